@@ -21,6 +21,7 @@ F32 = 0
 BF16 = 1
 F64 = 2  # the host library (CPU tensors) only
 F16 = 3  # the host library (CPU tensors) only
+E4M3 = 4  # what the pages of a key/value cache may hold
 TILE_CTR_INTS = 16  # ABACUS_MOE_TILE_CTR_INTS
 
 _P = ctypes.c_void_p
@@ -97,6 +98,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "abacus_cross_entropy_bwd": (_I, [_P, _P, _P, _P, _F, _I64, _I64, _I64, _I, _P, _P]),
     "abacus_cross_entropy_mean_fwd": (_I, [_P, _P, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P]),
     "abacus_cross_entropy_mean_bwd": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _P, _P]),
+    "abacus_kv_write": (_I, [_P, _P, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P]),
+    "abacus_kv_read": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _I64, _I, _P, _P, _P]),
+    "abacus_paged_attention_ws_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "abacus_paged_attention": (_I, [_P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P,
+                                    _P, _F, _I64, _I, _P, _P, _I64, _P]),
+    "abacus_verify_drafts_ws_bytes": (_I64, [_I64, _I64, _I64]),
+    "abacus_verify_drafts": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _D, _P, _P, _P, _I64, _P]),
     "abacus_adamw_step": (_I, [_P, _P, _P, _P, _P, _P, _I, _D, _D, _D, _D, _D, _I, _P]),
 }
 

@@ -1,0 +1,347 @@
+// The paged key/value cache: written (as it is, or quantised to e4m3) and read back.
+//
+// Key pages are (page, head, slot, dim), value pages (page, head, dim, slot):
+// the attention multiplies V^T by P^T, whose operand is 8 consecutive keys of one
+// dim, so with the values turned once here, where each is touched once, the
+// attention reads them as they lie on every later token.
+//
+// e4m3: one exponent byte per token and head.  With amax the largest magnitude,
+// e = the smallest integer with amax <= 448 * 2^e and byte = e + 127 (e = 0 for
+// amax = 0, and never below -110, so that every value a code stands for is a
+// normal bf16 number); codes are x * 2^-e rounded to nearest even.  The scale is a
+// power of two because it costs a floating-point code no precision, makes what a
+// code stands for exact in bf16, and is applied by the conversion instruction.  A
+// token's head with an infinity or NaN in its key or its value gets key codes NaN
+// and value codes 0: whoever sees the key gets NaN from its score, and nobody else
+// anything from 0 * V.
+//
+// Both kernels are bound by their bytes.  A work-group takes 16 (row, head) pairs
+// of one 16-slot group of one sequence, 16 lanes with 8 dims each per pair, so
+// that a full group is turned through LDS into whole 16-slot runs; a step's single
+// row (one group each) takes its 16 heads at once instead.
+#include <algorithm>
+
+#include "paged_rows.h"
+
+namespace abacus {
+namespace {
+
+constexpr int kGroup = 16;   // slots of a group: a divisor of every page size
+constexpr int kMaxK = 128;
+constexpr uint8_t kNaNCode = 0x7f;
+
+struct Pages {
+  void *k, *v;
+  uint8_t *k_scale, *v_scale;  // null unless e4m3
+  int H, K;
+};
+
+// 8 values at p as fp32
+template <typename T>
+__device__ inline void load8(const T* p, float (&x)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    const Vec16 v = ld16(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = lo_bf16(v.w[i]);
+      x[2 * i + 1] = hi_bf16(v.w[i]);
+    }
+  } else {
+    const Vec16 a = ld16(p), b = ld16(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = bits_f32(a.w[i]);
+      x[4 + i] = bits_f32(b.w[i]);
+    }
+  }
+}
+
+// 8 values to 8 of T
+template <typename T>
+__device__ inline void store8(T* to, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    Vec16 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w.w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    st16(to, w);
+  } else {
+    Vec16 w, z;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w.w[i] = f32_bits(x[i]);
+      z.w[i] = f32_bits(x[4 + i]);
+    }
+    st16(to, w);
+    st16(to + 4, z);
+  }
+}
+
+// The exponent byte of a row whose largest magnitude is amax (finite): 448 = 1.75 * 2^8.
+__device__ inline int scale_byte(float amax) {
+  const uint32_t u = f32_bits(amax);
+  const int e = (int)(u >> 23) - 127 - ((u & 0x7fffffu) <= 0x600000u ? 8 : 7);
+  return amax == 0.f ? 127 : max(e, -110) + 127;
+}
+
+// 8 values to 8 e4m3 codes of 2^(byte - 127) each
+__device__ inline uint2 codes8(const float (&x)[8], int byte) {
+  const float f = bits_f32((uint32_t)(254 - byte) << 23);  // (byte is 17 to 247)
+  uint2 c;
+  int w = 0;
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * f, x[1] * f, w, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * f, x[3] * f, w, true);
+  c.x = (uint32_t)w;
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4] * f, x[5] * f, w, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(x[6] * f, x[7] * f, w, true);
+  c.y = (uint32_t)w;
+  return c;
+}
+
+// C: what a slot holds (uint16_t bf16, float, uint8_t e4m3 code); T: what the rows are.
+template <typename T, typename C>
+__global__ __launch_bounds__(256) void kv_write_kernel(const T* __restrict__ k, const T* __restrict__ v, PagedRows a,
+                                                       Pages p) {
+  constexpr bool kCodes = sizeof(C) == 1;
+  __shared__ __attribute__((aligned(16))) C turned[kGroup][kMaxK + 16 / sizeof(C)];
+  const int tid = threadIdx.x, H = p.H, K = p.K;
+  int seq, local;
+  const bool any = find_unit(a.S, blockIdx.x, [&](int s) {
+    const SeqRows r = seq_rows(a, s);
+    return r.n > 0 && r.len > 0 ? (r.len - 1) / kGroup - max(r.len - r.n, 0) / kGroup + 1 : 0;
+  }, seq, local);
+  if (!any) return;
+  const SeqRows r = seq_rows(a, seq);
+  const int g0 = (max(r.len - r.n, 0) / kGroup + local) * kGroup;  // the group's first position
+  const int p0 = max(g0, r.len - r.n), p1 = min(g0 + kGroup, r.len), rows = p1 - p0;
+  const int pair0 = blockIdx.y * 16;
+  if (pair0 >= rows * H) return;
+  bool bad;
+  const int page = page_of(a, seq, g0, bad);
+  if (bad || r.bad) return;
+  const int in_page = g0 & ((1 << a.shift) - 1);
+
+  // this thread's pair and 8 dims
+  const int pair = pair0 + tid / 16, d0 = (tid % 16) * 8;
+  const int head = pair / rows, pos = p0 + pair % rows;
+  const bool mine = pair < rows * H && d0 < K;
+  const int64_t row = r.first + pos - (r.len - r.n);
+  float x[8] = {}, y[8] = {};
+  if (mine) {
+    load8(k + (row * H + head) * K + d0, x);
+    load8(v + (row * H + head) * K + d0, y);
+  }
+  const int64_t tile = (int64_t)page * H + head;  // (page, head)
+  if constexpr (kCodes) {
+    float mk = 0.f, mv = 0.f, bad_sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      mk = fmaxf(mk, fabsf(x[i]));
+      mv = fmaxf(mv, fabsf(y[i]));
+      bad_sum += x[i] * 0.f + y[i] * 0.f;  // 0, or NaN where an infinity or NaN is among them
+    }
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) {
+      mk = fmaxf(mk, __shfl_xor(mk, off, 64));
+      mv = fmaxf(mv, __shfl_xor(mv, off, 64));
+      bad_sum += __shfl_xor(bad_sum, off, 64);
+    }
+    const bool poison = !(bad_sum == 0.f);
+    const int bk = poison ? 127 : scale_byte(mk), bv = poison ? 127 : scale_byte(mv);
+    uint2 ck = codes8(x, bk), cv = codes8(y, bv);
+    if (poison) {
+      ck.x = ck.y = kNaNCode * 0x01010101u;
+      cv.x = cv.y = 0;
+    }
+    if (mine) {
+      const int64_t slot = (tile << a.shift) + in_page + (pos - g0);
+      *reinterpret_cast<uint2*>((uint8_t*)p.k + slot * K + d0) = ck;
+      if (d0 == 0) {
+        p.k_scale[slot] = (uint8_t)bk;
+        p.v_scale[slot] = (uint8_t)bv;
+      }
+    }
+    *reinterpret_cast<uint2*>(&turned[tid / 16][d0]) = cv;
+  } else {
+    if (mine) store8((C*)p.k + ((tile << a.shift) + in_page + (pos - g0)) * K + d0, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) turned[tid / 16][d0 + i] = from_f32<C>(y[i]);
+  }
+  __syncthreads();
+  // the values, slot by slot of one dim
+  if (rows == kGroup) {  // 16 pairs are one head's 16 slots
+    for (int i = tid; i < K * 2; i += 256) {
+      const int d = i / 2, s0 = (i % 2) * 8;
+      C* to = (C*)p.v + ((((int64_t)page * H + pair0 / kGroup) * K + d) << a.shift) + in_page + s0;
+      union { C c[8]; uint32_t w[2 * sizeof(C)]; } run;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) run.c[j] = turned[s0 + j][d];
+#pragma unroll
+      for (int j = 0; j < (int)(2 * sizeof(C)); j += 2) {
+        uint2 w;
+        w.x = run.w[j];
+        w.y = run.w[j + 1];
+        *reinterpret_cast<uint2*>((uint32_t*)to + j) = w;
+      }
+    }
+  } else {
+    for (int i = tid; i < 16 * K; i += 256) {
+      const int q = i / K, d = i % K, pr = pair0 + q;
+      if (pr >= rows * H) break;
+      const int off = in_page + p0 - g0 + pr % rows;
+      ((C*)p.v)[((((int64_t)page * H + pr / rows) * K + d) << a.shift) + off] = turned[q][d];
+    }
+  }
+}
+
+// 8 held values (codes: times 2^(byte - 127)) as fp32
+template <typename C>
+__device__ inline void widen8(const C* p, int byte, float (&x)[8]) {
+  if constexpr (sizeof(C) == 1) {
+    const uint2 c = *reinterpret_cast<const uint2*>(p);
+    const float s = bits_f32((uint32_t)byte << 23);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int w = (int)(h ? c.y : c.x);
+      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+      x[4 * h] = lo[0] * s;
+      x[4 * h + 1] = lo[1] * s;
+      x[4 * h + 2] = hi[0] * s;
+      x[4 * h + 3] = hi[1] * s;
+    }
+  } else {
+    load8(p, x);
+  }
+}
+
+// Rows (s, l) of out, l < L: position l of sequence s, 0 past its length.  A block
+// takes 16 positions of one head.
+template <typename C, typename T>
+__global__ __launch_bounds__(256) void kv_read_kernel(PagedRows a, Pages p, int64_t L, T* __restrict__ k,
+                                                      T* __restrict__ v) {
+  __shared__ __attribute__((aligned(16))) C turned[kMaxK][kGroup + (sizeof(C) == 1 ? 0 : 16 / sizeof(C))];
+  const int tid = threadIdx.x, H = p.H, K = p.K;
+  const int seq = blockIdx.z, head = blockIdx.x, g0 = blockIdx.y * kGroup;
+  const int pos = g0 + tid / 16, d0 = (tid % 16) * 8;
+  const int given = a.lengths[seq], most = a.P << a.shift, len = min(max(given, 0), most);
+  float x[8] = {}, y[8] = {};
+  if (g0 < len) {
+    bool bad;
+    const int page = page_of(a, seq, g0, bad);
+    bad |= given > most;
+    const int in_page = g0 & ((1 << a.shift) - 1);
+    const int64_t tile = (int64_t)page * H + head, slot = (tile << a.shift) + in_page + tid / 16;
+    for (int d = tid; d < K; d += 256) {
+      const C* from = (const C*)p.v + ((tile * K + d) << a.shift) + in_page;
+#pragma unroll
+      for (int j = 0; j < (int)sizeof(C); ++j)
+        *reinterpret_cast<Vec16*>((char*)turned[d] + 16 * j) = ld16((const char*)from + 16 * j);
+    }
+    __syncthreads();
+    if (pos < len && d0 < K) {
+      int bk = 127, bv = 127;
+      bool poison = bad;
+      if constexpr (sizeof(C) == 1) {
+        bk = p.k_scale[slot];
+        bv = p.v_scale[slot];
+        poison |= (((const uint8_t*)p.k)[slot * K] & 0x7f) == kNaNCode;
+      }
+      widen8((const C*)p.k + slot * K + d0, bk, x);
+      C run[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) run[i] = turned[d0 + i][tid / 16];
+      if constexpr (sizeof(C) == 1) {
+        uint2 c;
+        c.x = run[0] | run[1] << 8 | run[2] << 16 | (uint32_t)run[3] << 24;
+        c.y = run[4] | run[5] << 8 | run[6] << 16 | (uint32_t)run[7] << 24;
+        widen8((const C*)&c, bv, y);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = to_f32(run[i]);
+      }
+      if (poison) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = bad ? __builtin_nanf("") : x[i], y[i] = __builtin_nanf("");
+      }
+    }
+  }
+  if (pos < L && d0 < K) {
+    const int64_t at = ((seq * L + pos) * H + head) * K + d0;
+    store8(k + at, x);
+    store8(v + at, y);
+  }
+}
+
+int check_pages(const char* what, const void* k, const void* v, const void* k_scale, const void* v_scale, int dtype,
+                int held) {
+  ABACUS_CHECK_ARG(dtype == kF32 || dtype == kBF16, "%s: dtype code %d", what, dtype);
+  ABACUS_CHECK_ARG(held == dtype || held == ABACUS_E4M3, "%s: a cache of dtype code %d with rows of %d", what, held, dtype);
+  ABACUS_CHECK_ARG(k && v && (held != ABACUS_E4M3 || (k_scale && v_scale)), "%s: null pointer", what);
+  ABACUS_CHECK_ARG(((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_scale | (uintptr_t)v_scale) % 16 == 0,
+                   "%s: pages must be 16-byte aligned", what);
+  return 0;
+}
+
+}  // namespace
+}  // namespace abacus
+
+using namespace abacus;
+
+extern "C" int abacus_kv_write(const void* k_THK, const void* v_THK, int64_t T, int64_t H, int64_t K, int dtype,
+                               const int32_t* page_table_SP, const int32_t* query_start, const int32_t* lengths,
+                               int64_t S, int64_t P, int64_t page_size, int64_t n_pages, int held, void* k_pages,
+                               void* v_pages, void* k_scale, void* v_scale, void* stream) {
+  if (check_paged_rows("kv_write", page_table_SP, query_start, lengths, S, P, T, page_size, n_pages, H, K)) return 1;
+  if (check_pages("kv_write", k_pages, v_pages, k_scale, v_scale, dtype, held)) return 1;
+  if (T == 0) return 0;
+  ABACUS_CHECK_ARG(k_THK && v_THK && ((uintptr_t)k_THK | (uintptr_t)v_THK) % 16 == 0,
+                   "kv_write: k and v must be there, and 16-byte aligned");
+  PagedRows a{page_table_SP, query_start, lengths, (int)S, (int)P, (int)T, __builtin_ctzll(page_size), (int)n_pages};
+  Pages p{k_pages, v_pages, (uint8_t*)k_scale, (uint8_t*)v_scale, (int)H, (int)K};
+  // a sequence's rows touch at most n / 16 groups and the two at their ends
+  const int64_t groups = std::min<int64_t>(T, T / kGroup + 2 * S);
+  const dim3 grid((unsigned)groups, (unsigned)H);  // 16 pairs a block, at most 16 H in a group
+  hipStream_t s = (hipStream_t)stream;
+  if (held == ABACUS_E4M3 && dtype == kBF16)
+    hipLaunchKernelGGL((kv_write_kernel<uint16_t, uint8_t>), grid, dim3(256), 0, s, (const uint16_t*)k_THK,
+                       (const uint16_t*)v_THK, a, p);
+  else if (held == ABACUS_E4M3)
+    hipLaunchKernelGGL((kv_write_kernel<float, uint8_t>), grid, dim3(256), 0, s, (const float*)k_THK,
+                       (const float*)v_THK, a, p);
+  else if (dtype == kBF16)
+    hipLaunchKernelGGL((kv_write_kernel<uint16_t, uint16_t>), grid, dim3(256), 0, s, (const uint16_t*)k_THK,
+                       (const uint16_t*)v_THK, a, p);
+  else
+    hipLaunchKernelGGL((kv_write_kernel<float, float>), grid, dim3(256), 0, s, (const float*)k_THK,
+                       (const float*)v_THK, a, p);
+  ABACUS_CHECK_LAUNCH("kv_write");
+  return 0;
+}
+
+extern "C" int abacus_kv_read(const int32_t* page_table_SP, const int32_t* lengths, int64_t S, int64_t P,
+                              int64_t page_size, int64_t n_pages, int64_t H, int64_t K, int held, const void* k_pages,
+                              const void* v_pages, const void* k_scale, const void* v_scale, int64_t L, int dtype,
+                              void* k_SLHK, void* v_SLHK, void* stream) {
+  if (check_paged_rows("kv_read", page_table_SP, lengths, lengths, S, P, 0, page_size, n_pages, H, K)) return 1;
+  if (check_pages("kv_read", k_pages, v_pages, k_scale, v_scale, dtype, held)) return 1;
+  ABACUS_CHECK_ARG(S <= 65535 && L >= 0 && L <= 65535 * kGroup, "kv_read: %lld sequences of %lld tokens", (long long)S,
+                   (long long)L);
+  if (L == 0) return 0;
+  ABACUS_CHECK_ARG(k_SLHK && v_SLHK && ((uintptr_t)k_SLHK | (uintptr_t)v_SLHK) % 16 == 0,
+                   "kv_read: k and v must be there, and 16-byte aligned");
+  PagedRows a{page_table_SP, nullptr, lengths, (int)S, (int)P, 0, __builtin_ctzll(page_size), (int)n_pages};
+  Pages p{(void*)k_pages, (void*)v_pages, (uint8_t*)k_scale, (uint8_t*)v_scale, (int)H, (int)K};
+  const dim3 grid((unsigned)H, (unsigned)((L + kGroup - 1) / kGroup), (unsigned)S);
+  hipStream_t s = (hipStream_t)stream;
+  if (held == ABACUS_E4M3 && dtype == kBF16)
+    hipLaunchKernelGGL((kv_read_kernel<uint8_t, uint16_t>), grid, dim3(256), 0, s, a, p, L, (uint16_t*)k_SLHK,
+                       (uint16_t*)v_SLHK);
+  else if (held == ABACUS_E4M3)
+    hipLaunchKernelGGL((kv_read_kernel<uint8_t, float>), grid, dim3(256), 0, s, a, p, L, (float*)k_SLHK, (float*)v_SLHK);
+  else if (dtype == kBF16)
+    hipLaunchKernelGGL((kv_read_kernel<uint16_t, uint16_t>), grid, dim3(256), 0, s, a, p, L, (uint16_t*)k_SLHK,
+                       (uint16_t*)v_SLHK);
+  else
+    hipLaunchKernelGGL((kv_read_kernel<float, float>), grid, dim3(256), 0, s, a, p, L, (float*)k_SLHK, (float*)v_SLHK);
+  ABACUS_CHECK_LAUNCH("kv_read");
+  return 0;
+}

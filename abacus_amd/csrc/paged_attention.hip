@@ -1,0 +1,645 @@
+// Attention of new tokens over a paged key/value cache.
+//
+// Row j of a sequence's n new tokens has position len - n + j and sees the keys
+// up to it: o = sum_j softmax(scale q . k_j) v_j, query head h with key head h / G.
+// One pass over the keys with the running maximum and sum of the softmax in fp32.
+//
+// Work: rows r = (token, query head of the group) of one key head are packed, R to a
+// unit, so that shared key heads and drafted tokens fill a matrix instruction's
+// columns; a unit's keys are cut into `split` pieces of whole 64-key tiles where
+// there are too few units for the GPU, each piece gives its rows' maximum, sum and
+// unscaled output, and a second kernel joins them in order.  The piece length is the
+// same for the whole call: all (unit, key head, tile)s spread over kTarget pieces,
+// at least kLeast tiles each.  Which unit a block has is found from the device's
+// lengths by a scan (paged_rows.h), the launch being sized for the most there can be.
+//
+// In registers (v_mfma_f32_16x16x32_bf16: lane l gives A[l % 16][8 (l / 16) .. +7] and
+// B[8 (l / 16) .. +7][l % 16], and holds D[4 (l / 16) + r][l % 16] in register r):
+// S^T = K Q^T takes the keys of a 64-key tile in four products t = 0..3 whose row i is
+// key 16 (i / 4) + 4 t + i % 4.  Lane l then holds the scores of query l % 16 against
+// keys 16 (l / 16) + 4 t + r, 16 consecutive ones, and those are, as they lie, the
+// operand P^T of O^T = V^T P^T with V^T rows of 16 consecutive keys: neither the scores
+// nor a tile of keys or values goes through LDS.
+#include <algorithm>
+
+#include "paged_rows.h"
+
+namespace abacus {
+namespace {
+
+constexpr int kTile = 64;      // keys of a tile
+constexpr int kTarget = 2048;  // pieces the work is cut into, about
+constexpr int kLeast = 8;      // tiles of a piece, at least
+
+typedef __bf16 pa_bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 pa_bf16x2 __attribute__((ext_vector_type(2)));
+typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
+// 16 bytes of operands.  A vector and not Vec16's four words: of words loaded together and
+// masked on a branch the compiler (ROCm 7.2) let some be overwritten before their use.
+typedef uint32_t pa_u32x4 __attribute__((ext_vector_type(4)));
+
+struct PagedArgs {
+  PagedRows a;
+  const void *q, *k, *v;
+  const uint8_t *k_scale, *v_scale;
+  void* o;
+  float* part;  // (item, key head): R x K outputs, then R maxima, R sums
+  int H, Hk, G, K;
+  float scale_log2;
+  int zero_rest;  // rows of no sequence: 0, or left as they are
+};
+
+// How the rows of a call are cut, the same on every wave and in both kernels.
+struct Cut {
+  int chunk;  // tiles of a piece, at least
+};
+
+__host__ __device__ inline int units_of(int n, int G, int R) { return (int)(((int64_t)n * G + R - 1) / R); }
+
+template <int R>
+__device__ inline Cut cut_of(const PagedArgs& p) {
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0;  // tiles of one key head
+  for (int s = lane; s < p.a.S; s += 64) {
+    const SeqRows r = seq_rows(p.a, s);
+    total += (int64_t)units_of(r.n, p.G, R) * ((r.len + kTile - 1) / kTile);
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) total += __shfl_xor(total, off, 64);
+  const int64_t want = (kTarget + p.Hk - 1) / p.Hk;
+  Cut c;
+  c.chunk = (int)max((int64_t)kLeast, (total + want - 1) / want);
+  return c;
+}
+
+__device__ inline int splits_of(const SeqRows& r, const Cut& c) {
+  const int tiles = (r.len + kTile - 1) / kTile;
+  return max(1, (tiles + c.chunk - 1) / c.chunk);
+}
+
+// Rows r0 .. r0 + rows - 1 (of n * G) of unit u: the tiles that any of them sees.
+__device__ inline int seen_of(const SeqRows& r, int last_row, int G) {
+  return max(0, r.len - r.n + last_row / G + 1);  // keys
+}
+
+__device__ inline float group_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16, 64));
+  return fmaxf(x, __shfl_xor(x, 32, 64));
+}
+__device__ inline float group_sum(float x) {
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+
+__device__ inline pa_u32x4 load16(const void* p) { return *reinterpret_cast<const pa_u32x4*>(p); }
+
+__device__ inline void mfma16(pa_f32x4& acc, pa_u32x4 a, pa_u32x4 b) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8, a), __builtin_bit_cast(pa_bf16x8, b), acc,
+                                                0, 0, 0);
+}
+__device__ inline void mfma16_f32(pa_f32x4& acc, float a, float b) {
+  acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0);
+}
+
+// 4 codes (a dword), times 2^(exponent of s), as bf16 or fp32
+__device__ inline uint2 codes_bf16(uint32_t w, float s) {
+  uint2 r;
+  r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
+  r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true));
+  return r;
+}
+__device__ inline pa_u32x4 codes_f32(uint32_t w, float s) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  pa_u32x4 r;
+  r[0] = f32_bits(lo[0] * s);
+  r[1] = f32_bits(lo[1] * s);
+  r[2] = f32_bits(hi[0] * s);
+  r[3] = f32_bits(hi[1] * s);
+  return r;
+}
+__device__ inline float byte_scale(uint32_t w, int i) { return bits_f32(((w >> (8 * i)) & 0xffu) << 23); }
+
+// Bytes of one 16-lane row of operands.  Q: uint16_t (bf16 products) or float (fp32
+// products); Cd: whether the cache holds codes.  KD: the head dim the registers are
+// laid out for, K <= KD the one there is (Full: K == KD).
+template <typename Q, bool Cd, int KD, bool Full>
+struct Tile {
+  static constexpr bool kBf = sizeof(Q) == 2;
+  static constexpr int kHeld = Cd ? 1 : (int)sizeof(Q);  // bytes of a held value
+  static constexpr int kPer = 16 / kHeld;                // dims of a 16-byte load
+  static constexpr int NC = KD / (4 * kPer) > 0 ? KD / (4 * kPer) : 1;  // key loads of a lane and product
+  static constexpr int NS = kPer / (kBf ? 8 : 4) * NC;   // operands of those (8 bf16 or 4 fp32 dims each)
+  static constexpr int ND = KD / 16;                     // rows of 16 dims of V^T
+  static constexpr int NV = 16 / kPer;                   // value loads of a lane and 16 dims
+  pa_u32x4 k[4][NC], v[ND][NV];
+  pa_u32x4 ks, vs;  // exponent bytes: of the lane's key group's rows, of its value keys
+
+  // dims of key load c in lane group g
+  __device__ static inline int dim_of(int c, int g) { return (4 * c + g) * kPer; }
+
+  __device__ inline void load_k(const PagedArgs& p, int64_t tile, int off, int lane) {
+    const int i = lane & 15, g = lane >> 4, ps = p.a.shift;
+    const char* base = (const char*)p.k + (((tile << ps) + off + (i & 3)) * p.K) * kHeld;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int d = dim_of(c, g);
+        const bool in = Full || d < p.K;
+        k[t][c] = load16(base + (int64_t)(4 * t * p.K + (in ? d : 0)) * kHeld);
+        if constexpr (!Full)
+          if (!in) k[t][c] = pa_u32x4{0, 0, 0, 0};
+      }
+    if constexpr (Cd) ks = load16(p.k_scale + (tile << ps) + off);
+  }
+  __device__ inline void load_v(const PagedArgs& p, int64_t tile, int off, int lane) {
+    const int ps = p.a.shift;
+    const char* base = (const char*)p.v + ((tile * p.K) << ps) * kHeld;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) {
+      const int d = dt * 16 + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        v[dt][j] = load16(base + (((int64_t)(Full || d < p.K ? d : 0) << ps) + off + j * kPer) * kHeld);
+    }
+    if constexpr (Cd) vs = load16(p.v_scale + (tile << ps) + off);
+  }
+};
+
+// A block: the rows of one unit and key head against one piece of its keys, the
+// tiles dealt out to its four waves.
+template <typename Q, bool Cd, int KD, bool Full, int QT>
+__global__ __launch_bounds__(256, QT == 1 && sizeof(Q) == 2 ? 2 : 1) void paged_few_kernel(PagedArgs p) {
+  using TileT = Tile<Q, Cd, KD, Full>;
+  constexpr bool kBf = TileT::kBf;
+  constexpr int R = 16 * QT, ND = TileT::ND, NS = TileT::NS;
+  constexpr int kPitch = KD + 4;  // floats of a row's output in LDS
+  __shared__ __attribute__((aligned(16))) float merged[4][R][kPitch];
+  __shared__ float stat_m[4][R], stat_l[4][R];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, g = lane >> 4;
+  const int item = blockIdx.x / p.Hk, kh = blockIdx.x % p.Hk, G = p.G, K = p.K;
+
+  if (p.zero_rest) {
+    const int first = min(max(p.a.query_start[0], 0), p.a.T), end = min(max(p.a.query_start[p.a.S], first), p.a.T);
+    const int rest = p.a.T - (end - first), items = gridDim.x / p.Hk;
+    for (int r = item; r < rest; r += items) {
+      Q* row = (Q*)p.o + ((int64_t)(r < first ? r : end + r - first) * p.H + kh * G) * K;
+      for (int d = tid; d < G * K; d += 256) row[d] = from_f32<Q>(0.f);
+    }
+  }
+  const Cut cut = cut_of<R>(p);
+  int seq, local;
+  if (!find_unit(p.a.S, item, [&](int s) {
+        const SeqRows r = seq_rows(p.a, s);
+        return units_of(r.n, G, R) * splits_of(r, cut);
+      }, seq, local))
+    return;
+  const SeqRows r = seq_rows(p.a, seq);
+  const int split = splits_of(r, cut), units = units_of(r.n, G, R);
+  const int unit = units - 1 - local / split, piece = local % split;  // the units with the most keys first
+  const int row0 = unit * R, rows = min(R, r.n * G - row0);
+  const int seen = seen_of(r, row0 + rows - 1, G), least = seen_of(r, row0, G);
+  const int tiles = (seen + kTile - 1) / kTile, per = (tiles + split - 1) / split;
+  const int t0 = min(piece * per, tiles), t1 = min(t0 + per, tiles);
+
+  // Q^T operands, and how many keys the lane's rows see
+  pa_u32x4 qf[QT][NS];
+  int vis[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int m = qt * 16 + i, row = row0 + min(m, rows - 1);
+    const int token = row / G, head = kh * G + row % G;
+    vis[qt] = m < rows ? max(0, r.len - r.n + token + 1) : 0;
+    const Q* at = (const Q*)p.q + ((int64_t)(r.first + token) * p.H + head) * K;
+#pragma unroll
+    for (int c = 0; c < TileT::NC; ++c)
+#pragma unroll
+      for (int j = 0; j < NS / TileT::NC; ++j) {
+        const int d = TileT::dim_of(c, g) + j * (kBf ? 8 : 4);
+        const bool in = Full || d < K;
+        pa_u32x4 x = load16(at + (in ? d : 0));
+        if (!in) x = pa_u32x4{0, 0, 0, 0};
+        qf[qt][c * (NS / TileT::NC) + j] = x;
+      }
+  }
+
+  pa_f32x4 acc[QT][ND];
+  float m_run[QT], l_run[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    m_run[qt] = -__builtin_inff();
+    l_run[qt] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt) acc[qt][dt] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // The pages of a tile's four groups of 16 keys: the lane's key rows are in group
+  // i / 4, its value keys in group g.  Groups past the last key seen take the first.
+  struct Place { int64_t k, v; int ko, vo; bool bad; };
+  const int in_mask = (1 << p.a.shift) - 1;
+  auto place = [&](int tile) __attribute__((always_inline)) {
+    Place w;
+    const int pk = tile * kTile + (i >> 2) * 16, pv = tile * kTile + g * 16;
+    const int ck = pk < seen ? pk : 0, cv = pv < seen ? pv : 0;
+    bool bad_k, bad_v;
+    w.k = (int64_t)page_of(p.a, seq, ck, bad_k) * p.Hk + kh;
+    w.v = (int64_t)page_of(p.a, seq, cv, bad_v) * p.Hk + kh;
+    w.ko = ck & in_mask;
+    w.vo = cv & in_mask;
+    w.bad = bad_v && pv < seen;
+    return w;
+  };
+
+  TileT x;
+  Place here;
+  const int first = t0 + wave;
+  if (first < t1) {
+    here = place(first);
+    x.load_k(p, here.k, here.ko, lane);
+    x.load_v(p, here.v, here.vo, lane);
+  }
+  for (int tile = first; tile < t1; tile += 4) {
+    const int key0 = tile * kTile + g * 16;  // the lane's first key
+    const bool more = tile + 4 < t1;
+    const Place next = more ? place(tile + 4) : here;
+    // scores
+    pa_f32x4 s[QT][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) s[qt][t] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
+      const float sc = Cd ? byte_scale(x.ks[t], i & 3) : 1.f;
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        pa_u32x4 kf;
+        if constexpr (Cd && kBf) {
+          const uint2 a = codes_bf16(x.k[t][n / 2][2 * (n % 2)], sc), b = codes_bf16(x.k[t][n / 2][2 * (n % 2) + 1], sc);
+          kf[0] = a.x, kf[1] = a.y, kf[2] = b.x, kf[3] = b.y;
+        } else if constexpr (Cd) {
+          kf = codes_f32(x.k[t][n / 4][n % 4], sc);
+        } else {
+          kf = x.k[t][n];
+        }
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          if constexpr (kBf) {
+            mfma16(s[qt][t], kf, qf[qt][n]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mfma16_f32(s[qt][t], bits_f32(kf[e]), bits_f32(qf[qt][n][e]));
+          }
+        }
+      }
+    }
+    if (more) x.load_k(p, next.k, next.ko, lane);
+    const bool edge = tile * kTile + kTile > least;  // some row does not see some key of the tile
+    if (__any(here.bad)) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[qt][t][e] = here.bad ? __builtin_nanf("") : s[qt][t][e];
+    }
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      if (edge) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key0 + 4 * t + e >= vis[qt]) s[qt][t][e] = -__builtin_inff();
+      }
+      float mx = s[qt][0][0];
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[qt][t][e]);
+      mx = group_max(mx) * p.scale_log2;
+      // the maximum moves only when it grows by more than 8 (base 2): probabilities
+      // stay below 2^8, and most tiles leave the accumulators alone
+      const bool grow = mx > m_run[qt] + 8.f;
+      if (__any(grow)) {
+        const float m_new = grow ? mx : m_run[qt];
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m_run[qt] - m_new) : 1.f;
+        l_run[qt] *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) acc[qt][dt] *= alpha;
+        m_run[qt] = m_new;
+      }
+      const float m_use = m_run[qt] == -__builtin_inff() ? 0.f : m_run[qt];  // (nothing seen yet)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qt][t][e], p.scale_log2, -m_use));
+          s[qt][t][e] = pr;
+          l_run[qt] += pr;
+        }
+    }
+    // Where a row does not look there may be anything, and 0 times an infinity or NaN is
+    // NaN.  Slots past the last key seen may hold what was there before: codes and
+    // exponents of those are cleared.  In a cache of the rows' own type a key that only
+    // some of the rows see may also be infinite or NaN (codes never are): such a tile
+    // goes key by key below.
+    bool poison = false;
+    if (edge) {
+      if constexpr (Cd) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int there = min(max(seen - key0 - 4 * t, 0), 4);
+          const uint32_t mask = there == 4 ? ~0u : (1u << (8 * there)) - 1u;
+          x.vs[t] &= mask;
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) x.v[dt][0][t] &= mask;
+        }
+      } else {
+        constexpr uint32_t top = kBf ? 0x7f80u : 0x7f800000u;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+          for (int j = 0; j < TileT::NV; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t w = x.v[dt][j][e];
+              poison |= (w & top) == top;
+              if constexpr (kBf) poison |= (w & (top << 16)) == (top << 16);
+            }
+      }
+    }
+    if (!__any(poison)) {
+      if constexpr (kBf) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          pa_u32x4 pf[QT];
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) {
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              w[e] = s[qt][2 * h + e / 4][e % 4];
+              if constexpr (Cd) w[e] *= byte_scale(x.vs[2 * h + e / 4], e % 4);  // exact: a power of two
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pf[qt][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
+          }
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) {
+            pa_u32x4 vf;
+            if constexpr (Cd) {
+              const uint2 a = codes_bf16(x.v[dt][0][2 * h], 1.f), b = codes_bf16(x.v[dt][0][2 * h + 1], 1.f);
+              vf[0] = a.x, vf[1] = a.y, vf[2] = b.x, vf[3] = b.y;
+            } else {
+              vf = x.v[dt][h];
+            }
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) mfma16(acc[qt][dt], vf, pf[qt]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if constexpr (Cd) {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[qt][t][e] *= byte_scale(x.vs[t], e);
+          }
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) {
+            pa_u32x4 vf;
+            if constexpr (Cd) vf = codes_f32(x.v[dt][0][t], 1.f);
+            else vf = x.v[dt][t];
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mfma16_f32(acc[qt][dt], bits_f32(vf[e]), s[qt][t][e]);
+          }
+        }
+      }
+    } else if constexpr (!Cd) {
+      // key by key: only the rows that see a key take its product
+      for (int key = 0; key < kTile; ++key) {
+        const int pos = tile * kTile + key;
+        if (pos >= seen) break;
+        const bool own = key >> 4 == g;
+        const int kt = (key >> 2) & 3, ke = key & 3;
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+          float pr = 0.f;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (own && t == kt && e == ke) pr = s[qt][t][e];
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) {
+            pa_f32x4 one = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (kBf) {
+              pa_u32x4 vf = pa_u32x4{0, 0, 0, 0}, pf = pa_u32x4{0, 0, 0, 0};
+              uint32_t w = 0;
+#pragma unroll
+              for (int n = 0; n < 8; ++n)
+                if (((key & 15) >> 1) == n) w = x.v[dt][n / 4][n % 4];
+              vf[0] = own ? (key & 1 ? w >> 16 : w & 0xffffu) : 0u;
+              pf[0] = pack_bf16x2(pr, 0.f);
+              mfma16(one, vf, pf);
+            } else {
+              uint32_t w = 0;
+#pragma unroll
+              for (int n = 0; n < 16; ++n)
+                if ((key & 15) == n) w = x.v[dt][n / 4][n % 4];
+              mfma16_f32(one, own ? bits_f32(w) : 0.f, pr);
+            }
+            if (pos < vis[qt]) acc[qt][dt] += one;
+          }
+        }
+      }
+    }
+    if (more) x.load_v(p, next.v, next.vo, lane);
+    here = next;
+  }
+
+  // the waves' parts, joined in their order
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const float l = group_sum(l_run[qt]);
+    if (g == 0) {
+      stat_m[wave][qt * 16 + i] = m_run[qt];
+      stat_l[wave][qt * 16 + i] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < ND; ++dt)
+      *reinterpret_cast<pa_f32x4*>(&merged[wave][qt * 16 + i][dt * 16 + g * 4]) = acc[qt][dt];
+  }
+  __syncthreads();
+  float* part = p.part + (int64_t)blockIdx.x * R * (K + 2);
+  for (int e = tid; e < rows * (K / 4); e += 256) {
+    const int m = e / (K / 4), d = e % (K / 4) * 4;
+    float top = stat_m[0][m];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, stat_m[w][m]);
+    float l = 0.f;
+    pa_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = stat_m[w][m] == -__builtin_inff() ? (stat_l[w][m] == 0.f ? 0.f : 1.f)
+                                                        : __builtin_amdgcn_exp2f(stat_m[w][m] - top);
+      l += f * stat_l[w][m];
+      o += f * *reinterpret_cast<const pa_f32x4*>(&merged[w][m][d]);
+    }
+    if (split > 1) {
+      *reinterpret_cast<pa_f32x4*>(part + (int64_t)m * K + d) = o;
+      if (d == 0) {
+        part[R * K + m] = top;
+        part[R * K + R + m] = l;
+      }
+    } else {
+      const int row = row0 + m, sees = r.len - r.n + row / G + 1;
+      const float inv = r.bad ? __builtin_nanf("") : 1.f / l;
+      Q* to = (Q*)p.o + ((int64_t)(r.first + row / G) * p.H + kh * G + row % G) * K + d;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) to[n] = from_f32<Q>(sees <= 0 && !r.bad ? 0.f : o[n] * inv);
+    }
+  }
+}
+
+// Joins the pieces of the units that were cut, one block per unit and key head.
+template <typename Q, int R>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
+  const int tid = threadIdx.x, G = p.G, K = p.K;
+  const int b = blockIdx.x / p.Hk, kh = blockIdx.x % p.Hk;
+  const Cut cut = cut_of<R>(p);
+  int seq, local;
+  if (!find_unit(p.a.S, b, [&](int s) { return units_of(seq_rows(p.a, s).n, G, R); }, seq, local)) return;
+  const SeqRows r = seq_rows(p.a, seq);
+  const int split = splits_of(r, cut), units = units_of(r.n, G, R);
+  if (split == 1) return;
+  // items before this sequence's: the same scan, to its end
+  const int lane = tid & 63;
+  int before = 0;
+  for (int s = lane; s < seq; s += 64) {
+    const SeqRows o = seq_rows(p.a, s);
+    before += units_of(o.n, G, R) * splits_of(o, cut);
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) before += __shfl_xor(before, off, 64);
+  const int row0 = local * R, rows = min(R, r.n * G - row0);
+  const int item = before + (units - 1 - local) * split;
+  const int64_t pitch = (int64_t)p.Hk * R * (K + 2);  // between a unit's pieces
+  const float* part = p.part + ((int64_t)item * p.Hk + kh) * R * (K + 2);
+  for (int e = tid; e < rows * (K / 4); e += 256) {
+    const int m = e / (K / 4), d = e % (K / 4) * 4;
+    float top = -__builtin_inff();
+    for (int i = 0; i < split; ++i) top = fmaxf(top, part[i * pitch + R * K + m]);
+    float l = 0.f;
+    pa_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < split; ++i) {
+      const float pm = part[i * pitch + R * K + m], pl = part[i * pitch + R * K + R + m];
+      const float f = pm == -__builtin_inff() ? (pl == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(pm - top);
+      l += f * pl;
+      o += f * *reinterpret_cast<const pa_f32x4*>(part + i * pitch + (int64_t)m * K + d);
+    }
+    const int row = row0 + m, sees = r.len - r.n + row / G + 1;
+    const float inv = r.bad ? __builtin_nanf("") : 1.f / l;
+    Q* to = (Q*)p.o + ((int64_t)(r.first + row / G) * p.H + kh * G + row % G) * K + d;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) to[n] = from_f32<Q>(sees <= 0 && !r.bad ? 0.f : o[n] * inv);
+  }
+}
+
+// What a launch is sized by.
+struct Plan {
+  int R;           // rows of a unit
+  int64_t units;   // at most
+  int64_t items;   // at most
+  bool cuts;       // whether any unit can be cut
+};
+
+Plan plan_of(int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G, int64_t Hk, int64_t max_new) {
+  Plan n;
+  const int64_t rows = std::min(T, max_new) * G;
+  n.R = rows <= 16 ? 16 : 32;
+  n.units = std::min(T * G, T * G / n.R + std::min(S, T));
+  const int64_t tiles = (P * page_size + kTile - 1) / kTile, most = (tiles + kLeast - 1) / kLeast;
+  n.cuts = most > 1;
+  n.items = std::min(n.units * most, n.units + (kTarget + Hk - 1) / Hk);
+  return n;
+}
+
+template <typename Q, bool Cd, int QT>
+void launch_few(const PagedArgs& p, unsigned blocks, hipStream_t s) {
+  if (p.K == 64) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 64, true, QT>), dim3(blocks), dim3(256), 0, s, p);
+  else if (p.K == 128) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 128, true, QT>), dim3(blocks), dim3(256), 0, s, p);
+  else if (p.K < 64) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 64, false, QT>), dim3(blocks), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 128, false, QT>), dim3(blocks), dim3(256), 0, s, p);
+}
+
+template <typename Q>
+int launch(const PagedArgs& p, const Plan& n, bool codes, hipStream_t s) {
+  const unsigned blocks = (unsigned)(n.items * p.Hk);
+  if (n.R == 16) codes ? launch_few<Q, true, 1>(p, blocks, s) : launch_few<Q, false, 1>(p, blocks, s);
+  else codes ? launch_few<Q, true, 2>(p, blocks, s) : launch_few<Q, false, 2>(p, blocks, s);
+  ABACUS_CHECK_LAUNCH("paged_attention");
+  if (n.cuts) {
+    const dim3 grid((unsigned)(n.units * p.Hk));
+    if (n.R == 16) hipLaunchKernelGGL((paged_join_kernel<Q, 16>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((paged_join_kernel<Q, 32>), grid, dim3(256), 0, s, p);
+    ABACUS_CHECK_LAUNCH("paged_attention (join)");
+  }
+  return 0;
+}
+
+}  // namespace
+}  // namespace abacus
+
+using namespace abacus;
+
+extern "C" int64_t abacus_paged_attention_ws_bytes(int64_t T, int64_t H, int64_t Hk, int64_t K, int64_t S, int64_t P,
+                                                   int64_t page_size, int64_t max_new) {
+  if (T < 1 || Hk < 1 || H % Hk != 0) return 0;
+  const Plan n = plan_of(T, S, P, page_size, H / Hk, Hk, max_new);
+  return n.cuts ? n.items * Hk * n.R * (K + 2) * 4 : 0;
+}
+
+extern "C" int abacus_paged_attention(const void* q_THK, int64_t T, int64_t H, int64_t Hk, int64_t K, int dtype,
+                                      const int32_t* page_table_SP, const int32_t* query_start,
+                                      const int32_t* lengths, int64_t S, int64_t P, int64_t page_size,
+                                      int64_t n_pages, int held, const void* k_pages, const void* v_pages,
+                                      const void* k_scale, const void* v_scale, float scale, int64_t max_new,
+                                      int zero_rest, void* o_THK, void* ws, int64_t ws_bytes, void* stream) {
+  if (check_paged_rows("paged_attention", page_table_SP, query_start, lengths, S, P, T, page_size, n_pages, Hk, K))
+    return 1;
+  ABACUS_CHECK_ARG(dtype == kF32 || dtype == kBF16, "paged_attention: dtype code %d", dtype);
+  ABACUS_CHECK_ARG(held == dtype || held == ABACUS_E4M3, "paged_attention: a cache of dtype code %d with queries of %d",
+                   held, dtype);
+  ABACUS_CHECK_ARG(H >= Hk && H % Hk == 0 && H <= 1024, "paged_attention: %lld heads over %lld key heads", (long long)H,
+                   (long long)Hk);
+  ABACUS_CHECK_ARG(T * H < (1ll << 31), "paged_attention: %lld rows of %lld heads are too many", (long long)T, (long long)H);
+  ABACUS_CHECK_ARG(scale > 0.f && scale < __builtin_inff(), "paged_attention: scale %g", (double)scale);
+  ABACUS_CHECK_ARG(max_new >= 1, "paged_attention: max_new %lld", (long long)max_new);
+  if (T == 0) return 0;
+  ABACUS_CHECK_ARG(q_THK && k_pages && v_pages && o_THK && (held != ABACUS_E4M3 || (k_scale && v_scale)),
+                   "paged_attention: null pointer");
+  ABACUS_CHECK_ARG(((uintptr_t)q_THK | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_scale |
+                    (uintptr_t)v_scale | (uintptr_t)o_THK | (uintptr_t)ws) % 16 == 0,
+                   "paged_attention: tensors must be 16-byte aligned");
+  const Plan n = plan_of(T, S, P, page_size, H / Hk, Hk, max_new);
+  const int64_t need = n.cuts ? n.items * Hk * n.R * (K + 2) * 4 : 0;
+  ABACUS_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "paged_attention: workspace of %lld bytes, need %lld",
+                   (long long)ws_bytes, (long long)need);
+  ABACUS_CHECK_ARG(n.items * Hk < (1ll << 31), "paged_attention: %lld rows of %lld heads are too many", (long long)T,
+                   (long long)H);
+  PagedArgs p;
+  p.a = PagedRows{page_table_SP, query_start, lengths, (int)S, (int)P, (int)T, __builtin_ctzll(page_size), (int)n_pages};
+  p.q = q_THK, p.k = k_pages, p.v = v_pages;
+  p.k_scale = (const uint8_t*)k_scale, p.v_scale = (const uint8_t*)v_scale;
+  p.o = o_THK, p.part = (float*)ws;
+  p.H = (int)H, p.Hk = (int)Hk, p.G = (int)(H / Hk), p.K = (int)K;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.zero_rest = zero_rest;
+  hipStream_t s = (hipStream_t)stream;
+  const bool codes = held == ABACUS_E4M3;
+  return dtype == kBF16 ? launch<uint16_t>(p, n, codes, s) : launch<float>(p, n, codes, s);
+}

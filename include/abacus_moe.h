@@ -43,6 +43,10 @@ extern "C" {
  * float), so its f_E and fp32 loss stay fp32. */
 enum { ABACUS_F32 = 0, ABACUS_BF16 = 1, ABACUS_F64 = 2, ABACUS_F16 = 3 };
 
+/* What the pages of a key/value cache may hold beside fp32 and bf16: e4m3 codes
+ * with one exponent byte per token and head. */
+enum { ABACUS_E4M3 = 4 };
+
 /* int32 elements of the tile-counter workspace (tile_ctr) that the weight-gradient
  * entry points take: device memory the call clears on its stream and then uses
  * for the launch's work counters.  Calls in flight at the same time need
@@ -413,6 +417,68 @@ int abacus_cross_entropy_mean_fwd(const void* logits_NV, const int64_t* targets_
 int abacus_cross_entropy_mean_bwd(const void* logits_NV, const int64_t* targets_N, const float* lse_N,
                                   const void* grad_loss, const float* count, int64_t N, int64_t V,
                                   int64_t ignore_index, int dtype, void* dlogits_NV, void* stream);
+
+/* The paged key/value cache of a decoding program (no counterpart in the reference).
+ * T rows of S sequences lie one after the other: rows query_start[s] ..
+ * query_start[s + 1] - 1 (S + 1 values) are the last positions of sequence s,
+ * which has lengths[s] tokens with them.  Position p of s lies in slot
+ * p % page_size of page page_table_SP[s][p / page_size] (P pages a row).
+ * Key pages are (n_pages, H, page_size, K), value pages (n_pages, H, K, page_size),
+ * `held` is what they hold: the rows' dtype, or ABACUS_E4M3 with exponent bytes
+ * k_scale and v_scale (n_pages, H, page_size): a code stands for
+ * code * 2^(byte - 127).  page_size: a power of two, 16 to 256; K: a multiple of 16 up to 128.
+ * The three index arrays are device memory: a range of rows outside [0, T] is taken
+ * as empty, rows whose sequence is longer than its table or whose pages lie outside the
+ * pool are not written, and read or attended to as NaN.
+ *
+ * write: k_THK and v_THK (T, H, K) into the pages.  e4m3: per row and head,
+ * e = the smallest integer (at least -110) with max|x| <= 448 * 2^e, 0 for a row of
+ * zeros; byte = e + 127; codes are x * 2^-e to nearest even.  Where a key or a value
+ * holds an infinity or NaN, both read back as NaN. */
+int abacus_kv_write(const void* k_THK, const void* v_THK, int64_t T, int64_t H, int64_t K, int dtype,
+                    const int32_t* page_table_SP, const int32_t* query_start, const int32_t* lengths, int64_t S,
+                    int64_t P, int64_t page_size, int64_t n_pages, int held, void* k_pages, void* v_pages,
+                    void* k_scale, void* v_scale, void* stream);
+
+/* Read back: row (s, l) of k_SLHK and v_SLHK (S, L, H, K) is position l of sequence s, 0 past its length. */
+int abacus_kv_read(const int32_t* page_table_SP, const int32_t* lengths, int64_t S, int64_t P, int64_t page_size,
+                   int64_t n_pages, int64_t H, int64_t K, int held, const void* k_pages, const void* v_pages,
+                   const void* k_scale, const void* v_scale, int64_t L, int dtype, void* k_SLHK, void* v_SLHK,
+                   void* stream);
+
+/* Attention of the T rows q_THK (T, H, K) over the pages of Hk heads, query head h with
+ * key head h / (H / Hk): o = softmax(scale q k^T) v over the positions up to the row's
+ * own, statistics and sums in fp32, probabilities rounded to bf16 where q is bf16; a
+ * row that sees nothing gives 0.  max_new: the most rows of one sequence, as far as the
+ * caller knows (T otherwise); it chooses the kernels and changes no result beyond
+ * rounding.  zero_rest: rows of no sequence become 0 (otherwise they are left as they
+ * are).  ws: device workspace of abacus_paged_attention_ws_bytes bytes. */
+int64_t abacus_paged_attention_ws_bytes(int64_t T, int64_t H, int64_t Hk, int64_t K, int64_t S, int64_t P,
+                                        int64_t page_size, int64_t max_new);
+int abacus_paged_attention(const void* q_THK, int64_t T, int64_t H, int64_t Hk, int64_t K, int dtype,
+                           const int32_t* page_table_SP, const int32_t* query_start, const int32_t* lengths,
+                           int64_t S, int64_t P, int64_t page_size, int64_t n_pages, int held, const void* k_pages,
+                           const void* v_pages, const void* k_scale, const void* v_scale, float scale,
+                           int64_t max_new, int zero_rest, void* o_THK, void* ws, int64_t ws_bytes, void* stream);
+
+/* Drafted tokens against the target's probabilities (no counterpart in the reference).
+ * Row t of target_TV (T, V) holds the logits of the token after tokens_T[t]; of a
+ * sequence's rows the first is its last known token and the others are drafts, and
+ * row t of draft_TV (NULL: the drafter was certain) holds the logits that tokens_T[t + 1]
+ * was drawn from.  With p = softmax(target / temperature) and q likewise, the draft after row t
+ * is accepted where uniforms_T2[t][0] * q(x) < p(x); after the last row r accepted,
+ * next_S[s] is the smallest i with sum_{j <= i} max(p_j - q_j, 0) > uniforms_T2[r][1]
+ * times the whole sum (p alone where every draft was accepted, or where the sum is 0).
+ * temperature 0: a draft is accepted where it is the row's largest logit (the lowest
+ * index of equals), and next is that one; uniforms_T2 and draft_TV are not read.
+ * accepted_S: drafts accepted.  A sequence without rows gives 0 and -1; a row without
+ * a distribution (a NaN, +inf, or -inf throughout) accepts nothing and gives -1.
+ * Exponentials and sums are in 64 bits.  ws: abacus_verify_drafts_ws_bytes bytes. */
+int64_t abacus_verify_drafts_ws_bytes(int64_t T, int64_t V, int64_t S);
+int abacus_verify_drafts(const void* target_TV, const void* draft_TV, const int64_t* tokens_T,
+                         const int32_t* query_start, const float* uniforms_T2, int64_t T, int64_t V, int64_t S,
+                         int dtype, double temperature, int32_t* accepted_S, int64_t* next_S, void* ws,
+                         int64_t ws_bytes, void* stream);
 
 /* One AdamW step (optimizers/adamw.py:85-119, AdamW.step) over n tensors in
  * as few launches as possible: for tensor i, params[i], grads[i], exp_avgs[i]

@@ -1,0 +1,293 @@
+"""The paged cache's kernels against plain 64-bit forms: one token to long contexts, every page size, head dims, shared
+key heads, cut and uncut keys, masked places that hold infinities and NaN, graphs and streams.  (Tolerances:
+paged_check.attention_bound.)"""
+
+import math
+
+import pytest
+import torch
+
+import paged_check as pc
+from abacus_amd.kv_cache import E4M3, BatchRows, PagedKVCache
+
+pytestmark = pytest.mark.gpu
+
+KINDS = [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32), (torch.bfloat16, E4M3), (torch.float32, E4M3)]
+
+
+def _filled(plan, H, K, page, dtype, held, seed=0, fill=None, max_new=None, spread=1.0):
+    """Pages that hold random keys and values of the plan's whole sequences, and those rows."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rows, n = pc.rows_of(plan, page, "cuda", seed=seed, max_new=max_new)
+    pages = pc.pages_of(n, H, page, K, held, "cuda", fill=fill)
+    whole = BatchRows(rows.page_table_SP, torch.tensor([0] + [length for _, length in plan]).cumsum(0).to(torch.int32).cuda(),
+                      rows.lengths)
+    total = sum(length for _, length in plan)
+    k, v = (spread * torch.randn(total, H, K, device="cuda", generator=g).to(dtype) for _ in range(2))
+    pages.write(k, v, whole)
+    return pages, rows, k, v, g
+
+
+def _check(pages, plan, rows, k, v, q, o, held, scale=None):
+    scale = 1 / math.sqrt(q.shape[-1]) if scale is None else scale
+    at = first = 0
+    for n, length in plan:
+        if n:
+            qs = q[first:first + n]
+            ks, vs = pc.held(k[at:at + length], held), pc.held(v[at:at + length], held)
+            want, weight = pc.attention(qs, ks, vs, scale)
+            got = o[first:first + n].double()
+            assert torch.equal(torch.isnan(got), torch.isnan(want)), (n, length)
+            off, most = (got - want).abs(), pc.attention_bound(qs, ks, want, weight, scale)
+            worst = float((off / most.clamp(min=1e-300)).nan_to_num(0.0).max())
+            assert worst <= 1.0, (n, length, worst)
+        at, first = at + length, first + n
+
+
+@pytest.mark.parametrize("dtype,held", KINDS)
+@pytest.mark.parametrize("K,page", [(16, 16), (64, 32), (80, 64), (128, 256)])
+def test_write_and_read(dtype, held, K, page):
+    """Whole groups, groups begun and ended inside, single rows: bit for bit what the cache should hold, and no other
+    slot is touched."""
+    H = 3
+    plan = [(1, 1), (40, 40), (0, 5), (17, 50), (1, 16), (1, 33), (300, 333), (2, 1)]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows, n = pc.rows_of(plan, page, "cuda")
+    fill = 0x55 if held == E4M3 else 3.0
+    pages = pc.pages_of(n, H, page, K, held, "cuda", fill=fill)
+    T = sum(n for n, _ in plan)
+    k, v = (torch.randn(T, H, K, device="cuda", generator=g).to(dtype) for _ in range(2))
+    k[3] = 0.0
+    k[5] *= 1e-30  # exponents at their least, and large
+    v[6] *= 1e30
+    pages.write(k, v, rows)
+    kr, vr = pages.read(rows, 340, torch.float32 if held == E4M3 else None)
+    untouched = 1.625 * 2.0 ** (3 + 0x55 - 127) if held == E4M3 else 3.0  # code 0x55: exponent 10 - 7, 1 + 5 / 8
+    first = 0
+    for s, (new, length) in enumerate(plan):
+        for got, x in ((kr, k), (vr, v)):
+            there = min(new, length)
+            assert torch.equal(got[s, length - there:length].double(), pc.held(x[first + new - there:first + new], held))
+            assert (got[s, :length - there] == untouched).all() and not got[s, length:].any()
+        first += new
+    taken = sum(min(new, length) for new, length in plan) * H * K
+    for t in (pages.k, pages.v):
+        other = (t.view(torch.uint8) == 0x55 if held == E4M3 else t == 3.0).sum()
+        assert int(other) >= t.numel() - taken
+
+
+@pytest.mark.parametrize("dtype,held", KINDS)
+@pytest.mark.parametrize("H,G,K,page,plan", [
+    (2, 1, 64, 16, [(1, 1), (1, 2), (1, 63), (1, 64), (1, 65), (1, 700)]),
+    (1, 4, 128, 64, [(1, 1500), (1, 40), (0, 9)]),
+    (2, 3, 80, 32, [(5, 5), (4, 130), (6, 1100)]),
+    (4, 8, 16, 128, [(3, 200), (9, 9)]),
+    (1, 16, 96, 16, [(1, 77), (2, 640)]),
+    (2, 2, 128, 16, [(40, 40), (1, 900), (130, 520), (1, 3)]),
+    (1, 1, 64, 256, [(257, 800)]),
+    (2, 5, 32, 64, [(70, 70), (3, 2)]),
+])
+def test_attention(dtype, held, H, G, K, page, plan):
+    pages, rows, k, v, g = _filled(plan, H, K, page, dtype, held)
+    T = sum(n for n, _ in plan)
+    q = torch.randn(T, H * G, K, device="cuda", generator=g).to(dtype)
+    o = pages.attend(q, rows)
+    _check(pages, plan, rows, k, v, q, o, held)
+    known = BatchRows(rows.page_table_SP, rows.query_start, rows.lengths, max_new=max(n for n, _ in plan))
+    _check(pages, plan, known, k, v, q, pages.attend(q, known, scale=0.3), held, 0.3)
+
+
+@pytest.mark.parametrize("dtype,held", KINDS)
+def test_long_context_is_cut_and_joined(dtype, held):
+    plan = [(1, 9000), (2, 33), (1, 20001)]
+    pages, rows, k, v, g = _filled(plan, 1, 64, 64, dtype, held, max_new=2)
+    q = 3 * torch.randn(4, 2, 64, device="cuda", generator=g).to(dtype)
+    o = pages.attend(q, rows)
+    _check(pages, plan, rows, k, v, q, o, held)
+    assert torch.equal(o, pages.attend(q, rows))  # the same bits again
+
+
+def test_many_sequences():
+    """More sequences than a wave scans at once, some without rows."""
+    plan = [((s * 7) % 3, 1 + (s * 37) % 90) for s in range(200)]
+    pages, rows, k, v, g = _filled(plan, 2, 64, 16, torch.bfloat16, torch.bfloat16)
+    T = sum(n for n, _ in plan)
+    q = torch.randn(T, 2, 64, device="cuda", generator=g).bfloat16()
+    _check(pages, plan, rows, k, v, q, pages.attend(q, rows), torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype,held", KINDS)
+@pytest.mark.parametrize("plan", [[(1, 5), (3, 70), (1, 130)], [(100, 300)]])
+def test_what_a_row_does_not_see_does_not_reach_it(dtype, held, plan):
+    """Pages full of NaN and infinities before the sequences are written; then a NaN and an infinity in the keys and
+    values of the last token: only the rows that see it have them, dim by dim as the formula has."""
+    K, H = 64, 2
+    for fill in ((0x7f, 0xff) if held == E4M3 else (math.nan, math.inf)):
+        pages, rows, k, v, g = _filled(plan, H, K, 32, dtype, held, fill=fill)
+        T = sum(n for n, _ in plan)
+        q = torch.randn(T, H, K, device="cuda", generator=g).to(dtype)
+        _check(pages, plan, rows, k, v, q, pages.attend(q, rows), held)
+    at = first = 0
+    for s, (n, length) in enumerate(plan):
+        last = at + length - 1
+        k[last, 0, 3] = math.nan
+        v[last, 1, 7] = math.inf
+        at += length
+    whole = BatchRows(rows.page_table_SP, torch.tensor([0] + [l for _, l in plan]).cumsum(0).to(torch.int32).cuda(), rows.lengths)
+    pages.write(k, v, whole)
+    o = pages.attend(q, rows)
+    at = first = 0
+    for n, length in plan:
+        for j in range(n):
+            row = o[first + j]
+            if j < n - 1:
+                assert torch.isfinite(row).all()
+            else:
+                assert torch.isnan(row[0]).all()
+                if held == E4M3:
+                    assert torch.isnan(row[1]).all()
+                else:
+                    assert row[1, 7] == math.inf and torch.isfinite(row[1, :7]).all() and torch.isfinite(row[1, 8:]).all()
+        if n > 1:  # the others as if it were not there
+            kk, vv = k[at:at + length].clone(), v[at:at + length].clone()
+            kk[-1], vv[-1] = 0.0, 0.0
+            want, weight = pc.attention(q[first:first + n], pc.held(kk, held), pc.held(vv, held), 1 / 8)
+            most = pc.attention_bound(q[first:first + n], pc.held(kk, held), want, weight, 1 / 8)
+            assert ((o[first:first + n].double() - want).abs() <= most)[:-1].all()
+        at, first = at + length, first + n
+
+
+@pytest.mark.parametrize("held", [torch.bfloat16, E4M3])
+def test_large_scores(held):
+    """Scores far beyond what exp holds without its running maximum, and a maximum that grows late."""
+    plan = [(2, 600)]
+    pages, rows, k, v, g = _filled(plan, 1, 64, 16, torch.bfloat16, held, spread=8.0)
+    q = 20 * torch.randn(2, 1, 64, device="cuda", generator=g).bfloat16()
+    _check(pages, plan, rows, k, v, q, pages.attend(q, rows), held)
+
+
+def test_refused_by_the_pages_on_the_device():
+    """Page ids outside the pool, lengths past the table, ranges of rows outside the batch: NaN or nothing, as on the
+    CPU (test_kv_cache.py)."""
+    for held in (torch.float32, E4M3):
+        rows, n = pc.rows_of([(1, 20), (1, 20), (1, 20), (1, 20)], 16, "cuda")
+        rows.page_table_SP[1, 1] = n
+        rows.lengths[2] = 33
+        rows.query_start[4] = 9  # past the batch: no rows
+        pages = pc.pages_of(n, 1, 16, 16, held, "cuda")
+        x = torch.ones(4, 1, 16, device="cuda")
+        pages.write(x, x, rows)
+        k, _ = pages.read(rows, 20, torch.float32)
+        assert torch.isnan(k[1, 16:]).all() and not torch.isnan(k[1, :16]).any() and torch.isnan(k[2]).all()
+        assert torch.equal(k[0, 19], x[0]) and not k[3].any()
+        out = torch.full_like(x, 7.0)
+        pages.attend(x, rows, out=out)
+        assert torch.isfinite(out[0]).all() and torch.isnan(out[1:3]).all() and (out[3] == 7.0).all()
+
+
+def test_rows_of_nothing():
+    rows, n = pc.rows_of([(2, 1), (1, 0)], 16, "cuda")
+    pages = pc.pages_of(n, 1, 16, 16, torch.float32, "cuda")
+    k = torch.ones(3, 1, 16, device="cuda")
+    pages.write(k, 2 * k, rows)
+    out = torch.full((5, 1, 16), 7.0, device="cuda")
+    q = torch.ones(5, 1, 16, device="cuda")
+    assert pages.attend(q, rows, out=out)[:, 0, 0].tolist() == [0.0, 2.0, 0.0, 7.0, 7.0]
+    assert pages.attend(q, rows)[:, 0, 0].tolist() == [0.0, 2.0, 0.0, 0.0, 0.0]
+    rows.query_start += 1  # a row before the first sequence
+    assert pages.attend(q, rows)[:, 0, 0].tolist() == [0.0, 0.0, 2.0, 0.0, 0.0]
+    assert pages.attend(q[:0], rows).shape == (0, 1, 16)
+
+
+def test_operands_of_any_stride():
+    plan = [(5, 90), (1, 33)]
+    pages, rows, k, v, g = _filled(plan, 2, 64, 16, torch.bfloat16, torch.bfloat16)
+    wide = torch.randn(6, 3, 4, 64, device="cuda", generator=g).bfloat16()
+    q = wide[:, 1]
+    assert not q.is_contiguous()
+    assert torch.equal(pages.attend(q, rows), pages.attend(q.contiguous(), rows))
+    flat = torch.empty(q.numel() + 1, device="cuda", dtype=q.dtype)
+    off = flat[1:].view(q.shape).copy_(q)
+    assert off.data_ptr() % 16 and torch.equal(pages.attend(off, rows), pages.attend(q.contiguous(), rows))
+    kn, vn = wide[:, 0, :2], wide[:, 2, 2:]
+    pages.write(kn, vn, rows)
+    kr, vr = pages.read(rows, 90)
+    assert torch.equal(kr[0, 85:], kn[:5]) and torch.equal(vr[0, 85:], vn[:5])
+    assert torch.equal(kr[1, 32], kn[5]) and torch.equal(vr[1, 32], vn[5])
+
+
+@pytest.mark.parametrize("held", [torch.bfloat16, E4M3])
+def test_captured_step_follows_its_rows(held):
+    """A write and an attention captured once: each replay writes and reads where the index tensors then say, and
+    eager work between the replays changes nothing."""
+    H, K, page, S = 2, 64, 16, 3
+    cache = PagedKVCache(1, 160, page, H, K, dtype=held, device="cuda")
+    pages = cache.layer(0)
+    twin = PagedKVCache(1, 160, page, H, K, dtype=held, device="cuda").layer(0)
+    seqs = [cache.add() for _ in range(S)]
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rand = lambda T, heads: torch.randn(T, heads, K, device="cuda", generator=g).bfloat16()
+    rows = cache.extend({s: 30 + 600 * s for s in seqs})
+    k, v = rand(int(rows.query_start[-1]), H), rand(int(rows.query_start[-1]), H)
+    pages.write(k, v, rows)
+    twin.write(k, v, rows)
+    static = BatchRows(torch.zeros(S, 100, dtype=torch.int32, device="cuda"), torch.zeros(S + 1, dtype=torch.int32, device="cuda"),
+                       torch.zeros(S, dtype=torch.int32, device="cuda"))
+    T = 9
+    q, k, v = rand(T, 2 * H), rand(T, H), rand(T, H)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        pages.attend(q, static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pages.write(k, v, static)
+        out = pages.attend(q, static)
+    for step in ({seqs[0]: 1, seqs[1]: 3, seqs[2]: 2}, {seqs[0]: 2, seqs[1]: 1, seqs[2]: 1}, {seqs[0]: 5, seqs[1]: 0, seqs[2]: 4}):
+        rows = cache.extend(step)
+        static.page_table_SP[:, :rows.page_table_SP.shape[1]] = rows.page_table_SP
+        static.query_start.copy_(rows.query_start)
+        static.lengths.copy_(rows.lengths)
+        for t, heads in ((q, 2 * H), (k, H), (v, H)):
+            t.copy_(rand(T, heads))
+        graph.replay()
+        twin.write(k, v, rows)
+        want = twin.attend(q, static)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert all(torch.equal(a, b) for a, b in zip(pages.read(rows, 1300), twin.read(rows, 1300)))
+
+
+def test_calls_on_two_streams():
+    plan = [(1, 5000), (1, 3000)]
+    pages, rows, k, v, g = _filled(plan, 2, 64, 64, torch.bfloat16, torch.bfloat16, max_new=1)
+    qs = [torch.randn(2, 2, 64, device="cuda", generator=g).bfloat16() for _ in range(2)]
+    want = [pages.attend(q, rows) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for q, stream in zip(qs, streams):
+            with torch.cuda.stream(stream):
+                got.append(pages.attend(q, rows))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_offsets_past_32_bits():
+    """A pool of more than 2^32 bytes (and 2^31 elements): its last pages are written and read."""
+    H, K, page = 8, 128, 256
+    n = (1 << 31) // (H * K * page) + 3  # 8195 pages of 2^18 elements
+    pages = pc.pages_of(n, H, page, K, torch.bfloat16, "cuda")
+    as_int = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    rows = BatchRows(as_int([[n - 2, n - 1], [0, 1]]), as_int([0, 300, 310]), as_int([300, 10]))
+    g = torch.Generator(device="cuda").manual_seed(2)
+    k, v = (torch.randn(310, H, K, device="cuda", generator=g).bfloat16() for _ in range(2))
+    pages.write(k, v, rows)
+    assert torch.equal(pages.k[n - 2].transpose(0, 1), k[:256])
+    assert torch.equal(pages.v[n - 1, :, :, :44].permute(2, 0, 1), v[256:300])
+    kr, vr = pages.read(rows, 300)
+    assert torch.equal(kr[0], k[:300]) and torch.equal(vr[0], v[:300]) and torch.equal(kr[1, :10], k[300:])
+    q = torch.randn(310, H, K, device="cuda", generator=g).bfloat16()
+    _check(pages, [(300, 300), (10, 10)], rows, k, v, q, pages.attend(q, rows), torch.bfloat16)
