@@ -24,6 +24,11 @@ reference's (scores, mask, softmax, weighted sum) as one autograd function
 whose batched products all take contiguous operands.  The dense projections
 and the embedding run on torch.  Tensor, sequence and context parallelism
 with more than one process are not implemented here (one GPU).
+
+``forward_cached`` (of the attention, the block and the model; no reference
+counterpart) runs only the new tokens of some sequences, over the paged cache of
+abacus_amd.kv_cache: the same norms, rotary tables and weights, so it gives what
+``forward`` gives for the whole sequences up to rounding.
 """
 
 from __future__ import annotations
@@ -34,6 +39,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
+from .kv_cache import BatchRows, KVPages, PagedKVCache
 from .moe import MoE, MoEExpertParallel, _contig, _rank_and_world_size
 
 __all__ = [
@@ -698,6 +704,46 @@ class MultiHeadAttention(torch.nn.Module):
         joined = out.permute(0, 2, 1, 3).reshape(B, L, H * K)
         return joined @ self.w_o_HKD.reshape(H * K, self.dim)  # (B, L, D)
 
+    @torch.no_grad()
+    def forward_cached(self, x_TD: torch.Tensor, pages: KVPages, rows: BatchRows, cos_TK: torch.Tensor | None = None,
+                       sin_TK: torch.Tensor | None = None) -> torch.Tensor:
+        """The attention of T new tokens (`rows` says whose) over `pages`, which their keys and values are written
+        into first.  cos_TK, sin_TK: the rotary tables at the rows' positions."""
+        if self.context_parallel or self.world_size > 1:
+            _single_process("attention parallelism")
+        _check_cached(self, x_TD, "(tokens, dim)", 2)
+        T, D = x_TD.shape
+        if T == 0:
+            return x_TD
+        H, K = self.local_heads, self.head_dim
+        q, k, v = ((x_TD @ w.reshape(D, H * K)).view(T, H, K) for w in (self.w_q_DHK, self.w_k_DHK, self.w_v_DHK))
+        q, k = self._norm_rope(q, k, cos_TK, sin_TK)
+        pages.write(k, v, rows)
+        return pages.attend(q, rows).view(T, H * K) @ self.w_o_HKD.reshape(H * K, self.dim)
+
+    def _norm_rope(self, q_THK, k_THK, cos_TK, sin_TK):
+        """The q and k norms and the rotary embedding, row t at the tables' row t."""
+        gamma_q, gamma_k = self.q_norm.w_gamma_D, self.k_norm.w_gamma_D
+        if cos_TK is None:
+            return self.q_norm(q_THK), self.k_norm(k_THK)
+        if not (_fused_rope_ok(q_THK, gamma_q, cos_TK, sin_TK) and _fused_rope_ok(k_THK, gamma_k, cos_TK, sin_TK)):
+            return apply_rotary_pos_emb(self.q_norm(q_THK), self.k_norm(k_THK), cos_TK[:, None], sin_TK[:, None])
+        T, H, K = q_THK.shape
+        qn, kn = torch.empty_like(q_THK), torch.empty_like(k_THK)
+        rstd = torch.empty(2, T * H, dtype=torch.float32, device=q_THK.device)
+        _lib.call("abacus_qk_norm_rope_fwd", _lib.ptr(_contig(q_THK)), _lib.ptr(_contig(k_THK)), _lib.ptr(_contig(gamma_q)),
+                  _lib.ptr(_contig(gamma_k)), _lib.ptr(_contig(cos_TK)), _lib.ptr(_contig(sin_TK)), T * H, T, H, K, 1e-5,
+                  _lib.dtype_code(q_THK.dtype), _lib.ptr(qn), _lib.ptr(kn), _lib.ptr(rstd), _lib.stream_of(q_THK.device))
+        return qn, kn
+
+
+def _check_cached(module: torch.nn.Module, x: torch.Tensor, shape: str, dims: int) -> None:
+    if module.training:
+        raise ValueError("forward_cached is the eval-mode forward: call eval() first (a training forward steps the "
+                         "router bias and has no cache)")
+    if x.dim() != dims:
+        raise ValueError(f"forward_cached takes {shape}, got {tuple(x.shape)}")
+
 
 class TransformerBlockMoe(torch.nn.Module):
     """x + attention(RMSNorm(x)), then x + MoE(RMSNorm(x)) (transformer_block.py:64-110)."""
@@ -737,6 +783,13 @@ class TransformerBlockMoe(torch.nn.Module):
         x_BLD = x_BLD + self.dropout(attn_BLD)
         moe_BLD = self.moe(self.norm_mlp(x_BLD))
         return x_BLD + self.dropout(moe_BLD)
+
+    @torch.no_grad()
+    def forward_cached(self, x_TD: torch.Tensor, pages: KVPages, rows: BatchRows, cos_TK: torch.Tensor | None = None,
+                       sin_TK: torch.Tensor | None = None) -> torch.Tensor:
+        _check_cached(self, x_TD, "(tokens, dim)", 2)
+        x_TD = x_TD + self.attention.forward_cached(self.norm_attention(x_TD), pages, rows, cos_TK, sin_TK)
+        return x_TD + self.moe(self.norm_mlp(x_TD))
 
 
 class TransformerMoe(torch.nn.Module):
@@ -786,3 +839,20 @@ class TransformerMoe(torch.nn.Module):
         for block in self.blocks:
             x_BLD = block(x_BLD, self.rotary)
         return self.norm(x_BLD) @ self.w_D_vocab  # (B, L, vocab)
+
+    @torch.no_grad()
+    def forward_cached(self, tokens_T: torch.Tensor, cache: PagedKVCache, rows: BatchRows,
+                       out_rows: torch.Tensor | None = None) -> torch.Tensor:
+        """Logits (T, vocab) of T new tokens of some sequences, or of the rows out_rows (int64) of them; their keys
+        and values are left in `cache` (a layer per block).  `rows` says which tokens belong to which sequence, as
+        ``cache.extend`` gives it."""
+        _check_cached(self, tokens_T, "(tokens,)", 1)
+        if cache.n_layers != self.n_blocks:
+            raise ValueError(f"a cache of {cache.n_layers} layers for {self.n_blocks} blocks")
+        x_TD = self.embedding(tokens_T)
+        cos, sin = self.rotary(x_TD, positions=rows.positions(tokens_T.shape[0]))  # (1, 1, T, K)
+        for i, block in enumerate(self.blocks):
+            x_TD = block.forward_cached(x_TD, cache.layer(i), rows, cos[0, 0], sin[0, 0])
+        if out_rows is not None:
+            x_TD = x_TD[out_rows]
+        return self.norm(x_TD) @ self.w_D_vocab

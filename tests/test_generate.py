@@ -1,0 +1,138 @@
+"""forward_cached and generate: the cached forward against the whole one, and the decoding loop with and without drafts."""
+
+import pytest
+import torch
+
+from abacus_amd.generate import generate
+from abacus_amd.kv_cache import E4M3, PagedKVCache
+from abacus_amd.transformer import TransformerMoe
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _model(seed=0, dim=32, heads=2, head_dim=16, blocks=2, vocab=50, device="cpu", dtype=torch.float32):
+    torch.manual_seed(seed)
+    model = TransformerMoe(dim, heads, head_dim, blocks, vocab, n_experts=4, top_k=2, hidden_dim=24)
+    return model.to(dtype).to(device).eval()
+
+
+def _whole(model, tokens):
+    with torch.no_grad():
+        return model(torch.tensor([tokens], device=model.w_D_vocab.device))[0]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("head_dim", [16, 64])
+def test_cached_forward_matches_the_whole_one(device, head_dim):
+    """fp32: token by token, in chunks and mixed, the logits are the whole forward's up to the rounding of fp32 sums
+    (relative 2^-24 of each of about dim + length terms, over the layers, well within 1e-4 of the largest logit)."""
+    model = _model(device=device, head_dim=head_dim)
+    g = torch.Generator().manual_seed(1)
+    seqs = [torch.randint(0, 50, (n,), generator=g).tolist() for n in (37, 5, 61)]
+    cache = PagedKVCache(2, 12, 16, 2, head_dim, dtype=torch.float32, device=device)
+    ids = [cache.add() for _ in seqs]
+    want = [_whole(model, s) for s in seqs]
+    at = [0, 0, 0]
+    for step in ((30, 1, 60), (1, 1, 0), (4, 1, 1), (2, 2, 0)):
+        new = {ids[i]: n for i, n in enumerate(step)}
+        tokens = [x for i, n in enumerate(step) for x in seqs[i][at[i]:at[i] + n]]
+        logits = model.forward_cached(torch.tensor(tokens, device=device), cache, cache.extend(new))
+        first = 0
+        for i, n in enumerate(step):
+            got = logits[first:first + n]
+            assert float((got - want[i][at[i]:at[i] + n]).abs().max()) <= 1e-4 * float(want[i].abs().max()) if n else True
+            at[i], first = at[i] + n, first + n
+    assert at == [37, 5, 61]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_greedy_generation_is_the_whole_forwards(device):
+    model = _model(device=device)
+    prompts = [[1, 2, 3], [7], list(range(20))]
+    got = generate(model, prompts, 12, page_size=16, prefill_chunk=7)
+    for prompt, new in zip(prompts, got):
+        assert len(new) == 12
+        logits = _whole(model, prompt + new)
+        for j, x in enumerate(new):
+            row = logits[len(prompt) + j - 1]
+            assert float(row[x]) >= float(row.max()) - 1e-4 * float(row.abs().max())  # the largest, up to rounding
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("drafter", ["itself", "another"])
+def test_drafts_change_the_steps_and_not_the_tokens(device, drafter, monkeypatch):
+    model = _model(device=device)
+    other = model if drafter == "itself" else _model(seed=9, dim=16, heads=1, blocks=1, device=device)
+    prompts = [[1, 2, 3], [7], list(range(20))]
+    plain = generate(model, prompts, 15, page_size=16)
+    steps = []
+    whole = TransformerMoe.forward_cached
+    monkeypatch.setattr(TransformerMoe, "forward_cached", lambda self, t, *a: (steps.append((self is model, t.numel())),
+                                                                             whole(self, t, *a))[1])
+    assert generate(model, prompts, 15, page_size=16, draft_model=other, n_draft=3) == plain
+    if drafter == "itself":  # every draft is accepted: four tokens a step
+        assert sum(n == 3 * 4 for _, n in steps) == 4  # 15 tokens, four at a time
+    stop = plain[0][4]
+    cut = generate(model, prompts, 15, page_size=16, draft_model=other, n_draft=3, stop_token=stop)
+    for a, b in zip(cut, plain):
+        end = b.index(stop) + 1 if stop in b else 15
+        assert a == b[:end]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sampling_follows_the_generator(device):
+    model, other = _model(device=device), _model(seed=9, dim=16, heads=1, blocks=1, device=device)
+    run = lambda seed, **more: generate(model, [[3, 4]] * 4, 8, temperature=0.9, page_size=16,
+                                        generator=torch.Generator(device=device).manual_seed(seed), **more)
+    assert run(0) == run(0) != run(1)
+    drafted = run(0, draft_model=other, n_draft=2)
+    assert drafted == run(0, draft_model=other, n_draft=2)
+    assert all(len(t) == 8 and all(0 <= x < 50 for x in t) for t in drafted)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_quantised_cache_runs(device):
+    model = _model(device=device, head_dim=64)
+    got = generate(model, [[5, 6], [1]], 6, page_size=16, cache_dtype=E4M3)
+    assert [len(t) for t in got] == [6, 6]
+
+
+def test_refusals():
+    model = _model()
+    cache = PagedKVCache(2, 4, 16, 2, 16, dtype=torch.float32)
+    seq = cache.add()
+    tokens = torch.tensor([1])
+    with pytest.raises(ValueError, match="eval"):
+        model.train().forward_cached(tokens, cache, cache.extend({seq: 1}))
+    model.eval()
+    rows = cache.rows({seq: 1})
+    with pytest.raises(ValueError, match="tokens"):
+        model.forward_cached(tokens[None], cache, rows)
+    with pytest.raises(ValueError, match="layers"):
+        model.forward_cached(tokens, PagedKVCache(1, 4, 16, 2, 16, dtype=torch.float32), rows)
+    for bad in (dict(prompts=[]), dict(prompts=[[]]), dict(prompts=[[50]]), dict(prompts=[[1]], max_new_tokens=-1)):
+        with pytest.raises(ValueError):
+            generate(model, **{"max_new_tokens": 3, **bad})
+    with pytest.raises(ValueError, match="drafter"):
+        generate(model, [[1]], 3, draft_model=_model(vocab=49))
+    assert generate(model, [[1]], 0) == [[]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("held", [torch.bfloat16, E4M3])
+def test_bf16_cached_forward_on_the_gpu(held):
+    """bf16 over two blocks: the cached logits against the fp32 model's whole forward, no further off than twice the bf16
+    whole forward (each rounds the same tensors once, independently: sqrt(2) of one side's error apart).  e4m3 pages: it
+    runs (what they hold and give is test_gpu_kv_cache's)."""
+    exact = _model(dim=128, head_dim=64, device="cuda")
+    model = _model(dim=128, head_dim=64, device="cuda", dtype=torch.bfloat16)
+    g = torch.Generator().manual_seed(1)
+    tokens = torch.randint(0, 50, (150,), generator=g).tolist()
+    cache = PagedKVCache(2, 5, 32, 2, 64, dtype=held, device="cuda")
+    seq, parts = cache.add(), []
+    for a, b in ((0, 100), (100, 101), (101, 150)):
+        parts.append(model.forward_cached(torch.tensor(tokens[a:b], device="cuda"), cache, cache.extend({seq: b - a})))
+    got, whole, want = torch.cat(parts).double(), _whole(model, tokens).double(), _whole(exact, tokens).double()
+    err = lambda x: float((x - want).norm() / want.norm())
+    assert torch.isfinite(got).all()
+    assert held == E4M3 or err(got) <= 2 * err(whole)
