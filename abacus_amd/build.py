@@ -47,10 +47,10 @@ def hipcc() -> str:
     return path
 
 
-# Per-file additions.  attention.hip: MFMA results in VGPRs, not AGPRs -- its
+# Per-file additions.  The attention kernels: MFMA results in VGPRs, not AGPRs -- their
 # score and output accumulators are read and rescaled by VALU code every tile,
 # and accumulators in AGPRs cost a move per element each way.
-FILE_FLAGS = {"attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("attention.hip", "paged_attention.hip")}
 
 
 def _compile(src: pathlib.Path, obj: pathlib.Path) -> None:

@@ -14,13 +14,15 @@
 // lengths by a scan (paged_rows.h), the launch being sized for the most there can be.
 //
 // In registers (v_mfma_f32_16x16x32_bf16: lane l gives A[l % 16][8 (l / 16) .. +7] and
-// B[8 (l / 16) .. +7][l % 16], and holds D[4 (l / 16) + r][l % 16] in register r):
-// S^T = K Q^T takes the keys of a 64-key tile in four products t = 0..3 whose row i is
-// key 16 (i / 4) + 4 t + i % 4.  Lane l then holds the scores of query l % 16 against
-// keys 16 (l / 16) + 4 t + r, 16 consecutive ones, and those are, as they lie, the
-// operand P^T of O^T = V^T P^T with V^T rows of 16 consecutive keys: neither the scores
-// nor a tile of keys or values goes through LDS.
+// B[8 (l / 16) .. +7][l % 16], and holds D[4 (l / 16) + r][l % 16] in register r; the fp32
+// product takes one element of each per lane): a wave's tile is four groups of KG keys, as
+// many as 16 bytes of values hold (16 codes, 8 bf16, 4 fp32).  S^T = K Q^T takes them in KG / 4
+// products t whose row i is key KG (i / 4) + 4 t + i % 4.  Lane l then holds the scores of
+// query l % 16 against the KG keys of group l / 16, in their order, and those are, as they
+// lie, the operand P^T of O^T = V^T P^T with 16 bytes of a V^T row: neither the scores nor a
+// tile of keys or values goes through LDS, and every load of the cache is 16 bytes a lane.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_rows.h"
 
@@ -82,13 +84,20 @@ __device__ inline int seen_of(const SeqRows& r, int last_row, int G) {
   return max(0, r.len - r.n + last_row / G + 1);  // keys
 }
 
+// The value of lanes l, l ^ 16, l ^ 32 and l ^ 48, combined (no LDS round trip).
+template <class Op>
+__device__ inline float over_groups(float x, Op op) {
+  uint32_t a = f32_bits(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  a = f32_bits(op(bits_f32(r[0]), bits_f32(r[1])));
+  const auto s = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+  return op(bits_f32(s[0]), bits_f32(s[1]));
+}
 __device__ inline float group_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16, 64));
-  return fmaxf(x, __shfl_xor(x, 32, 64));
+  return over_groups(x, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ inline float group_sum(float x) {
-  x += __shfl_xor(x, 16, 64);
-  return x + __shfl_xor(x, 32, 64);
+  return over_groups(x, [](float a, float b) { return a + b; });
 }
 
 __device__ inline pa_u32x4 load16(const void* p) { return *reinterpret_cast<const pa_u32x4*>(p); }
@@ -119,34 +128,35 @@ __device__ inline pa_u32x4 codes_f32(uint32_t w, float s) {
 }
 __device__ inline float byte_scale(uint32_t w, int i) { return bits_f32(((w >> (8 * i)) & 0xffu) << 23); }
 
-// Bytes of one 16-lane row of operands.  Q: uint16_t (bf16 products) or float (fp32
-// products); Cd: whether the cache holds codes.  KD: the head dim the registers are
-// laid out for, K <= KD the one there is (Full: K == KD).
+// One wave's tile.  Q: uint16_t (bf16 products) or float (fp32 products); Cd: whether the
+// cache holds codes.  KD: the head dim the registers are laid out for, K <= KD the one there
+// is (Full: K == KD).
 template <typename Q, bool Cd, int KD, bool Full>
 struct Tile {
   static constexpr bool kBf = sizeof(Q) == 2;
   static constexpr int kHeld = Cd ? 1 : (int)sizeof(Q);  // bytes of a held value
-  static constexpr int kPer = 16 / kHeld;                // dims of a 16-byte load
-  static constexpr int NC = KD / (4 * kPer) > 0 ? KD / (4 * kPer) : 1;  // key loads of a lane and product
-  static constexpr int NS = kPer / (kBf ? 8 : 4) * NC;   // operands of those (8 bf16 or 4 fp32 dims each)
+  static constexpr int KG = 16 / kHeld;                  // dims, or keys, of a 16-byte load
+  static constexpr int KT = 4 * KG;                      // keys
+  static constexpr int NT = KG / 4;                      // products of scores
+  static constexpr int NC = KD / KT;                     // key loads of a lane and product
+  static constexpr int NS = KG / (kBf ? 8 : 4) * NC;     // operands of those (8 bf16 or 4 fp32 dims each)
   static constexpr int ND = KD / 16;                     // rows of 16 dims of V^T
-  static constexpr int NV = 16 / kPer;                   // value loads of a lane and 16 dims
-  pa_u32x4 k[4][NC], v[ND][NV];
+  pa_u32x4 k[NT][NC], v[ND];
   pa_u32x4 ks, vs;  // exponent bytes: of the lane's key group's rows, of its value keys
 
   // dims of key load c in lane group g
-  __device__ static inline int dim_of(int c, int g) { return (4 * c + g) * kPer; }
+  __device__ static inline int dim_of(int c, int g) { return (4 * c + g) * KG; }
 
   __device__ inline void load_k(const PagedArgs& p, int64_t tile, int off, int lane) {
     const int i = lane & 15, g = lane >> 4, ps = p.a.shift;
     const char* base = (const char*)p.k + (((tile << ps) + off + (i & 3)) * p.K) * kHeld;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const int d = dim_of(c, g);
         const bool in = Full || d < p.K;
-        k[t][c] = load16(base + (int64_t)(4 * t * p.K + (in ? d : 0)) * kHeld);
+        k[t][c] = load16(base + (4 * t * p.K + (in ? d : 0)) * kHeld);
         if constexpr (!Full)
           if (!in) k[t][c] = pa_u32x4{0, 0, 0, 0};
       }
@@ -154,13 +164,14 @@ struct Tile {
   }
   __device__ inline void load_v(const PagedArgs& p, int64_t tile, int off, int lane) {
     const int ps = p.a.shift;
-    const char* base = (const char*)p.v + ((tile * p.K) << ps) * kHeld;
+    const char* at = (const char*)p.v + (((tile * p.K + (lane & 15)) << ps) + off) * kHeld;
+    int64_t step = (int64_t)(16 * kHeld) << ps;
+    if constexpr (Full) asm volatile("" : "+s"(step));  // (one address a row of loads, not ND kept)
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt) {
-      const int d = dt * 16 + (lane & 15);
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-        v[dt][j] = load16(base + (((int64_t)(Full || d < p.K ? d : 0) << ps) + off + j * kPer) * kHeld);
+      if constexpr (Full) v[dt] = load16(at);
+      else v[dt] = load16(at - (dt * 16 + (lane & 15) < p.K ? 0 : (int64_t)((dt * 16 + (lane & 15)) * kHeld) << ps));
+      at += step;
     }
     if constexpr (Cd) vs = load16(p.v_scale + (tile << ps) + off);
   }
@@ -169,10 +180,10 @@ struct Tile {
 // A block: the rows of one unit and key head against one piece of its keys, the
 // tiles dealt out to its four waves.
 template <typename Q, bool Cd, int KD, bool Full, int QT>
-__global__ __launch_bounds__(256, QT == 1 && sizeof(Q) == 2 ? 2 : 1) void paged_few_kernel(PagedArgs p) {
+__global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 : 1)) void paged_few_kernel(PagedArgs p) {
   using TileT = Tile<Q, Cd, KD, Full>;
   constexpr bool kBf = TileT::kBf;
-  constexpr int R = 16 * QT, ND = TileT::ND, NS = TileT::NS;
+  constexpr int R = 16 * QT, ND = TileT::ND, NS = TileT::NS, NT = TileT::NT, KG = TileT::KG, KT = TileT::KT;
   constexpr int kPitch = KD + 4;  // floats of a row's output in LDS
   __shared__ __attribute__((aligned(16))) float merged[4][R][kPitch];
   __shared__ float stat_m[4][R], stat_l[4][R];
@@ -200,8 +211,9 @@ __global__ __launch_bounds__(256, QT == 1 && sizeof(Q) == 2 ? 2 : 1) void paged_
   const int unit = units - 1 - local / split, piece = local % split;  // the units with the most keys first
   const int row0 = unit * R, rows = min(R, r.n * G - row0);
   const int seen = seen_of(r, row0 + rows - 1, G), least = seen_of(r, row0, G);
-  const int tiles = (seen + kTile - 1) / kTile, per = (tiles + split - 1) / split;
-  const int t0 = min(piece * per, tiles), t1 = min(t0 + per, tiles);
+  const int whole = (seen + kTile - 1) / kTile, per = (whole + split - 1) / split;
+  const int t0 = min(piece * per, whole) * (kTile / KT);  // tiles of this piece
+  const int t1 = min(t0 + per * (kTile / KT), (seen + KT - 1) / KT);
 
   // Q^T operands, and how many keys the lane's rows see
   pa_u32x4 qf[QT][NS];
@@ -234,13 +246,13 @@ __global__ __launch_bounds__(256, QT == 1 && sizeof(Q) == 2 ? 2 : 1) void paged_
     for (int dt = 0; dt < ND; ++dt) acc[qt][dt] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // The pages of a tile's four groups of 16 keys: the lane's key rows are in group
+  // The pages of a tile's four groups of keys: the lane's key rows are in group
   // i / 4, its value keys in group g.  Groups past the last key seen take the first.
   struct Place { int64_t k, v; int ko, vo; bool bad; };
   const int in_mask = (1 << p.a.shift) - 1;
   auto place = [&](int tile) __attribute__((always_inline)) {
     Place w;
-    const int pk = tile * kTile + (i >> 2) * 16, pv = tile * kTile + g * 16;
+    const int pk = tile * KT + (i >> 2) * KG, pv = tile * KT + g * KG;
     const int ck = pk < seen ? pk : 0, cv = pv < seen ? pv : 0;
     bool bad_k, bad_v;
     w.k = (int64_t)page_of(p.a, seq, ck, bad_k) * p.Hk + kh;
@@ -253,20 +265,15 @@ __global__ __launch_bounds__(256, QT == 1 && sizeof(Q) == 2 ? 2 : 1) void paged_
 
   TileT x;
   Place here;
-  const int first = t0 + wave;
-  if (first < t1) {
-    here = place(first);
-    x.load_k(p, here.k, here.ko, lane);
-    x.load_v(p, here.v, here.vo, lane);
-  }
-  for (int tile = first; tile < t1; tile += 4) {
-    const int key0 = tile * kTile + g * 16;  // the lane's first key
-    const bool more = tile + 4 < t1;
-    const Place next = more ? place(tile + 4) : here;
+  // One tile: scores, running maximum and sum, P V.  Edge: some row does not see some key of
+  // it.  `between` runs once the keys are used.
+  auto step = [&](int tile, auto edge_t, auto between) __attribute__((always_inline)) {
+    constexpr bool edge = decltype(edge_t)::value;
+    const int key0 = tile * KT + g * KG;  // the lane's first key
     // scores
-    pa_f32x4 s[QT][4];
+    pa_f32x4 s[QT][NT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) s[qt][t] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
       const float sc = Cd ? byte_scale(x.ks[t], i & 3) : 1.f;
@@ -292,28 +299,27 @@ __global__ __launch_bounds__(256, QT == 1 && sizeof(Q) == 2 ? 2 : 1) void paged_
         }
       }
     }
-    if (more) x.load_k(p, next.k, next.ko, lane);
-    const bool edge = tile * kTile + kTile > least;  // some row does not see some key of the tile
+    between();
     if (__any(here.bad)) {
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[qt][t][e] = here.bad ? __builtin_nanf("") : s[qt][t][e];
     }
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      if (edge) {
+      if constexpr (edge) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (key0 + 4 * t + e >= vis[qt]) s[qt][t][e] = -__builtin_inff();
       }
       float mx = s[qt][0][0];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[qt][t][e]);
       mx = group_max(mx) * p.scale_log2;
@@ -330,7 +336,7 @@ __global__ __launch_bounds__(256, QT == 1 && sizeof(Q) == 2 ? 2 : 1) void paged_
       }
       const float m_use = m_run[qt] == -__builtin_inff() ? 0.f : m_run[qt];  // (nothing seen yet)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qt][t][e], p.scale_log2, -m_use));
@@ -341,124 +347,153 @@ __global__ __launch_bounds__(256, QT == 1 && sizeof(Q) == 2 ? 2 : 1) void paged_
     // Where a row does not look there may be anything, and 0 times an infinity or NaN is
     // NaN.  Slots past the last key seen may hold what was there before: codes and
     // exponents of those are cleared.  In a cache of the rows' own type a key that only
-    // some of the rows see may also be infinite or NaN (codes never are): such a tile
-    // goes key by key below.
-    bool poison = false;
-    if (edge) {
+    // some of the rows see may also be infinite or NaN (codes never are).
+    [[maybe_unused]] bool poison = false;
+    if constexpr (edge) {
       if constexpr (Cd) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < NT; ++t) {
           const int there = min(max(seen - key0 - 4 * t, 0), 4);
           const uint32_t mask = there == 4 ? ~0u : (1u << (8 * there)) - 1u;
           x.vs[t] &= mask;
 #pragma unroll
-          for (int dt = 0; dt < ND; ++dt) x.v[dt][0][t] &= mask;
+          for (int dt = 0; dt < ND; ++dt) x.v[dt][t] &= mask;
         }
       } else {
         constexpr uint32_t top = kBf ? 0x7f80u : 0x7f800000u;
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-          for (int j = 0; j < TileT::NV; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t w = x.v[dt][j][e];
-              poison |= (w & top) == top;
-              if constexpr (kBf) poison |= (w & (top << 16)) == (top << 16);
-            }
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t w = x.v[dt][e];
+            poison |= (w & top) == top;
+            if constexpr (kBf) poison |= (w & (top << 16)) == (top << 16);
+          }
       }
     }
-    if (!__any(poison)) {
-      if constexpr (kBf) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          pa_u32x4 pf[QT];
+    if constexpr (edge && !Cd) {
+      if (__any(poison)) {  // those values' products one by one, to the rows that see them; 0 in their place below
+        for (int key = 0; key < KT && tile * KT + key < seen; ++key) {
+          const int from = key / KG * 16;
+          const int64_t pool = __shfl(here.v, from, 64);
+          const Q* at = (const Q*)p.v + ((pool * K) << p.a.shift) + __shfl(here.vo, from, 64) + key % KG;
+          int first_d = g * 4;
+          asm volatile("" : "+v"(first_d));  // (nothing of the addresses is kept over the loop)
 #pragma unroll
           for (int qt = 0; qt < QT; ++qt) {
-            float w[8];
+            float pr = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              w[e] = s[qt][2 * h + e / 4][e % 4];
-              if constexpr (Cd) w[e] *= byte_scale(x.vs[2 * h + e / 4], e % 4);  // exact: a power of two
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (key % KG == 4 * t + e) pr = s[qt][t][e];
+            pr = __shfl(pr, from + i, 64);
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) {
+              __builtin_amdgcn_sched_barrier(0);  // (few registers: the path above wants them)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int d = dt * 16 + first_d + e;
+                const float f = to_f32(at[(int64_t)(Full || d < K ? d : 0) << p.a.shift]);
+                if (tile * KT + key < vis[qt] && !(fabsf(f) < __builtin_inff())) acc[qt][dt][e] += pr * f;
+              }
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) pf[qt][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
-          }
-#pragma unroll
-          for (int dt = 0; dt < ND; ++dt) {
-            pa_u32x4 vf;
-            if constexpr (Cd) {
-              const uint2 a = codes_bf16(x.v[dt][0][2 * h], 1.f), b = codes_bf16(x.v[dt][0][2 * h + 1], 1.f);
-              vf[0] = a.x, vf[1] = a.y, vf[2] = b.x, vf[3] = b.y;
-            } else {
-              vf = x.v[dt][h];
-            }
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) mfma16(acc[qt][dt], vf, pf[qt]);
           }
         }
-      } else {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if constexpr (Cd) {
+        for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[qt][t][e] *= byte_scale(x.vs[t], e);
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w = x.v[dt][e];
+            if constexpr (kBf) {
+              if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+              if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+            } else if ((w & 0x7f800000u) == 0x7f800000u) {
+              w = 0;
+            }
+            x.v[dt][e] = w;
           }
-#pragma unroll
-          for (int dt = 0; dt < ND; ++dt) {
-            pa_u32x4 vf;
-            if constexpr (Cd) vf = codes_f32(x.v[dt][0][t], 1.f);
-            else vf = x.v[dt][t];
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) mfma16_f32(acc[qt][dt], bits_f32(vf[e]), s[qt][t][e]);
-          }
-        }
       }
-    } else if constexpr (!Cd) {
-      // key by key: only the rows that see a key take its product
-      for (int key = 0; key < kTile; ++key) {
-        const int pos = tile * kTile + key;
-        if (pos >= seen) break;
-        const bool own = key >> 4 == g;
-        const int kt = (key >> 2) & 3, ke = key & 3;
+    }
+    if constexpr (kBf) {
+#pragma unroll
+      for (int h = 0; h < KG / 8; ++h) {
+        pa_u32x4 pf[QT];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
-          float pr = 0.f;
+          float w[8];
 #pragma unroll
-          for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (own && t == kt && e == ke) pr = s[qt][t][e];
-#pragma unroll
-          for (int dt = 0; dt < ND; ++dt) {
-            pa_f32x4 one = {0.f, 0.f, 0.f, 0.f};
-            if constexpr (kBf) {
-              pa_u32x4 vf = pa_u32x4{0, 0, 0, 0}, pf = pa_u32x4{0, 0, 0, 0};
-              uint32_t w = 0;
-#pragma unroll
-              for (int n = 0; n < 8; ++n)
-                if (((key & 15) >> 1) == n) w = x.v[dt][n / 4][n % 4];
-              vf[0] = own ? (key & 1 ? w >> 16 : w & 0xffffu) : 0u;
-              pf[0] = pack_bf16x2(pr, 0.f);
-              mfma16(one, vf, pf);
-            } else {
-              uint32_t w = 0;
-#pragma unroll
-              for (int n = 0; n < 16; ++n)
-                if ((key & 15) == n) w = x.v[dt][n / 4][n % 4];
-              mfma16_f32(one, own ? bits_f32(w) : 0.f, pr);
-            }
-            if (pos < vis[qt]) acc[qt][dt] += one;
+          for (int e = 0; e < 8; ++e) {
+            w[e] = s[qt][2 * h + e / 4][e % 4];
+            if constexpr (Cd) w[e] *= byte_scale(x.vs[2 * h + e / 4], e % 4);  // exact: a power of two
           }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pf[qt][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
+        }
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+          pa_u32x4 vf;
+          if constexpr (Cd) {
+            const uint2 a = codes_bf16(x.v[dt][2 * h], 1.f), b = codes_bf16(x.v[dt][2 * h + 1], 1.f);
+            vf[0] = a.x, vf[1] = a.y, vf[2] = b.x, vf[3] = b.y;
+          } else {
+            vf = x.v[dt];
+          }
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) mfma16(acc[qt][dt], vf, pf[qt]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (Cd) {
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[qt][t][e] *= byte_scale(x.vs[t], e);
+        }
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+          pa_u32x4 vf;
+          if constexpr (Cd) vf = codes_f32(x.v[dt][t], 1.f);
+          else vf = x.v[dt];
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mfma16_f32(acc[qt][dt], bits_f32(vf[e]), s[qt][t][e]);
         }
       }
     }
-    if (more) x.load_v(p, next.v, next.vo, lane);
-    here = next;
+  };
+
+  int tile = t0 + wave;
+  if (tile < t1) {
+    here = place(tile);
+    x.load_k(p, here.k, here.ko, lane);
+    x.load_v(p, here.v, here.vo, lane);
+    // every row sees all of these: the next tile's keys are on their way while this one's
+    // scores are weighed, its values while the next one's scores are formed
+    while (tile * KT + KT <= least) {
+      const bool more = tile + 4 < t1;
+      const Place next = more ? place(tile + 4) : here;
+      step(tile, std::false_type{}, [&]() __attribute__((always_inline)) {
+        if (more) x.load_k(p, next.k, next.ko, lane);
+      });
+      if (more) x.load_v(p, next.v, next.vo, lane);
+      here = next;
+      tile += 4;
+      if (!more) break;
+    }
+    // the others, one at a time: their masks cost registers that the loop above would lack
+    while (tile < t1) {
+      step(tile, std::true_type{}, [] {});
+      tile += 4;
+      if (tile < t1) {
+        here = place(tile);
+        x.load_k(p, here.k, here.ko, lane);
+        x.load_v(p, here.v, here.vo, lane);
+      }
+    }
   }
 
   // the waves' parts, joined in their order
@@ -505,47 +540,74 @@ __global__ __launch_bounds__(256, QT == 1 && sizeof(Q) == 2 ? 2 : 1) void paged_
   }
 }
 
-// Joins the pieces of the units that were cut, one block per unit and key head.
+// Joins the pieces of the units that were cut: blockIdx (unit and key head, four rows), a wave
+// per row.  K / 4 lanes take a piece's row, 64 / (K / 4) pieces at a time, each lane four of
+// them in flight; with one thread for all the pieces of its four dims a row of 128 pieces
+// took 100 us, now 6.
 template <typename Q, int R>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
-  const int tid = threadIdx.x, G = p.G, K = p.K;
-  const int b = blockIdx.x / p.Hk, kh = blockIdx.x % p.Hk;
+  const int lane = threadIdx.x & 63, G = p.G, K = p.K, lanes = K / 4;
+  const int b = blockIdx.x / p.Hk, kh = blockIdx.x % p.Hk, m = blockIdx.y * 4 + (threadIdx.x >> 6);
   const Cut cut = cut_of<R>(p);
   int seq, local;
   if (!find_unit(p.a.S, b, [&](int s) { return units_of(seq_rows(p.a, s).n, G, R); }, seq, local)) return;
   const SeqRows r = seq_rows(p.a, seq);
   const int split = splits_of(r, cut), units = units_of(r.n, G, R);
-  if (split == 1) return;
-  // items before this sequence's: the same scan, to its end
-  const int lane = tid & 63;
-  int before = 0;
+  const int row = local * R + m;
+  if (split == 1 || row >= r.n * G) return;
+  int before = 0;  // the items of the sequences before this one
   for (int s = lane; s < seq; s += 64) {
     const SeqRows o = seq_rows(p.a, s);
     before += units_of(o.n, G, R) * splits_of(o, cut);
   }
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) before += __shfl_xor(before, off, 64);
-  const int row0 = local * R, rows = min(R, r.n * G - row0);
   const int item = before + (units - 1 - local) * split;
   const int64_t pitch = (int64_t)p.Hk * R * (K + 2);  // between a unit's pieces
   const float* part = p.part + ((int64_t)item * p.Hk + kh) * R * (K + 2);
-  for (int e = tid; e < rows * (K / 4); e += 256) {
-    const int m = e / (K / 4), d = e % (K / 4) * 4;
-    float top = -__builtin_inff();
-    for (int i = 0; i < split; ++i) top = fmaxf(top, part[i * pitch + R * K + m]);
-    float l = 0.f;
-    pa_f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < split; ++i) {
-      const float pm = part[i * pitch + R * K + m], pl = part[i * pitch + R * K + R + m];
-      const float f = pm == -__builtin_inff() ? (pl == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(pm - top);
+  float top = -__builtin_inff();
+  for (int i = lane; i < split; i += 64) top = fmaxf(top, part[i * pitch + R * K + m]);
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  const int sub = lane / lanes, subs = 64 / lanes, d = lane % lanes * 4;
+  float l = 0.f;
+  pa_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < split; i0 += 64) {
+    float f = 0.f;
+    if (i0 + lane < split) {
+      const float pm = part[(i0 + lane) * pitch + R * K + m], pl = part[(i0 + lane) * pitch + R * K + R + m];
+      f = pm == -__builtin_inff() ? (pl == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(pm - top);
       l += f * pl;
-      o += f * *reinterpret_cast<const pa_f32x4*>(part + i * pitch + (int64_t)m * K + d);
     }
-    const int row = row0 + m, sees = r.len - r.n + row / G + 1;
+    const int n = min(64, split - i0);
+    for (int j0 = 0; j0 < n; j0 += 4 * subs) {
+      pa_f32x4 x[4];
+      float w[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int j = j0 + c * subs + sub;
+        w[c] = __shfl(f, min(j, 63), 64);
+        const bool in = j < n && sub < subs;
+        if (!in) w[c] = 0.f;
+        x[c] = *reinterpret_cast<const pa_f32x4*>(part + (i0 + (in ? j : 0)) * pitch + (int64_t)m * K + d);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (w[c] != 0.f) o += w[c] * x[c];  // (an empty piece weighs nothing)
+    }
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off, 64);
+  pa_f32x4 sum = o;
+  for (int j = 1; j < subs; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] += __shfl(o[e], (lane + j * lanes) & 63, 64);
+  if (sub == 0) {
+    const int sees = r.len - r.n + row / G + 1;
     const float inv = r.bad ? __builtin_nanf("") : 1.f / l;
     Q* to = (Q*)p.o + ((int64_t)(r.first + row / G) * p.H + kh * G + row % G) * K + d;
 #pragma unroll
-    for (int n = 0; n < 4; ++n) to[n] = from_f32<Q>(sees <= 0 && !r.bad ? 0.f : o[n] * inv);
+    for (int n = 0; n < 4; ++n) to[n] = from_f32<Q>(sees <= 0 && !r.bad ? 0.f : sum[n] * inv);
   }
 }
 
@@ -583,7 +645,7 @@ int launch(const PagedArgs& p, const Plan& n, bool codes, hipStream_t s) {
   else codes ? launch_few<Q, true, 2>(p, blocks, s) : launch_few<Q, false, 2>(p, blocks, s);
   ABACUS_CHECK_LAUNCH("paged_attention");
   if (n.cuts) {
-    const dim3 grid((unsigned)(n.units * p.Hk));
+    const dim3 grid((unsigned)(n.units * p.Hk), (unsigned)(n.R / 4));
     if (n.R == 16) hipLaunchKernelGGL((paged_join_kernel<Q, 16>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((paged_join_kernel<Q, 32>), grid, dim3(256), 0, s, p);
     ABACUS_CHECK_LAUNCH("paged_attention (join)");
