@@ -50,7 +50,7 @@ def hipcc() -> str:
 # Per-file additions.  The attention kernels: MFMA results in VGPRs, not AGPRs -- their
 # score and output accumulators are read and rescaled by VALU code every tile,
 # and accumulators in AGPRs cost a move per element each way.
-FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("attention.hip", "paged_attention.hip")}
+FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for name in ("attention.hip", "paged_attention.hip", "paged_chunk.hip")}
 
 
 def _compile(src: pathlib.Path, obj: pathlib.Path) -> None:

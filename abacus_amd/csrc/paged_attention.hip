@@ -4,14 +4,9 @@
 // up to it: o = sum_j softmax(scale q . k_j) v_j, query head h with key head h / G.
 // One pass over the keys with the running maximum and sum of the softmax in fp32.
 //
-// Work: rows r = (token, query head of the group) of one key head are packed, R to a
-// unit, so that shared key heads and drafted tokens fill a matrix instruction's
-// columns; a unit's keys are cut into `split` pieces of whole 64-key tiles where
-// there are too few units for the GPU, each piece gives its rows' maximum, sum and
-// unscaled output, and a second kernel joins them in order.  The piece length is the
-// same for the whole call: all (unit, key head, tile)s spread over kTarget pieces,
-// at least kLeast tiles each.  Which unit a block has is found from the device's
-// lengths by a scan (paged_rows.h), the launch being sized for the most there can be.
+// How the work is cut over units of rows and pieces of keys is paged_cut.h's; sequences with
+// many rows go to paged_chunk.hip's kernel, the others, and every type and head dim that
+// one does not take, to this file's.
 //
 // In registers (v_mfma_f32_16x16x32_bf16: lane l gives A[l % 16][8 (l / 16) .. +7] and
 // B[8 (l / 16) .. +7][l % 16], and holds D[4 (l / 16) + r][l % 16] in register r; the fp32
@@ -24,14 +19,13 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "paged_rows.h"
+#include "paged_cut.h"
 
 namespace abacus {
 namespace {
 
-constexpr int kTile = 64;      // keys of a tile
-constexpr int kTarget = 2048;  // pieces the work is cut into, about
-constexpr int kLeast = 8;      // tiles of a piece, at least
+constexpr int kFewPieces = 2048;   // pieces the work of a launch is cut into, about
+constexpr int kChunkPieces = 512;  // (of the chunk kernel's: two work-groups a CU)
 
 typedef __bf16 pa_bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 pa_bf16x2 __attribute__((ext_vector_type(2)));
@@ -39,50 +33,6 @@ typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
 // 16 bytes of operands.  A vector and not Vec16's four words: of words loaded together and
 // masked on a branch the compiler (ROCm 7.2) let some be overwritten before their use.
 typedef uint32_t pa_u32x4 __attribute__((ext_vector_type(4)));
-
-struct PagedArgs {
-  PagedRows a;
-  const void *q, *k, *v;
-  const uint8_t *k_scale, *v_scale;
-  void* o;
-  float* part;  // (item, key head): R x K outputs, then R maxima, R sums
-  int H, Hk, G, K;
-  float scale_log2;
-  int zero_rest;  // rows of no sequence: 0, or left as they are
-};
-
-// How the rows of a call are cut, the same on every wave and in both kernels.
-struct Cut {
-  int chunk;  // tiles of a piece, at least
-};
-
-__host__ __device__ inline int units_of(int n, int G, int R) { return (int)(((int64_t)n * G + R - 1) / R); }
-
-template <int R>
-__device__ inline Cut cut_of(const PagedArgs& p) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;  // tiles of one key head
-  for (int s = lane; s < p.a.S; s += 64) {
-    const SeqRows r = seq_rows(p.a, s);
-    total += (int64_t)units_of(r.n, p.G, R) * ((r.len + kTile - 1) / kTile);
-  }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) total += __shfl_xor(total, off, 64);
-  const int64_t want = (kTarget + p.Hk - 1) / p.Hk;
-  Cut c;
-  c.chunk = (int)max((int64_t)kLeast, (total + want - 1) / want);
-  return c;
-}
-
-__device__ inline int splits_of(const SeqRows& r, const Cut& c) {
-  const int tiles = (r.len + kTile - 1) / kTile;
-  return max(1, (tiles + c.chunk - 1) / c.chunk);
-}
-
-// Rows r0 .. r0 + rows - 1 (of n * G) of unit u: the tiles that any of them sees.
-__device__ inline int seen_of(const SeqRows& r, int last_row, int G) {
-  return max(0, r.len - r.n + last_row / G + 1);  // keys
-}
 
 // The value of lanes l, l ^ 16, l ^ 32 and l ^ 48, combined (no LDS round trip).
 template <class Op>
@@ -110,13 +60,7 @@ __device__ inline void mfma16_f32(pa_f32x4& acc, float a, float b) {
   acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0);
 }
 
-// 4 codes (a dword), times 2^(exponent of s), as bf16 or fp32
-__device__ inline uint2 codes_bf16(uint32_t w, float s) {
-  uint2 r;
-  r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
-  r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true));
-  return r;
-}
+// 4 codes (a dword), times s, as fp32
 __device__ inline pa_u32x4 codes_f32(uint32_t w, float s) {
   const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
   pa_u32x4 r;
@@ -126,7 +70,6 @@ __device__ inline pa_u32x4 codes_f32(uint32_t w, float s) {
   r[3] = f32_bits(hi[1] * s);
   return r;
 }
-__device__ inline float byte_scale(uint32_t w, int i) { return bits_f32(((w >> (8 * i)) & 0xffu) << 23); }
 
 // One wave's tile.  Q: uint16_t (bf16 products) or float (fp32 products); Cd: whether the
 // cache holds codes.  KD: the head dim the registers are laid out for, K <= KD the one there
@@ -199,21 +142,11 @@ __global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 :
       for (int d = tid; d < G * K; d += 256) row[d] = from_f32<Q>(0.f);
     }
   }
-  const Cut cut = cut_of<R>(p);
-  int seq, local;
-  if (!find_unit(p.a.S, item, [&](int s) {
-        const SeqRows r = seq_rows(p.a, s);
-        return units_of(r.n, G, R) * splits_of(r, cut);
-      }, seq, local))
-    return;
-  const SeqRows r = seq_rows(p.a, seq);
-  const int split = splits_of(r, cut), units = units_of(r.n, G, R);
-  const int unit = units - 1 - local / split, piece = local % split;  // the units with the most keys first
-  const int row0 = unit * R, rows = min(R, r.n * G - row0);
-  const int seen = seen_of(r, row0 + rows - 1, G), least = seen_of(r, row0, G);
-  const int whole = (seen + kTile - 1) / kTile, per = (whole + split - 1) / split;
-  const int t0 = min(piece * per, whole) * (kTile / KT);  // tiles of this piece
-  const int t1 = min(t0 + per * (kTile / KT), (seen + KT - 1) / KT);
+  Item w;
+  if (!find_item<R>(p, item, w)) return;
+  const SeqRows r = w.r;
+  const int seq = w.seq, row0 = w.row0, rows = w.rows, seen = w.seen, least = w.least;
+  const int t0 = w.t0 * (kTile / KT), t1 = min(w.t1 * (kTile / KT), (seen + KT - 1) / KT);
 
   // Q^T operands, and how many keys the lane's rows see
   pa_u32x4 qf[QT][NS];
@@ -514,28 +447,24 @@ __global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 :
     const int m = e / (K / 4), d = e % (K / 4) * 4;
     float top = stat_m[0][m];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, stat_m[w][m]);
+    for (int v = 1; v < 4; ++v) top = fmaxf(top, stat_m[v][m]);
     float l = 0.f;
     pa_f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = stat_m[w][m] == -__builtin_inff() ? (stat_l[w][m] == 0.f ? 0.f : 1.f)
-                                                        : __builtin_amdgcn_exp2f(stat_m[w][m] - top);
-      l += f * stat_l[w][m];
-      o += f * *reinterpret_cast<const pa_f32x4*>(&merged[w][m][d]);
+    for (int v = 0; v < 4; ++v) {
+      const float f = stat_m[v][m] == -__builtin_inff() ? (stat_l[v][m] == 0.f ? 0.f : 1.f)
+                                                        : __builtin_amdgcn_exp2f(stat_m[v][m] - top);
+      l += f * stat_l[v][m];
+      o += f * *reinterpret_cast<const pa_f32x4*>(&merged[v][m][d]);
     }
-    if (split > 1) {
+    if (w.split > 1) {
       *reinterpret_cast<pa_f32x4*>(part + (int64_t)m * K + d) = o;
       if (d == 0) {
         part[R * K + m] = top;
         part[R * K + R + m] = l;
       }
     } else {
-      const int row = row0 + m, sees = r.len - r.n + row / G + 1;
-      const float inv = r.bad ? __builtin_nanf("") : 1.f / l;
-      Q* to = (Q*)p.o + ((int64_t)(r.first + row / G) * p.H + kh * G + row % G) * K + d;
-#pragma unroll
-      for (int n = 0; n < 4; ++n) to[n] = from_f32<Q>(sees <= 0 && !r.bad ? 0.f : o[n] * inv);
+      store_row4<Q>(p, r, kh, row0 + m, d, o, l);
     }
   }
 }
@@ -548,17 +477,17 @@ template <typename Q, int R>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
   const int lane = threadIdx.x & 63, G = p.G, K = p.K, lanes = K / 4;
   const int b = blockIdx.x / p.Hk, kh = blockIdx.x % p.Hk, m = blockIdx.y * 4 + (threadIdx.x >> 6);
-  const Cut cut = cut_of<R>(p);
+  const int chunk = piece_tiles<R>(p);
   int seq, local;
-  if (!find_unit(p.a.S, b, [&](int s) { return units_of(seq_rows(p.a, s).n, G, R); }, seq, local)) return;
+  if (!find_unit(p.a.S, b, [&](int s) { return units_of<R>(p, seq_rows(p.a, s)); }, seq, local)) return;
   const SeqRows r = seq_rows(p.a, seq);
-  const int split = splits_of(r, cut), units = units_of(r.n, G, R);
+  const int split = pieces_of(r, chunk), units = units_of<R>(p, r);
   const int row = local * R + m;
   if (split == 1 || row >= r.n * G) return;
   int before = 0;  // the items of the sequences before this one
   for (int s = lane; s < seq; s += 64) {
     const SeqRows o = seq_rows(p.a, s);
-    before += units_of(o.n, G, R) * splits_of(o, cut);
+    before += units_of<R>(p, o) * pieces_of(o, chunk);
   }
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) before += __shfl_xor(before, off, 64);
@@ -602,31 +531,50 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
   for (int j = 1; j < subs; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) sum[e] += __shfl(o[e], (lane + j * lanes) & 63, 64);
-  if (sub == 0) {
-    const int sees = r.len - r.n + row / G + 1;
-    const float inv = r.bad ? __builtin_nanf("") : 1.f / l;
-    Q* to = (Q*)p.o + ((int64_t)(r.first + row / G) * p.H + kh * G + row % G) * K + d;
-#pragma unroll
-    for (int n = 0; n < 4; ++n) to[n] = from_f32<Q>(sees <= 0 && !r.bad ? 0.f : sum[n] * inv);
-  }
+  if (sub == 0) store_row4<Q>(p, r, kh, row, d, sum, l);
 }
 
-// What a launch is sized by.
-struct Plan {
-  int R;           // rows of a unit
-  int64_t units;   // at most
-  int64_t items;   // at most
-  bool cuts;       // whether any unit can be cut
+// A launch, as it is sized on the host.
+struct Part {
+  int R;          // rows of a unit, 0: no launch
+  int over, upto; // the sequences it takes, by their rows of a key head
+  int target;     // pieces
+  int64_t units, items;  // at most
+  bool cuts;      // whether a unit can be cut
+  int64_t floats(int64_t Hk, int64_t K) const { return cuts ? items * Hk * R * (K + 2) : 0; }
 };
 
-Plan plan_of(int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G, int64_t Hk, int64_t max_new) {
-  Plan n;
-  const int64_t rows = std::min(T, max_new) * G;
-  n.R = rows <= 16 ? 16 : 32;
-  n.units = std::min(T * G, T * G / n.R + std::min(S, T));
+// A launch of the sequences with at most 16 or 32 rows of a key head, and, where there may be
+// others that it serves better, one of paged_chunk.hip's kernel.
+struct Plan {
+  Part few, many;
+};
+
+Part part_of(int R, int64_t over, int64_t upto, int target, int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G,
+             int64_t Hk) {
+  Part n;
+  n.R = R, n.over = (int)over, n.upto = (int)upto, n.target = target;
+  n.units = std::min(T * G, T * G / R + std::min(S, T));
   const int64_t tiles = (P * page_size + kTile - 1) / kTile, most = (tiles + kLeast - 1) / kLeast;
   n.cuts = most > 1;
-  n.items = std::min(n.units * most, n.units + (kTarget + Hk - 1) / Hk);
+  n.items = std::min(n.units * most, n.units + (target + Hk - 1) / Hk);
+  return n;
+}
+
+Plan plan_of(int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G, int64_t Hk, int64_t K, int dtype,
+             int64_t max_new) {
+  constexpr int64_t kAll = 0x7fffffff;
+  const int64_t rows = std::min(T, max_new) * G;
+  const bool chunks = dtype == kBF16 && (K == 64 || K == 128);
+  Plan n;
+  n.many.R = 0, n.many.cuts = false;
+  if (rows <= 32 || !chunks) {
+    n.few = part_of(rows <= 16 ? 16 : 32, 0, kAll, kFewPieces, T, S, P, page_size, G, Hk);
+  } else {
+    const int few = G <= 16 ? 16 : 32;
+    n.few = part_of(few, 0, few, kFewPieces, T, S, P, page_size, G, Hk);
+    n.many = part_of(kChunkRows, few, kAll, kChunkPieces, T, S, P, page_size, G, Hk);
+  }
   return n;
 }
 
@@ -639,15 +587,29 @@ void launch_few(const PagedArgs& p, unsigned blocks, hipStream_t s) {
 }
 
 template <typename Q>
-int launch(const PagedArgs& p, const Plan& n, bool codes, hipStream_t s) {
-  const unsigned blocks = (unsigned)(n.items * p.Hk);
-  if (n.R == 16) codes ? launch_few<Q, true, 1>(p, blocks, s) : launch_few<Q, false, 1>(p, blocks, s);
+int launch(PagedArgs p, const Plan& n, bool codes, float* ws, int64_t rows, hipStream_t s) {
+  auto set = [&](const Part& part, float* at) {
+    p.over = part.over, p.upto = part.upto, p.target = part.target, p.part = at;
+    return (unsigned)(part.items * p.Hk);
+  };
+  auto join_grid = [&](const Part& part) {
+    return dim3((unsigned)(part.units * p.Hk), (unsigned)((std::min<int64_t>(part.R, rows) + 3) / 4));
+  };
+  const unsigned blocks = set(n.few, ws);
+  if (n.few.R == 16) codes ? launch_few<Q, true, 1>(p, blocks, s) : launch_few<Q, false, 1>(p, blocks, s);
   else codes ? launch_few<Q, true, 2>(p, blocks, s) : launch_few<Q, false, 2>(p, blocks, s);
   ABACUS_CHECK_LAUNCH("paged_attention");
-  if (n.cuts) {
-    const dim3 grid((unsigned)(n.units * p.Hk), (unsigned)(n.R / 4));
-    if (n.R == 16) hipLaunchKernelGGL((paged_join_kernel<Q, 16>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((paged_join_kernel<Q, 32>), grid, dim3(256), 0, s, p);
+  if (n.few.cuts) {
+    if (n.few.R == 16) hipLaunchKernelGGL((paged_join_kernel<Q, 16>), join_grid(n.few), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((paged_join_kernel<Q, 32>), join_grid(n.few), dim3(256), 0, s, p);
+    ABACUS_CHECK_LAUNCH("paged_attention (join)");
+  }
+  if (n.many.R == 0) return 0;
+  p.zero_rest = 0;
+  const unsigned chunks = set(n.many, ws + n.few.floats(p.Hk, p.K));
+  if (launch_chunk(p, chunks, codes, s)) return 2;
+  if (n.many.cuts) {
+    hipLaunchKernelGGL((paged_join_kernel<Q, kChunkRows>), join_grid(n.many), dim3(256), 0, s, p);
     ABACUS_CHECK_LAUNCH("paged_attention (join)");
   }
   return 0;
@@ -658,11 +620,11 @@ int launch(const PagedArgs& p, const Plan& n, bool codes, hipStream_t s) {
 
 using namespace abacus;
 
-extern "C" int64_t abacus_paged_attention_ws_bytes(int64_t T, int64_t H, int64_t Hk, int64_t K, int64_t S, int64_t P,
-                                                   int64_t page_size, int64_t max_new) {
+extern "C" int64_t abacus_paged_attention_ws_bytes(int64_t T, int64_t H, int64_t Hk, int64_t K, int dtype, int64_t S,
+                                                   int64_t P, int64_t page_size, int64_t max_new) {
   if (T < 1 || Hk < 1 || H % Hk != 0) return 0;
-  const Plan n = plan_of(T, S, P, page_size, H / Hk, Hk, max_new);
-  return n.cuts ? n.items * Hk * n.R * (K + 2) * 4 : 0;
+  const Plan n = plan_of(T, S, P, page_size, H / Hk, Hk, K, dtype, max_new);
+  return (n.few.floats(Hk, K) + n.many.floats(Hk, K)) * 4;
 }
 
 extern "C" int abacus_paged_attention(const void* q_THK, int64_t T, int64_t H, int64_t Hk, int64_t K, int dtype,
@@ -687,21 +649,22 @@ extern "C" int abacus_paged_attention(const void* q_THK, int64_t T, int64_t H, i
   ABACUS_CHECK_ARG(((uintptr_t)q_THK | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_scale |
                     (uintptr_t)v_scale | (uintptr_t)o_THK | (uintptr_t)ws) % 16 == 0,
                    "paged_attention: tensors must be 16-byte aligned");
-  const Plan n = plan_of(T, S, P, page_size, H / Hk, Hk, max_new);
-  const int64_t need = n.cuts ? n.items * Hk * n.R * (K + 2) * 4 : 0;
+  const Plan n = plan_of(T, S, P, page_size, H / Hk, Hk, K, dtype, max_new);
+  const int64_t need = (n.few.floats(Hk, K) + n.many.floats(Hk, K)) * 4;
   ABACUS_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "paged_attention: workspace of %lld bytes, need %lld",
                    (long long)ws_bytes, (long long)need);
-  ABACUS_CHECK_ARG(n.items * Hk < (1ll << 31), "paged_attention: %lld rows of %lld heads are too many", (long long)T,
+  ABACUS_CHECK_ARG(n.few.items * Hk < (1ll << 31), "paged_attention: %lld rows of %lld heads are too many", (long long)T,
                    (long long)H);
   PagedArgs p;
   p.a = PagedRows{page_table_SP, query_start, lengths, (int)S, (int)P, (int)T, __builtin_ctzll(page_size), (int)n_pages};
   p.q = q_THK, p.k = k_pages, p.v = v_pages;
   p.k_scale = (const uint8_t*)k_scale, p.v_scale = (const uint8_t*)v_scale;
-  p.o = o_THK, p.part = (float*)ws;
+  p.o = o_THK;
   p.H = (int)H, p.Hk = (int)Hk, p.G = (int)(H / Hk), p.K = (int)K;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.zero_rest = zero_rest;
   hipStream_t s = (hipStream_t)stream;
   const bool codes = held == ABACUS_E4M3;
-  return dtype == kBF16 ? launch<uint16_t>(p, n, codes, s) : launch<float>(p, n, codes, s);
+  const int64_t rows = std::min(T, max_new) * (H / Hk);
+  return dtype == kBF16 ? launch<uint16_t>(p, n, codes, (float*)ws, rows, s) : launch<float>(p, n, codes, (float*)ws, rows, s);
 }

@@ -231,7 +231,8 @@ class KVPages:
         S, P = args[3:5]
         most = max(1, T) if rows.max_new is None else rows.max_new
         with _Guard(q.device):
-            nbytes = _lib.query("abacus_paged_attention_ws_bytes", T, H, self.n_heads, K, S, P, self.page_size, most)
+            nbytes = _lib.query("abacus_paged_attention_ws_bytes", T, H, self.n_heads, K, _lib.dtype_code(q.dtype), S, P,
+                                self.page_size, most)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
             _lib.call("abacus_paged_attention", q.data_ptr(), T, H, self.n_heads, K, _lib.dtype_code(q.dtype), *args,
                       scale, most, int(zero_rest), out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
