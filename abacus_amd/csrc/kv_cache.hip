@@ -105,12 +105,11 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const T* __restrict__ k, 
   __shared__ __attribute__((aligned(16))) C turned[kGroup][kMaxK + 16 / sizeof(C)];
   const int tid = threadIdx.x, H = p.H, K = p.K;
   int seq, local;
-  const bool any = find_unit(a.S, blockIdx.x, [&](int s) {
-    const SeqRows r = seq_rows(a, s);
-    return r.n > 0 && r.len > 0 ? (r.len - 1) / kGroup - max(r.len - r.n, 0) / kGroup + 1 : 0;
-  }, seq, local);
-  if (!any) return;
-  const SeqRows r = seq_rows(a, seq);
+  SeqRows r;
+  if (!SeqScan(a).find(blockIdx.x, [](const SeqRows& r) {
+        return r.n > 0 && r.len > 0 ? (r.len - 1) / kGroup - max(r.len - r.n, 0) / kGroup + 1 : 0;
+      }, seq, local, r))
+    return;
   const int g0 = (max(r.len - r.n, 0) / kGroup + local) * kGroup;  // the group's first position
   const int p0 = max(g0, r.len - r.n), p1 = min(g0 + kGroup, r.len), rows = p1 - p0;
   const int pair0 = blockIdx.y * 16;

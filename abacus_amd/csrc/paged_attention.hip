@@ -134,16 +134,21 @@ __global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 :
   const int i = lane & 15, g = lane >> 4;
   const int item = blockIdx.x / p.Hk, kh = blockIdx.x % p.Hk, G = p.G, K = p.K;
 
-  if (p.zero_rest) {
-    const int first = min(max(p.a.query_start[0], 0), p.a.T), end = min(max(p.a.query_start[p.a.S], first), p.a.T);
+  // rows of no sequence, read now and cleared last
+  const int rest0 = p.zero_rest ? p.a.query_start[0] : 0, rest1 = p.zero_rest ? p.a.query_start[p.a.S] : 0x7fffffff;
+  auto clear_rest = [&] {
+    const int first = min(max(rest0, 0), p.a.T), end = min(max(rest1, first), p.a.T);
     const int rest = p.a.T - (end - first), items = gridDim.x / p.Hk;
     for (int r = item; r < rest; r += items) {
       Q* row = (Q*)p.o + ((int64_t)(r < first ? r : end + r - first) * p.H + kh * G) * K;
       for (int d = tid; d < G * K; d += 256) row[d] = from_f32<Q>(0.f);
     }
-  }
+  };
   Item w;
-  if (!find_item<R>(p, item, w)) return;
+  if (!find_item<R>(p, item, w)) {
+    clear_rest();
+    return;
+  }
   const SeqRows r = w.r;
   const int seq = w.seq, row0 = w.row0, rows = w.rows, seen = w.seen, least = w.least;
   const int t0 = w.t0 * (kTile / KT), t1 = min(w.t1 * (kTile / KT), (seen + KT - 1) / KT);
@@ -467,71 +472,69 @@ __global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 :
       store_row4<Q>(p, r, kh, row0 + m, d, o, l);
     }
   }
+  clear_rest();
 }
 
-// Joins the pieces of the units that were cut: blockIdx (unit and key head, four rows), a wave
-// per row.  K / 4 lanes take a piece's row, 64 / (K / 4) pieces at a time, each lane four of
+// Joins the pieces of the units that were cut: blockIdx (unit and key head, every how many
+// rows), a wave per row.  K / 4 lanes take a piece's row, 64 / (K / 4) pieces at a time, each lane four of
 // them in flight; with one thread for all the pieces of its four dims a row of 128 pieces
 // took 100 us, now 6.
 template <typename Q, int R>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
-  const int lane = threadIdx.x & 63, G = p.G, K = p.K, lanes = K / 4;
-  const int b = blockIdx.x / p.Hk, kh = blockIdx.x % p.Hk, m = blockIdx.y * 4 + (threadIdx.x >> 6);
-  const int chunk = piece_tiles<R>(p);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = p.K, lanes = K / 4;
+  const int b = blockIdx.x / p.Hk, kh = blockIdx.x % p.Hk;
+  const SeqScan scan(p.a);
+  const int chunk = piece_tiles<R>(p, scan);
   int seq, local;
-  if (!find_unit(p.a.S, b, [&](int s) { return units_of<R>(p, seq_rows(p.a, s)); }, seq, local)) return;
-  const SeqRows r = seq_rows(p.a, seq);
+  SeqRows r;
+  if (!scan.find(b, [&](const SeqRows& r) { return units_of<R>(p, r); }, seq, local, r)) return;
   const int split = pieces_of(r, chunk), units = units_of<R>(p, r);
-  const int row = local * R + m;
-  if (split == 1 || row >= r.n * G) return;
-  int before = 0;  // the items of the sequences before this one
-  for (int s = lane; s < seq; s += 64) {
-    const SeqRows o = seq_rows(p.a, s);
-    before += units_of<R>(p, o) * pieces_of(o, chunk);
-  }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) before += __shfl_xor(before, off, 64);
+  if (split == 1) return;
+  const int before = scan.before(seq, [&](const SeqRows& r) { return units_of<R>(p, r) * pieces_of(r, chunk); });
   const int item = before + (units - 1 - local) * split;
   const int64_t pitch = (int64_t)p.Hk * R * (K + 2);  // between a unit's pieces
   const float* part = p.part + ((int64_t)item * p.Hk + kh) * R * (K + 2);
-  float top = -__builtin_inff();
-  for (int i = lane; i < split; i += 64) top = fmaxf(top, part[i * pitch + R * K + m]);
+  const int rows = min(R, r.n * p.G - local * R);
+  for (int m = blockIdx.y * 4 + wave; m < rows; m += gridDim.y * 4) {
+    float top = -__builtin_inff();
+    for (int i = lane; i < split; i += 64) top = fmaxf(top, part[i * pitch + R * K + m]);
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  const int sub = lane / lanes, subs = 64 / lanes, d = lane % lanes * 4;
-  float l = 0.f;
-  pa_f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = 0; i0 < split; i0 += 64) {
-    float f = 0.f;
-    if (i0 + lane < split) {
-      const float pm = part[(i0 + lane) * pitch + R * K + m], pl = part[(i0 + lane) * pitch + R * K + R + m];
-      f = pm == -__builtin_inff() ? (pl == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(pm - top);
-      l += f * pl;
-    }
-    const int n = min(64, split - i0);
-    for (int j0 = 0; j0 < n; j0 += 4 * subs) {
-      pa_f32x4 x[4];
-      float w[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int j = j0 + c * subs + sub;
-        w[c] = __shfl(f, min(j, 63), 64);
-        const bool in = j < n && sub < subs;
-        if (!in) w[c] = 0.f;
-        x[c] = *reinterpret_cast<const pa_f32x4*>(part + (i0 + (in ? j : 0)) * pitch + (int64_t)m * K + d);
+    for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    const int sub = lane / lanes, subs = 64 / lanes, d = lane % lanes * 4;
+    float l = 0.f;
+    pa_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < split; i0 += 64) {
+      float f = 0.f;
+      if (i0 + lane < split) {
+        const float pm = part[(i0 + lane) * pitch + R * K + m], pl = part[(i0 + lane) * pitch + R * K + R + m];
+        f = pm == -__builtin_inff() ? (pl == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(pm - top);
+        l += f * pl;
       }
+      const int n = min(64, split - i0);
+      for (int j0 = 0; j0 < n; j0 += 4 * subs) {
+        pa_f32x4 x[4];
+        float w[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (w[c] != 0.f) o += w[c] * x[c];  // (an empty piece weighs nothing)
+        for (int c = 0; c < 4; ++c) {
+          const int j = j0 + c * subs + sub;
+          w[c] = __shfl(f, min(j, 63), 64);
+          const bool in = j < n && sub < subs;
+          if (!in) w[c] = 0.f;
+          x[c] = *reinterpret_cast<const pa_f32x4*>(part + (i0 + (in ? j : 0)) * pitch + (int64_t)m * K + d);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (w[c] != 0.f) o += w[c] * x[c];  // (an empty piece weighs nothing)
+      }
     }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off, 64);
+    pa_f32x4 sum = o;
+    for (int j = 1; j < subs; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += __shfl(o[e], (lane + j * lanes) & 63, 64);
+    if (sub == 0) store_row4<Q>(p, r, kh, local * R + m, d, sum, l);
   }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) l += __shfl_xor(l, off, 64);
-  pa_f32x4 sum = o;
-  for (int j = 1; j < subs; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sum[e] += __shfl(o[e], (lane + j * lanes) & 63, 64);
-  if (sub == 0) store_row4<Q>(p, r, kh, row, d, sum, l);
 }
 
 // A launch, as it is sized on the host.
@@ -593,7 +596,7 @@ int launch(PagedArgs p, const Plan& n, bool codes, float* ws, int64_t rows, hipS
     return (unsigned)(part.items * p.Hk);
   };
   auto join_grid = [&](const Part& part) {
-    return dim3((unsigned)(part.units * p.Hk), (unsigned)((std::min<int64_t>(part.R, rows) + 3) / 4));
+    return dim3((unsigned)(part.units * p.Hk), (unsigned)((std::min<int64_t>(part.R, std::min<int64_t>(rows, 16)) + 3) / 4));
   };
   const unsigned blocks = set(n.few, ws);
   if (n.few.R == 16) codes ? launch_few<Q, true, 1>(p, blocks, s) : launch_few<Q, false, 1>(p, blocks, s);

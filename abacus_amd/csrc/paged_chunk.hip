@@ -29,9 +29,9 @@ struct ChunkLds {
   uint8_t vs[kStages][kTile];
 };
 
-// The four 16-key groups of a tile: their pages and places, the same for the whole block.
+// The pages of a tile's four 16-key groups, the same for the whole block.
 struct Groups {
-  int page[4], off[4];
+  int page[4];
   int bad;  // bit per group that lies in no page
 };
 
@@ -40,10 +40,9 @@ __device__ inline Groups groups_of(const PagedArgs& p, int seq, int key0, int se
   g.bad = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int pos = key0 + 16 * j < seen ? key0 + 16 * j : 0;  // (past the last key seen: anything that exists)
+    const int pos = key0 + 16 * j < seen ? key0 + 16 * j : 0;  // (past the last key seen: any page that exists)
     bool bad;
     g.page[j] = __builtin_amdgcn_readfirstlane(page_of(p.a, seq, pos, bad));
-    g.off[j] = __builtin_amdgcn_readfirstlane(pos & ((1 << p.a.shift) - 1));
     if (__builtin_amdgcn_readfirstlane(bad)) g.bad |= 1 << j;
   }
   return g;
@@ -57,18 +56,19 @@ __device__ inline T pick(const T (&x)[4], int j) {
 
 // bf16 pages: 16 bytes a lane and instruction, straight into the swizzled tile.
 template <int HD>
-__device__ inline void dma_tile(const PagedArgs& p, int kh, const Groups& g, char* kt, char* vt) {
+__device__ inline void dma_tile(const PagedArgs& p, int kh, const Groups& g, int key0, char* kt, char* vt) {
+  const int in_page = (1 << p.a.shift) - 1;  // group j's slots begin at (key0 + 16 j) & in_page
   constexpr int CH = HD / 8;  // chunks of a key row
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ps = p.a.shift;
 #pragma unroll
   for (int i = 0; i < HD / 32; ++i) {
     const int at = i * 256 + tid, row = at / CH, j = HD == 128 ? i : 2 * i + (wave >> 1);  // the row's group
-    const int64_t slot = (((int64_t)pick(g.page, j) * p.Hk + kh) << ps) + pick(g.off, j) + (row & 15);
+    const int64_t slot = (((int64_t)pick(g.page, j) * p.Hk + kh) << ps) + ((key0 + 16 * j) & in_page) + (row & 15);
     dma16((const uint16_t*)p.k + slot * HD + ((at % CH) ^ tile_swz<HD>(row)) * 8, kt + (i * 4 + wave) * 1024);
   }
   const int d0 = tid / 8, c = (tid % 8) ^ tile_swz<64>(d0);  // V^T rows d0 + 32 i: the swizzle is the same for all
   const int64_t page = (int64_t)pick(g.page, c >> 1) * p.Hk + kh;
-  const uint16_t* from = (const uint16_t*)p.v + ((page * HD + d0) << ps) + pick(g.off, c >> 1) + (c & 1) * 8;
+  const uint16_t* from = (const uint16_t*)p.v + ((page * HD + d0) << ps) + ((key0 + 8 * c) & in_page);
 #pragma unroll
   for (int i = 0; i < HD / 32; ++i) dma16(from + ((int64_t)(32 * i) << ps), vt + (i * 4 + wave) * 1024);
 }
@@ -81,18 +81,18 @@ struct Codes {
   U4 k[N], v[N];
   int ks[N];
   U4 vs;
-  __device__ inline void load(const PagedArgs& p, int kh, const Groups& g) {
-    const int tid = threadIdx.x, ps = p.a.shift;
+  __device__ inline void load(const PagedArgs& p, int kh, const Groups& g, int key0) {
+    const int tid = threadIdx.x, ps = p.a.shift, in_page = (1 << ps) - 1;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int row = (i * 256 + tid) / (HD / 16), c = tid % (HD / 16);
-      const int64_t slot = (((int64_t)pick(g.page, row >> 4) * p.Hk + kh) << ps) + pick(g.off, row >> 4) + (row & 15);
+      const int64_t slot = (((int64_t)pick(g.page, row >> 4) * p.Hk + kh) << ps) + ((key0 + row) & in_page);
       k[i] = *reinterpret_cast<const U4*>((const uint8_t*)p.k + slot * HD + c * 16);
       ks[i] = p.k_scale[slot];
       const int d = (i * 256 + tid) / 4, j = tid & 3;
       const int64_t page = (int64_t)pick(g.page, j) * p.Hk + kh;
-      v[i] = *reinterpret_cast<const U4*>((const uint8_t*)p.v + ((page * HD + d) << ps) + pick(g.off, j));
-      if (i == 0) vs = *reinterpret_cast<const U4*>(p.v_scale + (page << ps) + pick(g.off, j));
+      v[i] = *reinterpret_cast<const U4*>((const uint8_t*)p.v + ((page * HD + d) << ps) + ((key0 + 16 * j) & in_page));
+      if (i == 0) vs = *reinterpret_cast<const U4*>(p.v_scale + (page << ps) + ((key0 + 16 * j) & in_page));
     }
   }
   // `left`: keys of the tile that exist (past them there may be anything in V: 0)
@@ -143,12 +143,11 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedArgs p) {
   Item w;
   if (!find_item<R>(p, item, w)) return;
 
-  // this wave's rows, and the keys that the first and the last of them see
+  // this wave's rows, and the keys that the last of them sees
   const int m0 = wave * 32, m = m0 + (lane & 31);
   const int row = w.row0 + min(m, w.rows - 1);
   const int token = row / G, head = kh * G + row % G;
   const int vis = m < w.rows ? max(0, w.r.len - w.r.n + token + 1) : 0;
-  const int least = m0 < w.rows ? seen_of(w.r, w.row0 + m0, G) : 0;
   const int seen = m0 < w.rows ? seen_of(w.r, w.row0 + min(m0 + 31, w.rows - 1), G) : 0;
   const uint16_t* at = (const uint16_t*)p.q + ((int64_t)(w.r.first + token) * p.H + head) * HD;
   Vec16 qf[HD / 16];
@@ -222,6 +221,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedArgs p) {
       }
       poison = __any(poison);
       if (poison) {
+#pragma unroll 1
         for (int key = 0; key < kTile; ++key) {
           float pr = 0.f;
 #pragma unroll
@@ -230,11 +230,14 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedArgs p) {
             for (int r = 0; r < 16; ++r)
               if (32 * n + 16 * (r >> 3) + (r & 7) == (key & ~8)) pr = s[n][r];
           pr = __shfl(pr, (lane & 31) + 4 * (key & 8), 64);
+          int first_d = 4 * h;
+          asm volatile("" : "+v"(first_d));  // (nothing of the addresses is kept over the loop)
 #pragma unroll
           for (int t = 0; t < HD / 32; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const int d = 32 * t + 8 * (r >> 2) + 4 * h + (r & 3);
+              __builtin_amdgcn_sched_barrier(0);
+              const int d = 32 * t + 8 * (r >> 2) + first_d + (r & 3);
               const float f = to_f32(*reinterpret_cast<const uint16_t*>(vt + tile_off<64>(d, key >> 3) + 2 * (key & 7)));
               if (key0 + key < vis && !(fabsf(f) < __builtin_inff())) acc[t][r] += pr * f;
             }
@@ -274,34 +277,38 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedArgs p) {
   // The ring: tile t is in stage t % 2; once it has landed everywhere (this thread's wait,
   // then the barrier, after which no wave still reads the other stage) the next is sent.
   if (w.t0 < w.t1) {
-    Groups here = groups_of(p, w.seq, w.t0 * kTile, w.seen), next = here;
+    Groups next = groups_of(p, w.seq, w.t0 * kTile, w.seen);
+    int bad = next.bad;
     [[maybe_unused]] Codes<HD> codes;
     if constexpr (Cd) {
-      codes.load(p, kh, here);
+      codes.load(p, kh, next, w.t0 * kTile);
       codes.store(lds.k[0], lds.v[0], lds.vs[0], w.seen - w.t0 * kTile);
     } else {
-      dma_tile<HD>(p, kh, here, lds.k[0], lds.v[0]);
+      dma_tile<HD>(p, kh, next, w.t0 * kTile, lds.k[0], lds.v[0]);
     }
     if (w.t0 + 1 < w.t1) next = groups_of(p, w.seq, (w.t0 + 1) * kTile, w.seen);
-    for (int t = w.t0; t < w.t1; ++t) {
+    auto turn = [&](int t, auto edge_t) __attribute__((always_inline)) {
       const int st = (t - w.t0) % kStages, key0 = t * kTile;
       const bool more = t + 1 < w.t1;
       if constexpr (!Cd) wait_vmcnt<0>();
       __syncthreads();
       if (more) {
-        if constexpr (Cd) codes.load(p, kh, next);
-        else dma_tile<HD>(p, kh, next, lds.k[st ^ 1], lds.v[st ^ 1]);
+        if constexpr (Cd) codes.load(p, kh, next, key0 + kTile);
+        else dma_tile<HD>(p, kh, next, key0 + kTile, lds.k[st ^ 1], lds.v[st ^ 1]);
       }
-      Groups after = next;
-      if (t + 2 < w.t1) after = groups_of(p, w.seq, key0 + 2 * kTile, w.seen);
-      if (key0 + kTile <= least) step(lds.k[st], lds.v[st], lds.vs[st], key0, here.bad, std::false_type{});
-      else if (key0 < seen) step(lds.k[st], lds.v[st], lds.vs[st], key0, here.bad, std::true_type{});
+      const int next_bad = next.bad;
+      if (t + 2 < w.t1) next = groups_of(p, w.seq, key0 + 2 * kTile, w.seen);
+      if (!decltype(edge_t)::value || key0 < seen) step(lds.k[st], lds.v[st], lds.vs[st], key0, bad, edge_t);
       if constexpr (Cd) {
         if (more) codes.store(lds.k[st ^ 1], lds.v[st ^ 1], lds.vs[st ^ 1], w.seen - key0 - kTile);
       }
-      here = next;
-      next = after;
-    }
+      bad = next_bad;
+    };
+    // the tiles that every row sees whole, then the others (in a loop of their own: their
+    // masks cost registers that the first would lack)
+    int t = w.t0;
+    for (; t < min(w.t1, w.least / kTile); ++t) turn(t, std::false_type{});
+    for (; t < w.t1; ++t) turn(t, std::true_type{});
   }
   if (m >= w.rows) return;
   const float l = pair_sum(l_run);

@@ -37,19 +37,15 @@ __device__ inline int units_of(const PagedArgs& p, const SeqRows& r) {
   return rows > p.over && rows <= p.upto ? (rows + R - 1) / R : 0;
 }
 
-// Tiles of a piece, the same on every wave and in both kernels.
+// Tiles of a piece, the same on every wave and in both kernels.  (A sum in floats, taken
+// larger by more than they can be off: the launch has room for no more pieces.)
 template <int R>
-__device__ inline int piece_tiles(const PagedArgs& p) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;  // tiles of one key head
-  for (int s = lane; s < p.a.S; s += 64) {
-    const SeqRows r = seq_rows(p.a, s);
-    total += (int64_t)units_of<R>(p, r) * ((r.len + kTile - 1) / kTile);
-  }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) total += __shfl_xor(total, off, 64);
-  const int64_t want = (p.target + p.Hk - 1) / p.Hk;
-  return (int)max((int64_t)kLeast, (total + want - 1) / want);
+__device__ inline int piece_tiles(const PagedArgs& p, const SeqScan& scan) {
+  const float total = scan.sum([&](const SeqRows& r) {  // tiles of one key head
+    return (float)units_of<R>(p, r) * (float)((r.len + kTile - 1) / kTile);
+  });
+  const int want = (p.target + p.Hk - 1) / p.Hk;
+  return max(kLeast, (int)fminf(ceilf(total * 1.001f / (float)want), 1e9f));
 }
 
 // Pieces of each of a sequence's units.
@@ -70,14 +66,11 @@ __device__ inline int seen_of(const SeqRows& r, int row, int G) { return max(0, 
 // The whole block's item, false where there is none.
 template <int R>
 __device__ inline bool find_item(const PagedArgs& p, int item, Item& w) {
-  const int chunk = piece_tiles<R>(p);
+  const SeqScan scan(p.a);
+  const int chunk = piece_tiles<R>(p, scan);
   int local;
-  if (!find_unit(p.a.S, item, [&](int s) {
-        const SeqRows r = seq_rows(p.a, s);
-        return units_of<R>(p, r) * pieces_of(r, chunk);
-      }, w.seq, local))
+  if (!scan.find(item, [&](const SeqRows& r) { return units_of<R>(p, r) * pieces_of(r, chunk); }, w.seq, local, w.r))
     return false;
-  w.r = seq_rows(p.a, w.seq);
   w.split = pieces_of(w.r, chunk);
   const int units = units_of<R>(p, w.r);
   const int unit = units - 1 - local / w.split, piece = local % w.split;  // those with the most keys first

@@ -43,31 +43,86 @@ __device__ inline SeqRows seq_rows(const PagedRows& a, int s) {
   return r;
 }
 
-// Sequence and place of unit b where sequence s has count(s) units, for a whole
-// wave; false past the last one.
-template <class Count>
-__device__ inline bool find_unit(int S, int b, Count count, int& seq, int& local) {
-  const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int s0 = 0; s0 < S; s0 += 64) {
-    const int c = s0 + lane < S ? count(s0 + lane) : 0;
-    int upto = c;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int v = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += v;
-    }
-    const int total = __shfl(upto, 63, 64);
-    if (b < base + total) {
-      const int at = __ffsll((unsigned long long)__ballot(base + upto > b)) - 1;
-      seq = __builtin_amdgcn_readfirstlane(s0 + at);
-      local = __builtin_amdgcn_readfirstlane(b - base - __shfl(upto - c, at, 64));
-      return true;
-    }
-    base += total;
-  }
-  return false;
+// Sums over a wave without LDS: within rows of 16 lanes by DPP, then over the rows.
+template <int kCtrl> __device__ inline int dpp_or_0(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, kCtrl, 0xf, 0xf, true);
 }
+__device__ inline int wave_scan(int x, int& total) {  // inclusive; total: the whole wave's
+  x += dpp_or_0<0x111>(x);  // row_shr:1, 2, 4, 8
+  x += dpp_or_0<0x112>(x);
+  x += dpp_or_0<0x114>(x);
+  x += dpp_or_0<0x118>(x);
+  const int r0 = __builtin_amdgcn_readlane(x, 15), r1 = __builtin_amdgcn_readlane(x, 31),
+            r2 = __builtin_amdgcn_readlane(x, 47), row = (threadIdx.x & 63) >> 4;
+  x += (row > 0 ? r0 : 0) + (row > 1 ? r1 : 0) + (row > 2 ? r2 : 0);
+  total = __builtin_amdgcn_readlane(x, 63);
+  return x;
+}
+__device__ inline float wave_total(float x) {
+  x += bits_f32((uint32_t)dpp_or_0<0x121>((int)f32_bits(x)));  // row_ror:1, 2, 4, 8
+  x += bits_f32((uint32_t)dpp_or_0<0x122>((int)f32_bits(x)));
+  x += bits_f32((uint32_t)dpp_or_0<0x124>((int)f32_bits(x)));
+  x += bits_f32((uint32_t)dpp_or_0<0x128>((int)f32_bits(x)));
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) sum += bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(x), 16 * r));
+  return sum;
+}
+
+// The sequences as a wave looks through them: lane l has sequence l, 64 + l, ... ; the
+// first 64 are read once.
+struct SeqScan {
+  const PagedRows& a;
+  SeqRows first;
+  __device__ inline explicit SeqScan(const PagedRows& rows) : a(rows), first(at(0)) {}
+  __device__ inline SeqRows at(int s0) const {
+    const int s = s0 + (threadIdx.x & 63);
+    return s < a.S ? seq_rows(a, s) : SeqRows{0, 0, 0, false};
+  }
+  // sum of value(sequence) over all
+  template <class F>
+  __device__ inline float sum(F value) const {
+    float x = value(first);
+    for (int s0 = 64; s0 < a.S; s0 += 64) x += value(at(s0));
+    return wave_total(x);
+  }
+  // sum of count(sequence) over the sequences before `seq`
+  template <class F>
+  __device__ inline int before(int seq, F count) const {
+    int base = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+      const int c = count(s0 == 0 ? first : at(s0));
+      int total;
+      const int upto = wave_scan(c, total);
+      if (seq < s0 + 64) return base + __builtin_amdgcn_readlane(upto - c, seq - s0);
+      base += total;
+    }
+    return base;
+  }
+  // Sequence and place of unit b where a sequence has count(sequence) units; false past the last.
+  template <class F>
+  __device__ inline bool find(int b, F count, int& seq, int& local, SeqRows& r) const {
+    int base = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+      const SeqRows mine = s0 == 0 ? first : at(s0);
+      const int c = count(mine);
+      int total;
+      const int upto = wave_scan(c, total);
+      if (b < base + total) {
+        const int l = __ffsll((unsigned long long)__ballot(base + upto > b)) - 1;
+        seq = s0 + l;
+        local = b - base - __builtin_amdgcn_readlane(upto - c, l);
+        r.first = __builtin_amdgcn_readlane(mine.first, l);
+        r.n = __builtin_amdgcn_readlane(mine.n, l);
+        r.len = __builtin_amdgcn_readlane(mine.len, l);
+        r.bad = __builtin_amdgcn_readlane((int)mine.bad, l);
+        return true;
+      }
+      base += total;
+    }
+    return false;
+  }
+};
 
 // Page of a sequence's position; `bad` is set, and page 0 taken, where there is none.
 __device__ inline int page_of(const PagedRows& a, int seq, int pos, bool& bad) {

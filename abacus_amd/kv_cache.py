@@ -18,6 +18,7 @@ torch's operations.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -29,6 +30,13 @@ __all__ = ["BatchRows", "KVPages", "PagedKVCache"]
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 E4M3 = torch.float8_e4m3fn
+_CODES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+_HELD = {**_CODES, E4M3: _lib.E4M3}
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_ws_bytes(*sizes: int) -> int:
+    return _lib.query("abacus_paged_attention_ws_bytes", *sizes)
 
 
 def _index(name: str, t: torch.Tensor, shape: tuple[int, ...], device: torch.device) -> torch.Tensor:
@@ -36,7 +44,7 @@ def _index(name: str, t: torch.Tensor, shape: tuple[int, ...], device: torch.dev
         raise ValueError(f"{name} must be int32 on {device}, got {t.dtype} on {t.device}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 class BatchRows:
@@ -51,19 +59,21 @@ class BatchRows:
     The three are read on the device when a call runs, so a captured graph follows what they hold at each replay.
     """
 
-    __slots__ = ("page_table_SP", "query_start", "lengths", "max_new")
+    __slots__ = ("page_table_SP", "query_start", "lengths", "max_new", "device", "_sizes")
 
     def __init__(self, page_table_SP: torch.Tensor, query_start: torch.Tensor, lengths: torch.Tensor,
                  max_new: int | None = None):
-        if page_table_SP.dim() != 2 or 0 in page_table_SP.shape:
-            raise ValueError(f"page_table must be (sequences, pages), got {tuple(page_table_SP.shape)}")
-        S, device = page_table_SP.shape[0], page_table_SP.device
+        shape = page_table_SP.shape
+        if len(shape) != 2 or 0 in shape:
+            raise ValueError(f"page_table must be (sequences, pages), got {tuple(shape)}")
         if max_new is not None and max_new < 1:
             raise ValueError(f"max_new must be at least 1, got {max_new}")
-        self.page_table_SP = _index("page_table", page_table_SP, page_table_SP.shape, device)
+        S, P = shape
+        device = page_table_SP.device
+        self.page_table_SP = _index("page_table", page_table_SP, (S, P), device)
         self.query_start = _index("query_start", query_start, (S + 1,), device)
         self.lengths = _index("lengths", lengths, (S,), device)
-        self.max_new = max_new
+        self.max_new, self.device, self._sizes = max_new, device, (S, P)
 
     def positions(self, n_rows: int) -> torch.Tensor:
         """(n_rows,) int64: each row's position in its sequence (0 for rows of none)."""
@@ -75,22 +85,14 @@ class BatchRows:
         return torch.where((seq >= 0) & (seq < S) & (pos >= 0), pos, 0).long()
 
 
-class _Guard:
-    """Makes the tensors' device current where it is not (a launch takes place on the current one)."""
-
-    __slots__ = ("guard",)
-
-    def __init__(self, device: torch.device):
-        other = device.type == "cuda" and device.index is not None and device.index != torch.cuda.current_device()
-        self.guard = torch.cuda.device(device) if other else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(device: torch.device, name: str, *args) -> None:
+    """_lib.call on torch's current stream of `device`, which is made current where it is not (a launch takes place on
+    the current one)."""
+    if device.index == torch._C._cuda_getDevice():
+        _lib.call(name, *args, _lib.stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _lib.stream_of(device))
 
 
 class KVPages:
@@ -105,99 +107,95 @@ class KVPages:
     page_size is a power of two from 16 to 256, head_dim a multiple of 16 up to 128.
     """
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "n_heads", "page_size", "head_dim", "_held")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "n_heads", "page_size", "head_dim", "dtype", "device",
+                 "_args")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None):
-        if k.dim() != 4 or v.dim() != 4:
+        if k.dim() != 4:
             raise ValueError("pages must be (pages, heads, page_size, head_dim) and (pages, heads, head_dim, page_size)")
         n, H, page, K = k.shape
-        if v.shape != (n, H, K, page):
-            raise ValueError(f"value pages must be {(n, H, K, page)} beside key pages {tuple(k.shape)}, got {tuple(v.shape)}")
+        dtype, device = k.dtype, k.device
         if page not in PAGE_SIZES or K % 16 or not 16 <= K <= 128 or n < 1 or not 1 <= H <= 1024:
             raise ValueError(f"{n} pages of {H} heads, {page} slots and head_dim {K}: page_size is one of {PAGE_SIZES}, "
                              "head_dim a multiple of 16 up to 128")
-        if k.dtype not in (torch.float32, torch.bfloat16, E4M3):
-            raise TypeError(f"a cache holds float32, bfloat16 or float8_e4m3fn, got {k.dtype}")
-        scales = (k_scale, v_scale) if k.dtype == E4M3 else ()
-        if k.dtype == E4M3:
-            for s in scales:
+        if dtype not in _HELD:
+            raise TypeError(f"a cache holds float32, bfloat16 or float8_e4m3fn, got {dtype}")
+        if v.shape != (n, H, K, page) or v.dtype != dtype:
+            raise ValueError(f"value pages must be {dtype} of {(n, H, K, page)} beside key pages {tuple(k.shape)}, got "
+                             f"{v.dtype} of {tuple(v.shape)}")
+        tensors = (k, v)
+        if dtype == E4M3:
+            for s in (k_scale, v_scale):
                 if s is None or s.dtype != torch.uint8 or s.shape != (n, H, page):
                     raise ValueError(f"float8_e4m3fn pages need uint8 k_scale and v_scale of {(n, H, page)}")
+            tensors = (k, v, k_scale, v_scale)
         elif k_scale is not None or v_scale is not None:
-            raise ValueError(f"{k.dtype} pages have no scales")
-        for t in (v, *scales):
-            if t.device != k.device or (t is v and t.dtype != k.dtype):
-                raise ValueError("a layer's pages must have one dtype and be on one device")
-        for t in (k, v, *scales):
-            if not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f"{dtype} pages have no scales")
+        at = [t.data_ptr() for t in tensors]
+        for t, p in zip(tensors, at):
+            if t.device != device:
+                raise ValueError("a layer's pages must be on one device")
+            if p % 16 or not t.is_contiguous():
                 raise ValueError("pages must be contiguous and 16-byte aligned")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.n_pages, self.n_heads, self.page_size, self.head_dim = n, H, page, K
-        self._held = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, E4M3: _lib.E4M3}[k.dtype]
+        self.dtype, self.device = dtype, device
+        self._args = (page, n, _HELD[dtype], *at, *(None,) * (4 - len(at)))
 
-    def _check(self, name: str, x: torch.Tensor, rows: BatchRows, heads: int | None) -> None:
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads):
+    def _check(self, name: str, x: torch.Tensor, rows: BatchRows, heads: int | None) -> torch.Size:
+        shape, dtype = x.shape, x.dtype
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
             want = "heads" if heads is None else heads
-            raise ValueError(f"{name} must be (rows, {want}, {self.head_dim}), got {tuple(x.shape)}")
-        if x.dtype not in (torch.float32, torch.bfloat16) or self.k.dtype not in (x.dtype, E4M3):
-            raise TypeError(f"{name} of {x.dtype} over a cache of {self.k.dtype}: the cache holds the rows' dtype "
+            raise ValueError(f"{name} must be (rows, {want}, {self.head_dim}), got {tuple(shape)}")
+        if dtype not in _CODES or (self.dtype != dtype and self.dtype != E4M3):
+            raise TypeError(f"{name} of {dtype} over a cache of {self.dtype}: the cache holds the rows' dtype "
                             "(float32 or bfloat16) or float8_e4m3fn")
-        if x.device != self.k.device or rows.lengths.device != self.k.device:
+        if x.device != self.device or rows.device != self.device:
             raise ValueError(f"{name}, the rows and the pages must be on one device")
+        return shape
 
     def _rows_args(self, rows: BatchRows) -> tuple:
-        S, P = rows.page_table_SP.shape
-        return (rows.page_table_SP.data_ptr(), rows.query_start.data_ptr(), rows.lengths.data_ptr(), S, P,
-                self.page_size, self.n_pages, self._held, self.k.data_ptr(), self.v.data_ptr(),
-                None if self.k_scale is None else self.k_scale.data_ptr(),
-                None if self.v_scale is None else self.v_scale.data_ptr())
+        return (rows.page_table_SP.data_ptr(), rows.query_start.data_ptr(), rows.lengths.data_ptr(), *rows._sizes,
+                *self._args)
 
-    @torch.no_grad()
     def write(self, k_THK: torch.Tensor, v_THK: torch.Tensor, rows: BatchRows) -> None:
         """Keys and values (T, heads, head_dim) of the rows into their slots.
 
         Rows of no sequence, of a sequence longer than its table, or whose page is not in the pool are not
         written.  Two rows of a call with the same slot leave one or the other (of e4m3 pages possibly codes of
         one and exponents of the other): sequences may share pages that they only read."""
-        self._check("k", k_THK, rows, self.n_heads)
-        if v_THK.shape != k_THK.shape or v_THK.dtype != k_THK.dtype or v_THK.device != k_THK.device:
+        T, H, K = self._check("k", k_THK, rows, self.n_heads)
+        if v_THK.shape != k_THK.shape or v_THK.dtype != k_THK.dtype or v_THK.device != self.device:
             raise ValueError("k and v must have one shape, dtype and device")
-        if k_THK.device.type == "cpu":
+        if not k_THK.is_cuda:
             return self._write_cpu(k_THK, v_THK, rows)
-        T, H, K = k_THK.shape
         k_THK, v_THK = _contig(k_THK), _contig(v_THK)
-        with _Guard(k_THK.device):
-            _lib.call("abacus_kv_write", k_THK.data_ptr(), v_THK.data_ptr(), T, H, K, _lib.dtype_code(k_THK.dtype),
-                      *self._rows_args(rows), _lib.stream_of(k_THK.device))
+        _call(self.device, "abacus_kv_write", k_THK.data_ptr(), v_THK.data_ptr(), T, H, K, _CODES[k_THK.dtype],
+              *self._rows_args(rows))
 
-    @torch.no_grad()
     def read(self, rows: BatchRows, length: int, dtype: torch.dtype | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Keys and values (S, length, heads, head_dim): position l of sequence s in row (s, l), 0 past its length.
 
         dtype: the pages' own, or for e4m3 pages bfloat16 (which holds every value of theirs exactly; the
         default) or float32."""
         if dtype is None:
-            dtype = torch.bfloat16 if self.k.dtype == E4M3 else self.k.dtype
-        if dtype not in (torch.float32, torch.bfloat16) or self.k.dtype not in (dtype, E4M3):
-            raise TypeError(f"a cache of {self.k.dtype} is not read as {dtype}")
-        if rows.lengths.device != self.k.device:
+            dtype = torch.bfloat16 if self.dtype == E4M3 else self.dtype
+        if dtype not in _CODES or (self.dtype != dtype and self.dtype != E4M3):
+            raise TypeError(f"a cache of {self.dtype} is not read as {dtype}")
+        if rows.device != self.device:
             raise ValueError("the rows and the pages must be on one device")
         if length < 0:
             raise ValueError(f"length must not be negative, got {length}")
-        S, P = rows.page_table_SP.shape
+        S, P = rows._sizes
         shape = (S, length, self.n_heads, self.head_dim)
-        if self.k.device.type == "cpu":
+        if not self.k.is_cuda:
             return self._read_cpu(rows, shape, dtype)
-        k, v = (torch.empty(shape, dtype=dtype, device=self.k.device) for _ in range(2))
-        table, _, lengths, *rest = self._rows_args(rows)
-        S, P, page, n, *pages = rest
-        with _Guard(k.device):
-            _lib.call("abacus_kv_read", table, lengths, S, P, page, n, self.n_heads, self.head_dim, *pages, length,
-                      _lib.dtype_code(dtype), k.data_ptr(), v.data_ptr(), _lib.stream_of(k.device))
+        k, v = torch.empty((2, *shape), dtype=dtype, device=self.device).unbind()
+        _call(self.device, "abacus_kv_read", rows.page_table_SP.data_ptr(), rows.lengths.data_ptr(), S, P, *self._args[:2],
+              self.n_heads, self.head_dim, *self._args[2:], length, _CODES[dtype], k.data_ptr(), v.data_ptr())
         return k, v
 
-    @torch.no_grad()
     def attend(self, q_THK: torch.Tensor, rows: BatchRows, scale: float | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
         """softmax(scale q k^T) v of each row over the cached positions up to its own, which have to be written.
@@ -209,34 +207,28 @@ class KVPages:
 
         Statistics and sums are fp32; with bf16 queries the probabilities are rounded to bf16 for the product
         with the values, as the training kernels do.  No gradient is formed."""
-        self._check("q", q_THK, rows, None)
-        T, H, K = q_THK.shape
+        T, H, K = self._check("q", q_THK, rows, None)
         if H % self.n_heads or H < 1 or H > 1024:
             raise ValueError(f"{H} query heads over {self.n_heads} key heads: they must be a multiple (at most 1024)")
         scale = 1.0 / math.sqrt(K) if scale is None else float(scale)
         if not 0.0 < scale < math.inf:
             raise ValueError(f"scale must be positive, got {scale}")
         if out is not None:
-            if out.shape != q_THK.shape or out.dtype != q_THK.dtype or out.device != q_THK.device:
+            if out.shape != q_THK.shape or out.dtype != q_THK.dtype or out.device != self.device:
                 raise ValueError("out must have q's shape, dtype and device")
             if not out.is_contiguous() or out.data_ptr() % 16:
                 raise ValueError("out must be contiguous and 16-byte aligned")
-        if q_THK.device.type == "cpu":
+        if not q_THK.is_cuda:
             return self._attend_cpu(q_THK, rows, scale, out)
-        q = _contig(q_THK)
-        zero_rest = out is None
+        q, code = _contig(q_THK), _CODES[q_THK.dtype]
+        zero_rest = int(out is None)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        args = self._rows_args(rows)
-        S, P = args[3:5]
+            out = torch.empty_like(q)
         most = max(1, T) if rows.max_new is None else rows.max_new
-        with _Guard(q.device):
-            nbytes = _lib.query("abacus_paged_attention_ws_bytes", T, H, self.n_heads, K, _lib.dtype_code(q.dtype), S, P,
-                                self.page_size, most)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-            _lib.call("abacus_paged_attention", q.data_ptr(), T, H, self.n_heads, K, _lib.dtype_code(q.dtype), *args,
-                      scale, most, int(zero_rest), out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
-                      _lib.stream_of(q.device))
+        nbytes = _attention_ws_bytes(T, H, self.n_heads, K, code, *rows._sizes, self.page_size, most)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        _call(self.device, "abacus_paged_attention", q.data_ptr(), T, H, self.n_heads, K, code, *self._rows_args(rows), scale,
+              most, zero_rest, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
         return out
 
     # ------------------------------------------------------------ CPU tensors
@@ -244,7 +236,7 @@ class KVPages:
     def _sequences(self, rows: BatchRows, n_rows: int):
         """Of each sequence: its number, first row, rows, length, and (page, slot) of its positions; page None
         where the table does not hold the sequence or its pages are not in the pool."""
-        P = rows.page_table_SP.shape[1]
+        P = rows._sizes[1]
         start, lengths = rows.query_start.tolist(), rows.lengths.tolist()
         for s, length in enumerate(lengths):
             first, n = start[s], start[s + 1] - start[s]
@@ -260,6 +252,7 @@ class KVPages:
         e = torch.where(mantissa == 0, 0, (exponent - torch.where(mantissa <= 0.875, 9, 8)).clamp(min=-110))
         return (x.float() * _power(-e)[..., None]).to(E4M3), (e + 127).to(torch.uint8)
 
+    @torch.no_grad()
     def _write_cpu(self, k, v, rows):
         for _, first, n, length, page, slot, there in self._sequences(rows, k.shape[0]):
             new = min(n, length)
@@ -269,7 +262,7 @@ class KVPages:
             keep = there[at]
             page, slot = page[at][keep], slot[at][keep]
             kn, vn = (x[first + n - new:first + n][keep] for x in (k, v))
-            if self.k.dtype == E4M3:
+            if self.dtype == E4M3:
                 fine = (torch.isfinite(kn) & torch.isfinite(vn)).all(-1)
                 (kc, ks), (vc, vs) = (self._quantise(torch.where(fine[..., None], x, 0)) for x in (kn, vn))
                 kc = torch.where(fine[..., None], kc.view(torch.uint8), 0x7f)
@@ -282,7 +275,7 @@ class KVPages:
 
     def _values(self, page, slot, there, dtype=torch.float32):
         """Keys and values (positions, heads, head_dim); NaN where a position is in no page."""
-        if self.k.dtype == E4M3:
+        if self.dtype == E4M3:
             k = self.k.view(torch.uint8)[page, :, slot].view(E4M3).to(dtype) * _power(
                 self.k_scale[page, :, slot].int() - 127)[..., None]
             v = self.v.view(torch.uint8)[page, :, :, slot].view(E4M3).to(dtype) * _power(
@@ -293,6 +286,7 @@ class KVPages:
         there = there[:, None, None]
         return torch.where(there, k, math.nan), torch.where(there, v, math.nan)
 
+    @torch.no_grad()
     def _read_cpu(self, rows, shape, dtype):
         k, v = torch.zeros(shape, dtype=dtype), torch.zeros(shape, dtype=dtype)
         for s, _, _, _, page, slot, there in self._sequences(rows, 0):
@@ -301,6 +295,7 @@ class KVPages:
             k[s, :n], v[s, :n] = kn.to(dtype), vn.to(dtype)
         return k, v
 
+    @torch.no_grad()
     def _attend_cpu(self, q, rows, scale, out):
         if out is None:
             out = torch.zeros(q.shape, dtype=q.dtype)

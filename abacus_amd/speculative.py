@@ -12,12 +12,11 @@ import math
 import torch
 
 from . import _lib
-from .kv_cache import _Guard
+from .kv_cache import _call
 
 __all__ = ["verify_drafts"]
 
 
-@torch.no_grad()
 def verify_drafts(target_logits_TV: torch.Tensor, tokens_T: torch.Tensor, query_start: torch.Tensor,
                   uniforms_T2: torch.Tensor | None = None, draft_logits_TV: torch.Tensor | None = None,
                   temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
@@ -65,21 +64,20 @@ def verify_drafts(target_logits_TV: torch.Tensor, tokens_T: torch.Tensor, query_
         if t is not None and t.device != dev:
             raise ValueError("logits, tokens, query_start and uniforms must be on one device")
     S = query_start.shape[0] - 1
-    if dev.type == "cpu":
+    if not target_logits_TV.is_cuda:
         return _verify_cpu(target_logits_TV, tokens_T, query_start.tolist(), uniforms_T2, draft_logits_TV, temperature)
     if T > 65535 or S > 65535:
         raise ValueError(f"{T} rows of {S} sequences: at most 65535 at once")
     target, tokens, start = target_logits_TV.contiguous(), tokens_T.contiguous(), query_start.contiguous()
     draft = None if draft_logits_TV is None else draft_logits_TV.contiguous()
     uniforms = None if uniforms_T2 is None else uniforms_T2.contiguous()
-    with _Guard(dev):
-        nbytes = _lib.query("abacus_verify_drafts_ws_bytes", T, V, S)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        accepted = torch.empty(S, dtype=torch.int32, device=dev)
-        following = torch.empty(S, dtype=torch.int64, device=dev)
-        at = [None if t is None else t.data_ptr() for t in (target, draft, tokens, start, uniforms)]
-        _lib.call("abacus_verify_drafts", *at, T, V, S, _lib.dtype_code(target.dtype), temperature,
-                  accepted.data_ptr(), following.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_of(dev))
+    nbytes = _lib.query("abacus_verify_drafts_ws_bytes", T, V, S)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    accepted = torch.empty(S, dtype=torch.int32, device=dev)
+    following = torch.empty(S, dtype=torch.int64, device=dev)
+    at = [None if t is None else t.data_ptr() for t in (target, draft, tokens, start, uniforms)]
+    _call(dev, "abacus_verify_drafts", *at, T, V, S, _lib.dtype_code(target.dtype), temperature, accepted.data_ptr(),
+          following.data_ptr(), ws.data_ptr(), nbytes)
     return accepted, following
 
 
@@ -91,6 +89,7 @@ def _softmax(row: torch.Tensor, temperature: float) -> torch.Tensor | None:
     return e / e.sum()
 
 
+@torch.no_grad()
 def _verify_cpu(target, tokens, start, uniforms, draft, temperature):
     T, V = target.shape
     accepted, following = [], []
