@@ -25,6 +25,7 @@ namespace abacus {
 namespace {
 
 constexpr int kFewPieces = 2048;   // pieces the work of a launch is cut into, about
+constexpr int kFewJoined = 16;     // pieces that a wave joins for several rows at once
 constexpr int kChunkPieces = 512;  // (of the chunk kernel's: two work-groups a CU)
 
 typedef __bf16 pa_bf16x8 __attribute__((ext_vector_type(8)));
@@ -186,17 +187,22 @@ __global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 :
 
   // The pages of a tile's four groups of keys: the lane's key rows are in group
   // i / 4, its value keys in group g.  Groups past the last key seen take the first.
+  struct Ids { int k, v; };
   struct Place { int64_t k, v; int ko, vo; bool bad; };
   const int in_mask = (1 << p.a.shift) - 1;
-  auto place = [&](int tile) __attribute__((always_inline)) {
+  const int* table = p.a.table + (int64_t)seq * p.a.P;
+  auto ids_of = [&](int tile) __attribute__((always_inline)) {
+    const int pk = tile * KT + (i >> 2) * KG, pv = tile * KT + g * KG;
+    return Ids{table[(pk < seen ? pk : 0) >> p.a.shift], table[(pv < seen ? pv : 0) >> p.a.shift]};
+  };
+  auto place = [&](int tile, Ids id) __attribute__((always_inline)) {
     Place w;
     const int pk = tile * KT + (i >> 2) * KG, pv = tile * KT + g * KG;
-    const int ck = pk < seen ? pk : 0, cv = pv < seen ? pv : 0;
-    bool bad_k, bad_v;
-    w.k = (int64_t)page_of(p.a, seq, ck, bad_k) * p.Hk + kh;
-    w.v = (int64_t)page_of(p.a, seq, cv, bad_v) * p.Hk + kh;
-    w.ko = ck & in_mask;
-    w.vo = cv & in_mask;
+    const bool bad_k = (unsigned)id.k >= (unsigned)p.a.n_pages, bad_v = (unsigned)id.v >= (unsigned)p.a.n_pages;
+    w.k = (int64_t)(bad_k ? 0 : id.k) * p.Hk + kh;
+    w.v = (int64_t)(bad_v ? 0 : id.v) * p.Hk + kh;
+    w.ko = pk & in_mask;
+    w.vo = pv & in_mask;
     w.bad = bad_v && pv < seen;
     return w;
   };
@@ -404,16 +410,19 @@ __global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 :
     }
   };
 
+  // (page numbers are read two tiles ahead, as the loads of a tile wait for them)
   int tile = t0 + wave;
   if (tile < t1) {
-    here = place(tile);
+    Ids then = ids_of(min(tile + 4, t1 - 1));
+    here = place(tile, ids_of(tile));
     x.load_k(p, here.k, here.ko, lane);
     x.load_v(p, here.v, here.vo, lane);
     // every row sees all of these: the next tile's keys are on their way while this one's
     // scores are weighed, its values while the next one's scores are formed
     while (tile * KT + KT <= least) {
       const bool more = tile + 4 < t1;
-      const Place next = more ? place(tile + 4) : here;
+      const Place next = place(tile + 4, then);
+      then = ids_of(min(tile + 8, t1 - 1));
       step(tile, std::false_type{}, [&]() __attribute__((always_inline)) {
         if (more) x.load_k(p, next.k, next.ko, lane);
       });
@@ -427,7 +436,8 @@ __global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 :
       step(tile, std::true_type{}, [] {});
       tile += 4;
       if (tile < t1) {
-        here = place(tile);
+        here = place(tile, then);
+        then = ids_of(min(tile + 4, t1 - 1));
         x.load_k(p, here.k, here.ko, lane);
         x.load_v(p, here.v, here.vo, lane);
       }
@@ -495,6 +505,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
   const int64_t pitch = (int64_t)p.Hk * R * (K + 2);  // between a unit's pieces
   const float* part = p.part + ((int64_t)item * p.Hk + kh) * R * (K + 2);
   const int rows = min(R, r.n * p.G - local * R);
+  if (split <= kFewJoined) {  // as many rows at a time as the wave holds, piece by piece
+    const int sub = lane / lanes, subs = 64 / lanes, d = lane % lanes * 4;
+    for (int m0 = (blockIdx.y * 4 + wave) * subs; m0 < rows; m0 += gridDim.y * 4 * subs) {
+      const int m = min(m0 + sub, rows - 1);
+      float top = -__builtin_inff(), l = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < split; ++i) top = fmaxf(top, part[i * pitch + R * K + m]);
+      pa_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int i = 0; i < split; ++i) {
+        const float pm = part[i * pitch + R * K + m], pl = part[i * pitch + R * K + R + m];
+        const pa_f32x4 x = *reinterpret_cast<const pa_f32x4*>(part + i * pitch + (int64_t)m * K + d);
+        const float f = pm == -__builtin_inff() ? (pl == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(pm - top);
+        l += f * pl;
+        if (f != 0.f) o += f * x;  // (an empty piece weighs nothing)
+      }
+      if (sub < subs && m0 + sub < rows) store_row4<Q>(p, r, kh, local * R + m, d, o, l);
+    }
+    return;
+  }
   for (int m = blockIdx.y * 4 + wave; m < rows; m += gridDim.y * 4) {
     float top = -__builtin_inff();
     for (int i = lane; i < split; i += 64) top = fmaxf(top, part[i * pitch + R * K + m]);

@@ -15,7 +15,7 @@
 namespace abacus {
 
 constexpr int kTile = 64;   // keys of a tile
-constexpr int kLeast = 8;   // tiles of a piece, at least
+constexpr int kLeast = 16;  // tiles of a piece, at least
 
 struct PagedArgs {
   PagedRows a;
