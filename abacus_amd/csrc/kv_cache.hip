@@ -212,61 +212,104 @@ __device__ inline void widen8(const C* p, int byte, float (&x)[8]) {
   }
 }
 
-// Rows (s, l) of out, l < L: position l of sequence s, 0 past its length.  A block
-// takes 16 positions of one head.
+// 8 values of one position out of 8 rows of V^T, four positions of each at hand (C's of a row in
+// n dwords), as fp32.
+template <typename C, int N>
+__device__ inline void position_of(const uint32_t (&w)[8][N], int pos, int byte, float (&y)[8]) {
+  if constexpr (sizeof(C) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = bits_f32(w[i][pos]);
+  } else if constexpr (sizeof(C) == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = pos & 1 ? hi_bf16(w[i][pos / 2]) : lo_bf16(w[i][pos / 2]);
+  } else {
+    const int sel = 0x0c0c0400 + pos * 0x0101;  // byte pos of two words, side by side
+    uint2 c;
+    c.x = __builtin_amdgcn_perm(w[1][0], w[0][0], sel) | __builtin_amdgcn_perm(w[3][0], w[2][0], sel) << 16;
+    c.y = __builtin_amdgcn_perm(w[5][0], w[4][0], sel) | __builtin_amdgcn_perm(w[7][0], w[6][0], sel) << 16;
+    widen8((const C*)&c, byte, y);
+  }
+}
+
+// Rows (s, l) of out, l < L: position l of sequence s, 0 past its length.  A block takes
+// kSpan groups of one head, all their loads under way at once: with one group a block, blocks
+// of a few kilobytes came and went at 3.9 TB/s.
+constexpr int kSpan = 4;
 template <typename C, typename T>
 __global__ __launch_bounds__(256) void kv_read_kernel(PagedRows a, Pages p, int64_t L, T* __restrict__ k,
                                                       T* __restrict__ v) {
-  __shared__ __attribute__((aligned(16))) C turned[kMaxK][kGroup + (sizeof(C) == 1 ? 0 : 16 / sizeof(C))];
-  const int tid = threadIdx.x, H = p.H, K = p.K;
-  const int seq = blockIdx.z, head = blockIdx.x, g0 = blockIdx.y * kGroup;
-  const int pos = g0 + tid / 16, d0 = (tid % 16) * 8;
+  constexpr int N = (int)sizeof(C);  // dwords of four values
+  constexpr int kPitch = 4 * N + 1;  // dwords of a V^T row in LDS: 8 rows apart is 8 or 40 banks
+  __shared__ uint32_t turned[kSpan][kMaxK * kPitch];
+  const int tid = threadIdx.x, H = p.H, K = p.K, octets = K / 8;
+  const int seq = blockIdx.z, head = blockIdx.x, l0 = blockIdx.y * kGroup * kSpan;
   const int given = a.lengths[seq], most = a.P << a.shift, len = min(max(given, 0), most);
-  float x[8] = {}, y[8] = {};
-  if (g0 < len) {
-    bool bad;
-    const int page = page_of(a, seq, g0, bad);
-    bad |= given > most;
-    const int in_page = g0 & ((1 << a.shift) - 1);
-    const int64_t tile = (int64_t)page * H + head, slot = (tile << a.shift) + in_page + tid / 16;
-    for (int d = tid; d < K; d += 256) {
-      const C* from = (const C*)p.v + ((tile * K + d) << a.shift) + in_page;
+  const int in_page = (1 << a.shift) - 1;
+  int64_t tile[kSpan];  // (page, head) of each group; groups past the length take the first page
+  bool bad[kSpan];
 #pragma unroll
-      for (int j = 0; j < (int)sizeof(C); ++j)
-        *reinterpret_cast<Vec16*>((char*)turned[d] + 16 * j) = ld16((const char*)from + 16 * j);
-    }
-    __syncthreads();
-    if (pos < len && d0 < K) {
-      int bk = 127, bv = 127;
-      bool poison = bad;
-      if constexpr (sizeof(C) == 1) {
-        bk = p.k_scale[slot];
-        bv = p.v_scale[slot];
-        poison |= (((const uint8_t*)p.k)[slot * K] & 0x7f) == kNaNCode;
-      }
-      widen8((const C*)p.k + slot * K + d0, bk, x);
-      C run[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) run[i] = turned[d0 + i][tid / 16];
-      if constexpr (sizeof(C) == 1) {
-        uint2 c;
-        c.x = run[0] | run[1] << 8 | run[2] << 16 | (uint32_t)run[3] << 24;
-        c.y = run[4] | run[5] << 8 | run[6] << 16 | (uint32_t)run[7] << 24;
-        widen8((const C*)&c, bv, y);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = to_f32(run[i]);
-      }
-      if (poison) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = bad ? __builtin_nanf("") : x[i], y[i] = __builtin_nanf("");
-      }
-    }
+  for (int j = 0; j < kSpan; ++j) {
+    const int pos = l0 + j * kGroup;
+    tile[j] = (int64_t)page_of(a, seq, pos < len ? pos : 0, bad[j]) * H + head;
+    bad[j] |= given > most;
   }
-  if (pos < L && d0 < K) {
-    const int64_t at = ((seq * L + pos) * H + head) * K + d0;
-    store8(k + at, x);
-    store8(v + at, y);
+  // V^T into LDS, 16 bytes at a time
+  for (int i = tid; i < kSpan * K * N; i += 256) {
+    const int j = i / (K * N), d = i / N % K, c = i % N;
+    const int64_t at = j == 0 ? tile[0] : j == 1 ? tile[1] : j == 2 ? tile[2] : tile[3];
+    const Vec16 w = ld16((const C*)p.v + ((at * K + d) << a.shift) + ((l0 + j * kGroup) & in_page) + c * (16 / N));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) turned[j][d * kPitch + 4 * c + e] = w.w[e];
+  }
+  // keys: 8 dims of one position a thread
+#pragma unroll
+  for (int j = 0; j < kSpan; ++j)
+    for (int i = tid; i < kGroup * octets; i += 256) {
+      const int r = i / octets, d0 = i % octets * 8, l = l0 + j * kGroup + r;
+      if (l >= L) continue;
+      float x[8] = {};
+      if (l < len) {
+        const int64_t slot = (tile[j] << a.shift) + (l & in_page);
+        int byte = 127;
+        if constexpr (N == 1) byte = p.k_scale[slot];
+        widen8((const C*)p.k + slot * K + d0, byte, x);
+        if (bad[j])
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = __builtin_nanf("");
+      }
+      store8(k + ((seq * L + l) * H + head) * K + d0, x);
+    }
+  __syncthreads();
+  // values: 8 dims of four positions
+  for (int i = tid; i < kSpan * 4 * octets; i += 256) {
+    const int d0 = i % octets * 8, quad = i / octets % 4, j = i / octets / 4;
+    const int64_t at = j == 0 ? tile[0] : j == 1 ? tile[1] : j == 2 ? tile[2] : tile[3];
+    const bool none = j == 0 ? bad[0] : j == 1 ? bad[1] : j == 2 ? bad[2] : bad[3];
+    uint32_t w[8][N];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int n = 0; n < N; ++n) w[e][n] = turned[j][(d0 + e) * kPitch + quad * N + n];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int l = l0 + j * kGroup + quad * 4 + r;
+      if (l >= L) continue;
+      float y[8] = {};
+      if (l < len) {
+        int byte = 127;
+        bool poison = none;
+        if constexpr (N == 1) {
+          const int64_t slot = (at << a.shift) + (l & in_page);
+          byte = p.v_scale[slot];
+          poison |= (((const uint8_t*)p.k)[slot * K] & 0x7f) == kNaNCode;
+        }
+        position_of<C>(w, r, byte, y);
+        if (poison)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = __builtin_nanf("");
+      }
+      store8(v + ((seq * L + l) * H + head) * K + d0, y);
+    }
   }
 }
 
@@ -329,7 +372,7 @@ extern "C" int abacus_kv_read(const int32_t* page_table_SP, const int32_t* lengt
                    "kv_read: k and v must be there, and 16-byte aligned");
   PagedRows a{page_table_SP, nullptr, lengths, (int)S, (int)P, 0, __builtin_ctzll(page_size), (int)n_pages};
   Pages p{(void*)k_pages, (void*)v_pages, (uint8_t*)k_scale, (uint8_t*)v_scale, (int)H, (int)K};
-  const dim3 grid((unsigned)H, (unsigned)((L + kGroup - 1) / kGroup), (unsigned)S);
+  const dim3 grid((unsigned)H, (unsigned)((L + kGroup * kSpan - 1) / (kGroup * kSpan)), (unsigned)S);
   hipStream_t s = (hipStream_t)stream;
   if (held == ABACUS_E4M3 && dtype == kBF16)
     hipLaunchKernelGGL((kv_read_kernel<uint8_t, uint16_t>), grid, dim3(256), 0, s, a, p, L, (uint16_t*)k_SLHK,
