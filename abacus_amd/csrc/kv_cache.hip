@@ -56,23 +56,20 @@ __device__ inline void load8(const T* p, float (&x)[8]) {
   }
 }
 
-// 8 values to 8 of T
-template <typename T>
+// 8 values to 8 of T; Stream: past the caches, for what is written once and not read here
+template <bool Stream, typename T>
 __device__ inline void store8(T* to, const float (&x)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    Vec16 w;
+  constexpr int N = 8 * sizeof(T) / 16;
+  Vec16 w[N];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w.w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
-    st16(to, w);
-  } else {
-    Vec16 w, z;
+  for (int i = 0; i < 8 * (int)sizeof(T) / 4; ++i) {
+    if constexpr (sizeof(T) == 2) w[i / 4].w[i % 4] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    else w[i / 4].w[i % 4] = f32_bits(x[i]);
+  }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w.w[i] = f32_bits(x[i]);
-      z.w[i] = f32_bits(x[4 + i]);
-    }
-    st16(to, w);
-    st16(to + 4, z);
+  for (int n = 0; n < N; ++n) {
+    if constexpr (Stream) st16_stream((char*)to + 16 * n, w[n]);
+    else st16((char*)to + 16 * n, w[n]);
   }
 }
 
@@ -161,7 +158,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(const T* __restrict__ k, 
     }
     *reinterpret_cast<uint2*>(&turned[tid / 16][d0]) = cv;
   } else {
-    if (mine) store8((C*)p.k + ((tile << a.shift) + in_page + (pos - g0)) * K + d0, x);
+    if (mine) store8<false>((C*)p.k + ((tile << a.shift) + in_page + (pos - g0)) * K + d0, x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) turned[tid / 16][d0 + i] = from_f32<C>(y[i]);
   }
@@ -232,85 +229,101 @@ __device__ inline void position_of(const uint32_t (&w)[8][N], int pos, int byte,
 }
 
 // Rows (s, l) of out, l < L: position l of sequence s, 0 past its length.  A block takes
-// kSpan groups of one head, all their loads under way at once: with one group a block, blocks
-// of a few kilobytes came and went at 3.9 TB/s.
-constexpr int kSpan = 4;
-template <typename C, typename T>
+// Span groups of one head, all their loads under way at once: 4 where there are blocks enough
+// all the same (16 x 4096 e4m3 tokens of 16 x 64: 95 us with 1, 78 us with 4, 4.6 TB/s),
+// else 1 (1000 bf16 tokens of 8 x 128: 3.5 us, 6.4 us with 4).
+template <class T, int N> __device__ inline T pick_of(const T (&x)[N], int j) {
+  if constexpr (N == 1) return x[0];
+  const T a = j & 1 ? x[1] : x[0], b = j & 1 ? x[N - 1] : x[N / 2];
+  return j & 2 ? b : a;
+}
+template <typename C, typename T, int Span>
 __global__ __launch_bounds__(256) void kv_read_kernel(PagedRows a, Pages p, int64_t L, T* __restrict__ k,
                                                       T* __restrict__ v) {
+  static_assert(Span == 1 || Span == 4, "pick_of");
   constexpr int N = (int)sizeof(C);  // dwords of four values
   constexpr int kPitch = 4 * N + 1;  // dwords of a V^T row in LDS: 8 rows apart is 8 or 40 banks
-  __shared__ uint32_t turned[kSpan][kMaxK * kPitch];
+  __shared__ uint32_t turned[Span][kMaxK * kPitch];
+  __shared__ uint8_t exponents[Span * kGroup], nan[Span * kGroup];
   const int tid = threadIdx.x, H = p.H, K = p.K, octets = K / 8;
-  const int seq = blockIdx.z, head = blockIdx.x, l0 = blockIdx.y * kGroup * kSpan;
+  const int seq = blockIdx.z, head = blockIdx.x, l0 = blockIdx.y * kGroup * Span;
   const int given = a.lengths[seq], most = a.P << a.shift, len = min(max(given, 0), most);
   const int in_page = (1 << a.shift) - 1;
-  int64_t tile[kSpan];  // (page, head) of each group; groups past the length take the first page
-  bool bad[kSpan];
+  int64_t tile[Span];  // (page, head) of each group; groups past the length take the first page
+  bool bad[Span];
 #pragma unroll
-  for (int j = 0; j < kSpan; ++j) {
+  for (int j = 0; j < Span; ++j) {
     const int pos = l0 + j * kGroup;
     tile[j] = (int64_t)page_of(a, seq, pos < len ? pos : 0, bad[j]) * H + head;
     bad[j] |= given > most;
   }
-  // V^T into LDS, 16 bytes at a time
-  for (int i = tid; i < kSpan * K * N; i += 256) {
+  // V^T into LDS, 16 bytes at a time; of codes the values' exponents and which positions are NaN
+  for (int i = tid; i < Span * K * N; i += 256) {
     const int j = i / (K * N), d = i / N % K, c = i % N;
-    const int64_t at = j == 0 ? tile[0] : j == 1 ? tile[1] : j == 2 ? tile[2] : tile[3];
-    const Vec16 w = ld16((const C*)p.v + ((at * K + d) << a.shift) + ((l0 + j * kGroup) & in_page) + c * (16 / N));
+    const Vec16 w = ld16((const C*)p.v + ((pick_of(tile, j) * K + d) << a.shift) + ((l0 + j * kGroup) & in_page) + c * (16 / N));
 #pragma unroll
     for (int e = 0; e < 4; ++e) turned[j][d * kPitch + 4 * c + e] = w.w[e];
   }
-  // keys: 8 dims of one position a thread
-#pragma unroll
-  for (int j = 0; j < kSpan; ++j)
-    for (int i = tid; i < kGroup * octets; i += 256) {
-      const int r = i / octets, d0 = i % octets * 8, l = l0 + j * kGroup + r;
-      if (l >= L) continue;
-      float x[8] = {};
-      if (l < len) {
-        const int64_t slot = (tile[j] << a.shift) + (l & in_page);
-        int byte = 127;
-        if constexpr (N == 1) byte = p.k_scale[slot];
-        widen8((const C*)p.k + slot * K + d0, byte, x);
-        if (bad[j])
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = __builtin_nanf("");
-      }
-      store8(k + ((seq * L + l) * H + head) * K + d0, x);
+  if (tid < Span * kGroup) {
+    const int j = tid / kGroup, l = l0 + tid;
+    const int64_t slot = (pick_of(tile, j) << a.shift) + (l & in_page);
+    bool none = pick_of(bad, j);
+    if constexpr (N == 1) {
+      exponents[tid] = p.v_scale[slot];
+      none |= (((const uint8_t*)p.k)[slot * K] & 0x7f) == kNaNCode;
     }
+    nan[tid] = none;
+  }
+  // keys: 8 dims of one position a thread
+  for (int i = tid; i < Span * kGroup * octets; i += 256) {
+    const int r = i / octets, d0 = i % octets * 8, j = r / kGroup, l = l0 + r;
+    if (l >= L) break;
+    float x[8] = {};
+    if (l < len) {
+      const int64_t slot = (pick_of(tile, j) << a.shift) + (l & in_page);
+      int byte = 127;
+      if constexpr (N == 1) byte = p.k_scale[slot];
+      widen8((const C*)p.k + slot * K + d0, byte, x);
+      if (pick_of(bad, j))
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __builtin_nanf("");
+    }
+    store8<true>(k + ((seq * L + l) * H + head) * K + d0, x);
+  }
   __syncthreads();
   // values: 8 dims of four positions
-  for (int i = tid; i < kSpan * 4 * octets; i += 256) {
-    const int d0 = i % octets * 8, quad = i / octets % 4, j = i / octets / 4;
-    const int64_t at = j == 0 ? tile[0] : j == 1 ? tile[1] : j == 2 ? tile[2] : tile[3];
-    const bool none = j == 0 ? bad[0] : j == 1 ? bad[1] : j == 2 ? bad[2] : bad[3];
+  for (int i = tid; i < Span * 4 * octets; i += 256) {
+    const int d0 = i % octets * 8, quad = i / octets, j = quad / 4;
     uint32_t w[8][N];
 #pragma unroll
     for (int e = 0; e < 8; ++e)
 #pragma unroll
-      for (int n = 0; n < N; ++n) w[e][n] = turned[j][(d0 + e) * kPitch + quad * N + n];
+      for (int n = 0; n < N; ++n) w[e][n] = turned[j][(d0 + e) * kPitch + quad % 4 * N + n];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int l = l0 + j * kGroup + quad * 4 + r;
-      if (l >= L) continue;
+      const int at = quad * 4 + r, l = l0 + at;
+      if (l >= L) break;
       float y[8] = {};
       if (l < len) {
-        int byte = 127;
-        bool poison = none;
-        if constexpr (N == 1) {
-          const int64_t slot = (at << a.shift) + (l & in_page);
-          byte = p.v_scale[slot];
-          poison |= (((const uint8_t*)p.k)[slot * K] & 0x7f) == kNaNCode;
-        }
-        position_of<C>(w, r, byte, y);
-        if (poison)
+        position_of<C>(w, r, N == 1 ? exponents[at] : 127, y);
+        if (nan[at])
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] = __builtin_nanf("");
       }
-      store8(v + ((seq * L + l) * H + head) * K + d0, y);
+      store8<true>(v + ((seq * L + l) * H + head) * K + d0, y);
     }
   }
+}
+
+template <typename C, typename T>
+void launch_read(const PagedRows& a, const Pages& p, int64_t L, void* k, void* v, hipStream_t s) {
+  const int64_t groups = (L + kGroup - 1) / kGroup, spans = (groups + 3) / 4;
+  if (spans * p.H * a.S >= 2048)
+    hipLaunchKernelGGL((kv_read_kernel<C, T, 4>), dim3((unsigned)p.H, (unsigned)spans, (unsigned)a.S), dim3(256), 0, s, a, p,
+                       L, (T*)k, (T*)v);
+  else
+    hipLaunchKernelGGL((kv_read_kernel<C, T, 1>), dim3((unsigned)p.H, (unsigned)groups, (unsigned)a.S), dim3(256), 0, s, a, p,
+                       L, (T*)k, (T*)v);
 }
 
 int check_pages(const char* what, const void* k, const void* v, const void* k_scale, const void* v_scale, int dtype,
@@ -372,18 +385,11 @@ extern "C" int abacus_kv_read(const int32_t* page_table_SP, const int32_t* lengt
                    "kv_read: k and v must be there, and 16-byte aligned");
   PagedRows a{page_table_SP, nullptr, lengths, (int)S, (int)P, 0, __builtin_ctzll(page_size), (int)n_pages};
   Pages p{(void*)k_pages, (void*)v_pages, (uint8_t*)k_scale, (uint8_t*)v_scale, (int)H, (int)K};
-  const dim3 grid((unsigned)H, (unsigned)((L + kGroup * kSpan - 1) / (kGroup * kSpan)), (unsigned)S);
   hipStream_t s = (hipStream_t)stream;
-  if (held == ABACUS_E4M3 && dtype == kBF16)
-    hipLaunchKernelGGL((kv_read_kernel<uint8_t, uint16_t>), grid, dim3(256), 0, s, a, p, L, (uint16_t*)k_SLHK,
-                       (uint16_t*)v_SLHK);
-  else if (held == ABACUS_E4M3)
-    hipLaunchKernelGGL((kv_read_kernel<uint8_t, float>), grid, dim3(256), 0, s, a, p, L, (float*)k_SLHK, (float*)v_SLHK);
-  else if (dtype == kBF16)
-    hipLaunchKernelGGL((kv_read_kernel<uint16_t, uint16_t>), grid, dim3(256), 0, s, a, p, L, (uint16_t*)k_SLHK,
-                       (uint16_t*)v_SLHK);
-  else
-    hipLaunchKernelGGL((kv_read_kernel<float, float>), grid, dim3(256), 0, s, a, p, L, (float*)k_SLHK, (float*)v_SLHK);
+  if (held == ABACUS_E4M3 && dtype == kBF16) launch_read<uint8_t, uint16_t>(a, p, L, k_SLHK, v_SLHK, s);
+  else if (held == ABACUS_E4M3) launch_read<uint8_t, float>(a, p, L, k_SLHK, v_SLHK, s);
+  else if (dtype == kBF16) launch_read<uint16_t, uint16_t>(a, p, L, k_SLHK, v_SLHK, s);
+  else launch_read<float, float>(a, p, L, k_SLHK, v_SLHK, s);
   ABACUS_CHECK_LAUNCH("kv_read");
   return 0;
 }
