@@ -25,6 +25,7 @@ namespace abacus {
 namespace {
 
 constexpr int kFewPieces = 2048;   // pieces the work of a launch is cut into, about
+constexpr int kWavesOf16 = 4;      // waves of a block of 16 rows
 constexpr int kFewJoined = 16;     // pieces that a wave joins for several rows at once
 constexpr int kChunkPieces = 512;  // (of the chunk kernel's: two work-groups a CU)
 
@@ -70,6 +71,12 @@ __device__ inline pa_u32x4 codes_f32(uint32_t w, float s) {
   r[2] = f32_bits(hi[0] * s);
   r[3] = f32_bits(hi[1] * s);
   return r;
+}
+
+// What a part with maximum m and sum l weighs where the largest maximum is `top`: nothing if it
+// has seen nothing, and NaN stays.
+__device__ inline float weight_of(float m, float l, float top) {
+  return m == -__builtin_inff() ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - top);
 }
 
 // One wave's tile.  Q: uint16_t (bf16 products) or float (fp32 products); Cd: whether the
@@ -122,15 +129,16 @@ struct Tile {
 };
 
 // A block: the rows of one unit and key head against one piece of its keys, the
-// tiles dealt out to its four waves.
+// tiles dealt out to its waves.
+constexpr int few_waves(int QT) { return QT == 1 ? kWavesOf16 : 4; }
 template <typename Q, bool Cd, int KD, bool Full, int QT>
-__global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 : 1)) void paged_few_kernel(PagedArgs p) {
+__global__ __launch_bounds__(64 * few_waves(QT), QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 : 1)) void paged_few_kernel(PagedArgs p) {
   using TileT = Tile<Q, Cd, KD, Full>;
   constexpr bool kBf = TileT::kBf;
   constexpr int R = 16 * QT, ND = TileT::ND, NS = TileT::NS, NT = TileT::NT, KG = TileT::KG, KT = TileT::KT;
-  constexpr int kPitch = KD + 4;  // floats of a row's output in LDS
-  __shared__ __attribute__((aligned(16))) float merged[4][R][kPitch];
-  __shared__ float stat_m[4][R], stat_l[4][R];
+  constexpr int NW = few_waves(QT), kPitch = KD + 4;  // waves; floats of a row's output in LDS
+  __shared__ __attribute__((aligned(16))) float merged[NW][R][kPitch];
+  __shared__ float stat_m[NW][R], stat_l[NW][R];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4;
   const int item = blockIdx.x / p.Hk, kh = blockIdx.x % p.Hk, G = p.G, K = p.K;
@@ -142,7 +150,7 @@ __global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 :
     const int rest = p.a.T - (end - first), items = gridDim.x / p.Hk;
     for (int r = item; r < rest; r += items) {
       Q* row = (Q*)p.o + ((int64_t)(r < first ? r : end + r - first) * p.H + kh * G) * K;
-      for (int d = tid; d < G * K; d += 256) row[d] = from_f32<Q>(0.f);
+      for (int d = tid; d < G * K; d += 64 * NW) row[d] = from_f32<Q>(0.f);
     }
   };
   Item w;
@@ -413,31 +421,31 @@ __global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 :
   // (page numbers are read two tiles ahead, as the loads of a tile wait for them)
   int tile = t0 + wave;
   if (tile < t1) {
-    Ids then = ids_of(min(tile + 4, t1 - 1));
+    Ids then = ids_of(min(tile + NW, t1 - 1));
     here = place(tile, ids_of(tile));
     x.load_k(p, here.k, here.ko, lane);
     x.load_v(p, here.v, here.vo, lane);
     // every row sees all of these: the next tile's keys are on their way while this one's
     // scores are weighed, its values while the next one's scores are formed
     while (tile * KT + KT <= least) {
-      const bool more = tile + 4 < t1;
-      const Place next = place(tile + 4, then);
-      then = ids_of(min(tile + 8, t1 - 1));
+      const bool more = tile + NW < t1;
+      const Place next = place(tile + NW, then);
+      then = ids_of(min(tile + 2 * NW, t1 - 1));
       step(tile, std::false_type{}, [&]() __attribute__((always_inline)) {
         if (more) x.load_k(p, next.k, next.ko, lane);
       });
       if (more) x.load_v(p, next.v, next.vo, lane);
       here = next;
-      tile += 4;
+      tile += NW;
       if (!more) break;
     }
     // the others, one at a time: their masks cost registers that the loop above would lack
     while (tile < t1) {
       step(tile, std::true_type{}, [] {});
-      tile += 4;
+      tile += NW;
       if (tile < t1) {
         here = place(tile, then);
-        then = ids_of(min(tile + 4, t1 - 1));
+        then = ids_of(min(tile + NW, t1 - 1));
         x.load_k(p, here.k, here.ko, lane);
         x.load_v(p, here.v, here.vo, lane);
       }
@@ -458,17 +466,16 @@ __global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 :
   }
   __syncthreads();
   float* part = p.part + (int64_t)blockIdx.x * R * (K + 2);
-  for (int e = tid; e < rows * (K / 4); e += 256) {
+  for (int e = tid; e < rows * (K / 4); e += 64 * NW) {
     const int m = e / (K / 4), d = e % (K / 4) * 4;
     float top = stat_m[0][m];
 #pragma unroll
-    for (int v = 1; v < 4; ++v) top = fmaxf(top, stat_m[v][m]);
+    for (int v = 1; v < NW; ++v) top = fmaxf(top, stat_m[v][m]);
     float l = 0.f;
     pa_f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const float f = stat_m[v][m] == -__builtin_inff() ? (stat_l[v][m] == 0.f ? 0.f : 1.f)
-                                                        : __builtin_amdgcn_exp2f(stat_m[v][m] - top);
+    for (int v = 0; v < NW; ++v) {
+      const float f = weight_of(stat_m[v][m], stat_l[v][m], top);
       l += f * stat_l[v][m];
       o += f * *reinterpret_cast<const pa_f32x4*>(&merged[v][m][d]);
     }
@@ -485,10 +492,9 @@ __global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 :
   clear_rest();
 }
 
-// Joins the pieces of the units that were cut: blockIdx (unit and key head, every how many
-// rows), a wave per row.  K / 4 lanes take a piece's row, 64 / (K / 4) pieces at a time, each lane four of
-// them in flight; with one thread for all the pieces of its four dims a row of 128 pieces
-// took 100 us, now 6.
+// Joins the pieces of the units that were cut, K / 4 lanes to a row of a piece.  blockIdx: unit
+// and key head, and the first of the block's rows.  (With one thread for all the pieces of its
+// four dims a row of 128 pieces took 100 us, with one wave 19.)
 template <typename Q, int R>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = p.K, lanes = K / 4;
@@ -517,7 +523,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
       for (int i = 0; i < split; ++i) {
         const float pm = part[i * pitch + R * K + m], pl = part[i * pitch + R * K + R + m];
         const pa_f32x4 x = *reinterpret_cast<const pa_f32x4*>(part + i * pitch + (int64_t)m * K + d);
-        const float f = pm == -__builtin_inff() ? (pl == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(pm - top);
+        const float f = weight_of(pm, pl, top);
         l += f * pl;
         if (f != 0.f) o += f * x;  // (an empty piece weighs nothing)
       }
@@ -525,27 +531,30 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
     }
     return;
   }
-  for (int m = blockIdx.y * 4 + wave; m < rows; m += gridDim.y * 4) {
-    float top = -__builtin_inff();
-    for (int i = lane; i < split; i += 64) top = fmaxf(top, part[i * pitch + R * K + m]);
+  // a row at a time, its pieces dealt out to the waves in runs
+  __shared__ float wave_top[4], wave_l[4];
+  __shared__ __attribute__((aligned(16))) float wave_o[4][128];
+  const int sub = lane / lanes, subs = 64 / lanes, d = lane % lanes * 4;
+  const int run = (split + 3) / 4, begin = min(wave * run, split), end = min(begin + run, split);
+  for (int m = blockIdx.y; m < rows; m += gridDim.y) {
+    float top = -__builtin_inff(), l = 0.f;
+    for (int i = begin + lane; i < end; i += 64) top = fmaxf(top, part[i * pitch + R * K + m]);
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    const int sub = lane / lanes, subs = 64 / lanes, d = lane % lanes * 4;
-    float l = 0.f;
     pa_f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int i0 = 0; i0 < split; i0 += 64) {
+    for (int i0 = begin; i0 < end; i0 += 64) {
       float f = 0.f;
-      if (i0 + lane < split) {
+      if (i0 + lane < end) {
         const float pm = part[(i0 + lane) * pitch + R * K + m], pl = part[(i0 + lane) * pitch + R * K + R + m];
-        f = pm == -__builtin_inff() ? (pl == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(pm - top);
+        f = weight_of(pm, pl, top);
         l += f * pl;
       }
-      const int n = min(64, split - i0);
-      for (int j0 = 0; j0 < n; j0 += 4 * subs) {
-        pa_f32x4 x[4];
-        float w[4];
+      const int n = min(64, end - i0);
+      for (int j0 = 0; j0 < n; j0 += 8 * subs) {
+        pa_f32x4 x[8];
+        float w[8];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 8; ++c) {
           const int j = j0 + c * subs + sub;
           w[c] = __shfl(f, min(j, 63), 64);
           const bool in = j < n && sub < subs;
@@ -553,7 +562,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
           x[c] = *reinterpret_cast<const pa_f32x4*>(part + (i0 + (in ? j : 0)) * pitch + (int64_t)m * K + d);
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 8; ++c)
           if (w[c] != 0.f) o += w[c] * x[c];  // (an empty piece weighs nothing)
       }
     }
@@ -563,7 +572,23 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
     for (int j = 1; j < subs; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) sum[e] += __shfl(o[e], (lane + j * lanes) & 63, 64);
-    if (sub == 0) store_row4<Q>(p, r, kh, local * R + m, d, sum, l);
+    if (sub == 0) *reinterpret_cast<pa_f32x4*>(&wave_o[wave][d]) = sum;
+    if (lane == 0) wave_top[wave] = top, wave_l[wave] = l;
+    __syncthreads();
+    if (threadIdx.x < lanes) {
+      float all = wave_top[0];
+#pragma unroll
+      for (int v = 1; v < 4; ++v) all = fmaxf(all, wave_top[v]);
+      l = 0.f, o = pa_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float f = weight_of(wave_top[v], wave_l[v], all);
+        l += f * wave_l[v];
+        if (f != 0.f) o += f * *reinterpret_cast<const pa_f32x4*>(&wave_o[v][d]);
+      }
+      store_row4<Q>(p, r, kh, local * R + m, d, o, l);
+    }
+    __syncthreads();
   }
 }
 
@@ -571,7 +596,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs p) {
 struct Part {
   int R;          // rows of a unit, 0: no launch
   int over, upto; // the sequences it takes, by their rows of a key head
-  int target;     // pieces
+  int target, least;  // pieces, and tiles of one at least
   int64_t units, items;  // at most
   bool cuts;      // whether a unit can be cut
   int64_t floats(int64_t Hk, int64_t K) const { return cuts ? items * Hk * R * (K + 2) : 0; }
@@ -583,50 +608,57 @@ struct Plan {
   Part few, many;
 };
 
-Part part_of(int R, int64_t over, int64_t upto, int target, int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G,
+Part part_of(int R, int64_t over, int64_t upto, int target, int least, int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G,
              int64_t Hk) {
   Part n;
-  n.R = R, n.over = (int)over, n.upto = (int)upto, n.target = target;
-  n.units = std::min(T * G, T * G / R + std::min(S, T));
-  const int64_t tiles = (P * page_size + kTile - 1) / kTile, most = (tiles + kLeast - 1) / kLeast;
+  n.R = R, n.over = (int)over, n.upto = (int)upto, n.target = target, n.least = least;
+  // a sequence of this launch has more than `over` rows; at most R of them are one unit
+  const int64_t seqs = std::min(std::min(S, T), T * G / (over + 1) + (over == 0 ? T : 0));
+  n.units = upto <= R ? seqs : std::min(T * G, T * G / R + seqs);
+  const int64_t tiles = (P * page_size + kTile - 1) / kTile, most = (tiles + least - 1) / least;
   n.cuts = most > 1;
   n.items = std::min(n.units * most, n.units + (target + Hk - 1) / Hk);
   return n;
 }
 
 Plan plan_of(int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G, int64_t Hk, int64_t K, int dtype,
-             int64_t max_new) {
+             int held, int64_t max_new) {
   constexpr int64_t kAll = 0x7fffffff;
   const int64_t rows = std::min(T, max_new) * G;
+  // a piece of a quarter of a megabyte, 256 to 1024 keys: less and its block's beginning and the
+  // join take longer than its keys (700 bf16 tokens in one piece 9 us, in two 14)
+  const int64_t tile = 2 * kTile * K * (held == ABACUS_E4M3 ? 1 : held == kBF16 ? 2 : 4);
+  const int least = (int)std::min<int64_t>(std::max<int64_t>((256 << 10) / tile, 4), 16);
   const bool chunks = dtype == kBF16 && (K == 64 || K == 128);
   Plan n;
   n.many.R = 0, n.many.cuts = false;
   if (rows <= 32 || !chunks) {
-    n.few = part_of(rows <= 16 ? 16 : 32, 0, kAll, kFewPieces, T, S, P, page_size, G, Hk);
+    n.few = part_of(rows <= 16 ? 16 : 32, 0, kAll, kFewPieces, least, T, S, P, page_size, G, Hk);
   } else {
     const int few = G <= 16 ? 16 : 32;
-    n.few = part_of(few, 0, few, kFewPieces, T, S, P, page_size, G, Hk);
-    n.many = part_of(kChunkRows, few, kAll, kChunkPieces, T, S, P, page_size, G, Hk);
+    n.few = part_of(few, 0, few, kFewPieces, least, T, S, P, page_size, G, Hk);
+    n.many = part_of(kChunkRows, few, kAll, kChunkPieces, 16, T, S, P, page_size, G, Hk);
   }
   return n;
 }
 
 template <typename Q, bool Cd, int QT>
 void launch_few(const PagedArgs& p, unsigned blocks, hipStream_t s) {
-  if (p.K == 64) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 64, true, QT>), dim3(blocks), dim3(256), 0, s, p);
-  else if (p.K == 128) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 128, true, QT>), dim3(blocks), dim3(256), 0, s, p);
-  else if (p.K < 64) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 64, false, QT>), dim3(blocks), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 128, false, QT>), dim3(blocks), dim3(256), 0, s, p);
+  if (p.K == 64) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 64, true, QT>), dim3(blocks), dim3(64 * few_waves(QT)), 0, s, p);
+  else if (p.K == 128) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 128, true, QT>), dim3(blocks), dim3(64 * few_waves(QT)), 0, s, p);
+  else if (p.K < 64) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 64, false, QT>), dim3(blocks), dim3(64 * few_waves(QT)), 0, s, p);
+  else hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 128, false, QT>), dim3(blocks), dim3(64 * few_waves(QT)), 0, s, p);
 }
 
 template <typename Q>
 int launch(PagedArgs p, const Plan& n, bool codes, float* ws, int64_t rows, hipStream_t s) {
   auto set = [&](const Part& part, float* at) {
-    p.over = part.over, p.upto = part.upto, p.target = part.target, p.part = at;
+    p.over = part.over, p.upto = part.upto, p.target = part.target, p.least = part.least, p.part = at;
     return (unsigned)(part.items * p.Hk);
   };
   auto join_grid = [&](const Part& part) {
-    return dim3((unsigned)(part.units * p.Hk), (unsigned)((std::min<int64_t>(part.R, std::min<int64_t>(rows, 16)) + 3) / 4));
+    const int64_t at_once = std::min<int64_t>(std::min<int64_t>(part.R, rows), 16);
+    return dim3((unsigned)(part.units * p.Hk), (unsigned)(part.units * p.Hk < 128 ? at_once : (at_once + 3) / 4));
   };
   const unsigned blocks = set(n.few, ws);
   if (n.few.R == 16) codes ? launch_few<Q, true, 1>(p, blocks, s) : launch_few<Q, false, 1>(p, blocks, s);
@@ -653,10 +685,10 @@ int launch(PagedArgs p, const Plan& n, bool codes, float* ws, int64_t rows, hipS
 
 using namespace abacus;
 
-extern "C" int64_t abacus_paged_attention_ws_bytes(int64_t T, int64_t H, int64_t Hk, int64_t K, int dtype, int64_t S,
-                                                   int64_t P, int64_t page_size, int64_t max_new) {
+extern "C" int64_t abacus_paged_attention_ws_bytes(int64_t T, int64_t H, int64_t Hk, int64_t K, int dtype, int held,
+                                                   int64_t S, int64_t P, int64_t page_size, int64_t max_new) {
   if (T < 1 || Hk < 1 || H % Hk != 0) return 0;
-  const Plan n = plan_of(T, S, P, page_size, H / Hk, Hk, K, dtype, max_new);
+  const Plan n = plan_of(T, S, P, page_size, H / Hk, Hk, K, dtype, held, max_new);
   return (n.few.floats(Hk, K) + n.many.floats(Hk, K)) * 4;
 }
 
@@ -682,7 +714,7 @@ extern "C" int abacus_paged_attention(const void* q_THK, int64_t T, int64_t H, i
   ABACUS_CHECK_ARG(((uintptr_t)q_THK | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)k_scale |
                     (uintptr_t)v_scale | (uintptr_t)o_THK | (uintptr_t)ws) % 16 == 0,
                    "paged_attention: tensors must be 16-byte aligned");
-  const Plan n = plan_of(T, S, P, page_size, H / Hk, Hk, K, dtype, max_new);
+  const Plan n = plan_of(T, S, P, page_size, H / Hk, Hk, K, dtype, held, max_new);
   const int64_t need = (n.few.floats(Hk, K) + n.many.floats(Hk, K)) * 4;
   ABACUS_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "paged_attention: workspace of %lld bytes, need %lld",
                    (long long)ws_bytes, (long long)need);

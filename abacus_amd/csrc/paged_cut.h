@@ -4,7 +4,7 @@
 // unit's keys are cut into `split` pieces of whole 64-key tiles where there are too few
 // units for the GPU, and each piece gives its rows' maximum, sum and unscaled output,
 // which a second kernel joins in order.  The piece length is the same for the whole
-// launch: its (unit, key head, tile)s spread over `target` pieces, at least kLeast tiles
+// launch: its (unit, key head, tile)s spread over `target` pieces, at least `least` tiles
 // each.  The units are found from the device's lengths by a scan (paged_rows.h), a launch
 // being sized for the most there can be.  A launch takes the sequences whose rows of a key
 // head number more than `over` and at most `upto`.
@@ -15,7 +15,6 @@
 namespace abacus {
 
 constexpr int kTile = 64;   // keys of a tile
-constexpr int kLeast = 16;  // tiles of a piece, at least
 
 struct PagedArgs {
   PagedRows a;
@@ -27,7 +26,7 @@ struct PagedArgs {
   float scale_log2;
   int zero_rest;   // rows of no sequence: 0, or left as they are
   int over, upto;  // rows of a key head that a sequence of this launch has
-  int target;
+  int target, least;
 };
 
 // Units of a sequence in this launch.
@@ -45,7 +44,7 @@ __device__ inline int piece_tiles(const PagedArgs& p, const SeqScan& scan) {
     return (float)units_of<R>(p, r) * (float)((r.len + kTile - 1) / kTile);
   });
   const int want = (p.target + p.Hk - 1) / p.Hk;
-  return max(kLeast, (int)fminf(ceilf(total * 1.001f / (float)want), 1e9f));
+  return max(p.least, (int)fminf(ceilf(total * 1.001f / (float)want), 1e9f));
 }
 
 // Pieces of each of a sequence's units.

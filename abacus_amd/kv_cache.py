@@ -225,7 +225,7 @@ class KVPages:
         if out is None:
             out = torch.empty_like(q)
         most = max(1, T) if rows.max_new is None else rows.max_new
-        nbytes = _attention_ws_bytes(T, H, self.n_heads, K, code, *rows._sizes, self.page_size, most)
+        nbytes = _attention_ws_bytes(T, H, self.n_heads, K, code, self._args[2], *rows._sizes, self.page_size, most)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
         _call(self.device, "abacus_paged_attention", q.data_ptr(), T, H, self.n_heads, K, code, *self._rows_args(rows), scale,
               most, zero_rest, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)

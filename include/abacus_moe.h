@@ -453,8 +453,8 @@ int abacus_kv_read(const int32_t* page_table_SP, const int32_t* lengths, int64_t
  * caller knows (T otherwise); it chooses the kernels and changes no result beyond
  * rounding.  zero_rest: rows of no sequence become 0 (otherwise they are left as they
  * are).  ws: device workspace of abacus_paged_attention_ws_bytes bytes. */
-int64_t abacus_paged_attention_ws_bytes(int64_t T, int64_t H, int64_t Hk, int64_t K, int dtype, int64_t S, int64_t P,
-                                        int64_t page_size, int64_t max_new);
+int64_t abacus_paged_attention_ws_bytes(int64_t T, int64_t H, int64_t Hk, int64_t K, int dtype, int held, int64_t S,
+                                        int64_t P, int64_t page_size, int64_t max_new);
 int abacus_paged_attention(const void* q_THK, int64_t T, int64_t H, int64_t Hk, int64_t K, int dtype,
                            const int32_t* page_table_SP, const int32_t* query_start, const int32_t* lengths,
                            int64_t S, int64_t P, int64_t page_size, int64_t n_pages, int held, const void* k_pages,
