@@ -26,7 +26,7 @@ template <int HD>
 struct ChunkLds {
   char k[kStages][kTile * HD * 2];
   char v[kStages][HD * kTile * 2];
-  uint8_t vs[kStages][kTile];
+  float vs[kStages][kTile];  // what the value codes of a key are to be multiplied by
 };
 
 // The pages of a tile's four 16-key groups, the same for the whole block.
@@ -96,8 +96,19 @@ struct Codes {
     }
   }
   // `left`: keys of the tile that exist (past them there may be anything in V: 0)
-  __device__ inline void store(char* kt, char* vt, uint8_t* scales, int left) const {
+  __device__ inline void store(char* kt, char* vt, float* scales, int left) {
     const int tid = threadIdx.x;
+    if (left < kTile) {
+      const int j = tid & 3;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int there = min(max(left - 16 * j - 4 * e, 0), 4);
+        const uint32_t mask = there == 4 ? ~0u : (1u << (8 * there)) - 1u;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i][e] &= mask;
+        vs[e] &= mask;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int row = (i * 256 + tid) / (HD / 16), c = tid % (HD / 16), d = (i * 256 + tid) / 4, j = tid & 3;
@@ -108,25 +119,16 @@ struct Codes {
         Vec16 w;
         w.w[0] = a.x, w.w[1] = a.y, w.w[2] = b.x, w.w[3] = b.y;
         *reinterpret_cast<Vec16*>(kt + tile_off<HD>(row, 2 * c + h)) = w;
-        uint32_t x[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int there = min(max(left - 16 * j - 8 * h - 4 * e, 0), 4);
-          x[e] = v[i][2 * h + e] & (there == 4 ? ~0u : (1u << (8 * there)) - 1u);
-        }
-        const uint2 y = codes_bf16(x[0], 1.f), z = codes_bf16(x[1], 1.f);
+        const uint2 y = codes_bf16(v[i][2 * h], 1.f), z = codes_bf16(v[i][2 * h + 1], 1.f);
         w.w[0] = y.x, w.w[1] = y.y, w.w[2] = z.x, w.w[3] = z.y;
         *reinterpret_cast<Vec16*>(vt + tile_off<64>(d, 2 * j + h)) = w;
       }
     }
     if (tid < 4) {
-      U4 w;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int there = min(max(left - 16 * tid - 4 * e, 0), 4);
-        w[e] = vs[e] & (there == 4 ? ~0u : (1u << (8 * there)) - 1u);
-      }
-      *reinterpret_cast<U4*>(scales + 16 * tid) = w;
+      for (int e = 0; e < 4; ++e)
+        *reinterpret_cast<float4*>(scales + 16 * tid + 4 * e) = make_float4(byte_scale(vs[e], 0), byte_scale(vs[e], 1),
+                                                                            byte_scale(vs[e], 2), byte_scale(vs[e], 3));
     }
   }
 };
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedArgs p) {
   float m_run = -__builtin_inff(), l_run = 0.f;
   const int key_row = (lane & 0x13) | (lane & 4) << 1 | (lane & 8) >> 1;  // bits 2 and 3 of l % 32 exchanged
 
-  auto step = [&](const char* kt, const char* vt, const uint8_t* scales, int key0, int bad,
+  auto step = [&](const char* kt, const char* vt, const float* scales, int key0, int bad,
                   auto edge_t) __attribute__((always_inline)) {
     constexpr bool edge = decltype(edge_t)::value;
     attn_f32x16 s[2];
@@ -250,9 +252,11 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = s[c >> 1][8 * (c & 1) + e];
       if constexpr (Cd) {
-        const uint2 b = *reinterpret_cast<const uint2*>(scales + 16 * c + 8 * h);
+        const float4 a = *reinterpret_cast<const float4*>(scales + 16 * c + 8 * h);
+        const float4 b = *reinterpret_cast<const float4*>(scales + 16 * c + 8 * h + 4);
+        const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= byte_scale(e < 4 ? b.x : b.y, e & 3);  // exact: powers of two
+        for (int e = 0; e < 8; ++e) x[e] *= f[e];  // exact: powers of two
       }
       Vec16 pf;
 #pragma unroll

@@ -97,6 +97,50 @@ def test_attention(dtype, held, H, G, K, page, plan):
     _check(pages, plan, known, k, v, q, pages.attend(q, known, scale=0.3), held, 0.3)
 
 
+@pytest.mark.parametrize("held", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("H,G,K,page,plan", [
+    (1, 1, 64, 16, [(200, 2500), (1, 700), (17, 17)]),
+    (1, 3, 128, 64, [(150, 3000), (2, 90)]),
+    (2, 1, 128, 256, [(129, 129), (300, 1400), (0, 60), (1, 1)]),
+    (2, 8, 64, 32, [(31, 2100), (128, 128)]),
+])
+def test_chunks(held, H, G, K, page, plan):
+    """Chunks over what was cached before: units that are cut and units that are not, partly filled ones, and a
+    decode step beside them; padded rows behind."""
+    pages, rows, k, v, g = _filled(plan, H, K, page, torch.bfloat16, held)
+    T = sum(n for n, _ in plan)
+    q = torch.randn(T + 5, H * G, K, device="cuda", generator=g).bfloat16()
+    o = pages.attend(q, rows)
+    assert not o[T:].any()
+    _check(pages, plan, rows, k, v, q[:T], o[:T], held)
+    kept = torch.full_like(q, 7.0)
+    pages.attend(q, rows, out=kept)
+    assert torch.equal(kept[:T], o[:T]) and (kept[T:] == 7.0).all()
+
+
+@pytest.mark.parametrize("held", [torch.bfloat16, E4M3])
+def test_a_wrong_hint_changes_no_result(held):
+    """max_new says one row and there are many: other kernels, the same attention."""
+    plan = [(1, 40), (70, 900), (3, 2000)]
+    pages, rows, k, v, g = _filled(plan, 2, 64, 16, torch.bfloat16, held, max_new=1)
+    q = torch.randn(74, 4, 64, device="cuda", generator=g).bfloat16()
+    _check(pages, plan, rows, k, v, q, pages.attend(q, rows), held)
+
+
+@pytest.mark.parametrize("held", [torch.bfloat16, E4M3])
+def test_a_chunk_with_pages_outside_the_pool(held):
+    """Rows that see a position in no page are NaN, the others are not touched by it."""
+    plan = [(200, 600)]
+    pages, rows, k, v, g = _filled(plan, 1, 128, 32, torch.bfloat16, held)
+    q = torch.randn(200, 2, 128, device="cuda", generator=g).bfloat16()
+    whole = pages.attend(q, rows)
+    rows.page_table_SP[0, 16] = -1  # positions 512 to 543: rows 112 on see them
+    o = pages.attend(q, rows)
+    assert torch.equal(o[:112], whole[:112]) and torch.isnan(o[112:]).all()
+    rows.page_table_SP[0, 3] = 1 << 30
+    assert torch.isnan(pages.attend(q, rows)).all()
+
+
 @pytest.mark.parametrize("dtype,held", KINDS)
 def test_long_context_is_cut_and_joined(dtype, held):
     plan = [(1, 9000), (2, 33), (1, 20001)]
@@ -117,11 +161,11 @@ def test_many_sequences():
 
 
 @pytest.mark.parametrize("dtype,held", KINDS)
-@pytest.mark.parametrize("plan", [[(1, 5), (3, 70), (1, 130)], [(100, 300)]])
-def test_what_a_row_does_not_see_does_not_reach_it(dtype, held, plan):
+@pytest.mark.parametrize("plan,K", [([(1, 5), (3, 70), (1, 130)], 64), ([(100, 300)], 64), ([(2, 9), (140, 140)], 128)])
+def test_what_a_row_does_not_see_does_not_reach_it(dtype, held, plan, K):
     """Pages full of NaN and infinities before the sequences are written; then a NaN and an infinity in the keys and
     values of the last token: only the rows that see it have them, dim by dim as the formula has."""
-    K, H = 64, 2
+    H = 2
     for fill in ((0x7f, 0xff) if held == E4M3 else (math.nan, math.inf)):
         pages, rows, k, v, g = _filled(plan, H, K, 32, dtype, held, fill=fill)
         T = sum(n for n, _ in plan)
@@ -151,8 +195,8 @@ def test_what_a_row_does_not_see_does_not_reach_it(dtype, held, plan):
         if n > 1:  # the others as if it were not there
             kk, vv = k[at:at + length].clone(), v[at:at + length].clone()
             kk[-1], vv[-1] = 0.0, 0.0
-            want, weight = pc.attention(q[first:first + n], pc.held(kk, held), pc.held(vv, held), 1 / 8)
-            most = pc.attention_bound(q[first:first + n], pc.held(kk, held), want, weight, 1 / 8)
+            want, weight = pc.attention(q[first:first + n], pc.held(kk, held), pc.held(vv, held), K ** -0.5)
+            most = pc.attention_bound(q[first:first + n], pc.held(kk, held), want, weight, K ** -0.5)
             assert ((o[first:first + n].double() - want).abs() <= most)[:-1].all()
         at, first = at + length, first + n
 
