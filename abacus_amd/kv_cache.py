@@ -405,7 +405,12 @@ class PagedKVCache:
     def rows(self, new: dict[int, int]) -> BatchRows:
         """The BatchRows of sequences whose last new[s] tokens are the call's."""
         width = max(1, max(len(self._pages[s]) for s in new))
-        table = torch.tensor([self._pages[s] + [0] * (width - len(self._pages[s])) for s in new], dtype=torch.int32)
-        start = torch.tensor([0, *new.values()]).cumsum(0).to(torch.int32)
-        lengths = torch.tensor([self._lengths[s] for s in new], dtype=torch.int32)
-        return BatchRows(*(t.to(self.device) for t in (table, start, lengths)), max_new=max(1, max(new.values())))
+        table = [page for s in new for page in self._pages[s] + [0] * (width - len(self._pages[s]))]
+        lengths = [self._lengths[s] for s in new]
+        start = [0]
+        for n in new.values():
+            start.append(start[-1] + n)
+        S = len(lengths)
+        every = torch.tensor(table + start + lengths, dtype=torch.int32).to(self.device)  # one copy
+        return BatchRows(every[:S * width].view(S, width), every[S * width:S * width + S + 1], every[S * width + S + 1:],
+                         max_new=max(1, max(new.values())))

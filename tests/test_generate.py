@@ -136,3 +136,58 @@ def test_bf16_cached_forward_on_the_gpu(held):
     err = lambda x: float((x - want).norm() / want.norm())
     assert torch.isfinite(got).all()
     assert held == E4M3 or err(got) <= 2 * err(whole)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,held", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                        (torch.bfloat16, E4M3)])
+def test_captured_step_of_the_whole_path(dtype, held):
+    """A decoding step captured once (cached forward, verification of the drafts): every replay gives what the eager
+    calls give, with eager work and synchronisation between, on a second cache in step with the first."""
+    from abacus_amd.kv_cache import BatchRows
+    from abacus_amd.speculative import verify_drafts
+
+    model = _model(head_dim=64, device="cuda", dtype=dtype)
+    g = torch.Generator().manual_seed(3)
+    caches = [PagedKVCache(2, 40, 16, 2, 64, dtype=held, device="cuda") for _ in range(2)]
+    S, n = 3, 4
+    seqs = [caches[0].add() for _ in range(S)]
+    prompts = [torch.randint(0, 50, (m,), generator=g) for m in (5, 30, 61)]
+    rows = caches[0].extend({s: p.numel() for s, p in zip(seqs, prompts)})
+    for cache in caches:
+        model.forward_cached(torch.cat(prompts).cuda(), cache, rows)
+    tokens = torch.zeros(S * n, dtype=torch.int64, device="cuda")
+    uniforms = torch.zeros(S * n, 2, device="cuda")
+    static = BatchRows(torch.zeros(S, 10, dtype=torch.int32, device="cuda"),
+                       torch.arange(0, S * n + 1, n, dtype=torch.int32, device="cuda"),
+                       torch.full((S,), n, dtype=torch.int32, device="cuda"), max_new=n)
+
+    def step(cache):
+        logits = model.forward_cached(tokens, cache, static)
+        return logits, *verify_drafts(logits, tokens, static.query_start, uniforms, temperature=0.9)
+
+    def load(rows):
+        static.page_table_SP[:, :rows.page_table_SP.shape[1]] = rows.page_table_SP
+        static.lengths.copy_(rows.lengths)
+        tokens.copy_(torch.randint(0, 50, (S * n,), generator=g))
+        uniforms.copy_(torch.rand(S * n, 2, generator=g))
+
+    load(caches[0].extend({s: n for s in seqs}))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(caches[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(caches[0])
+    for _ in range(4):
+        graph.replay()
+        want = step(caches[1])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        kept = {s: caches[0].length(s) - n + 1 + int(a) for s, a in zip(seqs, want[1])}
+        for s, length in kept.items():
+            caches[0].truncate(s, length)
+        load(caches[0].extend({s: n for s in seqs}))
