@@ -5,8 +5,7 @@
 // One pass over the keys with the running maximum and sum of the softmax in fp32.
 //
 // How the work is cut over units of rows and pieces of keys is paged_cut.h's; sequences with
-// many rows go to paged_chunk.hip's kernel, the others, and every type and head dim that
-// one does not take, to this file's.
+// many bf16 rows go to paged_chunk.hip's kernel, the others and all fp32 ones to this file's.
 //
 // In registers (v_mfma_f32_16x16x32_bf16: lane l gives A[l % 16][8 (l / 16) .. +7] and
 // B[8 (l / 16) .. +7][l % 16], and holds D[4 (l / 16) + r][l % 16] in register r; the fp32
@@ -629,7 +628,7 @@ Plan plan_of(int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G, int6
   // join take longer than its keys (700 bf16 tokens in one piece 9 us, in two 14)
   const int64_t tile = 2 * kTile * K * (held == ABACUS_E4M3 ? 1 : held == kBF16 ? 2 : 4);
   const int least = (int)std::min<int64_t>(std::max<int64_t>((256 << 10) / tile, 4), 16);
-  const bool chunks = dtype == kBF16 && (K == 64 || K == 128);
+  const bool chunks = dtype == kBF16;
   Plan n;
   n.many.R = 0, n.many.cuts = false;
   if (rows <= 32 || !chunks) {

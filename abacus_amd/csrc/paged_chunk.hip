@@ -1,5 +1,7 @@
-// Attention of a chunk of new tokens over a paged cache: bf16 queries, head dim 64 or
-// 128, a cache in bf16 or e4m3.  Work and its cut: paged_cut.h.
+// Attention of a chunk of new tokens over a paged cache: bf16 queries, a cache in bf16 or
+// e4m3.  Work and its cut: paged_cut.h.  The tiles are laid out for head dim 64 or 128 (HD);
+// another one (K < HD, not Full) leaves their last dims 0, which are cleared once and not
+// loaded after.
 //
 // A work-group has 128 rows (token, query head) of one key head, 32 to a wave, and walks
 // its piece's 64-key tiles with a running maximum and sum in fp32.  A tile of K and of V^T
@@ -55,26 +57,29 @@ __device__ inline T pick(const T (&x)[4], int j) {
 }
 
 // bf16 pages: 16 bytes a lane and instruction, straight into the swizzled tile.
-template <int HD>
+template <int HD, bool Full>
 __device__ inline void dma_tile(const PagedArgs& p, int kh, const Groups& g, int key0, char* kt, char* vt) {
-  const int in_page = (1 << p.a.shift) - 1;  // group j's slots begin at (key0 + 16 j) & in_page
   constexpr int CH = HD / 8;  // chunks of a key row
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), ps = p.a.shift;
+  const int K = Full ? HD : p.K;
+  const int in_page = (1 << ps) - 1;  // group j's slots begin at (key0 + 16 j) & in_page
 #pragma unroll
   for (int i = 0; i < HD / 32; ++i) {
     const int at = i * 256 + tid, row = at / CH, j = HD == 128 ? i : 2 * i + (wave >> 1);  // the row's group
     const int64_t slot = (((int64_t)pick(g.page, j) * p.Hk + kh) << ps) + ((key0 + 16 * j) & in_page) + (row & 15);
-    dma16((const uint16_t*)p.k + slot * HD + ((at % CH) ^ tile_swz<HD>(row)) * 8, kt + (i * 4 + wave) * 1024);
+    const int c = (at % CH) ^ tile_swz<HD>(row);
+    if (Full || c * 8 < K) dma16((const uint16_t*)p.k + slot * K + c * 8, kt + (i * 4 + wave) * 1024);
   }
   const int d0 = tid / 8, c = (tid % 8) ^ tile_swz<64>(d0);  // V^T rows d0 + 32 i: the swizzle is the same for all
   const int64_t page = (int64_t)pick(g.page, c >> 1) * p.Hk + kh;
-  const uint16_t* from = (const uint16_t*)p.v + ((page * HD + d0) << ps) + ((key0 + 8 * c) & in_page);
+  const uint16_t* from = (const uint16_t*)p.v + ((page * K + d0) << ps) + ((key0 + 8 * c) & in_page);
 #pragma unroll
-  for (int i = 0; i < HD / 32; ++i) dma16(from + ((int64_t)(32 * i) << ps), vt + (i * 4 + wave) * 1024);
+  for (int i = 0; i < HD / 32; ++i)
+    if (Full || d0 + 32 * i < K) dma16(from + ((int64_t)(32 * i) << ps), vt + (i * 4 + wave) * 1024);
 }
 
 // Codes: loaded while the tile before is used, made bf16 and stored after it.
-template <int HD>
+template <int HD, bool Full>
 struct Codes {
   static constexpr int N = HD / 64;  // 16-byte loads of a thread, of keys and of values
   typedef uint32_t U4 __attribute__((ext_vector_type(4)));
@@ -82,21 +87,22 @@ struct Codes {
   int ks[N];
   U4 vs;
   __device__ inline void load(const PagedArgs& p, int kh, const Groups& g, int key0) {
-    const int tid = threadIdx.x, ps = p.a.shift, in_page = (1 << ps) - 1;
+    const int tid = threadIdx.x, ps = p.a.shift, in_page = (1 << ps) - 1, K = Full ? HD : p.K;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int row = (i * 256 + tid) / (HD / 16), c = tid % (HD / 16);
       const int64_t slot = (((int64_t)pick(g.page, row >> 4) * p.Hk + kh) << ps) + ((key0 + row) & in_page);
-      k[i] = *reinterpret_cast<const U4*>((const uint8_t*)p.k + slot * HD + c * 16);
+      k[i] = *reinterpret_cast<const U4*>((const uint8_t*)p.k + slot * K + (Full || c * 16 < K ? c * 16 : 0));
       ks[i] = p.k_scale[slot];
       const int d = (i * 256 + tid) / 4, j = tid & 3;
       const int64_t page = (int64_t)pick(g.page, j) * p.Hk + kh;
-      v[i] = *reinterpret_cast<const U4*>((const uint8_t*)p.v + ((page * HD + d) << ps) + ((key0 + 16 * j) & in_page));
+      v[i] = *reinterpret_cast<const U4*>((const uint8_t*)p.v + ((page * K + (Full || d < K ? d : 0)) << ps) +
+                                           ((key0 + 16 * j) & in_page));
       if (i == 0) vs = *reinterpret_cast<const U4*>(p.v_scale + (page << ps) + ((key0 + 16 * j) & in_page));
     }
   }
   // `left`: keys of the tile that exist (past them there may be anything in V: 0)
-  __device__ inline void store(char* kt, char* vt, float* scales, int left) {
+  __device__ inline void store(char* kt, char* vt, float* scales, int left, int K) {
     const int tid = threadIdx.x;
     if (left < kTile) {
       const int j = tid & 3;
@@ -118,10 +124,10 @@ struct Codes {
         const uint2 a = codes_bf16(k[i][2 * h], s), b = codes_bf16(k[i][2 * h + 1], s);
         Vec16 w;
         w.w[0] = a.x, w.w[1] = a.y, w.w[2] = b.x, w.w[3] = b.y;
-        *reinterpret_cast<Vec16*>(kt + tile_off<HD>(row, 2 * c + h)) = w;
+        if (Full || c * 16 < K) *reinterpret_cast<Vec16*>(kt + tile_off<HD>(row, 2 * c + h)) = w;
         const uint2 y = codes_bf16(v[i][2 * h], 1.f), z = codes_bf16(v[i][2 * h + 1], 1.f);
         w.w[0] = y.x, w.w[1] = y.y, w.w[2] = z.x, w.w[3] = z.y;
-        *reinterpret_cast<Vec16*>(vt + tile_off<64>(d, 2 * j + h)) = w;
+        if (Full || d < K) *reinterpret_cast<Vec16*>(vt + tile_off<64>(d, 2 * j + h)) = w;
       }
     }
     if (tid < 4) {
@@ -137,11 +143,11 @@ __device__ inline bool not_finite(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
-template <bool Cd, int HD>
+template <bool Cd, int HD, bool Full>
 __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedArgs p) {
   __shared__ __attribute__((aligned(1024))) ChunkLds<HD> lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int item = blockIdx.x / p.Hk, kh = blockIdx.x % p.Hk, G = p.G;
+  const int item = blockIdx.x / p.Hk, kh = blockIdx.x % p.Hk, G = p.G, K = Full ? HD : p.K;
   Item w;
   if (!find_item<R>(p, item, w)) return;
 
@@ -151,10 +157,10 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedArgs p) {
   const int token = row / G, head = kh * G + row % G;
   const int vis = m < w.rows ? max(0, w.r.len - w.r.n + token + 1) : 0;
   const int seen = m0 < w.rows ? seen_of(w.r, w.row0 + min(m0 + 31, w.rows - 1), G) : 0;
-  const uint16_t* at = (const uint16_t*)p.q + ((int64_t)(w.r.first + token) * p.H + head) * HD;
+  const uint16_t* at = (const uint16_t*)p.q + ((int64_t)(w.r.first + token) * p.H + head) * K;
   Vec16 qf[HD / 16];
 #pragma unroll
-  for (int c = 0; c < HD / 16; ++c) qf[c] = ld16(at + 16 * c + 8 * h);
+  for (int c = 0; c < HD / 16; ++c) qf[c] = Full || 16 * c < K ? ld16(at + 16 * c + 8 * h) : zero16();
 
   attn_f32x16 acc[HD / 32];
 #pragma unroll
@@ -281,14 +287,18 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedArgs p) {
   // The ring: tile t is in stage t % 2; once it has landed everywhere (this thread's wait,
   // then the barrier, after which no wave still reads the other stage) the next is sent.
   if (w.t0 < w.t1) {
+    if constexpr (!Full) {
+      for (int i = tid; i < (int)sizeof(lds) / 16; i += 256) reinterpret_cast<Vec16*>(&lds)[i] = zero16();
+      __syncthreads();
+    }
     Groups next = groups_of(p, w.seq, w.t0 * kTile, w.seen);
     int bad = next.bad;
-    [[maybe_unused]] Codes<HD> codes;
+    [[maybe_unused]] Codes<HD, Full> codes;
     if constexpr (Cd) {
       codes.load(p, kh, next, w.t0 * kTile);
-      codes.store(lds.k[0], lds.v[0], lds.vs[0], w.seen - w.t0 * kTile);
+      codes.store(lds.k[0], lds.v[0], lds.vs[0], w.seen - w.t0 * kTile, K);
     } else {
-      dma_tile<HD>(p, kh, next, w.t0 * kTile, lds.k[0], lds.v[0]);
+      dma_tile<HD, Full>(p, kh, next, w.t0 * kTile, lds.k[0], lds.v[0]);
     }
     if (w.t0 + 1 < w.t1) next = groups_of(p, w.seq, (w.t0 + 1) * kTile, w.seen);
     auto turn = [&](int t, auto edge_t) __attribute__((always_inline)) {
@@ -298,13 +308,13 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedArgs p) {
       __syncthreads();
       if (more) {
         if constexpr (Cd) codes.load(p, kh, next, key0 + kTile);
-        else dma_tile<HD>(p, kh, next, key0 + kTile, lds.k[st ^ 1], lds.v[st ^ 1]);
+        else dma_tile<HD, Full>(p, kh, next, key0 + kTile, lds.k[st ^ 1], lds.v[st ^ 1]);
       }
       const int next_bad = next.bad;
       if (t + 2 < w.t1) next = groups_of(p, w.seq, key0 + 2 * kTile, w.seen);
       if (!decltype(edge_t)::value || key0 < seen) step(lds.k[st], lds.v[st], lds.vs[st], key0, bad, edge_t);
       if constexpr (Cd) {
-        if (more) codes.store(lds.k[st ^ 1], lds.v[st ^ 1], lds.vs[st ^ 1], w.seen - key0 - kTile);
+        if (more) codes.store(lds.k[st ^ 1], lds.v[st ^ 1], lds.vs[st ^ 1], w.seen - key0 - kTile, K);
       }
       bad = next_bad;
     };
@@ -316,32 +326,35 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(PagedArgs p) {
   }
   if (m >= w.rows) return;
   const float l = pair_sum(l_run);
-  float* part = p.part + (int64_t)blockIdx.x * R * (HD + 2);
+  float* part = p.part + (int64_t)blockIdx.x * R * (K + 2);
 #pragma unroll
   for (int t = 0; t < HD / 32; ++t)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const int d = 32 * t + 8 * g + 4 * h;
+      if (!Full && d >= K) continue;
       const float o[4] = {acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]};
-      if (w.split > 1) *reinterpret_cast<float4*>(part + m * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
+      if (w.split > 1) *reinterpret_cast<float4*>(part + m * K + d) = make_float4(o[0], o[1], o[2], o[3]);
       else store_row4<uint16_t>(p, w.r, kh, row, d, o, l);
     }
   if (w.split > 1 && h == 0) {
-    part[R * HD + m] = m_run;
-    part[R * HD + R + m] = l;
+    part[R * K + m] = m_run;
+    part[R * K + R + m] = l;
   }
 }
 
 }  // namespace
 
+template <bool Cd>
+static void launch_chunk_of(const PagedArgs& p, unsigned blocks, hipStream_t s) {
+  if (p.K == 64) hipLaunchKernelGGL((paged_chunk_kernel<Cd, 64, true>), dim3(blocks), dim3(256), 0, s, p);
+  else if (p.K == 128) hipLaunchKernelGGL((paged_chunk_kernel<Cd, 128, true>), dim3(blocks), dim3(256), 0, s, p);
+  else if (p.K < 64) hipLaunchKernelGGL((paged_chunk_kernel<Cd, 64, false>), dim3(blocks), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((paged_chunk_kernel<Cd, 128, false>), dim3(blocks), dim3(256), 0, s, p);
+}
+
 int launch_chunk(const PagedArgs& p, unsigned blocks, bool codes, hipStream_t s) {
-  if (p.K == 64) {
-    if (codes) hipLaunchKernelGGL((paged_chunk_kernel<true, 64>), dim3(blocks), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((paged_chunk_kernel<false, 64>), dim3(blocks), dim3(256), 0, s, p);
-  } else {
-    if (codes) hipLaunchKernelGGL((paged_chunk_kernel<true, 128>), dim3(blocks), dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((paged_chunk_kernel<false, 128>), dim3(blocks), dim3(256), 0, s, p);
-  }
+  codes ? launch_chunk_of<true>(p, blocks, s) : launch_chunk_of<false>(p, blocks, s);
   ABACUS_CHECK_LAUNCH("paged_attention (chunk)");
   return 0;
 }

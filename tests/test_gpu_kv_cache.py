@@ -103,6 +103,10 @@ def test_attention(dtype, held, H, G, K, page, plan):
     (1, 3, 128, 64, [(150, 3000), (2, 90)]),
     (2, 1, 128, 256, [(129, 129), (300, 1400), (0, 60), (1, 1)]),
     (2, 8, 64, 32, [(31, 2100), (128, 128)]),
+    (1, 2, 96, 16, [(150, 2000), (3, 3)]),
+    (2, 1, 16, 64, [(260, 700), (1, 50)]),
+    (1, 1, 112, 128, [(90, 90)]),
+    (1, 5, 48, 32, [(40, 1500)]),
 ])
 def test_chunks(held, H, G, K, page, plan):
     """Chunks over what was cached before: units that are cut and units that are not, partly filled ones, and a
@@ -161,7 +165,7 @@ def test_many_sequences():
 
 
 @pytest.mark.parametrize("dtype,held", KINDS)
-@pytest.mark.parametrize("plan,K", [([(1, 5), (3, 70), (1, 130)], 64), ([(100, 300)], 64), ([(2, 9), (140, 140)], 128)])
+@pytest.mark.parametrize("plan,K", [([(1, 5), (3, 70), (1, 130)], 64), ([(100, 300)], 64), ([(2, 9), (140, 140)], 128), ([(100, 300)], 80)])
 def test_what_a_row_does_not_see_does_not_reach_it(dtype, held, plan, K):
     """Pages full of NaN and infinities before the sequences are written; then a NaN and an infinity in the keys and
     values of the last token: only the rows that see it have them, dim by dim as the formula has."""
