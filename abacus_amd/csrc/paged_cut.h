@@ -6,8 +6,8 @@
 // which a second kernel joins in order.  The piece length is the same for the whole
 // launch: its (unit, key head, tile)s spread over `target` pieces, at least `least` tiles
 // each.  The units are found from the device's lengths by a scan (paged_rows.h), a launch
-// being sized for the most there can be.  A launch takes the sequences whose rows of a key
-// head number more than `over` and at most `upto`.
+// being sized for the most there can be.  Blocks of a kind take the sequences whose rows
+// of a key head number more than `over` and at most `upto`.
 #pragma once
 
 #include "paged_rows.h"
@@ -25,11 +25,11 @@ struct PagedArgs {
   int H, Hk, G, K;
   float scale_log2;
   int zero_rest;   // rows of no sequence: 0, or left as they are
-  int over, upto;  // rows of a key head that a sequence of this launch has
+  int over, upto;  // rows of a key head that a sequence of these blocks has
   int target, least;
 };
 
-// Units of a sequence in this launch.
+// Units of a sequence for blocks of this kind.
 template <int R>
 __device__ inline int units_of(const PagedArgs& p, const SeqRows& r) {
   const int rows = r.n * p.G;
@@ -112,8 +112,10 @@ __device__ inline uint2 codes_bf16(uint32_t w, float s) {
 // 2^(byte i of w - 127)
 __device__ inline float byte_scale(uint32_t w, int i) { return bits_f32(((w >> (8 * i)) & 0xffu) << 23); }
 
-// Rows of a key head that paged_chunk.hip's kernel takes per unit, and its launch.
+// Rows of a key head that a chunk block has (paged_chunk.h), and the launch with blocks of both
+// kinds (paged_chunk.hip; few_rows: 16 or 32).
 constexpr int kChunkRows = 128;
-int launch_chunk(const PagedArgs& p, unsigned blocks, bool codes, hipStream_t s);
+int launch_both(const PagedArgs& few, const PagedArgs& many, unsigned few_blocks, unsigned many_blocks, int few_rows,
+                bool codes, hipStream_t s);
 
 }  // namespace abacus
