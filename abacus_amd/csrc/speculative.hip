@@ -117,24 +117,39 @@ __device__ inline double wave_scan64(double x, double& total) {
 // 2^y for y <= 0 (2^-1000 below that): y = n + f with |f| <= 1/2, and the polynomial of
 // degree 9 that is 2^f at the ten Chebyshev nodes, off by at most 1.9e-14 of it and the
 // roundings.  n comes from the addition that rounds and goes straight into the exponent's
-// bits.
-__device__ inline double exp2_64(double y) {
+// bits.  N values step by step, as each step waits for the one before.
+template <int N>
+__device__ inline void exp2_64(double (&y)[N]) {
   constexpr double kRound = 0x1.8p52;
-  y = fmax(y, -1000.0);
-  const double shifted = y + kRound, f = y - (shifted - kRound);
-  double s = 1.0205905413765595e-07;
-  s = fma(s, f, 1.325964524488711e-06);
-  s = fma(s, f, 1.5252672924850737e-05);
-  s = fma(s, f, 0.0001540343375125101);
-  s = fma(s, f, 0.0013333558200794592);
-  s = fma(s, f, 0.009618129193934313);
-  s = fma(s, f, 0.05550410866465167);
-  s = fma(s, f, 0.2402265069564034);
-  s = fma(s, f, 0.6931471805599462);
-  s = fma(s, f, 1.0000000000000135);
-  const uint32_t n = (uint32_t)__builtin_bit_cast(uint64_t, shifted) << 20;  // its low bits
-  const uint64_t u = __builtin_bit_cast(uint64_t, s);
-  return __builtin_bit_cast(double, (uint64_t)((uint32_t)(u >> 32) + n) << 32 | (uint32_t)u);
+  constexpr double c[] = {1.0205905413765595e-07, 1.325964524488711e-06, 1.5252672924850737e-05,
+                          0.0001540343375125101,  0.0013333558200794592, 0.009618129193934313,
+                          0.05550410866465167,    0.2402265069564034,    0.6931471805599462,
+                          1.0000000000000135};
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  uint32_t n[N];
+  double s[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    y[i] = fmax(y[i], -1000.0);
+    const double shifted = y[i] + kRound;
+    n[i] = (uint32_t)__builtin_bit_cast(uint64_t, shifted) << 20;  // its low bits
+    y[i] -= shifted - kRound;
+    s[i] = c[0];
+  }
+#pragma unroll
+  for (int k = 1; k < 10; ++k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = fma(s[i], y[i], c[k]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const u32x2 u = __builtin_bit_cast(u32x2, s[i]);
+    y[i] = __builtin_bit_cast(double, u32x2{u[0], u[1] + n[i]});
+  }
+}
+__device__ inline double exp2_64(double y) {
+  double x[1] = {y};
+  exp2_64(x);
+  return x[0];
 }
 
 // The rows of sequence s, clipped to what there is.
@@ -206,7 +221,13 @@ __global__ __launch_bounds__(Threads) void verify_rows_kernel(VerifyArgs a) {
   if (top > -__builtin_inff() && top < __builtin_inff()) {
     const double shift = -(double)top * a.to_log2;
 #pragma unroll
-    for (int e = 0; e < Each; ++e) sum += exp2_64(fma((double)x[e], a.to_log2, shift));
+    for (int e = 0; e < Each; e += 4) {
+      double y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = fma((double)x[e + i], a.to_log2, shift);
+      exp2_64(y);
+      sum += (y[0] + y[1]) + (y[2] + y[3]);
+    }
   }
   sum = wave_sum64(sum);
   if (lane == 0) sum_w[wave] = sum;
@@ -265,14 +286,17 @@ __device__ inline void masses(const VerifyArgs& a, int row, bool residual, int64
   if (residual && a.draft) load_logits((const T*)a.draft + row * a.V, i0, 0, a.V, y);
   const double p_shift = -(double)p.top * a.to_log2, q_shift = -(double)q.top * a.to_log2;
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    m[e] = exp2_64(fma((double)x[e], a.to_log2, p_shift));
-    m[e] = m[e] > 0x1p-999 ? m[e] * p.inv : 0.0;
-    if (residual) {
-      const double d = a.draft ? exp2_64(fma((double)y[e], a.to_log2, q_shift)) * q.inv : (i0 + e == drafted ? 1.0 : 0.0);
-      m[e] = fmax(m[e] - d, 0.0);
-    }
-  }
+  for (int e = 0; e < kEach; ++e) m[e] = fma((double)x[e], a.to_log2, p_shift);
+  exp2_64(m);
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) m[e] = m[e] > 0x1p-999 ? m[e] * p.inv : 0.0;
+  if (!residual) return;
+  double d[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) d[e] = a.draft ? fma((double)y[e], a.to_log2, q_shift) : 0.0;
+  if (a.draft) exp2_64(d);
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) m[e] = fmax(m[e] - (a.draft ? d[e] * q.inv : i0 + e == drafted ? 1.0 : 0.0), 0.0);
 }
 
 constexpr int kKept = 32;  // rows whose maximum and sum a block keeps, of those it decides on
