@@ -16,6 +16,7 @@ namespace abacus {
 namespace {
 
 constexpr int kFewPieces = 2048;   // pieces the work of a launch is cut into, about
+constexpr int kLeast = 4;          // tiles of one at least
 constexpr int kFewJoined = 16;     // pieces that a wave joins for several rows at once
 constexpr int kChunkPieces = 512;  // (of the chunk kernel's: two work-groups a CU)
 
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(256) void paged_join_both_kernel(PagedArgs few, Pag
 struct Part {
   int R;           // rows of a unit, 0: none of this kind
   int over, upto;  // the sequences they take, by their rows of a key head
-  int target, least;  // pieces, and tiles of one at least
+  int target, least, full;  // (paged_cut.h)
   int64_t units, items;  // at most
   bool cuts;      // whether a unit can be cut
   int64_t floats(int64_t Hk, int64_t K) const { return cuts ? items * Hk * R * (K + 2) : 0; }
@@ -157,16 +158,17 @@ struct Plan {
   Part few, many;
 };
 
-Part part_of(int R, int64_t over, int64_t upto, int target, int least, int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G,
-             int64_t Hk) {
+Part part_of(int R, int64_t over, int64_t upto, int target, int full, int64_t T, int64_t S, int64_t P,
+             int64_t page_size, int64_t G, int64_t Hk) {
   Part n;
-  n.R = R, n.over = (int)over, n.upto = (int)upto, n.target = target, n.least = least;
+  n.R = R, n.over = (int)over, n.upto = (int)upto, n.target = target, n.full = full;
   // a sequence of this launch has more than `over` rows; at most R of them are one unit
   const int64_t seqs = std::min(std::min(S, T), T * G / (over + 1) + (over == 0 ? T : 0));
   n.units = upto <= R ? seqs : std::min(T * G, T * G / R + seqs);
-  const int64_t tiles = (P * page_size + kTile - 1) / kTile, most = (tiles + least - 1) / least;
-  n.cuts = most > 1;
-  n.items = std::min(n.units * most, n.units + (target + Hk - 1) / Hk);
+  const int64_t tiles = (P * page_size + kTile - 1) / kTile;
+  n.cuts = tiles > full;  // a launch that can do without the join does
+  n.least = n.cuts ? kLeast : full;
+  n.items = std::min(n.units * ((tiles + n.least - 1) / n.least), n.units + (target + Hk - 1) / Hk);
   return n;
 }
 
@@ -174,20 +176,22 @@ Plan plan_of(int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G, int6
              int held, int64_t max_new) {
   constexpr int64_t kAll = 0x7fffffff;
   const int64_t rows = std::min(T, max_new) * G;
-  // a piece of a quarter of a megabyte, 256 to 1024 keys: less and its block's beginning and the
-  // join take longer than its keys (700 bf16 tokens in one piece 9 us, in two 14)
+  // a full piece is a quarter of a megabyte, 256 to 1024 keys: what is shorter takes its block's
+  // beginning and the join longer than its keys, and pays only where CUs would have nothing (one
+  // sequence of 1500 bf16 keys in pieces of 1024 12.6 us, of 256 9.7; 16 sequences of 3000 e4m3
+  // keys and 32 rows in pieces of 1024 20 us, of 256 28; 700 keys uncut 9 us, in two pieces 14)
   const int64_t tile = 2 * kTile * K * (held == ABACUS_E4M3 ? 1 : held == kBF16 ? 2 : 4);
-  const int least = (int)std::min<int64_t>(std::max<int64_t>((256 << 10) / tile, 4), 16);
+  const int full = (int)std::min<int64_t>(std::max<int64_t>((256 << 10) / tile, kLeast), 16);
   const bool chunks = dtype == kBF16;
   Plan n;
   n.many.R = 0, n.many.cuts = false;
   if (rows <= 32 || !chunks) {
-    n.few = part_of(rows <= 16 ? 16 : 32, 0, kAll, kFewPieces, least, T, S, P, page_size, G, Hk);
+    n.few = part_of(rows <= 16 ? 16 : 32, 0, kAll, kFewPieces, full, T, S, P, page_size, G, Hk);
   } else {
     const int few = G <= 16 ? 16 : 32;
-    n.few = part_of(few, 0, few, kFewPieces, least, T, S, P, page_size, G, Hk);
+    n.few = part_of(few, 0, few, kFewPieces, full, T, S, P, page_size, G, Hk);
     // (four tiles: 36 rows of 16 sequences over 3000 keys, K = 128, 54 us at 16, 44 at 4)
-    n.many = part_of(kChunkRows, few, kAll, kChunkPieces, 4, T, S, P, page_size, G, Hk);
+    n.many = part_of(kChunkRows, few, kAll, kChunkPieces, kLeast, T, S, P, page_size, G, Hk);
   }
   return n;
 }
@@ -204,7 +208,7 @@ template <typename Q>
 int launch(const PagedArgs& p, const Plan& n, bool codes, float* ws, int64_t rows, hipStream_t s) {
   auto args = [&](const Part& part, float* at) {
     PagedArgs a = p;
-    a.over = part.over, a.upto = part.upto, a.target = part.target, a.least = part.least, a.part = at;
+    a.over = part.over, a.upto = part.upto, a.target = part.target, a.least = part.least, a.full = part.full, a.part = at;
     return a;
   };
   const PagedArgs few = args(n.few, ws);

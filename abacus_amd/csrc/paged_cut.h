@@ -4,10 +4,11 @@
 // unit's keys are cut into `split` pieces of whole 64-key tiles where there are too few
 // units for the GPU, and each piece gives its rows' maximum, sum and unscaled output,
 // which a second kernel joins in order.  The piece length is the same for the whole
-// launch: its (unit, key head, tile)s spread over `target` pieces, at least `least` tiles
-// each.  The units are found from the device's lengths by a scan (paged_rows.h), a launch
-// being sized for the most there can be.  Blocks of a kind take the sequences whose rows
-// of a key head number more than `over` and at most `upto`.
+// launch: its (unit, key head, tile)s spread over kShort pieces of at least `least` tiles
+// each, and over up to `target` pieces as long as those have `full` tiles.  The units are
+// found from the device's lengths by a scan (paged_rows.h), a launch being sized for the
+// most there can be.  Blocks of a kind take the sequences whose rows of a key head number
+// more than `over` and at most `upto`.
 #pragma once
 
 #include "paged_rows.h"
@@ -26,8 +27,11 @@ struct PagedArgs {
   float scale_log2;
   int zero_rest;   // rows of no sequence: 0, or left as they are
   int over, upto;  // rows of a key head that a sequence of these blocks has
-  int target, least;
+  int target, least, full;
 };
+
+// Pieces there may be before they have to be full ones: one a CU, as the sequences' last add to them.
+constexpr int kShort = 192;
 
 // Units of a sequence for blocks of this kind.
 template <int R>
@@ -43,8 +47,10 @@ __device__ inline int piece_tiles(const PagedArgs& p, const SeqScan& scan) {
   const float total = scan.sum([&](const SeqRows& r) {  // tiles of one key head
     return (float)units_of<R>(p, r) * (float)((r.len + kTile - 1) / kTile);
   });
-  const int want = (p.target + p.Hk - 1) / p.Hk;
-  return max(p.least, (int)fminf(ceilf(total * 1.001f / (float)want), 1e9f));
+  auto spread = [&](int pieces) {
+    return (int)fminf(ceilf(total * 1.001f / (float)((pieces + p.Hk - 1) / p.Hk)), 1e9f);
+  };
+  return max(max(p.least, spread(p.target)), min(p.full, spread(kShort)));
 }
 
 // Pieces of each of a sequence's units.
