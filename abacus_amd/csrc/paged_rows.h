@@ -5,9 +5,10 @@
 // query_start[s + 1] - 1 are the last n_s positions of sequence s, which has
 // lengths[s] tokens in all.  Position p lies in slot p % page_size of page
 // table[s][p / page_size].  All of this is device memory that no host check
-// has seen, so every value is bounded here: a range of rows outside [0, T] is
-// empty, a length past the table marks its sequence, a page id outside the
-// pool marks its positions.  Nothing is kept between calls: each wave finds its
+// has seen, so every value is bounded here: from the first range that runs backwards
+// or out of [0, T] on every sequence is without rows (so no two share one, and there
+// are at most T in all, which launches and workspaces are sized by), a length past the
+// table marks its sequence, a page id outside the pool marks its positions.  Nothing is kept between calls: each wave finds its
 // place by a scan over the sequences, one load per 64 of them.
 #pragma once
 
@@ -31,10 +32,10 @@ struct SeqRows {
   bool bad;   // the table has no place for that many
 };
 
-__device__ inline SeqRows seq_rows(const PagedRows& a, int s) {
+__device__ inline SeqRows seq_rows(const PagedRows& a, int s, bool& in) {
   SeqRows r;
   const int first = a.query_start[s], end = a.query_start[s + 1], len = a.lengths[s];
-  const bool in = first >= 0 && end >= first && end <= a.T;
+  in = first >= 0 && end >= first && end <= a.T;
   const int most = a.P << a.shift;
   r.first = in ? first : 0;
   r.n = in ? end - first : 0;
@@ -73,25 +74,40 @@ __device__ inline float wave_total(float x) {
 // first 64 are read once.
 struct SeqScan {
   const PagedRows& a;
+  bool first_ended = false;
   SeqRows first;
-  __device__ inline explicit SeqScan(const PagedRows& rows) : a(rows), first(at(0)) {}
-  __device__ inline SeqRows at(int s0) const {
-    const int s = s0 + (threadIdx.x & 63);
-    return s < a.S ? seq_rows(a, s) : SeqRows{0, 0, 0, false};
+  __device__ inline explicit SeqScan(const PagedRows& rows) : a(rows) { first = next(0, first_ended); }
+  // sequences s0 .. s0 + 63; `ended`: whether there was a bad range before them, among them
+  __device__ inline SeqRows next(int s0, bool& ended) const {
+    const int lane = threadIdx.x & 63, s = s0 + lane;
+    SeqRows r{0, 0, 0, false};
+    bool in = true;
+    if (s < a.S) r = seq_rows(a, s, in);
+    const uint64_t out = __ballot(!in);
+    if (ended || (out & ((1ull << lane) - 1))) r.n = 0;
+    ended |= out != 0;
+    return r;
+  }
+  __device__ inline SeqRows at(int s0, bool& ended) const {
+    if (s0 > 0) return next(s0, ended);
+    ended = first_ended;
+    return first;
   }
   // sum of value(sequence) over all
   template <class F>
   __device__ inline float sum(F value) const {
-    float x = value(first);
-    for (int s0 = 64; s0 < a.S; s0 += 64) x += value(at(s0));
+    bool ended;
+    float x = value(at(0, ended));
+    for (int s0 = 64; s0 < a.S; s0 += 64) x += value(at(s0, ended));
     return wave_total(x);
   }
   // sum of count(sequence) over the sequences before `seq`
   template <class F>
   __device__ inline int before(int seq, F count) const {
     int base = 0;
+    bool ended;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
-      const int c = count(s0 == 0 ? first : at(s0));
+      const int c = count(at(s0, ended));
       int total;
       const int upto = wave_scan(c, total);
       if (seq < s0 + 64) return base + __builtin_amdgcn_readlane(upto - c, seq - s0);
@@ -103,8 +119,9 @@ struct SeqScan {
   template <class F>
   __device__ inline bool find(int b, F count, int& seq, int& local, SeqRows& r) const {
     int base = 0;
+    bool ended;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
-      const SeqRows mine = s0 == 0 ? first : at(s0);
+      const SeqRows mine = at(s0, ended);
       const int c = count(mine);
       int total;
       const int upto = wave_scan(c, total);

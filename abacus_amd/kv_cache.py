@@ -52,7 +52,8 @@ class BatchRows:
 
     page_table_SP: (S, P) int32, page of positions 0 .. page_size - 1 of each sequence, and so on (entries past
     its length are not read).  query_start: (S + 1,) int32, sequence s has the rows query_start[s] ..
-    query_start[s + 1] - 1, none among them.  lengths: (S,) int32, its tokens in all, the new ones included: its
+    query_start[s + 1] - 1, none among them (from the first range that runs backwards or past the rows on, sequences
+    are taken to have none).  lengths: (S,) int32, its tokens in all, the new ones included: its
     last row is position lengths[s] - 1.  max_new: the most rows of one sequence, where the caller knows; it
     chooses the kernels and bounds nothing.
 
@@ -238,9 +239,11 @@ class KVPages:
         where the table does not hold the sequence or its pages are not in the pool."""
         P = rows._sizes[1]
         start, lengths = rows.query_start.tolist(), rows.lengths.tolist()
+        ended = False
         for s, length in enumerate(lengths):
             first, n = start[s], start[s + 1] - start[s]
-            if first < 0 or n < 0 or start[s + 1] > n_rows:
+            ended = ended or first < 0 or n < 0 or start[s + 1] > n_rows
+            if ended:
                 first, n = 0, 0
             at = torch.arange(min(max(length, 0), P * self.page_size))
             page = rows.page_table_SP[s].long()[at // self.page_size]

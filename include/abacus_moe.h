@@ -427,8 +427,8 @@ int abacus_cross_entropy_mean_bwd(const void* logits_NV, const int64_t* targets_
  * `held` is what they hold: the rows' dtype, or ABACUS_E4M3 with exponent bytes
  * k_scale and v_scale (n_pages, H, page_size): a code stands for
  * code * 2^(byte - 127).  page_size: a power of two, 16 to 256; K: a multiple of 16 up to 128.
- * The three index arrays are device memory: a range of rows outside [0, T] is taken
- * as empty, rows whose sequence is longer than its table or whose pages lie outside the
+ * The three index arrays are device memory: from the first range of rows that runs
+ * backwards or out of [0, T] on, sequences are taken to have none; rows whose sequence is longer than its table or whose pages lie outside the
  * pool are not written, and read or attended to as NaN.
  *
  * write: k_THK and v_THK (T, H, K) into the pages.  e4m3: per row and head,

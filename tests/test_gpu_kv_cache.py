@@ -233,6 +233,26 @@ def test_refused_by_the_pages_on_the_device():
         assert torch.isfinite(out[0]).all() and torch.isnan(out[1:3]).all() and (out[3] == 7.0).all()
 
 
+@pytest.mark.parametrize("S", [3, 201])
+@pytest.mark.parametrize("dtype,T", [(torch.float32, 40), (torch.bfloat16, 300)])
+def test_no_rows_after_a_range_that_runs_backwards(dtype, T, S):
+    """Ranges 0..T, T..0, 0..T, ...: only the first counts, and the others' pieces have no room in the workspace."""
+    context = 2000
+    rows, n = pc.rows_of([(T, context)] + [(0, context)] * (S - 1), 64, "cuda", n_pages=-(-context // 64) * S)
+    pages = pc.pages_of(n, 2, 64, 64, dtype, "cuda")
+    g = torch.Generator("cuda").manual_seed(3)
+    for held in (pages.k, pages.v):
+        held.copy_(torch.randn(held.shape, device="cuda", generator=g))
+    new = torch.randn(2, T, 2, 64, device="cuda", generator=g).to(dtype)
+    q = torch.randn(T, 4, 64, device="cuda", generator=g).to(dtype)
+    pages.write(*new, rows)
+    want, held = pages.attend(q, rows), (pages.k.clone(), pages.v.clone())
+    rows.query_start[2::2] = 0
+    pages.write(*new, rows)
+    assert torch.equal(pages.k, held[0]) and torch.equal(pages.v, held[1])
+    assert torch.equal(pages.attend(q, rows), want)
+
+
 def test_rows_of_nothing():
     rows, n = pc.rows_of([(2, 1), (1, 0)], 16, "cuda")
     pages = pc.pages_of(n, 1, 16, 16, torch.float32, "cuda")

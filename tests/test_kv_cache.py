@@ -75,6 +75,18 @@ def test_pages_outside_the_pool_and_lengths_past_the_table(held):
     assert torch.isfinite(o[0]).all() and torch.isnan(o[1:]).all()
 
 
+def test_no_rows_after_a_range_that_runs_backwards():
+    """Overlapping ranges would be more rows than the call has: what comes after the bad range has none."""
+    rows, n = pc.rows_of([(2, 2), (0, 0), (2, 2)], 16, "cpu")
+    rows.query_start.copy_(torch.tensor([0, 2, 0, 2]))
+    pages = pc.pages_of(n, 1, 16, 16, torch.float32, "cpu")
+    x = torch.ones(2, 1, 16)
+    pages.write(x, 3 * x, rows)
+    _, v = pages.read(rows, 2)
+    assert (v[0] == 3.0).all() and not v[2].any()
+    assert (pages.attend(x, rows) == 3.0).all()
+
+
 def test_nonfinite_rows_of_a_quantised_cache():
     rows, n = pc.rows_of([(3, 3)], 16, "cpu")
     pages = pc.pages_of(n, 2, 16, 16, E4M3, "cpu")
