@@ -44,7 +44,9 @@ def _index(name: str, t: torch.Tensor, shape: tuple[int, ...], device: torch.dev
         raise ValueError(f"{name} must be int32 on {device}, got {t.dtype} on {t.device}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-    return t if t.is_contiguous() else t.contiguous()
+    if not t.is_contiguous():  # (a copy would not follow what the caller writes there later)
+        raise ValueError(f"{name} must be contiguous")
+    return t
 
 
 class BatchRows:

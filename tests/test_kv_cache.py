@@ -75,6 +75,16 @@ def test_pages_outside_the_pool_and_lengths_past_the_table(held):
     assert torch.isfinite(o[0]).all() and torch.isnan(o[1:]).all()
 
 
+def test_rows_are_not_copied():
+    """A call reads what the caller's tensors hold then, so a strided view, which would be copied, is refused."""
+    table, start, lengths = torch.zeros(2, 8, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    assert BatchRows(table, start, lengths).page_table_SP.data_ptr() == table.data_ptr()
+    for bad in ((table[:, :4], start, lengths), (table, torch.zeros(6, dtype=torch.int32)[::2], lengths),
+                (table, start, torch.ones(4, dtype=torch.int32)[::2])):
+        with pytest.raises(ValueError, match="contiguous"):
+            BatchRows(*bad)
+
+
 def test_no_rows_after_a_range_that_runs_backwards():
     """Overlapping ranges would be more rows than the call has: what comes after the bad range has none."""
     rows, n = pc.rows_of([(2, 2), (0, 0), (2, 2)], 16, "cpu")
