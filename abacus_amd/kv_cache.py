@@ -49,6 +49,11 @@ def _index(name: str, t: torch.Tensor, shape: tuple[int, ...], device: torch.dev
     return t
 
 
+def _no_gradient(name: str) -> None:
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient, and a cache gives none: call it under torch.no_grad()")
+
+
 class BatchRows:
     """The T rows of a call, new tokens of S sequences one after the other.
 
@@ -156,6 +161,8 @@ class KVPages:
                             "(float32 or bfloat16) or float8_e4m3fn")
         if x.device != self.device or rows.device != self.device:
             raise ValueError(f"{name}, the rows and the pages must be on one device")
+        if x.requires_grad:
+            _no_gradient(name)
         return shape
 
     def _rows_args(self, rows: BatchRows) -> tuple:
@@ -171,6 +178,8 @@ class KVPages:
         T, H, K = self._check("k", k_THK, rows, self.n_heads)
         if v_THK.shape != k_THK.shape or v_THK.dtype != k_THK.dtype or v_THK.device != self.device:
             raise ValueError("k and v must have one shape, dtype and device")
+        if v_THK.requires_grad:
+            _no_gradient("v")
         if not k_THK.is_cuda:
             return self._write_cpu(k_THK, v_THK, rows)
         k_THK, v_THK = _contig(k_THK), _contig(v_THK)
@@ -209,7 +218,7 @@ class KVPages:
         left as they are there.
 
         Statistics and sums are fp32; with bf16 queries the probabilities are rounded to bf16 for the product
-        with the values, as the training kernels do.  No gradient is formed."""
+        with the values, as the training kernels do.  No gradient is formed: rows that ask for one are refused."""
         T, H, K = self._check("q", q_THK, rows, None)
         if H % self.n_heads or H < 1 or H > 1024:
             raise ValueError(f"{H} query heads over {self.n_heads} key heads: they must be a multiple (at most 1024)")

@@ -85,6 +85,19 @@ def test_rows_are_not_copied():
             BatchRows(*bad)
 
 
+def test_no_gradient():
+    """Rows that ask for a gradient are refused, not cut off from it silently."""
+    rows, n = pc.rows_of([(2, 5)], 16, "cpu")
+    pages = pc.pages_of(n, 2, 16, 16, torch.float32, "cpu")
+    x = torch.ones(2, 2, 16)
+    leaf = x.clone().requires_grad_()
+    for call in (lambda: pages.attend(leaf, rows), lambda: pages.write(leaf, x, rows), lambda: pages.write(x, leaf, rows)):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            call()
+        with torch.no_grad():
+            call()
+
+
 def test_no_rows_after_a_range_that_runs_backwards():
     """Overlapping ranges would be more rows than the call has: what comes after the bad range has none."""
     rows, n = pc.rows_of([(2, 2), (0, 0), (2, 2)], 16, "cpu")
