@@ -34,7 +34,7 @@ struct VerifyArgs {
   const float* uniforms;
   int T, S, slices, mass_slices;
   int64_t V;
-  double to_log2;  // log2(e) / temperature
+  double to_log2;  // log2(e) / temperature, for logits less their maximum (products first would lose digits)
   bool greedy;
   int32_t* accepted;
   int64_t* next;
@@ -219,12 +219,12 @@ __global__ __launch_bounds__(Threads) void verify_rows_kernel(VerifyArgs a) {
   }
   double sum = 0.0;
   if (top > -__builtin_inff() && top < __builtin_inff()) {
-    const double shift = -(double)top * a.to_log2;
+    const double t = (double)top;
 #pragma unroll
     for (int e = 0; e < Each; e += 4) {
       double y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = fma((double)x[e + i], a.to_log2, shift);
+      for (int i = 0; i < 4; ++i) y[i] = ((double)x[e + i] - t) * a.to_log2;
       exp2_64(y);
       sum += (y[0] + y[1]) + (y[2] + y[3]);
     }
@@ -284,16 +284,16 @@ __device__ inline void masses(const VerifyArgs& a, int row, bool residual, int64
   float x[kEach], y[kEach];
   load_logits((const T*)a.target + row * a.V, i0, 0, a.V, x);
   if (residual && a.draft) load_logits((const T*)a.draft + row * a.V, i0, 0, a.V, y);
-  const double p_shift = -(double)p.top * a.to_log2, q_shift = -(double)q.top * a.to_log2;
+  const double p_top = (double)p.top, q_top = (double)q.top;
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) m[e] = fma((double)x[e], a.to_log2, p_shift);
+  for (int e = 0; e < kEach; ++e) m[e] = ((double)x[e] - p_top) * a.to_log2;
   exp2_64(m);
 #pragma unroll
   for (int e = 0; e < kEach; ++e) m[e] = m[e] > 0x1p-999 ? m[e] * p.inv : 0.0;
   if (!residual) return;
   double d[kEach];
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) d[e] = a.draft ? fma((double)y[e], a.to_log2, q_shift) : 0.0;
+  for (int e = 0; e < kEach; ++e) d[e] = a.draft ? ((double)y[e] - q_top) * a.to_log2 : 0.0;
   if (a.draft) exp2_64(d);
 #pragma unroll
   for (int e = 0; e < kEach; ++e) m[e] = fmax(m[e] - (a.draft ? d[e] * q.inv : i0 + e == drafted ? 1.0 : 0.0), 0.0);
@@ -511,7 +511,7 @@ extern "C" int abacus_verify_drafts(const void* target_TV, const void* draft_TV,
   a.query_start = query_start, a.uniforms = uniforms_T2;
   a.T = (int)T, a.S = (int)S, a.slices = (int)n, a.mass_slices = (int)mass_slices_of(V), a.V = V;
   a.greedy = temperature == 0.0;
-  a.to_log2 = a.greedy ? 0.0 : 1.4426950408889634 / temperature;
+  a.to_log2 = a.greedy ? 0.0 : std::min(1.4426950408889634 / temperature, 1e300);  // (0 times infinity)
   a.accepted = accepted_S, a.next = next_S;
   a.sums = (double*)ws;
   a.mass = a.sums + 2 * T * n;

@@ -68,6 +68,30 @@ def test_matches_the_restatement(device, dtype, V, sizes, drafter, temperature):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("drafter", [False, True])
+@pytest.mark.parametrize("temperature", [1e-3, 1e-15, 1e-30, 1e-310, 1e30])
+def test_temperatures_far_from_one(device, drafter, temperature):
+    """Far below 1 the tokens that share the largest logit share the row, whatever its size; far above all do."""
+    V, T = 9001, 6
+    g = torch.Generator().manual_seed(7)
+    target = torch.randn(T, V, generator=g) + 50.3
+    draft = torch.randn(T, V, generator=g) - 77.7 if drafter else None
+    tokens = torch.tensor([0, 100, 8500, 3, 100, 100])
+    for row in range(T):
+        target[row, [100, 8500, 40]] = 61.7
+        if drafter:
+            draft[row, [100, 8500, 7, 8]] = -60.3
+    start = torch.tensor([0, 1, 3, 6], dtype=torch.int32)
+    for seed in range(6):
+        u = torch.rand(T, 2, generator=g.manual_seed(seed))
+        want = _restated(target.tolist(), tokens.tolist(), start.tolist(), u.tolist(), draft.tolist() if drafter else None,
+                         temperature)
+        got = verify_drafts(target.to(device), tokens.to(device), start.to(device), u.to(device),
+                            draft.to(device) if drafter else None, temperature)
+        assert (got[0].tolist(), got[1].tolist()) == want
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_temperature_zero_takes_the_lowest_of_equals(device, dtype):
     V = 8200
