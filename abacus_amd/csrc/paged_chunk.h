@@ -143,16 +143,18 @@ __device__ inline bool not_finite(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
-template <bool Cd, int HD, bool Full>
-__device__ __attribute__((always_inline)) inline void chunk_block(const PagedArgs& p, int block, ChunkLds<HD>& lds) {
+// N: 32-key halves of a tile that a wave takes.  With 1 (at most 64 rows) waves 2 and 3 have the
+// rows of 0 and 1 and the tiles' other halves, which are joined at the end.
+template <bool Cd, int HD, bool Full, int N>
+__device__ __attribute__((always_inline)) inline void chunk_rows(const PagedArgs& p, int block, const Item& w,
+                                                                 ChunkLds<HD>& lds) {
   constexpr int R = kChunkRows;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int item = block / p.Hk, kh = block % p.Hk, G = p.G, K = Full ? HD : p.K;
-  Item w;
-  if (!find_item<R>(p, item, w)) return;
+  const int kh = block % p.Hk, G = p.G, K = Full ? HD : p.K;
+  const int half = N == 1 ? wave >> 1 : 0;
 
   // this wave's rows, and the keys that the last of them sees
-  const int m0 = wave * 32, m = m0 + (lane & 31);
+  const int m0 = (N == 1 ? wave & 1 : wave) * 32, m = m0 + (lane & 31);
   const int row = w.row0 + min(m, w.rows - 1);
   const int token = row / G, head = kh * G + row % G;
   const int vis = m < w.rows ? max(0, w.r.len - w.r.n + token + 1) : 0;
@@ -171,31 +173,31 @@ __device__ __attribute__((always_inline)) inline void chunk_block(const PagedArg
   auto step = [&](const char* kt, const char* vt, const float* scales, int key0, int bad,
                   auto edge_t) __attribute__((always_inline)) {
     constexpr bool edge = decltype(edge_t)::value;
-    attn_f32x16 s[2];
+    attn_f32x16 s[N];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < N; ++n) {
       s[n] = attn_f32x16{};
 #pragma unroll
       for (int c = 0; c < HD / 16; ++c)
-        mfma32(s[n], *reinterpret_cast<const Vec16*>(kt + tile_off<HD>(32 * n + key_row, 2 * c + h)), qf[c]);
+        mfma32(s[n], *reinterpret_cast<const Vec16*>(kt + tile_off<HD>(32 * (n + half) + key_row, 2 * c + h)), qf[c]);
     }
     if (bad) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (bad >> (2 * n + r / 8) & 1) s[n][r] = __builtin_nanf("");
+          if (bad >> (2 * (n + half) + r / 8) & 1) s[n][r] = __builtin_nanf("");
     }
     if constexpr (edge) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (key0 + 32 * n + 16 * (r >> 3) + 8 * h + (r & 7) >= vis) s[n][r] = -__builtin_inff();
+          if (key0 + 32 * (n + half) + 16 * (r >> 3) + 8 * h + (r & 7) >= vis) s[n][r] = -__builtin_inff();
     }
     float mx = s[0][0];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[n][r]);
     mx = pair_max(mx) * p.scale_log2;
@@ -213,7 +215,7 @@ __device__ __attribute__((always_inline)) inline void chunk_block(const PagedArg
     }
     const float m_use = m_run == -__builtin_inff() ? 0.f : m_run;  // (nothing seen yet)
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[n][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][r], p.scale_log2, -m_use));
@@ -230,13 +232,13 @@ __device__ __attribute__((always_inline)) inline void chunk_block(const PagedArg
       poison = __any(poison);
       if (poison) {
 #pragma unroll 1
-        for (int key = 0; key < kTile; ++key) {
+        for (int key = 32 * half; key < 32 * (half + N); ++key) {
           float pr = 0.f;
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-              if (32 * n + 16 * (r >> 3) + (r & 7) == (key & ~8)) pr = s[n][r];
+              if (32 * (n + half) + 16 * (r >> 3) + (r & 7) == (key & ~8)) pr = s[n][r];
           pr = __shfl(pr, (lane & 31) + 4 * (key & 8), 64);
           int first_d = 4 * h;
           asm volatile("" : "+v"(first_d));  // (nothing of the addresses is kept over the loop)
@@ -253,13 +255,13 @@ __device__ __attribute__((always_inline)) inline void chunk_block(const PagedArg
       }
     }
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < 2 * N; ++c) {
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = s[c >> 1][8 * (c & 1) + e];
       if constexpr (Cd) {
-        const float4 a = *reinterpret_cast<const float4*>(scales + 16 * c + 8 * h);
-        const float4 b = *reinterpret_cast<const float4*>(scales + 16 * c + 8 * h + 4);
+        const float4 a = *reinterpret_cast<const float4*>(scales + 16 * (c + 2 * half) + 8 * h);
+        const float4 b = *reinterpret_cast<const float4*>(scales + 16 * (c + 2 * half) + 8 * h + 4);
         const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= f[e];  // exact: powers of two
@@ -269,7 +271,7 @@ __device__ __attribute__((always_inline)) inline void chunk_block(const PagedArg
       for (int e = 0; e < 4; ++e) pf.w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
 #pragma unroll
       for (int t = 0; t < HD / 32; ++t) {
-        Vec16 vf = *reinterpret_cast<const Vec16*>(vt + tile_off<64>(32 * t + (lane & 31), 2 * c + h));
+        Vec16 vf = *reinterpret_cast<const Vec16*>(vt + tile_off<64>(32 * t + (lane & 31), 2 * (c + 2 * half) + h));
         if constexpr (edge && !Cd) {
           if (poison) {
 #pragma unroll
@@ -312,7 +314,7 @@ __device__ __attribute__((always_inline)) inline void chunk_block(const PagedArg
       }
       const int next_bad = next.bad;
       if (t + 2 < w.t1) next = groups_of(p, w.seq, key0 + 2 * kTile, w.seen);
-      if (!decltype(edge_t)::value || key0 < seen) step(lds.k[st], lds.v[st], lds.vs[st], key0, bad, edge_t);
+      if (!decltype(edge_t)::value || key0 + 32 * half < seen) step(lds.k[st], lds.v[st], lds.vs[st], key0, bad, edge_t);
       if constexpr (Cd) {
         if (more) codes.store(lds.k[st ^ 1], lds.v[st ^ 1], lds.vs[st ^ 1], w.seen - key0 - kTile, K);
       }
@@ -323,6 +325,25 @@ __device__ __attribute__((always_inline)) inline void chunk_block(const PagedArg
     int t = w.t0;
     for (; t < min(w.t1, w.least / kTile); ++t) turn(t, std::false_type{});
     for (; t < w.t1; ++t) turn(t, std::true_type{});
+  }
+  if constexpr (N == 1) {  // waves 2 and 3 hand over what they have
+    constexpr int kAcc = HD / 2;  // of a lane
+    static_assert(sizeof(ChunkLds<HD>) >= 2 * (kAcc + 2) * 64 * 4, "two waves' sums");
+    float* to = reinterpret_cast<float*>(&lds) + (wave & 1) * (kAcc + 2) * 64 + lane;
+    __syncthreads();
+    if (wave >= 2) {
+#pragma unroll
+      for (int i = 0; i < kAcc; ++i) to[i * 64] = acc[i / 16][i % 16];
+      to[kAcc * 64] = m_run, to[(kAcc + 1) * 64] = l_run;
+    }
+    __syncthreads();
+    if (wave >= 2) return;
+    const float other = to[kAcc * 64], top = fmaxf(m_run, other), from = top == -__builtin_inff() ? 0.f : top;
+    const float a = __builtin_amdgcn_exp2f(m_run - from), b = __builtin_amdgcn_exp2f(other - from);
+    m_run = top;
+    l_run = a * l_run + b * to[(kAcc + 1) * 64];
+#pragma unroll
+    for (int i = 0; i < kAcc; ++i) acc[i / 16][i % 16] = a * acc[i / 16][i % 16] + b * to[i * 64];
   }
   if (m >= w.rows) return;
   const float l = pair_sum(l_run);
@@ -341,6 +362,14 @@ __device__ __attribute__((always_inline)) inline void chunk_block(const PagedArg
     part[R * K + m] = m_run;
     part[R * K + R + m] = l;
   }
+}
+
+template <bool Cd, int HD, bool Full>
+__device__ __attribute__((always_inline)) inline void chunk_block(const PagedArgs& p, int block, ChunkLds<HD>& lds) {
+  Item w;
+  if (!find_item<kChunkRows>(p, block / p.Hk, w)) return;
+  if (w.rows > kChunkRows / 2) chunk_rows<Cd, HD, Full, 2>(p, block, w, lds);
+  else chunk_rows<Cd, HD, Full, 1>(p, block, w, lds);
 }
 
 }  // namespace abacus

@@ -123,6 +123,30 @@ def test_chunks(held, H, G, K, page, plan):
 
 
 @pytest.mark.parametrize("held", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("K", [16, 64, 80, 128])
+def test_chunk_units_of_at_most_64_rows(held, K):
+    """Two waves have the same rows and half of each tile: rows of one wave and of two, pieces that end inside a half,
+    sequences shorter than one, what no row sees, and a page that is missing."""
+    plan = [(33, 2100), (64, 64), (40, 1000), (50, 97), (36, 40), (1, 300), (192, 500)]
+    pages, rows, k, v, g = _filled(plan, 1, K, 32, torch.bfloat16, held, fill=0x7f if held == E4M3 else math.nan)
+    T = sum(n for n, _ in plan)
+    q = torch.randn(T, 1, K, device="cuda", generator=g).bfloat16()
+    o = pages.attend(q, rows)
+    _check(pages, plan, rows, k, v, q, o, held)
+    v[2099, 0, 5], k[2099 + 64, 0, 3] = math.inf, math.nan  # the last positions of the first two sequences
+    whole = BatchRows(rows.page_table_SP, torch.tensor([0] + [n for _, n in plan]).cumsum(0).to(torch.int32).cuda(), rows.lengths)
+    pages.write(k, v, whole)
+    got = pages.attend(q, rows)
+    same = torch.ones(T, dtype=torch.bool, device="cuda")
+    same[[32, 96]] = False
+    assert torch.isfinite(got[same]).all() and not torch.isfinite(got[32, 0, 5]) and not torch.isfinite(got[96]).any()
+    rows.page_table_SP[2, 30] = -1  # positions 960 to 991: all 40 rows see the first of them
+    rows.page_table_SP[3, 2] = -1   # positions 64 to 95: rows 17 on
+    got = pages.attend(q, rows)
+    assert torch.isnan(got[97:137]).all() and torch.isfinite(got[137:154]).all() and torch.isnan(got[154:187]).all()
+
+
+@pytest.mark.parametrize("held", [torch.bfloat16, E4M3])
 def test_a_wrong_hint_changes_no_result(held):
     """max_new says one row and there are many: other kernels, the same attention."""
     plan = [(1, 40), (70, 900), (3, 2000)]
