@@ -21,7 +21,7 @@ constexpr int kFewJoined = 16;     // pieces that a wave joins for several rows 
 constexpr int kChunkPieces = 512;  // (of the chunk kernel's: two work-groups a CU)
 
 template <typename Q, bool Cd, int KD, bool Full, int QT>
-__global__ __launch_bounds__(256, QT == 1 ? (KD == 64 ? 3 : 2) : (KD == 64 ? 2 : 1)) void paged_few_kernel(PagedArgs p) {
+__global__ __launch_bounds__(256, QT == 1 ? (KD <= 64 ? 3 : 2) : (KD <= 64 ? 2 : 1)) void paged_few_kernel(PagedArgs p) {
   __shared__ __attribute__((aligned(16))) FewLds<KD, QT> lds;
   few_block<Q, Cd, KD, Full, QT>(p, blockIdx.x, gridDim.x, lds);
 }
@@ -198,10 +198,20 @@ Plan plan_of(int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G, int6
 
 template <typename Q, bool Cd, int QT>
 void launch_few(const PagedArgs& p, unsigned blocks, hipStream_t s) {
-  if (p.K == 64) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 64, true, QT>), dim3(blocks), dim3(256), 0, s, p);
-  else if (p.K == 128) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 128, true, QT>), dim3(blocks), dim3(256), 0, s, p);
-  else if (p.K < 64) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 64, false, QT>), dim3(blocks), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 128, false, QT>), dim3(blocks), dim3(256), 0, s, p);
+  const dim3 grid(blocks), threads(256);
+  // laid out for 32 dims instead of 64: 48 fp32 rows over 54074 keys 112 us, 63; not for codes, as
+  // 16 bytes in each lane group are 64 dims there
+  if constexpr (!Cd) {
+    if (p.K <= 32) {
+      if (p.K == 32) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 32, true, QT>), grid, threads, 0, s, p);
+      else hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 32, false, QT>), grid, threads, 0, s, p);
+      return;
+    }
+  }
+  if (p.K == 64) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 64, true, QT>), grid, threads, 0, s, p);
+  else if (p.K == 128) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 128, true, QT>), grid, threads, 0, s, p);
+  else if (p.K < 64) hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 64, false, QT>), grid, threads, 0, s, p);
+  else hipLaunchKernelGGL((paged_few_kernel<Q, Cd, 128, false, QT>), grid, threads, 0, s, p);
 }
 
 template <typename Q>

@@ -86,6 +86,8 @@ def test_write_and_read(dtype, held, K, page):
     (2, 2, 128, 16, [(40, 40), (1, 900), (130, 520), (1, 3)]),
     (1, 1, 64, 256, [(257, 800)]),
     (2, 5, 32, 64, [(70, 70), (3, 2)]),
+    (2, 4, 32, 16, [(1, 3000), (4, 1100), (1, 1)]),
+    (3, 1, 16, 256, [(20, 1700), (1, 31)]),
 ])
 def test_attention(dtype, held, H, G, K, page, plan):
     pages, rows, k, v, g = _filled(plan, H, K, page, dtype, held)
@@ -189,7 +191,8 @@ def test_many_sequences():
 
 
 @pytest.mark.parametrize("dtype,held", KINDS)
-@pytest.mark.parametrize("plan,K", [([(1, 5), (3, 70), (1, 130)], 64), ([(100, 300)], 64), ([(2, 9), (140, 140)], 128), ([(100, 300)], 80)])
+@pytest.mark.parametrize("plan,K", [([(1, 5), (3, 70), (1, 130)], 64), ([(100, 300)], 64), ([(2, 9), (140, 140)], 128), ([(100, 300)], 80),
+                                    ([(1, 5), (3, 70), (1, 130)], 32), ([(20, 300), (2, 40)], 16)])
 def test_what_a_row_does_not_see_does_not_reach_it(dtype, held, plan, K):
     """Pages full of NaN and infinities before the sequences are written; then a NaN and an infinity in the keys and
     values of the last token: only the rows that see it have them, dim by dim as the formula has."""
