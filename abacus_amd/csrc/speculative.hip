@@ -41,6 +41,7 @@ struct VerifyArgs {
   double* sums;   // [2][T][slices]: of exp((x - slice max) / temperature)
   double* mass;   // [S][mass_slices]
   float* tops;    // [2][T][slices]: slice maxima, NaN where there is one
+  float* drafted; // [2][T]: the logit of the draft after the row
   int* at;        // [T][slices]: where (greedy)
   int* ended;     // [S]: blocks that are done with the sequence
 };
@@ -182,6 +183,11 @@ __global__ __launch_bounds__(Threads) void verify_rows_kernel(VerifyArgs a) {
   if (which == 0 && slice == 0 && tid == 0)
     for (int s = row; s < a.S; s += a.T) a.ended[s] = 0;
   const int64_t i0 = (int64_t)slice * kSlice + tid * 8;
+  if (tid == 0 && !a.greedy && row + 1 < a.T) {  // read here, where nothing waits for it
+    const int64_t x = a.tokens[row + 1];
+    if (x >= 0 && x < a.V && x / kSlice == slice)
+      a.drafted[which * a.T + row] = to_f32(((const T*)(which ? a.draft : a.target))[row * a.V + x]);
+  }
   float x[Each];
   load_logits((const T*)(which ? a.draft : a.target) + row * a.V, i0, 8 * Threads, a.V, x);
   if (which == 1) {  // a sequence's last row has no draft after it
@@ -222,6 +228,7 @@ __global__ __launch_bounds__(Threads) void verify_rows_kernel(VerifyArgs a) {
     const double t = (double)top;
 #pragma unroll
     for (int e = 0; e < Each; e += 4) {
+      if ((int64_t)slice * kSlice + e / 8 * 8 * Threads >= a.V) break;  // (the same for all)
       double y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[i] = ((double)x[e + i] - t) * a.to_log2;
@@ -286,25 +293,32 @@ __device__ inline void masses(const VerifyArgs& a, int row, bool residual, int64
   if (residual && a.draft) load_logits((const T*)a.draft + row * a.V, i0, 0, a.V, y);
   const double p_top = (double)p.top, q_top = (double)q.top;
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) m[e] = ((double)x[e] - p_top) * a.to_log2;
-  exp2_64(m);
+  for (int e0 = 0; e0 < kEach; e0 += 4) {  // (four at a time, for registers)
+    double u[4], d[4] = {};
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) m[e] = m[e] > 0x1p-999 ? m[e] * p.inv : 0.0;
-  if (!residual) return;
-  double d[kEach];
+    for (int e = 0; e < 4; ++e) u[e] = ((double)x[e0 + e] - p_top) * a.to_log2;
+    exp2_64(u);
+    if (residual && a.draft) {
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) d[e] = a.draft ? ((double)y[e] - q_top) * a.to_log2 : 0.0;
-  if (a.draft) exp2_64(d);
+      for (int e = 0; e < 4; ++e) d[e] = ((double)y[e0 + e] - q_top) * a.to_log2;
+      exp2_64(d);
+    }
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) m[e] = fmax(m[e] - (a.draft ? d[e] * q.inv : i0 + e == drafted ? 1.0 : 0.0), 0.0);
+    for (int e = 0; e < 4; ++e) {
+      u[e] = u[e] > 0x1p-999 ? u[e] * p.inv : 0.0;
+      if (residual) u[e] = fmax(u[e] - (a.draft ? d[e] * q.inv : i0 + e0 + e == drafted ? 1.0 : 0.0), 0.0);
+      m[e0 + e] = u[e];
+    }
+  }
 }
 
 constexpr int kKept = 32;  // rows whose maximum and sum a block keeps, of those it decides on
 
 // blockIdx: slice, sequence.  Every block of a sequence decides alike and sums its slice's
-// mass; the last to end draws.
+// mass; the last to end draws.  (Six waves a SIMD, three blocks a CU: 124 fp32 sequences of
+// 32000 logits 41 us with two, 38 with three.)
 template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_decide_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(kThreads, 6) void verify_decide_kernel(VerifyArgs a) {
   __shared__ int stop, order;
   __shared__ double sum_w[kWaves];
   __shared__ RowStat kept[2][kKept];
@@ -330,8 +344,7 @@ __global__ __launch_bounds__(kThreads) void verify_decide_kernel(VerifyArgs a) {
     const RowParts pp = parts_of(a, 0, row), qp = both ? parts_of(a, 1, row) : pp;
     const int64_t x = draft ? a.tokens[row + 1] : -1;
     const bool known = x >= 0 && x < a.V;
-    const float px = known ? to_f32(((const T*)a.target)[row * a.V + x]) : 0.f;
-    const float qx = known && both ? to_f32(((const T*)a.draft)[row * a.V + x]) : 0.f;
+    const float px = a.drafted[row], qx = both ? a.drafted[a.T + row] : 0.f;  // (anything, where it is not known)
     const float u = draft ? a.uniforms[2 * row] : 0.f;
     const RowStat p = row_stat(a, 0, row, pp), q = both ? row_stat(a, 1, row, qp) : p;
     if (j < kKept && lane == 0) kept[0][j] = p, kept[1][j] = q;
@@ -363,23 +376,24 @@ __global__ __launch_bounds__(kThreads) void verify_decide_kernel(VerifyArgs a) {
   if (lane == 0) sum_w[wave] = sum;
   __syncthreads();
   double* mass = a.mass + (int64_t)seq * a.mass_slices;
+  const bool alone = a.mass_slices == 1;
   // What passes between the blocks does so in agent-scope operations, which do not stop at
   // this XCD's L2; the store has ended before the count goes up.  (A release would write the
   // whole L2 back, once a block.)
-  if (tid == 0) {
+  if (tid == 0 && !alone) {
     __hip_atomic_store(mass + slice, block_sum(sum_w), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     order = __hip_atomic_fetch_add(a.ended + seq, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  if (order != a.mass_slices - 1) return;
+  if (!alone && order != a.mass_slices - 1) return;
 
   // the draw: the border, the slice whose end passes it first, the token in it
   auto mass_of = [&](int i) {
     return i < a.mass_slices ? __hip_atomic_load(mass + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
   };
-  double total = 0.0, before = 0.0;
-  for (int s0 = 0; s0 < a.mass_slices; s0 += 64) {
+  double total = alone ? block_sum(sum_w) : 0.0, before = 0.0;
+  for (int s0 = 0; !alone && s0 < a.mass_slices; s0 += 64) {
     double part;
     wave_scan64(mass_of(s0 + lane), part);
     total += part;
@@ -388,7 +402,7 @@ __global__ __launch_bounds__(kThreads) void verify_decide_kernel(VerifyArgs a) {
   if (plain) residual = false, total = 1.0;
   const double border = fmin((double)a.uniforms[2 * row + 1], 1.0 - 0x1p-53) * total;
   int at = 0;
-  for (int s0 = 0; !plain && s0 < a.mass_slices; s0 += 64) {
+  for (int s0 = 0; !plain && !alone && s0 < a.mass_slices; s0 += 64) {
     double part;
     const double x = mass_of(s0 + lane), upto = wave_scan64(x, part);
     const unsigned long long has = __ballot(s0 + lane < a.mass_slices && before + upto > border);
@@ -400,10 +414,12 @@ __global__ __launch_bounds__(kThreads) void verify_decide_kernel(VerifyArgs a) {
     }
     before += part;
   }
+  bool held = !plain;   // whether m are this block's slice's
   long long last = -1;  // the last token with any mass, should rounding leave none past the border
   for (; at < a.mass_slices; ++at) {
     const int64_t i0 = (int64_t)at * kMassSlice + tid * kEach;
-    masses<T>(a, row, residual, drafted, p, q, i0, m);
+    if (!held || at != slice) masses<T>(a, row, residual, drafted, p, q, i0, m);
+    held = false;
     own = 0.0;
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
@@ -412,6 +428,7 @@ __global__ __launch_bounds__(kThreads) void verify_decide_kernel(VerifyArgs a) {
     }
     double part;
     const double upto = wave_scan64(own, part);
+    __syncthreads();  // (what was in sum_w is read)
     if (lane == 0) sum_w[wave] = part;
     __syncthreads();
     double run = before + (upto - own);
@@ -487,7 +504,7 @@ using namespace abacus;
 
 extern "C" int64_t abacus_verify_drafts_ws_bytes(int64_t T, int64_t V, int64_t S) {
   const int64_t n = slices_of(V);
-  return (2 * T * n + S * mass_slices_of(V)) * 8 + 2 * T * n * 4 + T * n * 4 + S * 4;
+  return (2 * T * n + S * mass_slices_of(V)) * 8 + 2 * T * n * 4 + 2 * T * 4 + T * n * 4 + S * 4;
 }
 
 extern "C" int abacus_verify_drafts(const void* target_TV, const void* draft_TV, const int64_t* tokens_T,
@@ -516,7 +533,8 @@ extern "C" int abacus_verify_drafts(const void* target_TV, const void* draft_TV,
   a.sums = (double*)ws;
   a.mass = a.sums + 2 * T * n;
   a.tops = (float*)(a.mass + S * a.mass_slices);
-  a.at = (int*)(a.tops + 2 * T * n);
+  a.drafted = a.tops + 2 * T * n;
+  a.at = (int*)(a.drafted + 2 * T);
   a.ended = a.at + T * n;
   hipStream_t s = (hipStream_t)stream;
   const dim3 rows((unsigned)n, (unsigned)T, a.draft ? 2 : 1), decide((unsigned)a.mass_slices, (unsigned)S);
