@@ -9,6 +9,12 @@
 // query l % 16 against the KG keys of group l / 16, in their order, and those are, as they
 // lie, the operand P^T of O^T = V^T P^T with 16 bytes of a V^T row: neither the scores nor a
 // tile of keys or values goes through LDS, and every load of the cache is 16 bytes a lane.
+//
+// Bound by the bytes of the cache.  4 query heads a key head, K = 128: 64 tokens over up to 8192
+// e4m3 keys 132 us (5.3 TB/s; the vector unit is busy a quarter of it), 2 over
+// 131072 bf16 keys 190 us (5.6 TB/s).  The tiles of a block's piece are dealt out to its four
+// waves in turn: runs of tiles a wave took 230 us for the first, eight waves 156.  With more
+// than 16 rows the fp32 products weigh as much (90 TF/s of 154 for a chunk of K = 128).
 #pragma once
 
 #include <type_traits>
