@@ -16,6 +16,7 @@ namespace abacus {
 namespace {
 
 constexpr int kFewPieces = 2048;   // pieces the work of a launch is cut into, about: eight a CU, as sequences differ
+constexpr int kOnePieces = 448;    // where a CU holds one work-group: two turns, less the sequences' last pieces
 constexpr int kLeast = 4;          // tiles of one at least
 constexpr int kFewJoined = 16;     // pieces that a wave joins for several rows at once
 constexpr int kChunkPieces = 512;  // (of the chunk kernel's: two work-groups a CU; 768 gains 7% where K = 64 and no
@@ -159,16 +160,17 @@ struct Plan {
   Part few, many;
 };
 
-Part part_of(int R, int64_t over, int64_t upto, int target, int full, int64_t T, int64_t S, int64_t P,
+Part part_of(int R, int64_t over, int64_t upto, int target, int full, int uncut, int64_t T, int64_t S, int64_t P,
              int64_t page_size, int64_t G, int64_t Hk) {
   Part n;
-  n.R = R, n.over = (int)over, n.upto = (int)upto, n.target = target, n.full = full;
+  n.R = R, n.over = (int)over, n.upto = (int)upto, n.target = target;
   // a sequence of this launch has more than `over` rows; at most R of them are one unit
   const int64_t seqs = std::min(std::min(S, T), T * G / (over + 1) + (over == 0 ? T : 0));
   n.units = upto <= R ? seqs : std::min(T * G, T * G / R + seqs);
   const int64_t tiles = (P * page_size + kTile - 1) / kTile;
-  n.cuts = tiles > full;  // a launch that can do without the join does
-  n.least = n.cuts ? kLeast : full;
+  n.cuts = tiles > uncut;  // a launch that can do without the join does
+  n.least = n.cuts ? kLeast : uncut;
+  n.full = n.cuts ? full : uncut;
   n.items = std::min(n.units * ((tiles + n.least - 1) / n.least), n.units + (target + Hk - 1) / Hk);
   return n;
 }
@@ -187,12 +189,16 @@ Plan plan_of(int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G, int6
   Plan n;
   n.many.R = 0, n.many.cuts = false;
   if (rows <= 32 || !chunks) {
-    n.few = part_of(rows <= 16 ? 16 : 32, 0, kAll, kFewPieces, full, T, S, P, page_size, G, Hk);
+    // a work-group fills a CU's registers: few turns of long pieces, as nothing covers a piece's
+    // beginning (20 rows of 16 sequences over 9000 bf16 keys in pieces as the others 120 us, 87 so)
+    const bool one = rows > 16 && K > 64;
+    n.few = part_of(rows <= 16 ? 16 : 32, 0, kAll, one ? kOnePieces : kFewPieces, one ? 32 : full, full, T, S, P,
+                    page_size, G, Hk);
   } else {
     const int few = G <= 16 ? 16 : 32;
-    n.few = part_of(few, 0, few, kFewPieces, full, T, S, P, page_size, G, Hk);
+    n.few = part_of(few, 0, few, kFewPieces, full, full, T, S, P, page_size, G, Hk);
     // (four tiles: 36 rows of 16 sequences over 3000 keys, K = 128, 54 us at 16, 44 at 4)
-    n.many = part_of(kChunkRows, few, kAll, kChunkPieces, kLeast, T, S, P, page_size, G, Hk);
+    n.many = part_of(kChunkRows, few, kAll, kChunkPieces, kLeast, kLeast, T, S, P, page_size, G, Hk);
   }
   return n;
 }
