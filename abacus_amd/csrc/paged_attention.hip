@@ -19,8 +19,10 @@ constexpr int kFewPieces = 2048;   // pieces the work of a launch is cut into, a
 constexpr int kOnePieces = 448;    // where a CU holds one work-group: two turns, less the sequences' last pieces
 constexpr int kLeast = 4;          // tiles of one at least
 constexpr int kFewJoined = 16;     // pieces that a wave joins for several rows at once
-constexpr int kChunkPieces = 512;  // (of the chunk kernel's: two work-groups a CU; 768 gains 7% where K = 64 and no
-                                   // single tokens are there to fill the CUs, and loses 20% beside them)
+// Of the chunk kernel's: two work-groups a CU, less the sequences' last pieces (259 tokens of 16 heads
+// over 8, K = 80, over 48042 keys: 219 us with 512, 155).  768 gains 7% where K = 64 and no single
+// tokens are there to fill the CUs, and loses 20% beside them.
+constexpr int kChunkPieces = 480;
 
 template <typename Q, bool Cd, int KD, bool Full, int QT>
 __global__ __launch_bounds__(256, QT == 1 ? (KD <= 64 ? 3 : 2) : (KD <= 64 ? 2 : 1)) void paged_few_kernel(PagedArgs p) {
