@@ -22,7 +22,9 @@ constexpr int kFewJoined = 16;     // pieces that a wave joins for several rows 
 // Of the chunk kernel's: two work-groups a CU, less the sequences' last pieces (259 tokens of 16 heads
 // over 8, K = 80, over 48042 keys: 219 us with 512, 155).  768 gains 7% where K = 64 and no single
 // tokens are there to fill the CUs, and loses 20% beside them.
-constexpr int kChunkPieces = 480;
+// Where the units, if they are all alike, would be more pieces than run at once, the last few of
+// those would run alone: a finer cut (576 tokens of 64 heads over 8, K = 128, over 7085 keys: 255 us, 215).
+constexpr int kChunkPieces = 480, kChunkPlaces = 512, kChunkFiner = 960;
 
 template <typename Q, bool Cd, int KD, bool Full, int QT>
 __global__ __launch_bounds__(256, QT == 1 ? (KD <= 64 ? 3 : 2) : (KD <= 64 ? 2 : 1)) void paged_few_kernel(PagedArgs p) {
@@ -200,7 +202,12 @@ Plan plan_of(int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G, int6
     const int few = G <= 16 ? 16 : 32;
     n.few = part_of(few, 0, few, kFewPieces, full, full, T, S, P, page_size, G, Hk);
     // (four tiles: 36 rows of 16 sequences over 3000 keys, K = 128, 54 us at 16, 44 at 4)
-    n.many = part_of(kChunkRows, few, kAll, kChunkPieces, kLeast, kLeast, T, S, P, page_size, G, Hk);
+    int target = kChunkPieces;
+    if (T == S * std::min(T, max_new)) {  // every sequence has a chunk of max_new
+      const int64_t units = S * ((rows + kChunkRows - 1) / kChunkRows) * Hk;
+      if ((kChunkPieces + units - 1) / units * units > kChunkPlaces) target = kChunkFiner;
+    }
+    n.many = part_of(kChunkRows, few, kAll, target, kLeast, kLeast, T, S, P, page_size, G, Hk);
   }
   return n;
 }
