@@ -186,7 +186,7 @@ Plan plan_of(int64_t T, int64_t S, int64_t P, int64_t page_size, int64_t G, int6
   // a full piece is a quarter of a megabyte, 256 to 1024 keys: what is shorter takes its block's
   // beginning and the join longer than its keys, and pays only where CUs would have nothing (one
   // sequence of 1500 bf16 keys in pieces of 1024 12.6 us, of 256 9.7; 16 sequences of 3000 e4m3
-  // keys and 32 rows in pieces of 1024 20 us, of 256 28; 700 keys uncut 9 us, in two pieces 14)
+  // keys, 8 heads of 128, in pieces of 1024 23 us, of 256 26; 700 keys uncut 9 us, in two pieces 14)
   const int64_t tile = 2 * kTile * K * (held == ABACUS_E4M3 ? 1 : held == kBF16 ? 2 : 4);
   const int full = (int)std::min<int64_t>(std::max<int64_t>((256 << 10) / tile, kLeast), 16);
   const bool chunks = dtype == kBF16;

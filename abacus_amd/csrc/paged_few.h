@@ -14,7 +14,7 @@
 // e4m3 keys 132 us (5.3 TB/s; the vector unit is busy a quarter of it), 2 over
 // 131072 bf16 keys 190 us (5.6 TB/s).  The tiles of a block's piece are dealt out to its four
 // waves in turn: runs of tiles a wave took 230 us for the first, eight waves 156.  With more
-// than 16 rows the fp32 products weigh as much (90 TF/s of 154 for a chunk of K = 128).
+// than 16 rows the fp32 products weigh as much (97 TF/s of 154 for a chunk of K = 128).
 #pragma once
 
 #include <type_traits>
