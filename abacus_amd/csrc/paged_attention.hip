@@ -44,7 +44,8 @@ __device__ inline void join_block(const PagedArgs& p, int block, JoinLds& lds) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, K = p.K, lanes = K / 4;
   const int b = block / p.Hk, kh = block % p.Hk;
   const SeqScan scan(p.a);
-  const int chunk = piece_tiles<R>(p, scan);
+  int given;
+  const int chunk = piece_tiles<R>(p, scan, given);
   int seq, local;
   SeqRows r;
   if (!scan.find(b, [&](const SeqRows& r) { return units_of<R>(p, r); }, seq, local, r)) return;

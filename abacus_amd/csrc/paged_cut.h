@@ -42,11 +42,15 @@ __device__ inline int units_of(const PagedArgs& p, const SeqRows& r) {
 
 // Tiles of a piece, the same on every wave and in both kernels.  (A sum in floats, taken
 // larger by more than they can be off: the launch has room for no more pieces.)
+// `given`: the rows that the sequences have, of both kinds (in floats too: at most 2^24).
 template <int R>
-__device__ inline int piece_tiles(const PagedArgs& p, const SeqScan& scan) {
+__device__ inline int piece_tiles(const PagedArgs& p, const SeqScan& scan, int& given) {
+  float rows = 0.f;
   const float total = scan.sum([&](const SeqRows& r) {  // tiles of one key head
+    rows += (float)r.n;
     return (float)units_of<R>(p, r) * (float)((r.len + kTile - 1) / kTile);
   });
+  given = (int)wave_total(rows);
   auto spread = [&](int pieces) {
     return (int)fminf(ceilf(total * 1.001f / (float)((pieces + p.Hk - 1) / p.Hk)), 1e9f);
   };
@@ -64,15 +68,16 @@ struct Item {
   int seq, split, row0, rows;
   int seen, least;  // keys that the last, the first of the rows sees
   int t0, t1;
+  int given;  // rows that the call's sequences have, one after the other from query_start[0] on
 };
 
 __device__ inline int seen_of(const SeqRows& r, int row, int G) { return max(0, r.len - r.n + row / G + 1); }
 
-// The whole block's item, false where there is none.
+// The whole block's item, false where there is none (`given` is set all the same).
 template <int R>
 __device__ inline bool find_item(const PagedArgs& p, int item, Item& w) {
   const SeqScan scan(p.a);
-  const int chunk = piece_tiles<R>(p, scan);
+  const int chunk = piece_tiles<R>(p, scan, w.given);
   int local;
   if (!scan.find(item, [&](const SeqRows& r) { return units_of<R>(p, r) * pieces_of(r, chunk); }, w.seq, local, w.r))
     return false;

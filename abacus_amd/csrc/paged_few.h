@@ -145,17 +145,20 @@ __device__ __attribute__((always_inline)) inline void few_block(const PagedArgs&
   const int i = lane & 15, g = lane >> 4;
   const int item = block / p.Hk, kh = block % p.Hk, G = p.G, K = p.K;
 
-  // rows of no sequence, read now and cleared last
-  const int rest0 = p.zero_rest ? p.a.query_start[0] : 0, rest1 = p.zero_rest ? p.a.query_start[p.a.S] : 0x7fffffff;
+  Item w;
+  // Rows of no sequence, cleared last: those before and behind the rows that the scan gives the
+  // sequences, which no block stores.  (The last entry of query_start does not say where those
+  // end: it may lie behind a range that runs backwards or past the call's rows.)
+  const int start = p.zero_rest ? p.a.query_start[0] : 0;  // read now
   auto clear_rest = [&] {
-    const int first = min(max(rest0, 0), p.a.T), end = min(max(rest1, first), p.a.T);
-    const int rest = p.a.T - (end - first), items = blocks / p.Hk;
-    for (int r = item; r < rest; r += items) {
-      Q* row = (Q*)p.o + ((int64_t)(r < first ? r : end + r - first) * p.H + kh * G) * K;
+    if (!p.zero_rest) return;
+    const int rest = p.a.T - w.given, items = blocks / p.Hk;
+    for (int r = item; r < rest; r += items) {  // (no sequence has a row: any start will do)
+      const int at = w.given > 0 && r >= start ? r + w.given : r;
+      Q* row = (Q*)p.o + ((int64_t)at * p.H + kh * G) * K;
       for (int d = tid; d < G * K; d += 64 * NW) row[d] = from_f32<Q>(0.f);
     }
   };
-  Item w;
   if (!find_item<R>(p, item, w)) {
     clear_rest();
     return;

@@ -280,6 +280,40 @@ def test_no_rows_after_a_range_that_runs_backwards(dtype, T, S):
     assert torch.equal(pages.attend(q, rows), want)
 
 
+# Ranges of rows and the rows of the call: (query_start, T, how many sequences count).
+CUT_SHORT = [([0, 2, 0], 2, 1), ([0, 1, 2, 0], 3, 2), ([0, 5, 20], 10, 1), ([0, 5, 3, 10], 10, 1), ([0, 1, 2, 3, 9], 4, 3),
+             ([2, 5, 5, 4, 8], 8, 2), ([-1, 3, 6], 6, 0), ([4, 2, 6], 6, 0), ([9, 9, 9], 6, 0), ([3, 3, 3], 6, 2),
+             ([0, 6, *[6] * 70, 7, *[0] * 60], 9, 72)]
+
+
+@pytest.mark.parametrize("dtype,held", KINDS)
+@pytest.mark.parametrize("G", [1, 8])  # (8 heads a key head: the launch that has chunks as well)
+@pytest.mark.parametrize("start,T,good", CUT_SHORT, ids=[str(i) for i in range(len(CUT_SHORT))])
+def test_every_row_of_no_sequence_is_cleared_and_no_other(dtype, held, G, start, T, good):
+    """From the first bad range on sequences have no rows, whatever the last entry says: the rows before it are those of
+    a call in which the others have none, bit for bit, and all the others are 0."""
+    S, H, K, page = len(start) - 1, 2, 64, 32
+    g = torch.Generator("cuda").manual_seed(1)
+    table = torch.randperm(2 * S, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(S, 2).cuda()
+    pages = pc.pages_of(2 * S, H, page, K, held, "cuda")
+    lengths = torch.tensor([30 + s % 35 for s in range(S)], dtype=torch.int32, device="cuda")
+    new = torch.randn(2, int(lengths.sum()), H, K, device="cuda", generator=g).to(dtype)
+    as_start = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    pages.write(*new, BatchRows(table, as_start([0] + lengths.cumsum(0).tolist()), lengths))
+    q = torch.randn(T, H * G, K, device="cuda", generator=g).to(dtype)
+    end = start[good] if good else 0
+    clean = BatchRows(table, as_start(start[:good + 1] + [end] * (S - good) if good else [0] * (S + 1)), lengths)
+    want = torch.zeros_like(q)
+    pages.attend(q, clean, out=want)
+    for _ in range(3):
+        dirty = torch.full_like(q, 7.0)  # what the next allocation of this size holds
+        del dirty
+        got = pages.attend(q, BatchRows(table, as_start(start), lengths))
+        assert torch.equal(got, want)
+    first = start[0] if good else 0
+    assert not want[:first].any() and not want[end:].any() and (end == first or want[first:end].abs().sum(-1).min() > 0)
+
+
 def test_rows_of_nothing():
     rows, n = pc.rows_of([(2, 1), (1, 0)], 16, "cuda")
     pages = pc.pages_of(n, 1, 16, 16, torch.float32, "cuda")

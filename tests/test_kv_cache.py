@@ -110,6 +110,19 @@ def test_no_rows_after_a_range_that_runs_backwards():
     assert (pages.attend(x, rows) == 3.0).all()
 
 
+@pytest.mark.parametrize("start,T,valid", [([0, 2, 0], 2, (0, 2)), ([0, 5, 20], 10, (0, 5)), ([0, 5, 3, 10], 10, (0, 5)),
+                                           ([2, 5, 5, 4, 8], 8, (2, 5)), ([-1, 3, 6], 6, (0, 0)), ([4, 2, 6], 6, (0, 0))])
+def test_rows_of_no_sequence_are_cleared_and_no_others(start, T, valid):
+    S = len(start) - 1
+    table = torch.arange(S, dtype=torch.int32)[:, None]
+    pages = pc.pages_of(S, 1, 16, 16, torch.float32, "cpu", fill=1.0)
+    rows = BatchRows(table, torch.tensor(start, dtype=torch.int32), torch.full((S,), 16, dtype=torch.int32))
+    got = pages.attend(torch.ones(T, 1, 16), rows)
+    want = torch.zeros(T, 1, 16)
+    want[valid[0]:valid[1]] = 1.0
+    assert torch.allclose(got, want, rtol=0, atol=17 * 2.0 ** -24)  # a mean of 16 ones
+
+
 def test_nonfinite_rows_of_a_quantised_cache():
     rows, n = pc.rows_of([(3, 3)], 16, "cpu")
     pages = pc.pages_of(n, 2, 16, 16, E4M3, "cpu")
