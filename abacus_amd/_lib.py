@@ -98,6 +98,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "abacus_cross_entropy_bwd": (_I, [_P, _P, _P, _P, _F, _I64, _I64, _I64, _I, _P, _P]),
     "abacus_cross_entropy_mean_fwd": (_I, [_P, _P, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P]),
     "abacus_cross_entropy_mean_bwd": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _P, _P]),
+    "abacus_batch_positions": (_I, [_P, _P, _I64, _I64, _P, _P]),
     "abacus_kv_write": (_I, [_P, _P, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P]),
     "abacus_kv_read": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _I64, _I, _P, _P, _P]),
     "abacus_paged_attention_ws_bytes": (_I64, [_I64, _I64, _I64, _I64, _I, _I, _I64, _I64, _I64, _I64]),

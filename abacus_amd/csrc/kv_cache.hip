@@ -328,6 +328,22 @@ void launch_read(const PagedRows& a, const Pages& p, int64_t L, void* k, void* v
                        L, (T*)k, (T*)v);
 }
 
+// Each row's position in its sequence, 0 for rows of none: a thread a row, by bisection of the
+// ranges that count.
+__global__ __launch_bounds__(256) void batch_positions_kernel(PagedRows a, int64_t* __restrict__ positions) {
+  const int good = good_sequences(a.query_start, a.S, a.T), row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= a.T) return;
+  int lo = 0, hi = good;  // the first sequence whose range ends behind the row
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (a.query_start[mid + 1] > row) hi = mid;
+    else lo = mid + 1;
+  }
+  int64_t pos = 0;
+  if (lo < good && row >= a.query_start[0]) pos = (int64_t)a.lengths[lo] - a.query_start[lo + 1] + row;
+  positions[row] = pos > 0 ? pos : 0;
+}
+
 int check_pages(const char* what, const void* k, const void* v, const void* k_scale, const void* v_scale, int dtype,
                 int held) {
   ABACUS_CHECK_ARG(dtype == kF32 || dtype == kBF16, "%s: dtype code %d", what, dtype);
@@ -342,6 +358,19 @@ int check_pages(const char* what, const void* k, const void* v, const void* k_sc
 }  // namespace abacus
 
 using namespace abacus;
+
+extern "C" int abacus_batch_positions(const int32_t* query_start, const int32_t* lengths, int64_t S, int64_t T,
+                                      int64_t* positions_T, void* stream) {
+  ABACUS_CHECK_ARG(S >= 1 && S <= (1 << 20) && T >= 0 && T < (1ll << 24), "batch_positions: %lld rows of %lld sequences",
+                   (long long)T, (long long)S);
+  ABACUS_CHECK_ARG(query_start && lengths && (T == 0 || positions_T), "batch_positions: null pointer");
+  if (T == 0) return 0;
+  PagedRows a{nullptr, query_start, lengths, (int)S, 0, (int)T, 0, 0};
+  hipLaunchKernelGGL(batch_positions_kernel, dim3((unsigned)((T + 255) / 256)), dim3(256), 0, (hipStream_t)stream, a,
+                     positions_T);
+  ABACUS_CHECK_LAUNCH("batch_positions");
+  return 0;
+}
 
 extern "C" int abacus_kv_write(const void* k_THK, const void* v_THK, int64_t T, int64_t H, int64_t K, int dtype,
                                const int32_t* page_table_SP, const int32_t* query_start, const int32_t* lengths,

@@ -32,16 +32,28 @@ struct SeqRows {
   bool bad;   // the table has no place for that many
 };
 
+__device__ inline bool range_in(int first, int end, int T) { return first >= 0 && end >= first && end <= T; }
+
 __device__ inline SeqRows seq_rows(const PagedRows& a, int s, bool& in) {
   SeqRows r;
   const int first = a.query_start[s], end = a.query_start[s + 1], len = a.lengths[s];
-  in = first >= 0 && end >= first && end <= a.T;
+  in = range_in(first, end, a.T);
   const int most = a.P << a.shift;
   r.first = in ? first : 0;
   r.n = in ? end - first : 0;
   r.len = min(max(len, 0), most);
   r.bad = len > most;
   return r;
+}
+
+// The sequences before the first bad range, by a wave.
+__device__ inline int good_sequences(const int* query_start, int S, int T) {
+  for (int s0 = 0; s0 < S; s0 += 64) {
+    const int s = s0 + (threadIdx.x & 63);
+    const uint64_t out = __ballot(s < S && !range_in(query_start[s], query_start[s + 1], T));
+    if (out) return s0 + __ffsll((unsigned long long)out) - 1;
+  }
+  return S;
 }
 
 // Sums over a wave without LDS: within rows of 16 lanes by DPP, then over the rows.

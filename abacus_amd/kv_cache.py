@@ -84,13 +84,20 @@ class BatchRows:
         self.max_new, self.device, self._sizes = max_new, device, (S, P)
 
     def positions(self, n_rows: int) -> torch.Tensor:
-        """(n_rows,) int64: each row's position in its sequence (0 for rows of none)."""
-        row = torch.arange(n_rows, device=self.lengths.device, dtype=torch.int32)
-        seq = torch.searchsorted(self.query_start, row, right=True) - 1
-        S = self.lengths.shape[0]
-        at = seq.clamp(0, S - 1)
-        pos = self.lengths[at] - self.query_start[at + 1] + row
-        return torch.where((seq >= 0) & (seq < S) & (pos >= 0), pos, 0).long()
+        """(n_rows,) int64: each row's position in its sequence (0 for rows of none and rows before position 0)."""
+        start, S = self.query_start, self._sizes[0]
+        pos = torch.empty(n_rows, dtype=torch.int64, device=self.device)
+        if pos.is_cuda:
+            _call(self.device, "abacus_batch_positions", start.data_ptr(), self.lengths.data_ptr(), S, n_rows, pos.data_ptr())
+            return pos
+        pos.zero_()
+        good = int(((start[:-1] >= 0) & (start[1:] >= start[:-1]) & (start[1:] <= n_rows)).cumprod(0).sum())
+        if good:
+            first, ends = int(start[0]), start[1:good + 1].long()
+            seq = torch.repeat_interleave(torch.arange(good), ends - start[:good])
+            row = first + torch.arange(len(seq))
+            pos[first:first + len(seq)] = (self.lengths[seq].long() - ends[seq] + row).clamp(min=0)
+        return pos
 
 
 def _call(device: torch.device, name: str, *args) -> None:

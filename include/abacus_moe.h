@@ -431,7 +431,11 @@ int abacus_cross_entropy_mean_bwd(const void* logits_NV, const int64_t* targets_
  * backwards or out of [0, T] on, sequences are taken to have none; rows whose sequence is longer than its table or whose pages lie outside the
  * pool are not written, and read or attended to as NaN.
  *
- * write: k_THK and v_THK (T, H, K) into the pages.  e4m3: per row and head,
+ * positions: of each of the T rows in its sequence, 0 for rows of none and rows before position 0. */
+int abacus_batch_positions(const int32_t* query_start, const int32_t* lengths, int64_t S, int64_t T,
+                           int64_t* positions_T, void* stream);
+
+/* write: k_THK and v_THK (T, H, K) into the pages.  e4m3: per row and head,
  * e = the smallest integer (at least -110) with max|x| <= 448 * 2^e, 0 for a row of
  * zeros; byte = e + 127; codes are x * 2^-e to nearest even.  Where a key or a value
  * holds an infinity or NaN, both read back as NaN. */

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from abacus_amd.generate import generate
-from abacus_amd.kv_cache import E4M3, PagedKVCache
+from abacus_amd.kv_cache import E4M3, BatchRows, PagedKVCache
 from abacus_amd.transformer import TransformerMoe
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -43,6 +43,23 @@ def test_cached_forward_matches_the_whole_one(device, head_dim):
             assert float((got - want[i][at[i]:at[i] + n]).abs().max()) <= 1e-4 * float(want[i].abs().max()) if n else True
             at[i], first = at[i] + n, first + n
     assert at == [37, 5, 61]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_unused_slots_of_a_step_change_nothing(device):
+    """A step whose last slots are still 0 is the step without them: the same logits and the same cache after it."""
+    model = _model(device=device)
+    as_int = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
+    logits, keys = [], []
+    for start in ([0, 1, 1, 1], [0, 1, 0, 0]):
+        cache = PagedKVCache(2, 4, 16, 2, 16, dtype=torch.float32, device=device)
+        seq = cache.add()
+        model.forward_cached(torch.tensor([3, 1, 4, 1], device=device), cache, cache.extend({seq: 4}))
+        page = int(cache.extend({seq: 1}).page_table_SP[0, 0])
+        rows = BatchRows(as_int([[page], [0], [0]]), as_int(start), as_int([5, 0, 0]))
+        logits.append(model.forward_cached(torch.tensor([5], device=device), cache, rows))
+        keys.append(cache.layer(1).read(cache.rows({seq: 1}), 5)[0])
+    assert torch.equal(*logits) and torch.equal(*keys)
 
 
 @pytest.mark.parametrize("device", DEVICES)

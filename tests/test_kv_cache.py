@@ -47,6 +47,28 @@ def test_positions():
     assert rows.positions(7).tolist() == [7, 8, 0, 0, 0, 1, 0]  # a row before position 0, and one of no sequence: 0
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("start,lengths,T,want", [
+    ([0, 1, 0, 0], [5, 9, 9], 1, [4]),
+    ([0, 2, 0, 3], [7, 8, 9], 3, [5, 6, 0]),
+    ([0, 2, 2, 5], [7, 8, 9], 4, [5, 6, 0, 0]),
+    ([-1, 2, 3], [4, 4], 3, [0, 0, 0]),
+    ([9, 9, 9], [4, 4], 3, [0, 0, 0]),
+    ([2, 1, 3], [4, 4], 3, [0, 0, 0]),
+    ([1, 1, 3, 3], [4, 6, 8], 4, [0, 4, 5, 0]),
+    ([0, 3], [2], 3, [0, 0, 1]),
+    ([0, 2], [2**31 - 1], 2, [2**31 - 3, 2**31 - 2]),
+    ([0, 2], [-(2**31)], 2, [0, 0]),
+    ([0, *range(300, 600, 2), 7, *range(598, 700, 2)], [1000 + s for s in range(202)], 700,
+     [*range(700, 1000), *(998 + s + j for s in range(1, 150) for j in (0, 1)), *[0] * 102])])
+def test_positions_end_where_the_ranges_do(device, start, lengths, T, want):
+    """From the first range that runs backwards or past the rows on sequences have none."""
+    as_int = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
+    rows = BatchRows(torch.zeros(len(lengths), 1, dtype=torch.int32, device=device), as_int(start), as_int(lengths))
+    got = rows.positions(T)
+    assert got.dtype == torch.int64 and got.tolist() == want and rows.positions(0).shape == (0,)
+
+
 def test_rows_of_nothing():
     """Rows of no sequence are 0, or left alone in `out`; rows that see nothing are 0."""
     rows, n = pc.rows_of([(2, 1), (1, 0)], 16, "cpu")
