@@ -49,6 +49,7 @@ struct VerifyArgs {
   float* drafted; // [2][T]: the logit of the draft after the row
   int* at;        // [T][slices]: where (greedy)
   int* ended;     // [S]: blocks that are done with the sequence
+  int* good;      // [1]: the sequences before the first bad range
 };
 
 template <typename T> struct alignas(sizeof(T)) Loose { T v[16 / sizeof(T)]; };  // 16 bytes at any element
@@ -158,10 +159,10 @@ __device__ inline double exp2_64(double y) {
   return x[0];
 }
 
-// The rows of sequence s, clipped to what there is.
+// The rows of sequence s, none from the first bad range on (as paged_rows.h has it).
 __device__ inline void rows_of(const VerifyArgs& a, int s, int& first, int& n) {
   const int b = a.query_start[s], e = a.query_start[s + 1];
-  const bool in = b >= 0 && e >= b && e <= a.T;
+  const bool in = range_in(b, e, a.T) && s < *a.good; // (with T = 0 nothing has counted them)
   first = in ? b : 0;
   n = in ? e - b : 0;
 }
@@ -183,6 +184,7 @@ __global__ __launch_bounds__(Threads) void verify_rows_kernel(VerifyArgs a) {
   __shared__ float top_w[Waves];
   __shared__ int at_w[Waves];
   __shared__ double sum_w[Waves];
+  __shared__ int first_bad;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int slice = blockIdx.x, row = blockIdx.y, which = blockIdx.z;
   if (which == 0 && slice == 0 && tid == 0)
@@ -195,10 +197,23 @@ __global__ __launch_bounds__(Threads) void verify_rows_kernel(VerifyArgs a) {
   }
   float x[Each];
   load_logits((const T*)(which ? a.draft : a.target) + row * a.V, i0, 8 * Threads, a.V, x);
-  if (which == 1) {  // a sequence's last row has no draft after it
-    bool last = false;
-    for (int s = lane; s < a.S; s += 64) last |= a.query_start[s + 1] == row + 1;
-    if (__any(last)) return;
+  if (which == 1) {  // a sequence's last row has no draft after it (those from the first bad range on do not count)
+    uint64_t bad = 0, end = 0;
+    for (int s = lane; s - lane < a.S && !(bad | end); s += 64) {
+      const int b = s < a.S ? a.query_start[s] : 0, e = s < a.S ? a.query_start[s + 1] : 0;
+      bad = __ballot(!range_in(b, e, a.T));
+      end = __ballot(e == row + 1);
+    }
+    if (end && (!bad || __builtin_ctzll(end) < __builtin_ctzll(bad))) return;
+  } else if (row == 0 && slice == 0) {  // the sequences before that range, for the second launch
+    if (tid == 0) first_bad = a.S;
+    __syncthreads();
+    int bad = a.S;
+    for (int s = tid; s < a.S; s += Threads)
+      if (!range_in(a.query_start[s], a.query_start[s + 1], a.T)) bad = min(bad, s);
+    if (bad < a.S) atomicMin(&first_bad, bad);
+    __syncthreads();
+    if (tid == 0) *a.good = first_bad;
   }
   float top = x[0];
 #pragma unroll
@@ -509,7 +524,7 @@ using namespace abacus;
 
 extern "C" int64_t abacus_verify_drafts_ws_bytes(int64_t T, int64_t V, int64_t S) {
   const int64_t n = slices_of(V);
-  return (2 * T * n + S * mass_slices_of(V)) * 8 + 2 * T * n * 4 + 2 * T * 4 + T * n * 4 + S * 4;
+  return (2 * T * n + S * mass_slices_of(V)) * 8 + 2 * T * n * 4 + 2 * T * 4 + T * n * 4 + (S + 1) * 4;
 }
 
 extern "C" int abacus_verify_drafts(const void* target_TV, const void* draft_TV, const int64_t* tokens_T,
@@ -541,6 +556,7 @@ extern "C" int abacus_verify_drafts(const void* target_TV, const void* draft_TV,
   a.drafted = a.tops + 2 * T * n;
   a.at = (int*)(a.drafted + 2 * T);
   a.ended = a.at + T * n;
+  a.good = a.ended + S;
   hipStream_t s = (hipStream_t)stream;
   const dim3 rows((unsigned)n, (unsigned)T, a.draft ? 2 : 1), decide((unsigned)a.mass_slices, (unsigned)S);
   const bool bf = dtype == kBF16;

@@ -23,7 +23,8 @@ def verify_drafts(target_logits_TV: torch.Tensor, tokens_T: torch.Tensor, query_
     """How many drafts of each sequence are accepted, and the token that follows them.
 
     The rows of sequence s are query_start[s] .. query_start[s + 1] - 1 (int32, (S + 1,)): its last known token,
-    then its drafts (int64 tokens_T).  Row t of target_logits_TV, and of draft_logits_TV, is what the target, and
+    then its drafts (int64 tokens_T).  As in ``BatchRows``, from the first range that runs backwards or past the
+    rows on sequences have none.  Row t of target_logits_TV, and of draft_logits_TV, is what the target, and
     the drafter, say about the token after row t; draft_logits_TV of a sequence's last row is not read.  Without
     draft_logits_TV the drafts are taken as certain (a lookup, a greedy drafter).
 
@@ -92,10 +93,11 @@ def _softmax(row: torch.Tensor, temperature: float) -> torch.Tensor | None:
 @torch.no_grad()
 def _verify_cpu(target, tokens, start, uniforms, draft, temperature):
     T, V = target.shape
-    accepted, following = [], []
+    accepted, following, ended = [], [], False
     for s in range(len(start) - 1):
         first, end = start[s], start[s + 1]
-        if first < 0 or end > T:
+        ended = ended or first < 0 or end < first or end > T
+        if ended:
             end = first
         n, token = 0, -1
         for t in range(first, end):

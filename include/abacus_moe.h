@@ -475,7 +475,8 @@ int abacus_paged_attention(const void* q_THK, int64_t T, int64_t H, int64_t Hk, 
  * times the whole sum (p alone where every draft was accepted, or where the sum is 0).
  * temperature 0: a draft is accepted where it is the row's largest logit (the lowest
  * index of equals), and next is that one; uniforms_T2 and draft_TV are not read.
- * accepted_S: drafts accepted.  A sequence without rows gives 0 and -1; a row without
+ * accepted_S: drafts accepted.  A sequence without rows (all are from the first range on that
+ * runs backwards or out of [0, T], as for the cache) gives 0 and -1; a row without
  * a distribution (a NaN, +inf, or -inf throughout) accepts nothing and gives -1.
  * Exponentials and sums are in 64 bits.  ws: abacus_verify_drafts_ws_bytes bytes. */
 int64_t abacus_verify_drafts_ws_bytes(int64_t T, int64_t V, int64_t S);

@@ -145,6 +145,29 @@ def test_rows_without_a_distribution(device, temperature):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("temperature,drafter", [(0.9, True), (0.9, False), (0.0, False)])
+@pytest.mark.parametrize("start,T,good", [([0, 2, 0, 3], 3, 1), ([0, 5, 3, 8], 8, 1), ([0, 3, 1, 3, 4], 4, 1), ([0, 2, 5, 9, 8], 8, 2),
+                                          ([-1, 2, 4], 4, 0), ([0, 4, 4, 8, 0, 0], 8, 3), ([8, 8], 4, 0), ([1, 4, 3, 8], 8, 1),
+                                          ([0, *range(2, 301, 2), 6, 300], 300, 150), ([0, *[4] * 1100, 2, 8], 8, 1100)])
+def test_no_rows_from_the_first_bad_range_on(device, temperature, drafter, start, T, good):
+    """What comes before a range that runs backwards or past the rows is as without the rest, whose ranges share
+    its rows; the rest has none.  (What a kernel left out would be what the last call of these sizes wrote.)"""
+    V, S = 9001, len(start) - 1
+    g = torch.Generator().manual_seed(T)
+    target = (2 * torch.randn(T, V, generator=g)).to(device)
+    draft = target + 0.3 * torch.randn(T, V, generator=g).to(device) if drafter else None
+    tokens = target.argmax(-1).roll(1)
+    u = torch.rand(T, 2, generator=g).to(device) * torch.tensor([0.5, 1.0], device=device)
+    call = lambda start, draft: [x.tolist() for x in verify_drafts(
+        target, tokens, torch.tensor(start, dtype=torch.int32, device=device), u, draft, temperature)]
+    want = call(start[:good + 1] + [start[good]] * (S - good) if good else [0] * (S + 1), draft)
+    assert want[0][good:] == [0] * (S - good) and want[1][good:] == [-1] * (S - good)
+    for other in (draft, None if draft is None else draft.flip(0)):
+        call([0] * (S + 1), other)
+        assert call(start, draft) == want
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_tokens_are_distributed_as_the_target(device):
     """The first token that comes out of a sequence (its draft or what replaces it) has the target's probabilities:
     over n sequences a token's count is within 5 standard deviations, 5 sqrt(n p (1 - p))."""
