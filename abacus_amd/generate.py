@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import torch
 
-from .kv_cache import PagedKVCache
+from .kv_cache import E4M3, PagedKVCache
 from .speculative import verify_drafts
 from .transformer import TransformerMoe
 
@@ -60,9 +60,10 @@ def generate(model: TransformerMoe, prompts: list[list[int]], max_new_tokens: in
     """The tokens that follow each prompt: at most max_new_tokens, up to and with stop_token.
 
     temperature 0 takes the likeliest token each time; above it tokens are drawn with random numbers of `generator`
-    (on the model's device).  draft_model (the same vocabulary) proposes n_draft tokens a step, which changes how many
-    steps it takes and not what the tokens are distributed as.  cache_dtype: the model's own, or
-    torch.float8_e4m3fn.  Both models must be in eval mode.
+    (on the model's device).  draft_model (the same vocabulary; of any dtype that a cache holds, on any device) proposes
+    n_draft tokens a step, which changes how many steps it takes and not what the tokens are distributed as: its logits
+    take the model's dtype before tokens are drawn from them.  cache_dtype: the model's own, or torch.float8_e4m3fn
+    (the drafter's cache then too, otherwise that has its own).  Both models must be in eval mode.
     """
     if not prompts or any(len(p) == 0 for p in prompts):
         raise ValueError("prompts must hold at least one token each")
@@ -77,8 +78,8 @@ def generate(model: TransformerMoe, prompts: list[list[int]], max_new_tokens: in
     n_draft = 0 if draft_model is None else n_draft
     room = [end + n_draft for end in ends]
     target = _Side(model, room, page_size, cache_dtype)
-    drafter = None if draft_model is None else _Side(draft_model, room, page_size, cache_dtype)
-    device = target.device
+    drafter = None if draft_model is None else _Side(draft_model, room, page_size, E4M3 if cache_dtype == E4M3 else None)
+    device, dtype = target.device, model.w_D_vocab.dtype
     target.prefill(known, prefill_chunk)
     if drafter is not None:
         drafter.prefill(known, prefill_chunk)
@@ -87,7 +88,7 @@ def generate(model: TransformerMoe, prompts: list[list[int]], max_new_tokens: in
         drafts, draft_logits = {s: [] for s in active}, []
         for _ in range(n_draft):
             new = {s: (known[s] + drafts[s])[drafter.cache.length(drafter.seqs[s]):] for s in active}
-            logits = drafter.feed(new, dict.fromkeys(active, 1))
+            logits = drafter.feed(new, dict.fromkeys(active, 1)).to(device=device, dtype=dtype)
             draft_logits.append(logits)
             # one row a sequence and no drafts: a token drawn from each
             start = torch.arange(len(active) + 1, dtype=torch.int32, device=device)

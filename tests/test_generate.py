@@ -5,6 +5,7 @@ import torch
 
 from abacus_amd.generate import generate
 from abacus_amd.kv_cache import E4M3, BatchRows, PagedKVCache
+from abacus_amd.speculative import verify_drafts
 from abacus_amd.transformer import TransformerMoe
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -94,6 +95,37 @@ def test_drafts_change_the_steps_and_not_the_tokens(device, drafter, monkeypatch
     for a, b in zip(cut, plain):
         end = b.index(stop) + 1 if stop in b else 15
         assert a == b[:end]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype,other,cache_dtype", [(torch.float32, torch.bfloat16, None), (torch.bfloat16, torch.float32, torch.bfloat16),
+                                                     (torch.float32, torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16, E4M3)])
+def test_a_drafter_of_another_dtype(device, dtype, other, cache_dtype, monkeypatch):
+    """It changes how many steps it takes: greedy tokens stay, drawn ones (the first of 600 sequences of one prompt, whose
+    draft comes from the other model) have the probabilities p of the logits that are verified: a count is within
+    5 sqrt(sum p (1 - p)) of sum p over the sequences."""
+    model, drafter = _model(device=device, dtype=dtype), _model(seed=9, dim=16, heads=1, blocks=1, device=device, dtype=other)
+    plain = generate(model, [[1, 2, 3], [7]], 6, page_size=16, cache_dtype=cache_dtype)
+    drafted = generate(model, [[1, 2, 3], [7]], 6, page_size=16, cache_dtype=cache_dtype, draft_model=drafter, n_draft=2)
+    assert [len(t) for t in drafted] == [6, 6]
+    if dtype == torch.float32 and cache_dtype != E4M3:
+        assert drafted == plain
+    n, calls = 600, []
+    verify = verify_drafts
+    monkeypatch.setattr("abacus_amd.generate.verify_drafts", lambda *a: (calls.append(a[0]), verify(*a))[1])
+    got = generate(model, [[3, 4]] * n, 1, temperature=0.9, page_size=16, cache_dtype=cache_dtype, draft_model=drafter, n_draft=1,
+                   generator=torch.Generator(device=device).manual_seed(1))
+    counts = torch.bincount(torch.tensor(got)[:, 0], minlength=50).double()
+    p = torch.softmax(calls[-1][::2].double() / 0.9, -1).cpu()  # rows: the prompt's last token, the draft
+    assert p.shape == (n, 50) and ((counts - p.sum(0)).abs() <= 5 * torch.sqrt((p * (1 - p)).sum(0))).all()
+
+
+@pytest.mark.gpu
+def test_a_drafter_on_another_device():
+    model, drafter = _model(device="cuda"), _model(seed=9, dim=16, heads=1, blocks=1)
+    prompts = [[1, 2, 3], [7]]
+    assert generate(model, prompts, 6, page_size=16, draft_model=drafter, n_draft=2) == generate(model, prompts, 6, page_size=16)
+    assert [len(t) for t in generate(model, prompts, 6, page_size=16, temperature=0.9, draft_model=drafter, n_draft=2)] == [6, 6]
 
 
 @pytest.mark.parametrize("device", DEVICES)
