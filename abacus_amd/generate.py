@@ -89,13 +89,18 @@ def generate(model: TransformerMoe, prompts: list[list[int]], max_new_tokens: in
         for _ in range(n_draft):
             new = {s: (known[s] + drafts[s])[drafter.cache.length(drafter.seqs[s]):] for s in active}
             logits = drafter.feed(new, dict.fromkeys(active, 1)).to(device=device, dtype=dtype)
-            draft_logits.append(logits)
             # one row a sequence and no drafts: a token drawn from each
             start = torch.arange(len(active) + 1, dtype=torch.int32, device=device)
             _, drawn = verify_drafts(logits, torch.zeros(len(active), dtype=torch.int64, device=device), start,
                                      _uniforms(len(active), temperature, generator, device), None, temperature)
-            for s, x in zip(active, drawn.tolist()):
-                drafts[s].append(max(x, 0))  # (-1, a row without a distribution: any token, it will not be accepted)
+            proposals = drawn.tolist()
+            if min(proposals) < 0:  # a row without a distribution proposes token 0, with certainty
+                certain = torch.full_like(logits[:1], -torch.inf)
+                certain[:, 0] = 0.0
+                logits = torch.where(drawn[:, None] < 0, certain, logits)
+            draft_logits.append(logits)
+            for s, x in zip(active, proposals):
+                drafts[s].append(max(x, 0))
         logits = target.feed({s: [known[s][-1], *drafts[s]] for s in active}, dict.fromkeys(active, n_draft + 1))
         T = len(active) * (n_draft + 1)
         tokens = torch.tensor([x for s in active for x in (known[s][-1], *drafts[s])], dtype=torch.int64).to(device)

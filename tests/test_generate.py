@@ -1,5 +1,7 @@
 """forward_cached and generate: the cached forward against the whole one, and the decoding loop with and without drafts."""
 
+import math
+
 import pytest
 import torch
 
@@ -118,6 +120,34 @@ def test_a_drafter_of_another_dtype(device, dtype, other, cache_dtype, monkeypat
     counts = torch.bincount(torch.tensor(got)[:, 0], minlength=50).double()
     p = torch.softmax(calls[-1][::2].double() / 0.9, -1).cpu()  # rows: the prompt's last token, the draft
     assert p.shape == (n, 50) and ((counts - p.sum(0)).abs() <= 5 * torch.sqrt((p * (1 - p)).sum(0))).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("bad", ["every row", "some rows"])
+def test_a_drafter_without_a_distribution(device, bad, monkeypatch):
+    """Its rows of NaN propose some token: greedy tokens stay, and drawn ones have the probabilities of the logits that are
+    verified (a count within 5 sqrt(sum p (1 - p)) of sum p).  The model's own rows of NaN are an error."""
+    model, drafter = _model(device=device), _model(seed=9, dim=16, heads=1, blocks=1, device=device)
+    def spoil(module, args, out):
+        out = out.clone()
+        out[::1 if bad == "every row" else 2] = math.nan
+        return out
+
+    drafter.norm.register_forward_hook(spoil)  # (the last one, before the logits)
+    prompts = [[1, 2, 3], [7], [8]]
+    assert generate(model, prompts, 9, page_size=16, draft_model=drafter) == generate(model, prompts, 9, page_size=16)
+    n, calls = 600, []
+    verify = verify_drafts
+    monkeypatch.setattr("abacus_amd.generate.verify_drafts", lambda *a: (calls.append(a[0]), verify(*a))[1])
+    got = generate(model, [[3, 4]] * n, 1, temperature=1.5, page_size=16, draft_model=drafter, n_draft=2,
+                   generator=torch.Generator(device=device).manual_seed(1))
+    counts = torch.bincount(torch.tensor(got)[:, 0], minlength=50).double()
+    p = torch.softmax(calls[-1][::3].double() / 1.5, -1).cpu()
+    assert p.shape == (n, 50) and ((counts - p.sum(0)).abs() <= 5 * torch.sqrt((p * (1 - p)).sum(0))).all()
+    with torch.no_grad():
+        model.w_D_vocab.fill_(math.nan)
+    with pytest.raises(RuntimeError, match="no distribution"):
+        generate(model, prompts, 2, page_size=16, temperature=0.9, draft_model=_model(device=device))
 
 
 @pytest.mark.gpu
