@@ -723,9 +723,9 @@ class MultiHeadAttention(torch.nn.Module):
 
     def _norm_rope(self, q_THK, k_THK, cos_TK, sin_TK):
         """The q and k norms and the rotary embedding, row t at the tables' row t."""
-        gamma_q, gamma_k = self.q_norm.w_gamma_D, self.k_norm.w_gamma_D
-        if cos_TK is None:
+        if cos_TK is None:  # (norms of any module)
             return self.q_norm(q_THK), self.k_norm(k_THK)
+        gamma_q, gamma_k = self.q_norm.w_gamma_D, self.k_norm.w_gamma_D
         if not (_fused_rope_ok(q_THK, gamma_q, cos_TK, sin_TK) and _fused_rope_ok(k_THK, gamma_k, cos_TK, sin_TK)):
             return apply_rotary_pos_emb(self.q_norm(q_THK), self.k_norm(k_THK), cos_TK[:, None], sin_TK[:, None])
         T, H, K = q_THK.shape

@@ -8,7 +8,7 @@ import torch
 from abacus_amd.generate import generate
 from abacus_amd.kv_cache import E4M3, BatchRows, PagedKVCache
 from abacus_amd.speculative import verify_drafts
-from abacus_amd.transformer import TransformerMoe
+from abacus_amd.transformer import MultiHeadAttention, TransformerMoe
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -174,6 +174,23 @@ def test_quantised_cache_runs(device):
     model = _model(device=device, head_dim=64)
     got = generate(model, [[5, 6], [1]], 6, page_size=16, cache_dtype=E4M3)
     assert [len(t) for t in got] == [6, 6]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_norms_of_any_module_without_a_rotary_embedding(device):
+    """As in forward: fp32, five products one after another of at most 32 terms each, 5 * 32 * 2^-24 = 1e-5 of the sums of
+    magnitudes, which are less than 10 times the largest output."""
+    torch.manual_seed(0)
+    attention = MultiHeadAttention(32, 2, 16).eval()
+    attention.q_norm, attention.k_norm = torch.nn.Identity(), torch.nn.LayerNorm(16)
+    attention = attention.to(device)
+    x = torch.randn(9, 32, device=device)
+    cache = PagedKVCache(1, 1, 16, 2, 16, dtype=torch.float32, device=device)
+    seq = cache.add()
+    with torch.no_grad():
+        want = attention(x[None])[0]
+    got = torch.cat([attention.forward_cached(x[a:b], cache.layer(0), cache.extend({seq: b - a})) for a, b in ((0, 5), (5, 9))])
+    assert float((got - want).abs().max()) <= 1e-4 * float(want.abs().max())
 
 
 def test_refusals():
