@@ -731,8 +731,9 @@ class MultiHeadAttention(torch.nn.Module):
         T, H, K = q_THK.shape
         qn, kn = torch.empty_like(q_THK), torch.empty_like(k_THK)
         rstd = torch.empty(2, T * H, dtype=torch.float32, device=q_THK.device)
-        _lib.call("abacus_qk_norm_rope_fwd", _lib.ptr(_contig(q_THK)), _lib.ptr(_contig(k_THK)), _lib.ptr(_contig(gamma_q)),
-                  _lib.ptr(_contig(gamma_k)), _lib.ptr(_contig(cos_TK)), _lib.ptr(_contig(sin_TK)), T * H, T, H, K, 1e-5,
+        # (copies, if any are needed, are held until the call is made: the next would take the place of one let go)
+        operands = [_contig(t) for t in (q_THK, k_THK, gamma_q, gamma_k, cos_TK, sin_TK)]
+        _lib.call("abacus_qk_norm_rope_fwd", *map(_lib.ptr, operands), T * H, T, H, K, 1e-5,
                   _lib.dtype_code(q_THK.dtype), _lib.ptr(qn), _lib.ptr(kn), _lib.ptr(rstd), _lib.stream_of(q_THK.device))
         return qn, kn
 

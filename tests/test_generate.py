@@ -193,6 +193,31 @@ def test_norms_of_any_module_without_a_rotary_embedding(device):
     assert float((got - want).abs().max()) <= 1e-4 * float(want.abs().max())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_weights_and_tables_at_any_element(dtype):
+    """Parameters that are views into one flat buffer, and tables likewise: each is copied to where the kernel can read it
+    and stays there until it has."""
+    torch.manual_seed(0)
+    attention = MultiHeadAttention(32, 2, 64).eval().to(dtype).cuda()
+    x = torch.randn(9, 32, device="cuda").to(dtype)
+    angles = torch.randn(9, 64, device="cuda")
+    parts = [1 + torch.rand(64, device="cuda"), 3 - torch.rand(64, device="cuda"), angles.cos(), angles.sin()]
+    results = []
+    for offset in (0, 1):
+        views = []
+        flat = torch.empty(sum(t.numel() for t in parts) + offset, device="cuda", dtype=dtype)
+        for t in parts:
+            at = offset + sum(v.numel() for v in views)
+            views.append(flat[at:at + t.numel()].view(t.shape).copy_(t))
+        attention.q_norm.w_gamma_D, attention.k_norm.w_gamma_D = (torch.nn.Parameter(v) for v in views[:2])
+        assert (attention.q_norm.w_gamma_D.data_ptr() % 16 == 0) == (offset == 0)
+        cache = PagedKVCache(1, 1, 16, 2, 64, dtype=dtype, device="cuda")
+        rows = cache.extend({cache.add(): 9})
+        results.append(attention.forward_cached(x, cache.layer(0), rows, *views[2:]))
+    assert torch.equal(*results)
+
+
 def test_refusals():
     model = _model()
     cache = PagedKVCache(2, 4, 16, 2, 16, dtype=torch.float32)
