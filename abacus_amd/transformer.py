@@ -528,9 +528,9 @@ class _AttentionFunction(torch.autograd.Function):
         qn, kn, o = torch.empty_like(q), torch.empty_like(k), torch.empty_like(q)
         rstd = torch.empty(2, rows, dtype=torch.float32, device=dev)
         lse = torch.empty(B, H, L, dtype=torch.float32, device=dev)
-        _lib.call("abacus_qk_norm_rope_fwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(gamma_q.contiguous()),
-                  _lib.ptr(gamma_k.contiguous()), _lib.ptr(cos_c), _lib.ptr(sin_c), rows, L, H, K, eps, _lib.BF16, _lib.ptr(qn), _lib.ptr(kn),
-                  _lib.ptr(rstd), s)
+        gammas = gamma_q.contiguous(), gamma_k.contiguous()  # (held: a copy let go gives its place to the next)
+        _lib.call("abacus_qk_norm_rope_fwd", _lib.ptr(q), _lib.ptr(k), *map(_lib.ptr, gammas), _lib.ptr(cos_c), _lib.ptr(sin_c),
+                  rows, L, H, K, eps, _lib.BF16, _lib.ptr(qn), _lib.ptr(kn), _lib.ptr(rstd), s)
         _lib.call("abacus_attention_any_fwd", _lib.ptr(qn), _lib.ptr(kn), _lib.ptr(v), B, L, H, K,
                   1.0 / math.sqrt(K), _lib.BF16, _lib.ptr(o), _lib.ptr(lse), s)
         ctx.save_for_backward(x_BLD, w_q, w_k, w_v, gamma_q, gamma_k, cos_c, sin_c, q, k, v, qn, kn, o, rstd, lse)

@@ -207,6 +207,27 @@ def test_rmsnorm_rope_matches_fp64(dtype, shape):
         assert _rel(a, t) <= max(2 * _rel(r, t), rtol), f"{name}: gpu {_rel(a, t):.3g} vs cpu {_rel(r, t):.3g}"
 
 
+def test_strided_norm_weights_of_the_joint_attention_node():
+    """q and k norm weights that are columns of one tensor: the attention and its gradients are bit for bit those of
+    contiguous ones (copies of both are there while their kernel runs)."""
+    from abacus_amd.transformer import MultiHeadAttention, Rotary
+
+    torch.manual_seed(0)
+    attention, rotary = MultiHeadAttention(64, 2, 64).bfloat16().cuda(), Rotary(64).bfloat16().cuda()
+    x, dy = torch.randn(2, 2, 40, 64, device="cuda").bfloat16()
+    columns = (0.5 + torch.rand(64, 2, device="cuda")).bfloat16()
+    results = []
+    for joined in (False, True):
+        gammas = [c if joined else c.contiguous() for c in columns.clone().unbind(1)]
+        attention.q_norm.w_gamma_D, attention.k_norm.w_gamma_D = map(torch.nn.Parameter, gammas)
+        assert attention.k_norm.w_gamma_D.is_contiguous() != joined
+        attention.zero_grad()
+        out = attention(x, rotary)
+        out.backward(dy)
+        results.append([out.detach(), *(p.grad.clone() for p in attention.parameters())])
+    assert len(results[0]) == 7 and all(torch.equal(a, b) for a, b in zip(*results))
+
+
 def test_trainer_step_matches_train_step():
     """abacus.trainer.Trainer(model).step (trainer.py:58-97, one process) is train_step with the
     reference's AdamW defaults: the same losses, parameters and moments over two steps; with
