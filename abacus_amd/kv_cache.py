@@ -22,6 +22,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .moe import _contig
@@ -49,9 +50,12 @@ def _index(name: str, t: torch.Tensor, shape: tuple[int, ...], device: torch.dev
     return t
 
 
-def _no_gradient(name: str) -> None:
-    if torch.is_grad_enabled():
+def _no_gradient(name: str, *tensors: torch.Tensor) -> None:
+    """Refuses tensors whose derivative a call would drop: backward's where it is recorded, forward mode's always."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} requires a gradient, and a cache gives none: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has a forward-mode tangent, and a cache carries none")
 
 
 class BatchRows:
@@ -168,9 +172,13 @@ class KVPages:
                             "(float32 or bfloat16) or float8_e4m3fn")
         if x.device != self.device or rows.device != self.device:
             raise ValueError(f"{name}, the rows and the pages must be on one device")
-        if x.requires_grad:
-            _no_gradient(name)
+        self._no_gradient(name, x)
         return shape
+
+    def _no_gradient(self, name: str, x: torch.Tensor) -> None:
+        if x.requires_grad or self.k.requires_grad or self.v.requires_grad or forward_ad._current_level >= 0:
+            _no_gradient(name, x)
+            _no_gradient("the cache", self.k, self.v)
 
     def _rows_args(self, rows: BatchRows) -> tuple:
         return (rows.page_table_SP.data_ptr(), rows.query_start.data_ptr(), rows.lengths.data_ptr(), *rows._sizes,
@@ -185,8 +193,7 @@ class KVPages:
         T, H, K = self._check("k", k_THK, rows, self.n_heads)
         if v_THK.shape != k_THK.shape or v_THK.dtype != k_THK.dtype or v_THK.device != self.device:
             raise ValueError("k and v must have one shape, dtype and device")
-        if v_THK.requires_grad:
-            _no_gradient("v")
+        self._no_gradient("v", v_THK)
         if not k_THK.is_cuda:
             return self._write_cpu(k_THK, v_THK, rows)
         k_THK, v_THK = _contig(k_THK), _contig(v_THK)
@@ -206,6 +213,7 @@ class KVPages:
             raise ValueError("the rows and the pages must be on one device")
         if length < 0:
             raise ValueError(f"length must not be negative, got {length}")
+        self._no_gradient("the cache", self.k)
         S, P = rows._sizes
         shape = (S, length, self.n_heads, self.head_dim)
         if not self.k.is_cuda:
@@ -225,7 +233,8 @@ class KVPages:
         left as they are there.
 
         Statistics and sums are fp32; with bf16 queries the probabilities are rounded to bf16 for the product
-        with the values, as the training kernels do.  No gradient is formed: rows that ask for one are refused."""
+        with the values, as the training kernels do.  No gradient is formed: rows, pages or an ``out`` that ask for one
+        are refused, and so are forward-mode tangents."""
         T, H, K = self._check("q", q_THK, rows, None)
         if H % self.n_heads or H < 1 or H > 1024:
             raise ValueError(f"{H} query heads over {self.n_heads} key heads: they must be a multiple (at most 1024)")
@@ -237,6 +246,7 @@ class KVPages:
                 raise ValueError("out must have q's shape, dtype and device")
             if not out.is_contiguous() or out.data_ptr() % 16:
                 raise ValueError("out must be contiguous and 16-byte aligned")
+            _no_gradient("out", out)
         if not q_THK.is_cuda:
             return self._attend_cpu(q_THK, rows, scale, out)
         q, code = _contig(q_THK), _CODES[q_THK.dtype]

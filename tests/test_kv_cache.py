@@ -120,6 +120,31 @@ def test_no_gradient():
             call()
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_no_gradient_of_pages_outputs_and_forward_mode(device):
+    """What a call would drop silently is refused: the gradient of pages and of `out`, and tangents, which no_grad keeps."""
+    forward_ad = torch.autograd.forward_ad
+    rows, n = pc.rows_of([(2, 5)], 16, device)
+    pages = pc.pages_of(n, 2, 16, 16, torch.float32, device)
+    x = torch.ones(2, 2, 16, device=device)
+    leaves = [KVPages(pages.k.clone().requires_grad_(), pages.v), KVPages(pages.k, pages.v.clone().requires_grad_())]
+    out = torch.empty_like(x).requires_grad_()
+    for call in (*(lambda p=p: p.attend(x, rows) for p in leaves), *(lambda p=p: p.read(rows, 5) for p in leaves),
+                 *(lambda p=p: p.write(x, x, rows) for p in leaves), lambda: pages.attend(x, rows, out=out)):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            call()
+        with torch.no_grad():
+            call()
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x)
+        held = KVPages(pages.k, forward_ad.make_dual(pages.v, pages.v))
+        for call in (lambda: pages.attend(dual, rows), lambda: pages.write(dual, x, rows), lambda: pages.write(x, dual, rows),
+                     lambda: held.attend(x, rows), lambda: held.read(rows, 5), lambda: held.write(x, x, rows)):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                call()
+        pages.attend(x, rows)
+
+
 def test_no_rows_after_a_range_that_runs_backwards():
     """Overlapping ranges would be more rows than the call has: what comes after the bad range has none."""
     rows, n = pc.rows_of([(2, 2), (0, 0), (2, 2)], 16, "cpu")
