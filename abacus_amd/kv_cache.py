@@ -232,7 +232,9 @@ class KVPages:
         a page outside the pool NaN.  Rows of no sequence give 0, or with ``out`` (T, G * heads, head_dim) are
         left as they are there.
 
-        Statistics and sums are fp32; with bf16 queries the probabilities are rounded to bf16 for the product
+        Statistics and sums are fp32, and a sum is divided once it is whole, with weights of up to 2^8: it is finite as
+        long as the largest |v| times 2^8 times the positions seen is below 2^128 (|v| to 2^100 at 2^20 positions), and
+        the products q . k, which are scaled after they are formed, are below 2^128 too.  With bf16 queries the probabilities are rounded to bf16 for the product
         with the values, as the training kernels do.  No gradient is formed: rows, pages or an ``out`` that ask for one
         are refused, and so are forward-mode tangents."""
         T, H, K = self._check("q", q_THK, rows, None)

@@ -452,8 +452,9 @@ int abacus_kv_read(const int32_t* page_table_SP, const int32_t* lengths, int64_t
 
 /* Attention of the T rows q_THK (T, H, K) over the pages of Hk heads, query head h with
  * key head h / (H / Hk): o = softmax(scale q k^T) v over the positions up to the row's
- * own, statistics and sums in fp32, probabilities rounded to bf16 where q is bf16; a
- * row that sees nothing gives 0.  max_new: the most rows of one sequence, as far as the
+ * own, statistics and sums in fp32, probabilities rounded to bf16 where q is bf16 (sums
+ * are divided once they are whole: finite while max|v| * 2^8 * positions and |q . k| are below
+ * 2^128); a row that sees nothing gives 0.  max_new: the most rows of one sequence, as far as the
  * caller knows (T otherwise); it chooses the kernels and changes no result beyond
  * rounding.  zero_rest: rows of no sequence become 0 (otherwise they are left as they
  * are).  ws: device workspace of abacus_paged_attention_ws_bytes bytes. */

@@ -241,6 +241,23 @@ def test_large_scores(held):
     _check(pages, plan, rows, k, v, q, pages.attend(q, rows), held)
 
 
+@pytest.mark.parametrize("dtype,held", KINDS)
+@pytest.mark.parametrize("exponent", [-100, 107])
+@pytest.mark.parametrize("plan", [[(2, 600), (1, 9)], [(70, 500)]])
+def test_small_and_large_values(dtype, held, exponent, plan):
+    """Values up to the documented limit (7 * 2^107 < 2^110, and 2^110 * 2^8 * 600 < 2^128) under scores that grow late,
+    and ones whose products with small probabilities are still normal numbers."""
+    pages, rows, k, v, g = _filled(plan, 2, 64, 16, dtype, held)
+    at = torch.arange(k.shape[0], device="cuda") / k.shape[0]
+    k = (k.float() * (0.5 + at[:, None, None])).to(dtype)
+    v = (v.float().clamp(-7, 7) * 2.0 ** exponent).to(dtype)
+    lengths = [length for _, length in plan]
+    whole = BatchRows(rows.page_table_SP, torch.tensor([0] + lengths).cumsum(0).to(torch.int32).cuda(), rows.lengths)
+    pages.write(k, v, whole)
+    q = 3 * torch.randn(sum(n for n, _ in plan), 4, 64, device="cuda", generator=g).to(dtype)
+    _check(pages, plan, rows, k, v, q, pages.attend(q, rows), held)
+
+
 def test_refused_by_the_pages_on_the_device():
     """Page ids outside the pool, lengths past the table, ranges of rows outside the batch: NaN or nothing, as on the
     CPU (test_kv_cache.py)."""
