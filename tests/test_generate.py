@@ -5,8 +5,9 @@ import math
 import pytest
 import torch
 
+import paged_check as pc
 from abacus_amd.generate import generate
-from abacus_amd.kv_cache import E4M3, BatchRows, PagedKVCache
+from abacus_amd.kv_cache import E4M3, BatchRows, KVPages, PagedKVCache
 from abacus_amd.speculative import verify_drafts
 from abacus_amd.transformer import MultiHeadAttention, TransformerMoe
 
@@ -216,6 +217,36 @@ def test_norm_weights_and_tables_at_any_element(dtype):
         rows = cache.extend({cache.add(): 9})
         results.append(attention.forward_cached(x, cache.layer(0), rows, *views[2:]))
     assert torch.equal(*results)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantised_cache_is_one_of_the_values_its_codes_stand_for(device, dtype, monkeypatch):
+    """The cached forward over e4m3 pages against the same over unquantised pages that are given what e4m3 holds of each
+    row.  One block, so both write the same rows.  fp32: five products of at most 61 terms, 5 * 64 * 2^-24 = 2e-5 of sums of
+    magnitudes less than 5 times the largest logit.  bf16: the attention's output rounds apart, by 2^-8, and what follows
+    rounds twice more (the projection, the residual): 3 * 2^-8 of the norm."""
+    model = _model(device=device, dtype=dtype, blocks=1, head_dim=64)
+    g = torch.Generator().manual_seed(1)
+    seqs = [torch.randint(0, 50, (n,), generator=g).tolist() for n in (37, 5, 61)]
+    write = KVPages.write
+    quantised = lambda x: pc.held(x.cpu(), E4M3).to(x.device, x.dtype)
+    outs = []
+    for held in (E4M3, dtype):
+        if held != E4M3:
+            monkeypatch.setattr(KVPages, "write", lambda self, k, v, rows: write(self, quantised(k), quantised(v), rows))
+        cache = PagedKVCache(1, 12, 16, 2, 64, dtype=held, device=device)
+        ids, at, logits = [cache.add() for _ in seqs], [0, 0, 0], []
+        for step in ((30, 1, 60), (1, 1, 0), (4, 1, 1), (2, 2, 0)):
+            tokens = [x for i, n in enumerate(step) for x in seqs[i][at[i]:at[i] + n]]
+            logits.append(model.forward_cached(torch.tensor(tokens, device=device), cache, cache.extend(dict(zip(ids, step)))))
+            at = [a + n for a, n in zip(at, step)]
+        outs.append(torch.cat(logits).double())
+    got, want = outs
+    if dtype == torch.float32:
+        assert float((got - want).abs().max()) <= 1e-4 * float(want.abs().max())
+    else:
+        assert float((got - want).norm()) <= 3 * 2.0 ** -8 * float(want.norm())
 
 
 def test_refusals():

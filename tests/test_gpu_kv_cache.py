@@ -77,6 +77,36 @@ def test_write_and_read(dtype, held, K, page):
 
 
 @pytest.mark.parametrize("dtype,held", KINDS)
+@pytest.mark.parametrize("H,K,page,L", [(2, 16, 16, 333), (3, 80, 64, 290), (1, 128, 256, 705)])
+def test_read_of_many_sequences(dtype, held, H, K, page, L):
+    """Blocks of four groups (2048 of them and more): ragged sequences, empty ones, some longer than what is read, a last
+    block that is not full, pages outside the pool and a length past its table."""
+    S = 220
+    plan = [(n, n) for n in ((s * 53) % (L + 40) if s % 9 else 0 for s in range(S))]
+    assert (-(-L // 64)) * H * S >= 2048 and L % 64
+    pages, rows, k, v, _ = _filled(plan, H, K, page, dtype, held, fill=0x55 if held == E4M3 else 3.0)
+    rows.page_table_SP[7, 2], rows.page_table_SP[8, 0] = -1, len(pages.k)
+    width = rows.page_table_SP.shape[1]
+    rows.lengths[12] = width * page + 1
+    kr, vr = pages.read(rows, L, torch.float32 if held == E4M3 else None)
+    at = 0
+    for s, (_, length) in enumerate(plan):
+        n = min(length, L)
+        bad = torch.zeros(L, dtype=torch.bool, device="cuda")
+        if s == 7:
+            bad[2 * page:3 * page] = True
+        if s in (8, 12):
+            bad[:page if s == 8 else min(width * page, L)] = True
+        there = torch.arange(L, device="cuda") < (L if s == 12 else n)
+        for got, x in ((kr[s], k), (vr[s], v)):
+            assert torch.equal(torch.isnan(got).all(-1).all(-1), bad & there)
+            fine = ~bad & (torch.arange(L, device="cuda") < n)
+            assert torch.equal(got[fine].double(), pc.held(x[at:at + n], held)[fine[:n]])
+            assert not got[~there].any()
+        at += length
+
+
+@pytest.mark.parametrize("dtype,held", KINDS)
 @pytest.mark.parametrize("H,G,K,page,plan", [
     (2, 1, 64, 16, [(1, 1), (1, 2), (1, 63), (1, 64), (1, 65), (1, 700)]),
     (1, 4, 128, 64, [(1, 1500), (1, 40), (0, 9)]),

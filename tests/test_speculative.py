@@ -67,6 +67,97 @@ def test_matches_the_restatement(device, dtype, V, sizes, drafter, temperature):
         assert got[0].tolist() == want[0] and got[1].tolist() == want[1]
 
 
+def _restated64(target, tokens, start, u, draft, temperature):
+    """The same in torch's 64-bit operations, for large vocabularies; p itself where p - q leaves nothing."""
+    V, accepted, following = target.shape[1], [], []
+    for a, b in zip(start, start[1:]):
+        n, token = 0, -1
+        for t in range(a, b):
+            x = tokens[t + 1] if t + 1 < b else None
+            p = torch.softmax(target[t].double() / temperature, 0)
+            q = torch.zeros_like(p)
+            if x is not None and draft is not None:
+                q = torch.softmax(draft[t].double() / temperature, 0)
+            elif x is not None and 0 <= x < V:
+                q[x] = 1.0
+            if x is not None and 0 <= x < V and u[t][0] * float(q[x]) < float(p[x]):
+                n += 1
+                continue
+            mass = (p - q).clamp(min=0.0)
+            upto = (mass if float(mass.sum()) > 0 else p).cumsum(0)
+            token = int((upto <= u[t][1] * float(upto[-1])).sum())
+            break
+        accepted.append(n)
+        following.append(token)
+    return accepted, following
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,sizes,drafter", [
+    (9001, [4] * 40, True),       # blocks enough for 32 logits a thread, a slice that is not full
+    (8193, [3] * 100, False),
+    (300007, [3, 1], True),       # more than 64 slices of the second launch
+    (600011, [2, 2], True),       # and of the first
+    (600011, [3], False),
+    (5003, [41, 33, 2], True),    # more rows than a block keeps
+])
+def test_sizes_that_other_launches_serve(device, dtype, V, sizes, drafter):
+    g = torch.Generator().manual_seed(V)
+    T = sum(sizes)
+    start = torch.tensor([0, *sizes]).cumsum(0).to(torch.int32)
+    target = (3 * torch.randn(T, V, generator=g)).to(dtype)
+    draft = (target.float() + 0.2 * torch.randn(T, V, generator=g)).to(dtype) if drafter else None
+    tokens = (draft if drafter else target).float().argmax(-1).roll(1)  # likely ones: long runs are accepted
+    accepted = []
+    for seed in range(3):
+        u = torch.rand(T, 2, generator=g.manual_seed(seed))
+        if max(sizes) > 32:
+            u[:, 0] *= 0.02 * (seed + 1)  # a rejection late in the long sequences, or none
+        if seed == 2:
+            tokens[start[1:-1].long() - 1] = V - 1  # an unlikely last draft
+        want = _restated64(target, tokens.tolist(), start.tolist(), u.tolist(), draft, 0.8)
+        got = verify_drafts(target.to(device), tokens.to(device), start.to(device), u.to(device),
+                            draft.to(device) if drafter else None, 0.8)
+        assert (got[0].tolist(), got[1].tolist()) == want
+        accepted += want[0]
+    assert max(sizes) <= 32 or max(accepted) > 32
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [3000, 9001, 300007])
+def test_no_mass_is_left_of_the_difference(device, dtype, V):
+    """A draft outside the vocabulary from a drafter that agrees with the target: the next token is drawn from p."""
+    g = torch.Generator().manual_seed(V)
+    target = (2 * torch.randn(3, V, generator=g)).to(dtype)
+    tokens, start = torch.tensor([0, V, 1]), torch.tensor([0, 2, 3], dtype=torch.int32)
+    for u1 in (0.0, 0.3, 0.77, 1.0 - 2.0 ** -24):
+        u = torch.tensor([[0.0, u1], [0.0, 0.0], [0.0, u1]])
+        want = _restated64(target, tokens.tolist(), start.tolist(), u.tolist(), target, 1.1)
+        got = verify_drafts(target.to(device), tokens.to(device), start.to(device), u.to(device), target.to(device), 1.1)
+        assert (got[0].tolist(), got[1].tolist()) == want and want[0] == [0, 0]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V,T", [(600011, 3), (9001, 300)])
+def test_temperature_zero_over_many_slices(device, dtype, V, T):
+    """The lowest of the largest logits, wherever its slice is; a NaN in the last slice is found."""
+    g = torch.Generator().manual_seed(V)
+    target = torch.randn(T, V, generator=g).to(dtype)
+    at = torch.randint(0, V, (T, 2), generator=g)
+    target.scatter_(1, at, 50.0)
+    target[T - 1, V - 1] = math.nan
+    best = at.amin(1)
+    start = torch.arange(T + 1, dtype=torch.int32)
+    got = verify_drafts(target.to(device), torch.zeros(T, dtype=torch.int64, device=device), start.to(device), temperature=0.0)
+    assert not got[0].any() and got[1].tolist() == [*best[:-1].tolist(), -1]
+    one = torch.tensor([0, T], dtype=torch.int32, device=device)
+    got = verify_drafts(target.to(device), best.roll(1).to(device), one, temperature=0.0)
+    assert (got[0].item(), got[1].item()) == (T - 1, -1)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("drafter", [False, True])
 @pytest.mark.parametrize("temperature", [1e-3, 1e-15, 1e-30, 1e-310, 1e30])
