@@ -311,8 +311,10 @@ extern "C" int abacus_paged_attention(const void* q_THK, int64_t T, int64_t H, i
   const int64_t need = (n.few.floats(Hk, K) + n.many.floats(Hk, K)) * 4;
   ABACUS_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "paged_attention: workspace of %lld bytes, need %lld",
                    (long long)ws_bytes, (long long)need);
-  ABACUS_CHECK_ARG(n.few.items * Hk < (1ll << 31), "paged_attention: %lld rows of %lld heads are too many", (long long)T,
-                   (long long)H);
+  // a launch holds fewer than 2^32 threads, 256 to a block
+  ABACUS_CHECK_ARG((n.few.items + (n.many.R > 0 ? n.many.items : 0)) * Hk < (1ll << 24),
+                   "paged_attention: %lld rows of %lld heads in %lld sequences are too many", (long long)T, (long long)H,
+                   (long long)S);
   PagedArgs p;
   p.a = PagedRows{page_table_SP, query_start, lengths, (int)S, (int)P, (int)T, __builtin_ctzll(page_size), (int)n_pages};
   p.q = q_THK, p.k = k_pages, p.v = v_pages;

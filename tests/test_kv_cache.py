@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import paged_check as pc
+from abacus_amd import _lib
 from abacus_amd.kv_cache import E4M3, BatchRows, KVPages, PagedKVCache
 
 PLANS = [[(1, 1)], [(3, 3), (1, 40), (0, 17), (5, 21)], [(2, 0 + 2), (0, 0), (33, 50)]]
@@ -229,6 +230,16 @@ def test_refusals():
         BatchRows(rows.page_table_SP, rows.query_start[:1], rows.lengths)
     with pytest.raises(ValueError, match="max_new"):
         BatchRows(rows.page_table_SP, rows.query_start, rows.lengths, max_new=0)
+
+
+@pytest.mark.parametrize("dtype", [_lib.F32, _lib.BF16])
+def test_more_blocks_than_a_launch_holds_are_refused(dtype):
+    """2^30 (row, head) pairs of single tokens, 256 threads each: a launch has at most 2^32 threads."""
+    T = S = 1 << 20
+    assert _lib.query("abacus_paged_attention_ws_bytes", T, 1024, 1024, 64, dtype, dtype, S, 1, 16, 1) == 0
+    with pytest.raises(RuntimeError, match="too many"):
+        _lib.call("abacus_paged_attention", 16, T, 1024, 1024, 64, dtype, 16, 16, 16, S, 1, 16, 1, dtype, 16, 16, None, None, 0.125,
+                  1, 1, 16, None, 0, None)
 
 
 def test_bookkeeping():
