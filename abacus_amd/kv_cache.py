@@ -123,7 +123,8 @@ class KVPages:
     code * 2^(byte - 127), the byte the least that keeps the row's largest magnitude within 448.  Where a key or a
     value of a token's head holds an infinity or NaN, e4m3 pages give NaN for both.
 
-    page_size is a power of two from 16 to 256, head_dim a multiple of 16 up to 128.
+    page_size is a power of two from 16 to 256, head_dim a multiple of 16 up to 128.  The tensors stay where they are:
+    once one has been given other memory (``.data``, ``resize_``), calls are refused.
     """
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "n_pages", "n_heads", "page_size", "head_dim", "dtype", "device",
@@ -173,7 +174,14 @@ class KVPages:
         if x.device != self.device or rows.device != self.device:
             raise ValueError(f"{name}, the rows and the pages must be on one device")
         self._no_gradient(name, x)
+        self._in_place()
         return shape
+
+    def _in_place(self) -> None:
+        at = self._args[3:]
+        if self.k.data_ptr() != at[0] or self.v.data_ptr() != at[1] or (at[2] is not None and (
+                self.k_scale.data_ptr() != at[2] or self.v_scale.data_ptr() != at[3])):
+            raise RuntimeError("the pages are no longer where they were: make KVPages of them anew")
 
     def _no_gradient(self, name: str, x: torch.Tensor) -> None:
         if x.requires_grad or self.k.requires_grad or self.v.requires_grad or forward_ad._current_level >= 0:
@@ -214,6 +222,7 @@ class KVPages:
         if length < 0:
             raise ValueError(f"length must not be negative, got {length}")
         self._no_gradient("the cache", self.k)
+        self._in_place()
         S, P = rows._sizes
         shape = (S, length, self.n_heads, self.head_dim)
         if not self.k.is_cuda:

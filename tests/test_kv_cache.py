@@ -232,6 +232,23 @@ def test_refusals():
         BatchRows(rows.page_table_SP, rows.query_start, rows.lengths, max_new=0)
 
 
+@pytest.mark.parametrize("held", [torch.float32, E4M3])
+def test_pages_that_were_given_other_memory_are_refused(held):
+    """Calls take the addresses that the pages had when they were checked."""
+    rows, n = pc.rows_of([(2, 5)], 16, "cpu")
+    x = torch.ones(2, 2, 16)
+    for name in ("k", "v", *(("k_scale", "v_scale") if held == E4M3 else ())):
+        pages = pc.pages_of(n, 2, 16, 16, held, "cpu")
+        pages.write(x, x, rows)
+        tensor = getattr(pages, name)
+        before, tensor.data = tensor.data, tensor.data.view(torch.uint8).clone().view(tensor.dtype)
+        for call in (lambda: pages.attend(x, rows), lambda: pages.write(x, x, rows), lambda: pages.read(rows, 5)):
+            with pytest.raises(RuntimeError, match="no longer"):
+                call()
+        tensor.data = before
+        pages.read(rows, 5)
+
+
 @pytest.mark.parametrize("dtype", [_lib.F32, _lib.BF16])
 def test_more_blocks_than_a_launch_holds_are_refused(dtype):
     """2^30 (row, head) pairs of single tokens, 256 threads each: a launch has at most 2^32 threads."""
