@@ -173,20 +173,19 @@ class KVPages:
                             "(float32 or bfloat16) or float8_e4m3fn")
         if x.device != self.device or rows.device != self.device:
             raise ValueError(f"{name}, the rows and the pages must be on one device")
-        self._no_gradient(name, x)
-        self._in_place()
+        self._usable(name, x)
         return shape
 
-    def _in_place(self) -> None:
-        at = self._args[3:]
-        if self.k.data_ptr() != at[0] or self.v.data_ptr() != at[1] or (at[2] is not None and (
-                self.k_scale.data_ptr() != at[2] or self.v_scale.data_ptr() != at[3])):
+    def _usable(self, name: str, x: torch.Tensor) -> None:
+        """The pages lie where they were checked, and neither they nor x have a derivative to carry."""
+        k, v = self.k, self.v
+        _, _, _, k_at, v_at, k_scale_at, v_scale_at = self._args
+        if k.data_ptr() != k_at or v.data_ptr() != v_at or k_scale_at is not None and (
+                self.k_scale.data_ptr() != k_scale_at or self.v_scale.data_ptr() != v_scale_at):
             raise RuntimeError("the pages are no longer where they were: make KVPages of them anew")
-
-    def _no_gradient(self, name: str, x: torch.Tensor) -> None:
-        if x.requires_grad or self.k.requires_grad or self.v.requires_grad or forward_ad._current_level >= 0:
+        if x.requires_grad or k.requires_grad or v.requires_grad or forward_ad._current_level >= 0:
             _no_gradient(name, x)
-            _no_gradient("the cache", self.k, self.v)
+            _no_gradient("the cache", k, v)
 
     def _rows_args(self, rows: BatchRows) -> tuple:
         return (rows.page_table_SP.data_ptr(), rows.query_start.data_ptr(), rows.lengths.data_ptr(), *rows._sizes,
@@ -201,7 +200,8 @@ class KVPages:
         T, H, K = self._check("k", k_THK, rows, self.n_heads)
         if v_THK.shape != k_THK.shape or v_THK.dtype != k_THK.dtype or v_THK.device != self.device:
             raise ValueError("k and v must have one shape, dtype and device")
-        self._no_gradient("v", v_THK)
+        if v_THK.requires_grad or forward_ad._current_level >= 0:
+            _no_gradient("v", v_THK)
         if not k_THK.is_cuda:
             return self._write_cpu(k_THK, v_THK, rows)
         k_THK, v_THK = _contig(k_THK), _contig(v_THK)
@@ -221,8 +221,7 @@ class KVPages:
             raise ValueError("the rows and the pages must be on one device")
         if length < 0:
             raise ValueError(f"length must not be negative, got {length}")
-        self._no_gradient("the cache", self.k)
-        self._in_place()
+        self._usable("the cache", self.k)
         S, P = rows._sizes
         shape = (S, length, self.n_heads, self.head_dim)
         if not self.k.is_cuda:
