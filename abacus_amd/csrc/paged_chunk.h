@@ -15,8 +15,9 @@
 // + 0..7 in registers 8 c .. 8 c + 7, which is the operand P^T of O^T = V^T P^T as it lies.
 //
 // Bound by the products and the exponentials together: two chunks of 2048 tokens over 8192 (32
-// heads over 8, K = 128) take 650 to 720 us, 860 to 950 TF/s, the matrix unit busy 0.40 of the
-// cycles, the vector unit 0.46, at the 2.0 GHz that the power limit leaves.  K = 64, where the
+// heads over 8, K = 128) take 667 us, 930 TF/s, in a long row of calls, the matrix unit busy 0.40
+// of the 1.46 million cycles, the vector unit 0.46.  The clock decides: the first 20 calls after a
+// pause take 716 to 850 us, calls among others with their join 650 to 720.  K = 64, where the
 // products are half as much, 610 TF/s; codes 790.  Two work-groups a CU hide a tile's loads, so two
 // stages are enough; the next tile's scores formed under this one's exponentials won nothing
 // (705 to 712 against 717 us) and spilled.
@@ -273,6 +274,9 @@ __device__ __attribute__((always_inline)) inline void chunk_rows(const PagedArgs
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] *= f[e];  // exact: powers of two
       }
+      // Rounded to bf16 for the product with the values, and summed unrounded: fp32 products run at
+      // an eighth of the rate, and o's own rounding is as large (o is 0.0023 off the formula,
+      // normwise, where its rounding alone is 0.0017).
       Vec16 pf;
 #pragma unroll
       for (int e = 0; e < 4; ++e) pf.w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);

@@ -11,8 +11,8 @@
 // tile of keys or values goes through LDS, and every load of the cache is 16 bytes a lane.
 //
 // Bound by the bytes of the cache.  4 query heads a key head, K = 128: 64 tokens over up to 8192
-// e4m3 keys 132 us (5.3 TB/s; the vector unit is busy a quarter of it), 2 over
-// 131072 bf16 keys 190 us (5.6 TB/s).  The tiles of a block's piece are dealt out to its four
+// e4m3 keys 133 us (5.3 TB/s; the vector unit is busy a quarter of it), 2 over
+// 131072 bf16 keys 193 us (5.6 TB/s).  The tiles of a block's piece are dealt out to its four
 // waves in turn: runs of tiles a wave took 230 us for the first, eight waves 156.  With more
 // than 16 rows the fp32 products weigh as much (97 TF/s of 154 for a chunk of K = 128).
 #pragma once
@@ -375,7 +375,7 @@ __device__ __attribute__((always_inline)) inline void few_block(const PagedArgs&
     if constexpr (kBf) {
 #pragma unroll
       for (int h = 0; h < KG / 8; ++h) {
-        pa_u32x4 pf[QT];
+        pa_u32x4 pf[QT];  // probabilities in bf16, as in paged_chunk.h; fp32 rows keep theirs
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
           float w[8];

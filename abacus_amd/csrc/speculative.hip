@@ -19,7 +19,7 @@
 //
 // The first launch is bound by its exponentials: some 20 instructions of 64 bits a logit, 10 us
 // of arithmetic for the 576 rows of 32000 bf16 logits that 64 sequences with 4 drafts have,
-// beside 6 us of reading; it takes 20 us.  The second is bound by latency (14 us there): what
+// beside 6 us of reading; it takes 20 us.  The second is bound by latency (15 us there): what
 // it reads depends on what it has read, from the row numbers to the blocks' counts.
 #include <algorithm>
 
