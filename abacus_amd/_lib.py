@@ -98,6 +98,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "abacus_cross_entropy_bwd": (_I, [_P, _P, _P, _P, _F, _I64, _I64, _I64, _I, _P, _P]),
     "abacus_cross_entropy_mean_fwd": (_I, [_P, _P, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P]),
     "abacus_cross_entropy_mean_bwd": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _P, _P]),
+    "abacus_linear_cross_entropy_ws_bytes": (_I64, [_I64, _I64, _I64, _I, _I]),
+    "abacus_linear_cross_entropy": (_I, [_P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _P, _P, _P, _P, _P, _I64, _P]),
+    "abacus_scale_by": (_I, [_P, _I64, _I, _P, _P]),
+    "abacus_embedding_fwd": (_I, [_P, _P, _I64, _I64, _I64, _F, _I, _P, _P]),
+    "abacus_embedding_bwd_ws_bytes": (_I64, [_I64, _I64, _I64]),
+    "abacus_embedding_bwd": (_I, [_P, _P, _I64, _I64, _I64, _F, _I, _P, _P, _I64, _P]),
+    "abacus_residual_norm_fwd": (_I, [_P, _P, _P, _P, _P, _I, _I64, _I64, _F, _F, _I, _P, _P, _P, _P, _P]),
+    "abacus_residual_norm_bwd_ws_bytes": (_I64, [_I64, _I64, _I, _I]),
+    "abacus_residual_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I64, _I64, _F, _I, _P, _P, _P, _P, _P, _P,
+                                      _I64, _P]),
     "abacus_batch_positions": (_I, [_P, _P, _I64, _I64, _P, _P]),
     "abacus_kv_write": (_I, [_P, _P, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P]),
     "abacus_kv_read": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _I64, _I, _P, _P, _P]),

@@ -1,0 +1,191 @@
+"""The decoder's two ends over the vocabulary: the embedding of tokens, and the loss of the head's product.
+
+``embedding`` is embedding.py's indexing with a scale; its gradient adds the rows of each token in fp32, by tokens
+sorted by id (csrc/embedding.hip).
+
+``linear_cross_entropy`` is the cross-entropy of ``x @ w`` without its logits in memory: the products, the softmax and
+the gradients of both operands run over them piece by piece (csrc/linear_cross_entropy.hip).  The reference takes the
+two steps one after the other (transformer_moe.py:75, kernels/liger.py:12-47).
+
+CPU tensors take the same steps in torch's operations.
+"""
+
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+
+from . import _lib
+from .moe import _contig
+
+__all__ = ["embedding", "linear_cross_entropy"]
+
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}  # ABACUS_LOSS_ROWS, _SUM, _MEAN
+
+
+def _plain_loss(x_TD, w_DV, targets_T, ignore_index: int, reduction: str):
+    """The loss in torch's operations, fp32 (fp64 for fp64 operands)."""
+    wide = torch.promote_types(x_TD.dtype, torch.float32)
+    return F.cross_entropy(x_TD.to(wide) @ w_DV.to(wide), targets_T, ignore_index=ignore_index, reduction=reduction)
+
+
+def _loss_call(x_TD, w_DV, targets_T, ignore_index: int, reduction: str, row_grad=None, want=(False, False), want_loss=True):
+    """(loss or None, dx or None, dw or None) of one call of the kernels."""
+    T, D = x_TD.shape
+    V = w_DV.shape[1]
+    dev, dt = x_TD.device, _lib.dtype_code(x_TD.dtype, x_TD.device)
+    loss = torch.empty((T,) if reduction == "none" else (), dtype=torch.float32, device=dev) if want_loss else None
+    dx = torch.empty(T, D, dtype=x_TD.dtype, device=dev) if want[0] else None
+    dw = torch.empty(D, V, dtype=w_DV.dtype, device=dev) if want[1] else None
+    nbytes = _lib.query("abacus_linear_cross_entropy_ws_bytes", T, D, V, dt, int(any(want)))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    w = _contig(w_DV)
+    _lib.call("abacus_linear_cross_entropy", x_TD.data_ptr(), x_TD.stride(0), _lib.ptr(w), targets_T.data_ptr(), T, D, V,
+              ignore_index, dt, _REDUCTIONS[reduction], _lib.ptr(row_grad), _lib.ptr(loss), _lib.ptr(dx), _lib.ptr(dw),
+              _lib.ptr(ws), nbytes, _lib.stream_of(dev))
+    return loss, dx, dw
+
+
+def _scaled(grad: torch.Tensor | None, g: torch.Tensor):
+    """grad times the scalar g, in place; left alone (on the device) where g is 1."""
+    if grad is not None:
+        _lib.call("abacus_scale_by", _lib.ptr(grad), grad.numel(), _lib.dtype_code(grad.dtype), g.data_ptr(),
+                  _lib.stream_of(grad.device))
+    return grad
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    """Loss and gradients in one pass over the logits: of a mean or a sum the forward forms both gradients, and the
+    backward multiplies them by the loss's own.  The losses of rows have gradients a row that only the
+    backward knows, so it makes the pass once more; so does a second backward of a mean or a sum."""
+
+    @staticmethod
+    def forward(ctx, x_TD, w_DV, targets_T, ignore_index: int, reduction: str):
+        ctx.save_for_backward(x_TD, w_DV, targets_T)
+        ctx.args = ignore_index, reduction
+        now = ctx.needs_input_grad[:2] if reduction != "none" else (False, False)
+        loss, *ctx.grads = _loss_call(x_TD, w_DV, targets_T, ignore_index, reduction, want=now)
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        from .transformer import _by_kernel
+
+        x, w, targets = ctx.saved_tensors
+        ignore_index, reduction = ctx.args
+        op = lambda x, w: _plain_loss(x, w, targets, ignore_index, reduction)
+        return (*_by_kernel(op, lambda: _LinearCrossEntropy.gradients(ctx, g, x, w, targets), g, x, w), None, None, None)
+
+    @staticmethod
+    def gradients(ctx, g, x, w, targets):
+        ignore_index, reduction = ctx.args
+        g = g.contiguous()
+        if reduction == "none":
+            return _loss_call(x, w, targets, ignore_index, reduction, g, ctx.needs_input_grad[:2], want_loss=False)[1:]
+        grads, ctx.grads = ctx.grads, None
+        if grads is None:  # handed over by an earlier backward of this graph
+            grads = _loss_call(x, w, targets, ignore_index, reduction, want=ctx.needs_input_grad[:2])[1:]
+        return tuple(_scaled(grad, g) for grad in grads)
+
+
+def linear_cross_entropy(x: torch.Tensor, w_DV: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """cross_entropy(x @ w_DV, targets) without the logits in memory: x (..., D), w_DV (D, V), targets (...) int64.
+
+    The loss is fp32, the mean over (or the sum of) the rows whose target is not ignore_index, or each row's loss
+    ("none", 0 where ignored).  A mean of no rows is NaN and its gradients are 0.  A target outside [0, V) other than
+    ignore_index makes its row's loss NaN, as train.cross_entropy on the GPU has it (on the CPU torch raises); nothing
+    waits on the host.  Logits and sums are fp32, whatever the operands' type; ignored rows cost no products.
+    """
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction is one of {', '.join(_REDUCTIONS)}, got {reduction!r}")
+    if x.dim() < 1 or w_DV.dim() != 2 or x.shape[-1] != w_DV.shape[0] or 0 in w_DV.shape:
+        raise ValueError(f"linear_cross_entropy takes x (..., D) and w (D, V), got {tuple(x.shape)} and {tuple(w_DV.shape)}")
+    if targets.shape != x.shape[:-1] or targets.dtype != torch.int64:
+        raise ValueError(f"linear_cross_entropy takes int64 targets {tuple(x.shape[:-1])}, got {targets.dtype} "
+                         f"{tuple(targets.shape)}")
+    if w_DV.dtype != x.dtype:
+        raise TypeError(f"x is {x.dtype} and w is {w_DV.dtype}")
+    if not x.device == w_DV.device == targets.device:
+        raise ValueError(f"x, w and targets are on {x.device}, {w_DV.device} and {targets.device}")
+    x_TD, targets_T = x.reshape(-1, x.shape[-1]), targets.reshape(-1).contiguous()
+    if x.device.type == "cpu" or x_TD.shape[0] == 0:
+        loss = _plain_loss(x_TD, w_DV, targets_T, ignore_index, reduction)
+    else:
+        _lib.dtype_code(x.dtype, x.device)  # refuses other types
+        if x_TD.stride(1) != 1 or x_TD.stride(0) < x_TD.shape[1]:
+            x_TD = x_TD.contiguous()
+        if torch.is_grad_enabled() and (x.requires_grad or w_DV.requires_grad):
+            loss = _LinearCrossEntropy.apply(x_TD, w_DV, targets_T, int(ignore_index), reduction)
+        else:
+            loss = _loss_call(x_TD, w_DV, targets_T, int(ignore_index), reduction)[0]
+    return loss.view(targets.shape) if reduction == "none" else loss
+
+
+class _Embedding(torch.autograd.Function):
+    """scale * w[tokens] and its gradient, the rows of each token added in a fixed order."""
+
+    @staticmethod
+    def forward(ctx, tokens, w_VD, scale: float):
+        ctx.save_for_backward(tokens)
+        ctx.shape, ctx.scale = w_VD.shape, scale
+        return _embed_call(tokens, w_VD, scale)
+
+    @staticmethod
+    def backward(ctx, d_out):
+        (tokens,) = ctx.saved_tensors
+        return None, _EmbeddingGradient.apply(d_out, tokens, ctx.shape, ctx.scale), None
+
+
+class _EmbeddingGradient(torch.autograd.Function):
+    """The gradient is linear in d_out, and its own derivative the embedding again."""
+
+    @staticmethod
+    def forward(ctx, d_out, tokens, shape, scale: float):
+        ctx.save_for_backward(tokens)
+        ctx.scale = scale
+        V, D = shape
+        T, dev = tokens.numel(), d_out.device
+        dw = torch.empty(V, D, dtype=d_out.dtype, device=dev)
+        nbytes = _lib.query("abacus_embedding_bwd_ws_bytes", T, V, D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        d_out = _contig(d_out)
+        _lib.call("abacus_embedding_bwd", tokens.data_ptr(), _lib.ptr(d_out), T, V, D, scale, _lib.dtype_code(d_out.dtype),
+                  _lib.ptr(dw), _lib.ptr(ws), nbytes, _lib.stream_of(dev))
+        return dw
+
+    @staticmethod
+    def backward(ctx, d_dw):
+        (tokens,) = ctx.saved_tensors
+        return _Embedding.apply(tokens, d_dw, ctx.scale), None, None, None
+
+
+def _embed_call(tokens, w_VD, scale: float):
+    V, D = w_VD.shape
+    w = _contig(w_VD)
+    out = torch.empty(*tokens.shape, D, dtype=w.dtype, device=w.device)
+    _lib.call("abacus_embedding_fwd", tokens.data_ptr(), _lib.ptr(w), tokens.numel(), V, D, scale,
+              _lib.dtype_code(w.dtype), _lib.ptr(out), _lib.stream_of(w.device))
+    return out
+
+
+def embedding(tokens: torch.Tensor, w_VD: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * w_VD[tokens] (embedding.py:20-23): tokens (...) int64, w_VD (V, D), out (..., D).
+
+    Negative tokens count from the end, as in torch's indexing.  A token outside [-V, V) gives a row of NaN and no
+    gradient on the GPU (on the CPU torch raises); nothing waits on the host.  The gradient of a row is the sum of its
+    tokens' in fp32, times the scale, rounded once, and the same bits every run.
+    """
+    if tokens.dtype != torch.int64:
+        raise ValueError(f"embedding takes int64 tokens, got {tokens.dtype}")
+    if w_VD.dim() != 2 or 0 in w_VD.shape:
+        raise ValueError(f"embedding takes a table (V, D), got {tuple(w_VD.shape)}")
+    if tokens.device != w_VD.device:
+        raise ValueError(f"tokens are on {tokens.device}, the table on {w_VD.device}")
+    if w_VD.device.type == "cpu":
+        return w_VD[tokens] if scale == 1.0 else w_VD[tokens] * scale
+    _lib.dtype_code(w_VD.dtype, w_VD.device)  # refuses other types
+    tokens = tokens.contiguous()
+    if torch.is_grad_enabled() and w_VD.requires_grad:
+        return _Embedding.apply(tokens, w_VD, float(scale))
+    return _embed_call(tokens, w_VD, float(scale))

@@ -418,6 +418,59 @@ int abacus_cross_entropy_mean_bwd(const void* logits_NV, const int64_t* targets_
                                   const void* grad_loss, const float* count, int64_t N, int64_t V,
                                   int64_t ignore_index, int dtype, void* dlogits_NV, void* stream);
 
+/* Cross-entropy of a linear head with the gradients of both operands, the logits never
+ * whole in memory (no counterpart in the reference, whose head and loss are two steps).
+ * Of l = x W, x_TD (T, D) with rows x_stride elements apart and w_DV (D, V), and int64
+ * targets_T: row t's loss is log(sum_v exp(l_tv)) - l[t, targets_T[t]] in fp32, 0 where
+ * its target is ignore_index, NaN where it is another value outside [0, V).
+ * reduction: ABACUS_LOSS_ROWS, loss is each row's (T values); ABACUS_LOSS_SUM and
+ * ABACUS_LOSS_MEAN (over the rows not ignored), one value.  loss may be NULL where a gradient is not.
+ * dx_TD (T, D), dw_DV (D, V), contiguous, `dtype`; NULL: not computed.  They are those of the
+ * sum or mean, or with ABACUS_LOSS_ROWS of the sum of row_grad_T[t] (fp32) times each
+ * row's loss (NULL without gradients, and for the others).  Logits, sums and
+ * gradients are fp32; P = s (softmax - onehot) is rounded to `dtype` for the products, the gradients once.
+ * Any D and V; x may start at any element, the other operands are 16-byte aligned.
+ * ws: device workspace of abacus_linear_cross_entropy_ws_bytes bytes (grad: with gradients).
+ *
+ * abacus_scale_by: n values of `dtype` times *g (device memory), left as they are where it is 1. */
+#define ABACUS_LOSS_ROWS 0
+#define ABACUS_LOSS_SUM 1
+#define ABACUS_LOSS_MEAN 2
+int64_t abacus_linear_cross_entropy_ws_bytes(int64_t T, int64_t D, int64_t V, int dtype, int grad);
+int abacus_linear_cross_entropy(const void* x_TD, int64_t x_stride, const void* w_DV, const int64_t* targets_T,
+                                int64_t T, int64_t D, int64_t V, int64_t ignore_index, int dtype, int reduction,
+                                const float* row_grad_T, float* loss, void* dx_TD, void* dw_DV, void* ws,
+                                int64_t ws_bytes, void* stream);
+int abacus_scale_by(void* t, int64_t n, int dtype, const float* g, void* stream);
+
+/* The embedding of tokens (embedding.py:20-23): out_TD[t] = scale * w_VD[tokens_T[t]], a
+ * negative token counted from the end; a token outside [-V, V) gives NaN and has no gradient.
+ * Backward: dw_VD[v] = scale * the sum of d_out_TD's rows of token v in fp32, in the
+ * order of t, rounded once; rows of no token are 0.  ws: abacus_embedding_bwd_ws_bytes bytes. */
+int abacus_embedding_fwd(const int64_t* tokens_T, const void* w_VD, int64_t T, int64_t V, int64_t D, float scale,
+                         int dtype, void* out_TD, void* stream);
+int64_t abacus_embedding_bwd_ws_bytes(int64_t T, int64_t V, int64_t D);
+int abacus_embedding_bwd(const int64_t* tokens_T, const void* d_out_TD, int64_t T, int64_t V, int64_t D, float scale,
+                         int dtype, void* dw_VD, void* ws, int64_t ws_bytes, void* stream);
+
+/* The residual stream between two blocks (transformer_block.py:98-100 with norm.py:26-31):
+ * of rows of D values, b = y, or with post_gamma post_gamma * y / sqrt(mean(y^2) + eps);
+ * r = x + scale * gate * b, rounded to `dtype`; h = gamma * r / sqrt(mean(r^2) + eps) of that r.
+ * gate_kind 0: no gate, 1: gate has D values, 2: (rows, D).  rstd and y_rstd (one fp32 a
+ * row, NULL where not wanted): the two inverse roots, for the backward.
+ * Backward, of dr and dh (NULL: zeros): dx, dy (may be dx's own memory or NULL where b is y and
+ * scale 1 without a gate: they are the same), dgamma, and dpost and dgate with post_gamma and gate; sums over rows in
+ * fp32, in a fixed order.  y is read with a gate or post_gamma only.
+ * ws: abacus_residual_norm_bwd_ws_bytes bytes.  D at most 16384 (bf16) or 8192 (fp32). */
+int abacus_residual_norm_fwd(const void* x, const void* y, const void* gamma, const void* post_gamma, const void* gate,
+                             int gate_kind, int64_t rows, int64_t D, float scale, float eps, int dtype, void* r,
+                             void* h, float* rstd, float* y_rstd, void* stream);
+int64_t abacus_residual_norm_bwd_ws_bytes(int64_t rows, int64_t D, int post, int gate_kind);
+int abacus_residual_norm_bwd(const void* dr, const void* dh, const void* r, const void* y, const void* gamma,
+                             const void* post_gamma, const void* gate, int gate_kind, const float* rstd,
+                             const float* y_rstd, int64_t rows, int64_t D, float scale, int dtype, void* dx, void* dy,
+                             void* dgamma, void* dpost, void* dgate, void* ws, int64_t ws_bytes, void* stream);
+
 /* The paged key/value cache of a decoding program (no counterpart in the reference).
  * T rows of S sequences lie one after the other: rows query_start[s] ..
  * query_start[s + 1] - 1 (S + 1 values) are the last positions of sequence s,
