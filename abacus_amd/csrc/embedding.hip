@@ -7,9 +7,9 @@
 //   1. sort: a work-group owns a range of ids.  It reads all tokens, counts its own (a counter for each wave's part of
 //      the tokens and id, in LDS) and those of ids before its range, which is where its part of the sorted list
 //      starts; a second reading writes the list.  No work-group waits for another and no order is left to chance.
-//   2. rows: a wave adds up a row of dw and writes it, zeros where no token has the id.  Ids with many tokens (kHot
-//      and more: padding, a frequent word) would keep one wave busy alone, so their sorted positions are
-//      added up in pieces of kPiece by work-groups of the same launch, in fp32;
+//   2. rows: a wave adds up 64 vectors of the rows of kIds ids and writes them, zeros where no token has the id.  Ids with
+//      many tokens (more than kHot: padding, a frequent word) would keep one wave busy alone, so their sorted
+//      positions are added up in pieces of kPiece by work-groups of the same launch, in fp32;
 //   3. join: which a last launch adds in order.
 #include <algorithm>
 
@@ -18,9 +18,12 @@
 namespace abacus {
 namespace {
 
-constexpr int kPiece = 64;     // sorted positions of a piece
+constexpr int kPiece = 32;     // sorted positions of a piece
 constexpr int kHot = kPiece;   // an id with more tokens goes by pieces: a piece then holds parts of two such ids at most
+constexpr int kIds = 4;        // of a wave
+constexpr int kRowsAhead = 8;  // rows of dy whose loads are in flight together
 constexpr int kSortWaves = 16;
+constexpr int kSortAhead = 8;  // tokens a lane, likewise
 constexpr int kMaxIds = 960;   // of a sorting work-group (its counters under 64 KB)
 
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
@@ -100,11 +103,22 @@ __global__ __launch_bounds__(kSortWaves * 64) void embedding_sort_kernel(const i
   const int part = ((T + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
   const int t0 = wave * part, t1 = min(T, t0 + part);
   int* count = count_s + wave * ids;
+  auto read = [&](int b, int (&v)[kSortAhead]) {  // ids of tokens b .. of this wave, -1 past its part
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      const int t = b + u * 64 + lane;
+      v[u] = t < t1 ? row_of(tokens[t], V) : -1;
+    }
+  };
   int before = 0;
-  for (int t = t0 + lane; t < t1; t += 64) {
-    const int v = row_of(tokens[t], V);
-    before += v >= 0 && v < lo;
-    if (v >= lo && v < lo + mine) atomicAdd(&count[v - lo], 1);
+  for (int b = t0; b < t1; b += 64 * kSortAhead) {
+    int v[kSortAhead];
+    read(b, v);
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      before += v[u] >= 0 && v[u] < lo;
+      if (v[u] >= lo && v[u] < lo + mine) atomicAdd(&count[v[u] - lo], 1);
+    }
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
@@ -139,44 +153,44 @@ __global__ __launch_bounds__(kSortWaves * 64) void embedding_sort_kernel(const i
   __syncthreads();
   // the same reading again: count[] is now the next free place
   volatile int* next = count;
-  for (int b = t0; b < t1; b += 64) {
-    const int t = b + lane;
-    const int v = t < t1 ? row_of(tokens[t], V) - lo : -1;
-    const bool in = v >= 0 && v < mine;
-    uint64_t left = __ballot(in);
-    while (left) {  // an id at a time
-      const int leader = __ffsll((unsigned long long)left) - 1;
-      const int id = __shfl(v, leader, 64);
-      const uint64_t same = __ballot(in && v == id);
-      const int place = next[id];
-      if (in && v == id) order[place + __popcll(same & ((1ull << lane) - 1))] = t;
-      if (lane == leader) next[id] = place + __popcll(same);
-      left &= ~same;
+  for (int b = t0; b < t1; b += 64 * kSortAhead) {
+    int ids_[kSortAhead];
+    read(b, ids_);
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      const int v = ids_[u] - lo;
+      const bool in = v >= 0 && v < mine;
+      uint64_t left = __ballot(in);
+      while (left) {  // an id at a time
+        const int leader = __ffsll((unsigned long long)left) - 1;
+        const int id = __shfl(v, leader, 64);
+        const uint64_t same = __ballot(in && v == id);
+        const int place = next[id];
+        if (in && v == id) order[place + __popcll(same & ((1ull << lane) - 1))] = b + u * 64 + lane;
+        if (lane == leader) next[id] = place + __popcll(same);
+        left &= ~same;
+      }
     }
   }
 }
 
-// Sum of dy's rows order[a] .. order[b - 1] at column c.
+// f = the sum of n rows of dy at column c, in order; row k's number is the k-th lane's `mine` (n at most 64).
 template <typename T>
-__device__ inline void add_rows(const T* dy, const int* order, int a, int b, int D, int c, float* f) {
+__device__ inline void add_rows(const T* dy, int mine, int n, int D, int c, float* f) {
   constexpr int EPV = VecTraits<T>::kN;
 #pragma unroll
   for (int k = 0; k < EPV; ++k) f[k] = 0.f;
-  int i = a;
-  for (; i + 4 <= b; i += 4) {
-    float g[4][EPV];
+  for (int i = 0; i < n; i += kRowsAhead) {
+    float g[kRowsAhead][EPV];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load_any<T>(dy + (int64_t)order[i + u] * D + c, D - c, g[u]);
+    for (int u = 0; u < kRowsAhead; ++u) {
+      const int t = __builtin_amdgcn_readlane(mine, min(i + u, n - 1));
+      load_any<T>(dy + (int64_t)t * D + c, i + u < n ? D - c : 0, g[u]);
+    }
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < kRowsAhead; ++u)
 #pragma unroll
       for (int k = 0; k < EPV; ++k) f[k] += g[u][k];
-  }
-  for (; i < b; ++i) {
-    float g[EPV];
-    load_any<T>(dy + (int64_t)order[i] * D + c, D - c, g);
-#pragma unroll
-    for (int k = 0; k < EPV; ++k) f[k] += g[k];
   }
 }
 
@@ -197,20 +211,27 @@ struct Piece {
   }
 };
 
+// Work-groups 0 .. 2 pieces - 1: (piece, slot); they note in `joins` which id, if any, a piece is the first of.
+// The others: a wave takes kIds ids and 64 vectors of their rows.
 template <typename T>
 __global__ __launch_bounds__(256) void embedding_rows_kernel(const int64_t* __restrict__ tokens, const T* __restrict__ dy,
                                                              const int* __restrict__ start, const int* __restrict__ order,
-                                                             int V, int D, float scale, int pieces,
-                                                             float* __restrict__ parts, T* __restrict__ dw) {
+                                                             int V, int D, int slabs, float scale, int pieces,
+                                                             int* __restrict__ joins, float* __restrict__ parts,
+                                                             T* __restrict__ dw) {
   constexpr int EPV = VecTraits<T>::kN;
   const int tid = threadIdx.x, lane = tid & 63;
   if ((int)blockIdx.x < 2 * pieces) {  // (the long ones first)
     Piece pc;
     const int p = blockIdx.x >> 1, slot = blockIdx.x & 1;
-    if (!pc.find(tokens, start, order, V, p, slot)) return;
-    for (int c = tid * EPV; c < D; c += 256 * EPV) {
+    const bool hot = pc.find(tokens, start, order, V, p, slot);
+    if (tid == 0) joins[blockIdx.x] = hot && pc.first >= p * kPiece ? pc.id : -1;
+    if (!hot) return;
+    const int n = pc.b - pc.a, mine = order[pc.a + min(lane, n - 1)];
+    for (int c0 = 0; c0 < D; c0 += 256 * EPV) {
+      const int c = c0 + tid * EPV;
       float f[EPV];
-      add_rows<T>(dy, order, pc.a, pc.b, D, c, f);
+      add_rows<T>(dy, mine, n, D, c, f);
       float* out = parts + (int64_t)blockIdx.x * D + c;
 #pragma unroll
       for (int k = 0; k < EPV; ++k)
@@ -218,38 +239,47 @@ __global__ __launch_bounds__(256) void embedding_rows_kernel(const int64_t* __re
     }
     return;
   }
-  const int v = ((int)blockIdx.x - 2 * pieces) * 4 + (tid >> 6);
-  if (v >= V) return;
-  const int a = start[v], b = start[v + 1];
-  if (b - a > kHot) return;
-  for (int c = lane * EPV; c < D; c += 64 * EPV) {
-    float f[EPV];
-    add_rows<T>(dy, order, a, b, D, c, f);
+  const int64_t task = ((int64_t)blockIdx.x - 2 * pieces) * 4 + (tid >> 6);
+  const int v0 = (int)(task / slabs) * kIds, c = (int)(task % slabs) * 64 * EPV + lane * EPV;
+  if (v0 >= V) return;
+  const int bound = start[min(v0 + min(lane, kIds), V)];
+  int a[kIds], n[kIds], mine[kIds];
 #pragma unroll
-    for (int k = 0; k < EPV; ++k) f[k] *= scale;
-    store_any<T>(dw + (int64_t)v * D + c, D - c, f);
+  for (int k = 0; k < kIds; ++k) {
+    a[k] = __builtin_amdgcn_readlane(bound, k);
+    n[k] = __builtin_amdgcn_readlane(bound, k + 1) - a[k];
+    mine[k] = lane < n[k] ? order[a[k] + lane] : 0;
+  }
+#pragma unroll
+  for (int k = 0; k < kIds; ++k) {
+    if (v0 + k >= V || n[k] > kHot) continue;
+    float f[EPV];
+    add_rows<T>(dy, mine[k], n[k], D, c, f);
+#pragma unroll
+    for (int i = 0; i < EPV; ++i) f[i] *= scale;
+    store_any<T>(dw + (int64_t)(v0 + k) * D + c, D - c, f);
   }
 }
 
-// Hot ids: the pieces' sums in order, 64 columns a work-group whose 16 waves take every 16th piece.
+// Hot ids: the pieces' sums in order, 64 columns a work-group whose 4 waves take every 4th piece.
 template <typename T>
-__global__ __launch_bounds__(1024) void embedding_join_kernel(const int64_t* __restrict__ tokens, const int* __restrict__ start,
-                                                              const int* __restrict__ order, int V, int D, float scale,
-                                                              const float* __restrict__ parts, T* __restrict__ dw) {
-  __shared__ float sum_s[16][64];
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.y * 64 + l;
-  const int p = blockIdx.x >> 1, slot = blockIdx.x & 1;
-  Piece pc;
-  if (!pc.find(tokens, start, order, V, p, slot) || pc.first < p * kPiece) return;  // (not the piece that it starts in)
-  const int n = (pc.last - 1) / kPiece - p + 1;
-  float s = 0.f;
-  for (int k = w; k < n; k += 16)
-    if (c < D) s += parts[((int64_t)(p + k) * 2 + (k == 0 ? slot : 0)) * D + c];
-  sum_s[w][l] = s;
-  __syncthreads();
-  if (w == 0 && c < D) {
-    for (int k = 1; k < 16; ++k) s += sum_s[k][l];
-    dw[(int64_t)pc.id * D + c] = from_f32<T>(s * scale);
+__global__ __launch_bounds__(256) void embedding_join_kernel(const int* __restrict__ start, const int* __restrict__ joins,
+                                                             int V, int D, float scale, const float* __restrict__ parts,
+                                                             T* __restrict__ dw) {
+  __shared__ float sum_s[4][64];
+  const int id = joins[blockIdx.x];
+  if (id < 0) return;
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int p = blockIdx.x >> 1, slot = blockIdx.x & 1, n = (start[id + 1] - 1) / kPiece - p + 1;
+  for (int c0 = blockIdx.y * 64; c0 < D; c0 += gridDim.y * 64) {
+    const int c = min(c0 + l, D - 1);
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = w; k < n; k += 4) s += parts[((int64_t)(p + k) * 2 + (k == 0 ? slot : 0)) * D + c];
+    sum_s[w][l] = s;
+    __syncthreads();
+    if (w == 0 && c0 + l < D) dw[(int64_t)id * D + c] = from_f32<T>((((s + sum_s[1][l]) + sum_s[2][l]) + sum_s[3][l]) * scale);
+    __syncthreads();
   }
 }
 
@@ -262,13 +292,15 @@ int check(const char* name, int64_t T, int64_t V, int64_t D, int dtype) {
 }
 
 struct Space {
-  int64_t start, order, parts, total;
+  int64_t start, order, joins, parts, total;
   Space(int64_t T, int64_t V, int64_t D) {
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     start = 0;
     order = up((V + 1) * 4);
-    parts = order + up(T * 4);
-    total = parts + (T > kHot ? (T + kPiece - 1) / kPiece * 2 * D * 4 : 0);
+    joins = order + up(T * 4);
+    const int64_t slots = T > kHot ? (T + kPiece - 1) / kPiece * 2 : 0;
+    parts = joins + up(slots * 4);
+    total = parts + slots * D * 4;
   }
 };
 
@@ -278,18 +310,22 @@ int backward(const int64_t* tokens, const void* dy, int64_t n, int64_t V, int64_
   const Space sp(n, V, D);
   int* start = (int*)(ws + sp.start);
   int* order = (int*)(ws + sp.order);
+  int* joins = (int*)(ws + sp.joins);
   float* parts = (float*)(ws + sp.parts);
   const int ids = (int)std::min<int64_t>(kMaxIds, (V + 255) / 256);
   hipLaunchKernelGGL(embedding_sort_kernel, dim3((unsigned)((V + ids - 1) / ids)), dim3(kSortWaves * 64),
                      kSortWaves * ids * 4, s, tokens, (int)n, (int)V, ids, start, order);
   ABACUS_CHECK_LAUNCH("embedding_bwd sort");
   const int pieces = n > kHot ? (int)((n + kPiece - 1) / kPiece) : 0;
-  hipLaunchKernelGGL(embedding_rows_kernel<T>, dim3((unsigned)(2 * pieces + (V + 3) / 4)), dim3(256), 0, s, tokens, (const T*)dy,
-                     start, order, (int)V, (int)D, scale, pieces, parts, (T*)dw);
+  const int slabs = (int)((D + 64 * VecTraits<T>::kN - 1) / (64 * VecTraits<T>::kN));
+  const int64_t tasks = (V + kIds - 1) / kIds * slabs, blocks = 2 * pieces + (tasks + 3) / 4;
+  ABACUS_CHECK_ARG(blocks < (1ll << 31), "embedding_bwd: a table of %lld x %lld", (long long)V, (long long)D);
+  hipLaunchKernelGGL(embedding_rows_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, tokens, (const T*)dy, start, order, (int)V,
+                     (int)D, slabs, scale, pieces, joins, parts, (T*)dw);
   ABACUS_CHECK_LAUNCH("embedding_bwd rows");
   if (pieces) {
-    hipLaunchKernelGGL(embedding_join_kernel<T>, dim3(2 * pieces, (unsigned)((D + 63) / 64)), dim3(1024), 0, s, tokens, start,
-                       order, (int)V, (int)D, scale, parts, (T*)dw);
+    hipLaunchKernelGGL(embedding_join_kernel<T>, dim3(2 * pieces, (unsigned)std::min<int64_t>((D + 63) / 64, 8)), dim3(256), 0, s,
+                       start, joins, (int)V, (int)D, scale, parts, (T*)dw);
     ABACUS_CHECK_LAUNCH("embedding_bwd join");
   }
   return 0;

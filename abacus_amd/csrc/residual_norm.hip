@@ -13,9 +13,12 @@
 // (norm.py:26-31); without post, gate and scale r and h have the bits of those two.  Each way is one pass:
 // everything but the outputs' rounding is fp32.
 //
-// Layout: a row is spread over lpr lanes of a wave (the RMSNorm kernels' layout, so the same sums), or over a
-// work-group of 4 waves where it is longer; a lane holds VPL vectors of 16 bytes.  Rows may start at any element: the last
-// vector of a D that is not whole vectors is taken element by element.
+// Layout: a lane holds VPL vectors of 16 bytes of a row, which is spread over
+//   kEven    lpr lanes of a wave that its vectors divide evenly (the RMSNorm kernels' layout, so the same sums),
+//   kWave    the 64 lanes of a wave,
+//   kGroup   the waves of a work-group: long rows, whose vectors and sums would crowd a lane's registers.
+// Rows may start at any element.  Where a row is not whole vectors the last one ends at the row's end and
+// overlaps the one before: its first elements are left out of sums and stores.
 // The sums over rows (dgamma, dpost, dgate) are added up by a lane over its rows, over the work-group's waves in
 // wave order, and over work-groups by a second kernel in block order: the same bits every run.
 #include <algorithm>
@@ -39,274 +42,354 @@ struct NormArgs {
   float scale, eps;
 };
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
-// The n (at most one vector's) values at p, at any element.
 template <typename T>
-__device__ inline void load_row(const T* p, int n, float* f) {
-  constexpr int EPV = VecTraits<T>::kN;
-  if (n >= EPV) {
-    const u32x4_any v = *reinterpret_cast<const u32x4_any*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 2) {
-        f[2 * i] = lo_bf16(v[i]);
-        f[2 * i + 1] = hi_bf16(v[i]);
-      } else {
-        f[i] = bits_f32(v[i]);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < EPV; ++i) f[i] = i < n ? to_f32<T>(p[i]) : 0.f;
-  }
+__device__ inline float get(const u32x4& v, int i) {
+  if constexpr (sizeof(T) == 2) return i & 1 ? hi_bf16(v[i >> 1]) : lo_bf16(v[i >> 1]);
+  else return bits_f32(v[i]);
 }
-
 template <typename T>
-__device__ inline void store_row(T* p, int n, const float* f) {
-  constexpr int EPV = VecTraits<T>::kN;
-  if (n >= EPV) {
-    u32x4_any v;
+__device__ inline u32x4 pack(const float* f) {
+  u32x4 v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 2) v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-      else v[i] = f32_bits(f[i]);
-    }
-    *reinterpret_cast<u32x4_any*>(p) = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < EPV; ++i)
-      if (i < n) p[i] = from_f32<T>(f[i]);
-  }
-}
-
-// A row's sum over its lanes.  WIDE: the work-group's; sum_s is free again after the next barrier.
-template <bool WIDE>
-__device__ inline float row_sum(float v, int lpr, float* sum_s) {
-  for (int off = lpr >> 1; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-  if constexpr (WIDE) {
-    if ((threadIdx.x & 63) == 0) sum_s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sum_s[0] + sum_s[1] + sum_s[2] + sum_s[3];
-    __syncthreads();
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 2) v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+    else v[i] = f32_bits(f[i]);
   }
   return v;
 }
 
-// The rows of a work-group of 4 waves, one after the other: the first, the step, a lane's place in its row.
-template <bool WIDE>
-struct Rows {
-  int lane, wave, li, sub;
-  int64_t first, step;
-  __device__ inline Rows(int lpr) {
-    lane = threadIdx.x & 63;
-    wave = threadIdx.x >> 6;
-    li = WIDE ? (int)threadIdx.x : lane % lpr;
-    sub = WIDE ? 0 : lane / lpr;
-    const int rpw = WIDE ? 1 : 64 / lpr;
-    first = WIDE ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x * 4 + wave) * rpw;
-    step = WIDE ? (int64_t)gridDim.x : (int64_t)gridDim.x * 4 * rpw;
+// Keeps a value in its packed registers: without it the compiler holds on to the unpacked floats of every use.
+__device__ inline void hold(u32x4& v) { asm volatile("" : "+v"(v)); }
+
+enum Layout : int { kEven = 0, kWave = 1, kGroup = 2 };
+
+// A lane's vector v: its column, and how many of its first elements are another vector's (EPV and more: all are).
+template <typename T, int LAYOUT>
+struct Place {
+  int col, skip;
+  __device__ inline Place(int li, int lanes, int v, int D) {
+    constexpr int EPV = VecTraits<T>::kN;
+    const int c = (li + v * lanes) * EPV;
+    col = LAYOUT == kEven ? c : min(c, D - EPV);
+    skip = c - col;
   }
 };
 
-template <typename T, int VPL, bool WIDE, bool PLAIN>
-__global__ __launch_bounds__(256) void residual_norm_fwd_kernel(NormArgs a) {
-  constexpr int EPV = VecTraits<T>::kN, NE = VPL * EPV;
-  __shared__ float sum_s[4];
-  const Rows<WIDE> at(a.lpr);
-  const int lanes = WIDE ? 256 : a.lpr, D = a.D;
+// Every load is made, in bounds, whatever the lane holds: loads without branches between them are in flight together.
+// What is another vector's or past the row is left out of sums by masking one factor of each term (own()), and is not stored.
+template <typename T, int LAYOUT>
+__device__ inline u32x4 load_vec(const T* row, const Place<T, LAYOUT>& p) {
+  return *reinterpret_cast<const u32x4_any*>(row + p.col);
+}
+template <typename T, int LAYOUT>
+__device__ inline u32x4 own(u32x4 v, const Place<T, LAYOUT>& p) {
+  if constexpr (LAYOUT != kEven) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) v[i] &= (2 * i < p.skip ? 0u : 0xffffu) | (2 * i + 1 < p.skip ? 0u : 0xffff0000u);
+      else v[i] = i < p.skip ? 0u : v[i];
+    }
+  }
+  return v;
+}
+template <typename T, int LAYOUT>
+__device__ inline void store_vec(T* row, const Place<T, LAYOUT>& p, const u32x4& v) {
+  constexpr int EPV = VecTraits<T>::kN;
+  if (LAYOUT == kEven || p.skip == 0) {
+    *reinterpret_cast<u32x4_any*>(row + p.col) = v;
+  } else if (p.skip < EPV) {
+#pragma unroll
+    for (int i = 1; i < EPV; ++i)
+      if (i >= p.skip) row[p.col + i] = from_f32<T>(get<T>(v, i));
+  }
+}
+
+// A row's sum over its lanes.  kGroup: the work-group's waves in order, through one of two places of sum_s in
+// turn (the barrier of the next sum is between this one's reads and the next writes to its place).
+template <int LAYOUT>
+__device__ inline float row_sum(float v, int lpr, float (*sum_s)[16], int& turn) {
+  for (int off = lpr >> 1; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  if constexpr (LAYOUT == kGroup) {
+    float* s = sum_s[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = s[0];
+    for (int w = 1; w < (int)blockDim.x >> 6; ++w) v += s[w];
+  }
+  return v;
+}
+
+// The rows of a work-group, one after the other: the first, the step, a lane's place in its row.
+template <int LAYOUT>
+struct Rows {
+  int lane, wave, li, sub, lanes, lpr;
+  int64_t first, step;
+  __device__ inline Rows(int lpr_) {
+    lpr = LAYOUT == kEven ? lpr_ : 64;
+    lane = threadIdx.x & 63;
+    wave = threadIdx.x >> 6;
+    lanes = LAYOUT == kGroup ? (int)blockDim.x : lpr;
+    li = LAYOUT == kGroup ? (int)threadIdx.x : lane % lpr;
+    sub = LAYOUT == kEven ? lane / lpr : 0;
+    const int rpw = 64 / lpr;
+    first = LAYOUT == kGroup ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x * 4 + wave) * rpw;
+    step = LAYOUT == kGroup ? (int64_t)gridDim.x : (int64_t)gridDim.x * 4 * rpw;
+  }
+};
+
+constexpr int threads_of(int layout) { return layout == kGroup ? 1024 : 256; }
+
+template <typename T, int VPL, int LAYOUT, bool PLAIN>
+__global__ __launch_bounds__(threads_of(LAYOUT)) void residual_norm_fwd_kernel(NormArgs a) {
+  constexpr int EPV = VecTraits<T>::kN;
+  __shared__ float sum_s[2][16];
+  int turn = 0;
+  const Rows<LAYOUT> at(a.lpr);
+  const int D = a.D;
   for (int64_t r0 = at.first; r0 < a.rows; r0 += at.step) {
     const int64_t row = r0 + at.sub;
-    const bool act = row < a.rows;
-    const int64_t o = row * D;
-    float x[NE], y[NE];
+    const bool act = LAYOUT == kGroup || row < a.rows;
+    const int64_t o = min(row, a.rows - 1) * D;  // (lanes past the last row read it again, and write nothing)
+    u32x4 x[VPL], y[VPL];
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-      const int c = (at.li + v * lanes) * EPV, n = act ? D - c : 0;
-      load_row<T>((const T*)a.x + o + c, n, x + v * EPV);
-      load_row<T>((const T*)a.y + o + c, n, y + v * EPV);
+      const Place<T, LAYOUT> c(at.li, at.lanes, v, D);
+      x[v] = load_vec((const T*)a.x + o, c);
+      y[v] = load_vec((const T*)a.y + o, c);
     }
-    if constexpr (!PLAIN) {
-      if (a.post) {
-        float ss = 0.f;
+    float p = 1.0f;
+    if (!PLAIN && a.post) {
+      float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < NE; ++i) ss += y[i] * y[i];
-        ss = row_sum<WIDE>(ss, WIDE ? 64 : a.lpr, sum_s);
-        const float p = 1.0f / sqrtf(ss / (float)D + a.eps);
-        if (act && at.li == 0 && a.y_rstd) a.y_rstd[row] = p;
+      for (int v = 0; v < VPL; ++v) {
+        const u32x4 mine = own(y[v], Place<T, LAYOUT>(at.li, at.lanes, v, D));
 #pragma unroll
-        for (int v = 0; v < VPL; ++v) {
-          const int c = (at.li + v * lanes) * EPV;
-          float f[EPV];
-          load_row<T>((const T*)a.post + c, D - c, f);
-#pragma unroll
-          for (int i = 0; i < EPV; ++i) y[v * EPV + i] = f[i] * (y[v * EPV + i] * p);
+        for (int i = 0; i < EPV; ++i) {
+          const float f = get<T>(mine, i);
+          ss += f * f;
         }
+        hold(y[v]);
       }
-      if (a.gate_kind != kNoGate) {
-#pragma unroll
-        for (int v = 0; v < VPL; ++v) {
-          const int c = (at.li + v * lanes) * EPV;
-          float f[EPV];
-          load_row<T>((const T*)a.gate + (a.gate_kind == kTokenGate ? o : 0) + c, act ? D - c : 0, f);
-#pragma unroll
-          for (int i = 0; i < EPV; ++i) y[v * EPV + i] *= f[i];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < NE; ++i) y[i] *= a.scale;
+      ss = row_sum<LAYOUT>(ss, at.lpr, sum_s, turn);
+      p = 1.0f / sqrtf(ss / (float)D + a.eps);
+      if (act && at.li == 0 && a.y_rstd) a.y_rstd[row] = p;
     }
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      x[i] = round_to<T>(x[i] + y[i]);
-      ss += x[i] * x[i];
+    for (int v = 0; v < VPL; ++v) {
+      const Place<T, LAYOUT> c(at.li, at.lanes, v, D);
+      float f[EPV];
+      if constexpr (PLAIN) {
+#pragma unroll
+        for (int i = 0; i < EPV; ++i) f[i] = get<T>(x[v], i) + get<T>(y[v], i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < EPV; ++i) f[i] = get<T>(y[v], i);
+        if (a.post) {
+          const u32x4 post = load_vec((const T*)a.post, c);
+#pragma unroll
+          for (int i = 0; i < EPV; ++i) f[i] = get<T>(post, i) * (f[i] * p);
+        }
+        if (a.gate_kind != kNoGate) {
+          const u32x4 gate = load_vec((const T*)a.gate + (a.gate_kind == kTokenGate ? o : 0), c);
+#pragma unroll
+          for (int i = 0; i < EPV; ++i) f[i] *= get<T>(gate, i);
+        }
+#pragma unroll
+        for (int i = 0; i < EPV; ++i) f[i] = get<T>(x[v], i) + f[i] * a.scale;
+      }
+      x[v] = own(pack<T>(f), c);  // r
+#pragma unroll
+      for (int i = 0; i < EPV; ++i) {
+        const float r = get<T>(x[v], i);
+        ss += r * r;
+      }
+      hold(x[v]);
     }
-    ss = row_sum<WIDE>(ss, WIDE ? 64 : a.lpr, sum_s);
+    ss = row_sum<LAYOUT>(ss, at.lpr, sum_s, turn);
     const float q = 1.0f / sqrtf(ss / (float)D + a.eps);
     if (!act) continue;
     if (at.li == 0 && a.rstd) a.rstd[row] = q;
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-      const int c = (at.li + v * lanes) * EPV;
-      store_row<T>((T*)a.r + o + c, D - c, x + v * EPV);
+      const Place<T, LAYOUT> c(at.li, at.lanes, v, D);
+      const u32x4 gamma = load_vec((const T*)a.gamma, c);
+      store_vec((T*)a.r + o, c, x[v]);
       float f[EPV];
-      load_row<T>((const T*)a.gamma + c, D - c, f);
 #pragma unroll
-      for (int i = 0; i < EPV; ++i) f[i] = f[i] * x[v * EPV + i] * q;
-      store_row<T>((T*)a.h + o + c, D - c, f);
+      for (int i = 0; i < EPV; ++i) f[i] = get<T>(gamma, i) * get<T>(x[v], i) * q;
+      store_vec((T*)a.h + o, c, pack<T>(f));
     }
   }
 }
 
+// The three tensors of a row that every backward reads; the next row's are loaded before this row's sums.
+template <typename T, int VPL, int LAYOUT>
+struct RowIn {
+  u32x4 r[VPL], dh[VPL], dr[VPL];
+  float q;
+  __device__ inline void load(const NormArgs& a, int64_t row, int li, int lanes) {
+    const bool here = LAYOUT == kGroup || row < a.rows;
+    row = min(row, a.rows - 1);
+    const int64_t o = row * a.D;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      const Place<T, LAYOUT> c(li, lanes, v, a.D);
+      r[v] = load_vec((const T*)a.r + o, c);
+      dh[v] = dr[v] = u32x4{0, 0, 0, 0};
+      if (a.dh) dh[v] = load_vec((const T*)a.dh + o, c);
+      if (a.dr) dr[v] = load_vec((const T*)a.dr + o, c);
+    }
+    q = here ? a.rstd[row] : 0.f;  // (lanes past the last row add nothing to the sums over rows)
+  }
+};
+
 // sums: dgamma, and where they are wanted dpost and the channel gate's, in that order.
-template <typename T, int VPL, bool WIDE, bool PLAIN>
-__global__ __launch_bounds__(256) void residual_norm_bwd_kernel(NormArgs a) {
+template <typename T, int VPL, int LAYOUT, bool PLAIN>
+__global__ __launch_bounds__(threads_of(LAYOUT)) void residual_norm_bwd_kernel(NormArgs a) {
   constexpr int EPV = VecTraits<T>::kN, NE = VPL * EPV, SUMS = PLAIN ? 1 : 3;
-  __shared__ float sum_s[4];
-  __shared__ float red_s[WIDE ? 1 : 4 * 64 * NE];
-  const Rows<WIDE> at(a.lpr);
-  const int lanes = WIDE ? 256 : a.lpr, D = a.D;
+  __shared__ float sum_s[2][16];
+  __shared__ float red_s[LAYOUT == kGroup ? 1 : 4 * 64 * NE];
+  int turn = 0;
+  const Rows<LAYOUT> at(a.lpr);
+  const int D = a.D;
   float sums[SUMS][NE];
 #pragma unroll
   for (int k = 0; k < SUMS; ++k)
 #pragma unroll
     for (int i = 0; i < NE; ++i) sums[k][i] = 0.f;
+  const bool need_y = !PLAIN && (a.post || a.gate_kind != kNoGate);
+  u32x4 gamma[VPL], post[VPL], gate[VPL];
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) {
+    const Place<T, LAYOUT> c(at.li, at.lanes, v, D);
+    gamma[v] = own(load_vec((const T*)a.gamma, c), c);
+    post[v] = gate[v] = u32x4{0, 0, 0, 0};
+    if (!PLAIN && a.post) post[v] = own(load_vec((const T*)a.post, c), c);
+    if (!PLAIN && a.gate_kind == kChannelGate) gate[v] = load_vec((const T*)a.gate, c);
+  }
+  RowIn<T, VPL, LAYOUT> next;
+  if (at.first < a.rows) next.load(a, at.first + at.sub, at.li, at.lanes);
   for (int64_t r0 = at.first; r0 < a.rows; r0 += at.step) {
     const int64_t row = r0 + at.sub;
-    const bool act = row < a.rows;
-    const int64_t o = row * D;
-    float g[NE], n[NE], d[NE];  // dh then g; r then n; dr
+    const bool act = LAYOUT == kGroup || row < a.rows;
+    const int64_t o = min(row, a.rows - 1) * D;
+    RowIn<T, VPL, LAYOUT> in = next;
+    u32x4 y[VPL];
+    if constexpr (!PLAIN) {
 #pragma unroll
-    for (int v = 0; v < VPL; ++v) {
-      const int c = (at.li + v * lanes) * EPV, left = act ? D - c : 0;
-      load_row<T>((const T*)a.r + o + c, left, n + v * EPV);
-      load_row<T>((const T*)a.dh + o + c, a.dh ? left : 0, g + v * EPV);
-      load_row<T>((const T*)a.dr + o + c, a.dr ? left : 0, d + v * EPV);
+      for (int v = 0; v < VPL; ++v) {
+        const Place<T, LAYOUT> c(at.li, at.lanes, v, D);
+        y[v] = u32x4{0, 0, 0, 0};
+        if (need_y) y[v] = load_vec((const T*)a.y + o, c);
+        if (a.gate_kind == kTokenGate) gate[v] = load_vec((const T*)a.gate + o, c);
+      }
     }
-    const float q = act ? a.rstd[row] : 0.f;
+    const float p = !PLAIN && a.post ? a.y_rstd[min(row, a.rows - 1)] : 1.0f;
+    if (r0 + at.step < a.rows) next.load(a, r0 + at.step + at.sub, at.li, at.lanes);
     float s = 0.f;
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
-      const int c = (at.li + v * lanes) * EPV;
-      float f[EPV];
-      load_row<T>((const T*)a.gamma + c, D - c, f);
 #pragma unroll
       for (int i = 0; i < EPV; ++i) {
-        const int e = v * EPV + i;
-        n[e] *= q;
-        sums[0][e] += g[e] * n[e];
-        g[e] *= f[i];
-        s += g[e] * n[e];
+        const float t = get<T>(in.dh[v], i) * (get<T>(in.r[v], i) * in.q);
+        sums[0][v * EPV + i] += t;
+        s += get<T>(gamma[v], i) * t;
       }
+      hold(in.dh[v]);
+      hold(in.r[v]);
+      hold(gamma[v]);
     }
-    s = row_sum<WIDE>(s, WIDE ? 64 : a.lpr, sum_s) / (float)D;
+    s = row_sum<LAYOUT>(s, at.lpr, sum_s, turn) / (float)D;
+    float d[PLAIN ? 1 : NE];
+    float t = 0.f;
+    const float scale = act ? a.scale : 0.f;  // (likewise)
 #pragma unroll
-    for (int i = 0; i < NE; ++i) d[i] += q * (g[i] - n[i] * s);
-    if (act) {
+    for (int v = 0; v < VPL; ++v) {
+      const Place<T, LAYOUT> c(at.li, at.lanes, v, D);
+      float f[EPV];
 #pragma unroll
-      for (int v = 0; v < VPL; ++v) {
-        const int c = (at.li + v * lanes) * EPV;
-        store_row<T>((T*)a.dx + o + c, D - c, d + v * EPV);
-      }
-    }
-    if constexpr (!PLAIN) {
-      // d becomes db; n the norm of y (or y) and g the branch b
-#pragma unroll
-      for (int i = 0; i < NE; ++i) d[i] *= a.scale;
-      const bool need_y = a.post || a.gate_kind != kNoGate;
-      const float p = a.post && act ? a.y_rstd[row] : 1.0f;
-#pragma unroll
-      for (int v = 0; v < VPL; ++v) {
-        const int c = (at.li + v * lanes) * EPV, left = act ? D - c : 0;
-        float post[EPV], gate[EPV];
-        load_row<T>((const T*)a.y + o + c, need_y ? left : 0, n + v * EPV);
-        load_row<T>((const T*)a.post + c, a.post ? D - c : 0, post);
-        load_row<T>((const T*)a.gate + (a.gate_kind == kTokenGate ? o : 0) + c, a.gate_kind != kNoGate ? left : 0, gate);
+      for (int i = 0; i < EPV; ++i)
+        f[i] = get<T>(in.dr[v], i) +
+               in.q * (get<T>(in.dh[v], i) * get<T>(gamma[v], i) - get<T>(in.r[v], i) * in.q * s);
+      if (act) store_vec((T*)a.dx + o, c, pack<T>(f));
+      if constexpr (!PLAIN) {
+        // f becomes db through the gate, then post's
+        float dg[EPV];
 #pragma unroll
         for (int i = 0; i < EPV; ++i) {
           const int e = v * EPV + i;
-          n[e] *= p;
-          const float b = a.post ? post[i] * n[e] : n[e];
+          const float m = get<T>(y[v], i) * p;
+          f[i] *= scale;
           if (a.gate_kind != kNoGate) {
-            const float dg = d[e] * b;
-            sums[2][e] += dg;
-            d[e] *= gate[i];
-            gate[i] = dg;
+            dg[i] = f[i] * (a.post ? get<T>(post[v], i) * m : m);
+            sums[2][e] += dg[i];
+            f[i] *= get<T>(gate[v], i);
           }
           if (a.post) {
-            sums[1][e] += d[e] * n[e];
-            d[e] *= post[i];
+            sums[1][e] += f[i] * m;
+            f[i] *= get<T>(post[v], i);
           }
+          d[e] = f[i];
+          t += f[i] * m;
         }
-        if (a.gate_kind == kTokenGate && act) store_row<T>((T*)a.dgate + o + c, D - c, gate);
+        hold(y[v]);
+        hold(post[v]);
+        hold(gate[v]);
+        if (a.gate_kind == kTokenGate && act) store_vec((T*)a.dgate + o, c, pack<T>(dg));
       }
-      if (a.post) {
-        float t = 0.f;
-#pragma unroll
-        for (int i = 0; i < NE; ++i) t += d[i] * n[i];
-        t = row_sum<WIDE>(t, WIDE ? 64 : a.lpr, sum_s) / (float)D;
-#pragma unroll
-        for (int i = 0; i < NE; ++i) d[i] = p * (d[i] - n[i] * t);
-      }
-      if (act && a.dy) {
+    }
+    if constexpr (!PLAIN) {
+      if (a.post) t = row_sum<LAYOUT>(t, at.lpr, sum_s, turn) / (float)D;
+      if (act) {
 #pragma unroll
         for (int v = 0; v < VPL; ++v) {
-          const int c = (at.li + v * lanes) * EPV;
-          store_row<T>((T*)a.dy + o + c, D - c, d + v * EPV);
+          float f[EPV];
+#pragma unroll
+          for (int i = 0; i < EPV; ++i) {
+            const int e = v * EPV + i;
+            f[i] = a.post ? p * (d[e] - get<T>(y[v], i) * p * t) : d[e];
+          }
+          store_vec((T*)a.dy + o, Place<T, LAYOUT>(at.li, at.lanes, v, D), pack<T>(f));
         }
       }
     }
   }
   // the work-group's sums, one row of the partials each
   const bool wanted[3] = {true, !PLAIN && a.post, !PLAIN && a.gate_kind == kChannelGate};
+  const int count = 1 + (int)wanted[1] + (int)wanted[2];
   int place = 0;
 #pragma unroll
   for (int k = 0; k < SUMS; ++k) {
     if (!wanted[k]) continue;
-    const int count = 1 + (int)wanted[1] + (int)wanted[2];
     float* out = a.partial + ((int64_t)blockIdx.x * count + place++) * D;
-    if constexpr (WIDE) {
+    if constexpr (LAYOUT == kGroup) {
 #pragma unroll
-      for (int v = 0; v < VPL; ++v)
+      for (int v = 0; v < VPL; ++v) {
+        const Place<T, LAYOUT> c(at.li, at.lanes, v, D);
 #pragma unroll
-        for (int i = 0; i < EPV; ++i) {
-          const int c = (at.li + v * lanes) * EPV + i;
-          if (c < D) out[c] = sums[k][v * EPV + i];
-        }
+        for (int i = 0; i < EPV; ++i)
+          if (i >= c.skip) out[c.col + i] = sums[k][v * EPV + i];
+      }
     } else {
+      // by element: a lane's vector v is vector li + v lanes of the row
 #pragma unroll
       for (int i = 0; i < NE; ++i) {
         float v = sums[k][i];
-        for (int off = a.lpr; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
+        for (int off = at.lpr; off < 64; off <<= 1) v += __shfl_xor(v, off, 64);
         if (at.sub == 0) red_s[(at.wave * 64 + at.li) * NE + i] = v;
       }
       __syncthreads();
       for (int c = threadIdx.x; c < D; c += 256) {
-        const int vec = c / EPV, l = vec % lanes, v = vec / lanes;
+        const int vec = c / EPV, l = vec % at.lanes, v = vec / at.lanes;
+        const int e = c - Place<T, LAYOUT>(l, at.lanes, v, D).col;
         float t = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) t += red_s[(w * 64 + l) * NE + v * EPV + c % EPV];
+        for (int w = 0; w < 4; ++w) t += red_s[(w * 64 + l) * NE + v * EPV + e];
         out[c] = t;
       }
       __syncthreads();
@@ -348,69 +431,73 @@ __global__ __launch_bounds__(1024) void residual_norm_sum_kernel(const float* __
 
 // ---------------------------------------------------------------- host
 
-constexpr int kBwdBlocks = 512;  // at most: a row of partials each
+constexpr int kBwdBlocks = 768;  // at most: a row of partials each
 constexpr int kFwdBlocks = 4096;
+// Waves of the backward that a CU holds at once, by its registers: a work-group more would wait for a place and
+// then work alone.
+constexpr int kBwdWavesPlain = 24, kBwdWaves = 16;
+constexpr int kWaveVectors = 2;   // of a lane in kWave; one in kGroup
 
 struct Shape {
-  int lpr, vpl;
-  bool wide;
+  int layout, lpr, vpl, threads;
   int64_t blocks(int64_t rows, int most) const {
-    const int64_t per = wide ? 1 : 4 * (64 / lpr);
+    const int64_t per = layout == kGroup ? 1 : 4 * (64 / lpr);
     return std::max<int64_t>(1, std::min<int64_t>((rows + per - 1) / per, most));
   }
 };
 
-// The RMSNorm kernels' lanes where they take D (the largest power of two that divides the row's vectors), or a whole
-// wave, up to `most` vectors a lane; else a work-group.
+// kEven where the RMSNorm kernels take D and a lane would hold at most `most` vectors; else kWave with up to two, else kGroup.
 Shape shape_of(int64_t D, int epv, int most) {
   const int64_t nvec = (D + epv - 1) / epv;
   int lpr = 64;
   while (lpr > 1 && nvec % lpr != 0) lpr >>= 1;
-  if (D % epv != 0 || nvec / lpr > most) lpr = 64;
-  int64_t v = (nvec + lpr - 1) / lpr;
-  const bool wide = v > most;
-  if (wide) v = (nvec + 255) / 256;
-  return {wide ? 64 : lpr, (int)(v <= 1 ? 1 : v <= 2 ? 2 : v <= 4 ? 4 : 8), wide};
+  const int64_t each = nvec / lpr;
+  if (D % epv == 0 && each <= most && (each & (each - 1)) == 0) return {kEven, lpr, (int)each, 256};
+  if (nvec <= 64 * kWaveVectors) return {kWave, 64, nvec <= 64 ? 1 : 2, 256};
+  return {kGroup, 64, 1, (int)((nvec + 63) / 64) * 64};
 }
 
-constexpr int kFwdVectors = 8, kBwdVectors = 2;  // of a lane before a row takes a work-group
+constexpr int kFwdVectors = 8, kBwdVectors = 2;  // of a lane in kEven
 
 int check(const char* name, int64_t rows, int64_t D, int gate_kind, bool gate, int dtype) {
   ABACUS_CHECK_ARG(dtype == kF32 || dtype == kBF16, "%s: unsupported dtype code %d (0 = fp32, 1 = bf16)", name, dtype);
   ABACUS_CHECK_ARG(rows >= 0, "%s: %lld rows", name, (long long)rows);
-  const int most = 256 * 8 * (dtype == kBF16 ? 8 : 4);
-  ABACUS_CHECK_ARG(D >= 1 && D <= most, "%s: dim %lld, at most %d", name, (long long)D, most);
+  const int least = dtype == kBF16 ? 8 : 4, most = 1024 * least;
+  ABACUS_CHECK_ARG(D >= least && D <= most, "%s: dim %lld, %d to %d", name, (long long)D, least, most);
   ABACUS_CHECK_ARG(gate_kind >= kNoGate && gate_kind <= kTokenGate && gate == (gate_kind != kNoGate), "%s: gate kind %d", name,
                    gate_kind);
   return 0;
 }
 
-template <typename T, bool WIDE, bool PLAIN, bool BWD>
-int launch(const NormArgs& a, int vpl, int64_t blocks, hipStream_t s) {
-#define ABACUS_GO(V)                                                                                               \
-  do {                                                                                                             \
-    if constexpr (BWD) hipLaunchKernelGGL((residual_norm_bwd_kernel<T, V, WIDE, PLAIN>), dim3((unsigned)blocks), dim3(256), 0, s, a); \
-    else hipLaunchKernelGGL((residual_norm_fwd_kernel<T, V, WIDE, PLAIN>), dim3((unsigned)blocks), dim3(256), 0, s, a); \
-  } while (0)
-  if (vpl == 1) ABACUS_GO(1);
-  else if (vpl == 2) ABACUS_GO(2);
-  else if constexpr (!BWD || WIDE) {
-    if (vpl == 4) ABACUS_GO(4);
-    else ABACUS_GO(8);
-  }
-#undef ABACUS_GO
+template <typename T, int VPL, int LAYOUT, bool PLAIN, bool BWD>
+int launch(const NormArgs& a, const Shape& sh, int64_t blocks, hipStream_t s) {
+  if constexpr (BWD)
+    hipLaunchKernelGGL((residual_norm_bwd_kernel<T, VPL, LAYOUT, PLAIN>), dim3((unsigned)blocks), dim3(sh.threads), 0, s, a);
+  else
+    hipLaunchKernelGGL((residual_norm_fwd_kernel<T, VPL, LAYOUT, PLAIN>), dim3((unsigned)blocks), dim3(sh.threads), 0, s, a);
   ABACUS_CHECK_LAUNCH("residual_norm");
   return 0;
 }
 
+template <typename T, bool PLAIN, bool BWD>
+int by_shape(const NormArgs& a, const Shape& sh, int64_t blocks, hipStream_t s) {
+  if (sh.layout == kGroup) return launch<T, 1, kGroup, PLAIN, BWD>(a, sh, blocks, s);
+  if (sh.layout == kWave)
+    return sh.vpl == 1 ? launch<T, 1, kWave, PLAIN, BWD>(a, sh, blocks, s) : launch<T, 2, kWave, PLAIN, BWD>(a, sh, blocks, s);
+  if (sh.vpl == 1) return launch<T, 1, kEven, PLAIN, BWD>(a, sh, blocks, s);
+  if (sh.vpl == 2) return launch<T, 2, kEven, PLAIN, BWD>(a, sh, blocks, s);
+  if constexpr (!BWD) {
+    if (sh.vpl == 4) return launch<T, 4, kEven, PLAIN, BWD>(a, sh, blocks, s);
+    return launch<T, 8, kEven, PLAIN, BWD>(a, sh, blocks, s);
+  }
+  return 1;  // (not reached: kBwdVectors is 2)
+}
+
 template <bool BWD>
 int dispatch(const NormArgs& a, const Shape& sh, int64_t blocks, int dtype, hipStream_t s) {
-  const bool plain = !a.post && a.gate_kind == kNoGate && a.scale == 1.0f;
-#define ABACUS_GO(T)                                                                                  \
-  (sh.wide ? (plain ? launch<T, true, true, BWD>(a, sh.vpl, blocks, s) : launch<T, true, false, BWD>(a, sh.vpl, blocks, s)) \
-           : (plain ? launch<T, false, true, BWD>(a, sh.vpl, blocks, s) : launch<T, false, false, BWD>(a, sh.vpl, blocks, s)))
-  return dtype == kBF16 ? ABACUS_GO(uint16_t) : ABACUS_GO(float);
-#undef ABACUS_GO
+  if (!a.post && a.gate_kind == kNoGate && a.scale == 1.0f)
+    return dtype == kBF16 ? by_shape<uint16_t, true, BWD>(a, sh, blocks, s) : by_shape<float, true, BWD>(a, sh, blocks, s);
+  return dtype == kBF16 ? by_shape<uint16_t, false, BWD>(a, sh, blocks, s) : by_shape<float, false, BWD>(a, sh, blocks, s);
 }
 
 int sums_of(bool post, int gate_kind) { return 1 + (post ? 1 : 0) + (gate_kind == kChannelGate ? 1 : 0); }
@@ -483,7 +570,9 @@ int abacus_residual_norm_bwd(const void* dr, const void* dh, const void* r, cons
   a.partial = (float*)ws;
   const Shape sh = shape_of(D, dtype == kBF16 ? 8 : 4, kBwdVectors);
   a.lpr = sh.lpr;
-  const int64_t blocks = sh.blocks(rows, kBwdBlocks);
+  const bool plain = !post_gamma && gate_kind == kNoGate && scale == 1.0f;
+  const int at_once = std::max(1, (plain ? kBwdWavesPlain : kBwdWaves) / (sh.threads / 64));
+  const int64_t blocks = sh.blocks(rows, std::min(kBwdBlocks, 256 * at_once));
   const hipStream_t s = (hipStream_t)stream;
   if (int rc = dispatch<true>(a, sh, blocks, dtype, s)) return rc;
   SumOut o{{dgamma, dgate, nullptr}};

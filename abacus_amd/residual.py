@@ -125,9 +125,9 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, gamma: torch.Tensor, post_ga
         raise ValueError("residual_norm takes tensors on one device")
     if x.device.type == "cpu" or x.numel() == 0:
         return _plain(x, y, gamma, post_gamma, gate, scale, eps)
-    most = 16384 if _lib.dtype_code(x.dtype, x.device) == _lib.BF16 else 8192
-    if D > most:
-        raise ValueError(f"residual_norm takes a dim of at most {most} for {x.dtype}, got {D}")
+    least, most = (8, 8192) if _lib.dtype_code(x.dtype, x.device) == _lib.BF16 else (4, 4096)
+    if not least <= D <= most:
+        raise ValueError(f"residual_norm takes a dim of {least} to {most} for {x.dtype} on the GPU, got {D}")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *tensors)):
         return _ResidualNorm.apply(x, y, gamma, post_gamma, gate, float(scale), float(eps))
     operands = [None if t is None else _contig(t) for t in (x, y, gamma, post_gamma, gate)]

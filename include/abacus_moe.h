@@ -461,7 +461,7 @@ int abacus_embedding_bwd(const int64_t* tokens_T, const void* d_out_TD, int64_t 
  * Backward, of dr and dh (NULL: zeros): dx, dy (may be dx's own memory or NULL where b is y and
  * scale 1 without a gate: they are the same), dgamma, and dpost and dgate with post_gamma and gate; sums over rows in
  * fp32, in a fixed order.  y is read with a gate or post_gamma only.
- * ws: abacus_residual_norm_bwd_ws_bytes bytes.  D at most 16384 (bf16) or 8192 (fp32). */
+ * ws: abacus_residual_norm_bwd_ws_bytes bytes.  D: 8 to 8192 (bf16), 4 to 4096 (fp32). */
 int abacus_residual_norm_fwd(const void* x, const void* y, const void* gamma, const void* post_gamma, const void* gate,
                              int gate_kind, int64_t rows, int64_t D, float scale, float eps, int dtype, void* r,
                              void* h, float* rstd, float* y_rstd, void* stream);
