@@ -47,6 +47,7 @@ struct LceArgs {
   int T, D, V, Dp, Vp;    // Dp, Vp: whole vectors; also the pitches of xc, P and the padded w
   int64_t ldv;
   int chunk, chunk_rows;  // this chunk's number, rows a chunk
+  int chunks;
   int reduction;          // ABACUS_LOSS_*
   int grad;               // P is wanted
   const float* row_grad;  // weights of the rows, or NULL
@@ -62,7 +63,7 @@ struct LceArgs {
   void* xc;               // kept rows of x
   float2* stats;          // (strip, chunk row): maximum, sum
   void* p;                // (chunk rows, Vp)
-  float* acc;             // dw over several chunks, (D, V)
+  float* acc;             // dw over several chunks
   float* parts;           // tiles of a sliced product
 };
 
@@ -74,18 +75,29 @@ __device__ inline int chunk_kept(const LceArgs& a) {
   return max(0, min(a.chunk_rows, *a.kept - a.chunk * a.chunk_rows));
 }
 
-// Slices of a product's reduction: as few rounds of the CUs as possible, a k-tile and its share of prologue and
-// epilogue counted alike (about 1 us), the partial tiles' way out and back at 4 TB/s.
-__host__ __device__ inline int slices_of(int tiles, int ktiles, int tile_kb) {
+// About what a tile's k-tile takes (us, with every CU at work), and its prologue and epilogue.
+template <typename T, int BMT> constexpr float kTileUs = sizeof(T) == 2 ? (BMT == BM ? 1.9f : 1.15f) : (BMT == BM ? 7.0f : 1.9f);
+template <int KIND, int BMT> constexpr float kEndsUs = (BMT == BM ? 8.f : 4.f) * (KIND == kLogits ? 1.5f : 1.f);
+
+// The time of a product cut into `slices` of its reduction: rounds of the CUs, and for partial tiles another launch
+// and their way out and back at 4 TB/s.
+template <typename T, int KIND, int BMT>
+__host__ __device__ inline float product_us(int64_t tiles, int ktiles, int slices) {
+  const float rounds = (float)((tiles * slices + kCUs - 1) / kCUs);
+  const float us = rounds * ((float)((ktiles + slices - 1) / slices) * kTileUs<T, BMT> + kEndsUs<KIND, BMT>);
+  return slices == 1 ? us : us + 6.f + (float)(tiles * slices) * (BMT * Geo<BMT, T>::BN * 4) * 2.f / 4.0e6f;
+}
+template <typename T, int KIND, int BMT>
+__host__ __device__ inline int slices_of(int64_t tiles, int ktiles) {
   int best = 1;
-  float least = 3.0e38f;
-  for (int s = 1; s <= kSlices && (s == 1 || (tiles * s <= kUnits && ktiles >= 4 * s)); ++s) {
-    const float rounds = (float)((tiles * s + kCUs - 1) / kCUs);
-    const float cost = rounds * ((float)((ktiles + s - 1) / s) + 4.f) +
-                       (s > 1 ? 4.f + (float)(tiles * s) * (float)tile_kb * 5e-4f : 0.f);
-    if (cost < least) {
-      least = cost;
-      best = s;
+  if constexpr (KIND != kLogits) {
+    float least = product_us<T, KIND, BMT>(tiles, ktiles, 1);
+    for (int s = 2; s <= kSlices && tiles * s <= kUnits && ktiles >= 4 * s; ++s) {
+      const float us = product_us<T, KIND, BMT>(tiles, ktiles, s);
+      if (us < least) {
+        least = us;
+        best = s;
+      }
     }
   }
   return best;
@@ -151,22 +163,60 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(LceArgs a, int rows_per)
   }
 }
 
-// w's rows of V values at a pitch of whole vectors, zeros behind them.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+// The vector at column c of a row of V values (V at least a vector), zeros past its end.  One load, always in bounds: near the
+// row's end that of its last vector, shifted.
 template <typename T>
-__global__ __launch_bounds__(256) void pad_w_kernel(const T* __restrict__ w, int64_t n, int V, int Vp, T* __restrict__ out) {
-  constexpr int VEC = kVec<T>;
-  const int vecs = Vp / VEC;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / vecs;
-    const int c = (int)(i - row * vecs) * VEC;
-    const T* src = w + row * V + c;
-    T v[VEC];
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) v[k] = c + k < V ? src[k] : from_f32<T>(0.f);
-    Vec16 o;
-    __builtin_memcpy(&o, v, 16);
-    st16(out + row * Vp + c, o);
+__device__ inline Vec16 load_end(const T* row, int c, int V) {
+  constexpr int VEC = kVec<T>, BITS = 8 * (int)sizeof(T);
+  const int at = min(c, V - VEC);
+  const u32x4_any v = *reinterpret_cast<const u32x4_any*>(row + at);
+  uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+  if (at < c) {
+    int sh = min(c - at, VEC) * BITS;
+    if (sh >= 64) {
+      lo = sh < 128 ? hi : 0;
+      hi = 0;
+      sh -= 64;
+    }
+    if (sh > 0 && sh < 64) {
+      lo = lo >> sh | hi << (64 - sh);
+      hi >>= sh;
+    }
   }
+  Vec16 o;
+  o.w[0] = (uint32_t)lo;
+  o.w[1] = (uint32_t)(lo >> 32);
+  o.w[2] = (uint32_t)hi;
+  o.w[3] = (uint32_t)(hi >> 32);
+  return o;
+}
+
+// w's rows of V values at a pitch of whole vectors, zeros behind them.  A thread takes a column of kPadRows vectors, so
+// that as many loads are in flight (2048 x 50257 bf16: 110 us a vector at a time).
+constexpr int kPadRows = 8;
+template <typename T>
+__global__ __launch_bounds__(256) void pad_w_kernel(const T* __restrict__ w, int D, int V, int Vp, T* __restrict__ out) {
+  constexpr int VEC = kVec<T>;
+  const int c = ((int)blockIdx.x * 256 + threadIdx.x) * VEC, row0 = blockIdx.y * kPadRows;
+  if (c >= Vp) return;
+  Vec16 v[kPadRows];
+#pragma unroll
+  for (int r = 0; r < kPadRows; ++r) {
+    const T* row = w + (int64_t)min(row0 + r, D - 1) * V;
+    if (V >= VEC) {
+      v[r] = load_end<T>(row, c, V);
+    } else {
+      T e[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) e[k] = k < V ? row[k] : from_f32<T>(0.f);
+      __builtin_memcpy(&v[r], e, 16);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kPadRows; ++r)
+    if (row0 + r < D) st16(out + (int64_t)(row0 + r) * Vp + c, v[r]);
 }
 
 // ---------------------------------------------------------------- the products
@@ -286,7 +336,7 @@ struct TileProduct {
       ktile(lfc, kt, false, false);
     };
     // few rows fill one fragment of a thin tile, or none of a wave's
-    if (wave_rows > 32 || FM > 2) run_tiles(std::integral_constant<int, FM>());
+    if (FM > 2 || wave_rows > 32) run_tiles(std::integral_constant<int, FM>());
     else if (wave_rows > 0) run_tiles(std::integral_constant<int, 1>());
     else run_tiles(std::integral_constant<int, 0>());
   }
@@ -309,28 +359,9 @@ __device__ inline void store_any(T* p, const float* f, int n) {
 
 // VEC finished values of a gradient at (row, col) of dx or dw; whole: rows of it are whole vectors.
 template <typename T, int KIND>
-__device__ inline void store_grad(const LceArgs& a, int kept, int row, int col, float* f, bool whole) {
-  constexpr int VEC = kVec<T>;
+__device__ inline void store_grad(const LceArgs& a, int row, int col, const float* f, bool whole) {
   const int N = KIND == kDx ? a.D : a.V;
-  T* out;
-  if (KIND == kDx) {
-    out = (T*)a.dx + (int64_t)a.idx[a.chunk * a.chunk_rows + row] * N + col;
-  } else {
-    const int64_t o = (int64_t)row * N + col;
-    const bool last = (a.chunk + 1) * (int64_t)a.chunk_rows >= kept;
-    if (a.chunk > 0) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (col + i < N) f[i] += a.acc[o + i];
-    }
-    if (!last) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (col + i < N) a.acc[o + i] = f[i];
-      return;
-    }
-    out = (T*)a.dw + o;
-  }
+  T* out = KIND == kDx ? (T*)a.dx + (int64_t)a.idx[a.chunk * a.chunk_rows + row] * N + col : (T*)a.dw + (int64_t)row * N + col;
   if (whole) {
     Vec16 v;
     if constexpr (sizeof(T) == 2) {
@@ -357,7 +388,9 @@ struct Cover {
     ktiles = (K + kBKT<T> - 1) / kBKT<T>;
     mt = (M + BMT - 1) / BMT;
     nt = (N + Geo<BMT, T>::BN - 1) / Geo<BMT, T>::BN;
-    slices = KIND == kLogits ? 1 : slices_of(mt * nt, ktiles, BMT * Geo<BMT, T>::BN / 256);
+    // (over several chunks dw's tiles are cut alike in each, as their sums go from one to the next)
+    const int most = KIND == kDw && a.chunks > 1 ? (a.chunk_rows + kBKT<T> - 1) / kBKT<T> : ktiles;
+    slices = slices_of<T, KIND, BMT>((int64_t)mt * nt, most);
   }
 };
 
@@ -397,15 +430,6 @@ __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
   // Fragment (i, j): lane l has row l % 32 and columns 8 g + 4 (l / 32) .. +3 for g = 0..3.
   const int rl = lane & 31, ch = 4 * (lane >> 5);
   if constexpr (KIND == kLogits) {
-    if (n0 + BN > a.V) {  // columns past the vocabulary are no logits
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-#pragma unroll
-        for (int q = 0; q < 16; ++q)
-          if (n0 + wn * WTN + j * 32 + 8 * (q >> 2) + ch + (q & 3) >= a.V)
-#pragma unroll
-            for (int i = 0; i < FM; ++i) acc[i][j][q] = -__builtin_inff();
-    }
     const int strip = n0 / WTN + wn, first = n0 + wn * WTN;
     uint16_t* tile = reinterpret_cast<uint16_t*>(lds);  // bf16: the exponentials' tile on its way out
     constexpr int LDC = GE::LDC, CV = BN / VEC;
@@ -413,23 +437,35 @@ __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int row = row0 + wm * WTM + i * 32 + rl;
-      float m = acc[i][0][0];
+      float l[FN][16];
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) m = fmaxf(m, acc[i][j][q]);
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
+        for (int q = 0; q < 16; ++q) l[j][q] = acc[i][j][q];
+      if (n0 + BN > a.V) {  // columns past the vocabulary are no logits
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            if (first + j * 32 + 8 * (q >> 2) + ch + (q & 3) >= a.V) l[j][q] = -__builtin_inff();
+      }
       if (row < n) {
         const int t = a.tgt[a.chunk * a.chunk_rows + row] - first;
         if (t >= 0 && t < WTN && ((t >> 2) & 1) == (lane >> 5)) {
-          float l = 0.f;
+          float at = 0.f;
 #pragma unroll
           for (int j = 0; j < FN; ++j)
 #pragma unroll
-            for (int q = 0; q < 16; ++q) l = t == j * 32 + 8 * (q >> 2) + ch + (q & 3) ? acc[i][j][q] : l;
-          a.target_logit[a.chunk * a.chunk_rows + row] = l;
+            for (int q = 0; q < 16; ++q) at = t == j * 32 + 8 * (q >> 2) + ch + (q & 3) ? l[j][q] : at;
+          a.target_logit[a.chunk * a.chunk_rows + row] = at;
         }
       }
+      float m = l[0][0];
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) m = fmaxf(m, l[j][q]);
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
       const float m2 = fmaxf(m * kLog2e, -3.0e38f);  // (finite in a strip of -inf, whose exponentials are 0)
       float s = 0.f;
 #pragma unroll
@@ -439,13 +475,18 @@ __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
           float e[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][4 * g + k], kLog2e, -m2));
+            e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(l[j][4 * g + k], kLog2e, -m2));
             s += e[k];
-            if constexpr (sizeof(T) == 4) acc[i][j][4 * g + k] = e[k];
           }
-          if (sizeof(T) == 2 && a.grad)
+          if (!a.grad) continue;
+          if constexpr (sizeof(T) == 2) {
             *reinterpret_cast<uint2*>(tile + (wm * WTM + i * 32 + rl) * LDC + wn * WTN + j * 32 + 8 * g + ch) =
                 make_uint2(encode2(e[0], e[1]), encode2(e[2], e[3]));
+          } else if (row < n && first + j * 32 + 8 * g + ch < a.Vp) {
+            // (fp32: 16 bytes of a row a lane; its tile is larger than LDS)
+            *reinterpret_cast<float4*>((float*)a.p + (int64_t)row * a.Vp + first + j * 32 + 8 * g + ch) =
+                make_float4(e[0], e[1], e[2], e[3]);
+          }
         }
       s += __shfl_xor(s, 32, 64);
       if (row < n && lane < 32 && first < a.V) a.stats[(int64_t)strip * a.chunk_rows + row] = make_float2(m2, s);
@@ -461,9 +502,9 @@ __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
     }
   }
 
-  if constexpr (KIND != kLogits || sizeof(T) == 4) {
+  if constexpr (KIND != kLogits) {
     __syncthreads();  // every fragment read is done: the tile goes out through the stages' LDS
-    if (KIND != kLogits && cv.slices > 1) {  // a slice's fp32 tile, for lce_reduce_kernel
+    if (cv.slices > 1) {  // a slice's fp32 tile, for lce_reduce_kernel
       float* out = a.parts + (int64_t)u * (BMT * BN);
 #pragma unroll
       for (int i = 0; i < FM; ++i)
@@ -473,6 +514,27 @@ __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
           for (int g = 0; g < 4; ++g)
             *reinterpret_cast<float4*>(out + (wm * WTM + i * 32 + rl) * BN + wn * WTN + j * 32 + 8 * g + ch) =
                 make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+      return;
+    }
+    // dw over several chunks: the sum so far, in the fragments' own order, whole lines a wave
+    const float4* sum = nullptr;
+    if (KIND == kDw && a.chunk > 0) sum = reinterpret_cast<const float4*>(a.acc) + (int64_t)r * (BMT * BN / 4) + tid;
+    auto value = [&](int i, int j, int g) __attribute__((always_inline)) {
+      float4 v = make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+      if (KIND == kDw && sum) {
+        const float4 x = sum[((i * FN + j) * 4 + g) * NT];
+        v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+      }
+      return v;
+    };
+    if (KIND == kDw && a.chunks > 1 && (a.chunk + 1) * (int64_t)a.chunk_rows < kept) {  // more to come
+      float4* to = reinterpret_cast<float4*>(a.acc) + (int64_t)r * (BMT * BN / 4) + tid;
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) to[((i * FN + j) * 4 + g) * NT] = value(i, j, g);
       return;
     }
     // fp32 bands of RB rows through LDS: whole rows of vectors go out
@@ -490,20 +552,17 @@ __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
 #pragma unroll
             for (int g = 0; g < 4; ++g)
               *reinterpret_cast<float4*>(band + (wm * WTM - pb * RB + i * 32 + rl) * LDB + wn * WTN + j * 32 + 8 * g + ch) =
-                  make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+                  value(i, j, g);
       }
       __syncthreads();
       for (int v = tid; v < RB * CV; v += NT) {
         const int row = row0 + pb * RB + v / CV, col = n0 + v % CV * VEC;
         const float* src = band + v / CV * LDB + v % CV * VEC;
-        if constexpr (KIND == kLogits) {
-          if (row < n && col < a.Vp)
-            *reinterpret_cast<float4*>((float*)a.p + (int64_t)row * a.Vp + col) = *reinterpret_cast<const float4*>(src);
-        } else if (row < cv.M && col < cv.N) {
+        if (row < cv.M && col < cv.N) {
           float f[VEC];
 #pragma unroll
           for (int k = 0; k < VEC; k += 4) *reinterpret_cast<float4*>(f + k) = *reinterpret_cast<const float4*>(src + k);
-          store_grad<T, KIND>(a, kept, row, col, f, whole);
+          store_grad<T, KIND>(a, row, col, f, whole);
         }
       }
       if (pb + 1 < BMT / RB) __syncthreads();
@@ -543,7 +602,17 @@ __global__ __launch_bounds__(256) void lce_reduce_kernel(LceArgs a) {
         f[k + 3] += x.w;
       }
     }
-    store_grad<T, KIND>(a, kept, row, col, f, whole);
+    if (KIND == kDw && a.chunks > 1) {  // the sum over the chunks so far, at the tile's place
+      float* sum = a.acc + (int64_t)r * (BMT * BN) + tr * BN + tc;
+      const bool done = (a.chunk + 1) * (int64_t)a.chunk_rows >= kept;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        if (a.chunk > 0) f[k] += sum[k];
+        if (!done) sum[k] = f[k];
+      }
+      if (!done) continue;
+    }
+    store_grad<T, KIND>(a, row, col, f, whole);
   }
 }
 
@@ -552,12 +621,15 @@ __global__ __launch_bounds__(256) void lce_reduce_kernel(LceArgs a) {
 // Rows of a block.  The strips' statistics of kRowsB rows are joined by 256 / kRowsB threads a row; then P takes the
 // place of the exponentials, P = exp(l - m) * (s exp(m - top) / sum), at the target s (p - 1) from its fp32 logit.
 constexpr int kRowsB = 8;
+constexpr int kStripsB = 512;  // strips whose factors are in LDS at a time
+constexpr int kAheadB = 4;     // vectors of a thread in flight
 
 template <typename T>
 __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip) {
   constexpr int VEC = kVec<T>, G = 256 / kRowsB;
   __shared__ float2 part_s[G][kRowsB];
   __shared__ float2 row_s[kRowsB];  // maximum, 1 / sum
+  __shared__ float factor_s[kStripsB];
   const int tid = threadIdx.x, n = chunk_kept(a), row0 = blockIdx.x * kRowsB, base = a.chunk * a.chunk_rows;
   if (row0 >= n) return;
   const int strips = (a.V + strip - 1) / strip;
@@ -595,37 +667,50 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip) {
   }
   if (!a.grad) return;
   __syncthreads();
-  const int kept = *a.kept, vecs = a.Vp / VEC;
+  const int kept = *a.kept;
   for (int r = 0; r < min(kRowsB, n - row0); ++r) {
     const int row = row0 + r;
     const float top = row_s[r].x, inv = row_s[r].y;
     const float s = a.row_grad ? a.row_grad[a.idx[base + row]] : a.reduction == ABACUS_LOSS_MEAN ? 1.0f / (float)kept : 1.0f;
     const int t = a.tgt[base + row];
     T* p = (T*)a.p + (int64_t)row * a.Vp;
-    for (int v = tid; v < vecs; v += 256) {
-      const int c = v * VEC;
-      const float f = s * inv * __builtin_amdgcn_exp2f(a.stats[(int64_t)(c / strip) * a.chunk_rows + row].x - top);
-      const Vec16 e = ld16(p + c);
-      float o[VEC];
+    for (int k0 = 0; k0 < strips; k0 += kStripsB) {
+      __syncthreads();
+      for (int k = tid; k < min(kStripsB, strips - k0); k += 256)
+        factor_s[k] = s * inv * __builtin_amdgcn_exp2f(a.stats[(int64_t)(k0 + k) * a.chunk_rows + row].x - top);
+      __syncthreads();
+      const int end = min(a.Vp, (k0 + kStripsB) * strip);
+      for (int c0 = k0 * strip + tid * VEC; c0 < end; c0 += 256 * VEC * kAheadB) {
+        Vec16 e[kAheadB];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        if constexpr (sizeof(T) == 2) o[k] = f * decode(k & 1 ? e.w[k >> 1] >> 16 : e.w[k >> 1] & 0xffffu);
-        else o[k] = f * bits_f32(e.w[k]);
+        for (int u = 0; u < kAheadB; ++u) e[u] = ld16(p + min(c0 + u * 256 * VEC, a.Vp - VEC));
+#pragma unroll
+        for (int u = 0; u < kAheadB; ++u) {
+          const int c = c0 + u * 256 * VEC;
+          if (c >= end) break;
+          const float f = factor_s[c / strip - k0];
+          float o[VEC];
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            if constexpr (sizeof(T) == 2) o[k] = f * decode(k & 1 ? e[u].w[k >> 1] >> 16 : e[u].w[k >> 1] & 0xffffu);
+            else o[k] = f * bits_f32(e[u].w[k]);
+          }
+          if (t >= c && t < c + VEC) {
+            const float pt = inv * __builtin_amdgcn_exp2f(__builtin_fmaf(a.target_logit[base + row], kLog2e, -top));
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) o[k] = t == c + k ? s * (pt - 1.0f) : o[k];
+          }
+          Vec16 out;
+          if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) out.w[k] = pack_bf16x2(o[2 * k], o[2 * k + 1]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) out.w[k] = f32_bits(o[k]);
+          }
+          st16(p + c, out);
+        }
       }
-      if (t >= c && t < c + VEC) {
-        const float pt = inv * __builtin_amdgcn_exp2f(__builtin_fmaf(a.target_logit[base + row], kLog2e, -top));
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) o[k] = t == c + k ? s * (pt - 1.0f) : o[k];
-      }
-      Vec16 out;
-      if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) out.w[k] = pack_bf16x2(o[2 * k], o[2 * k + 1]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) out.w[k] = f32_bits(o[k]);
-      }
-      st16(p + c, out);
     }
   }
 }
@@ -668,9 +753,34 @@ __global__ __launch_bounds__(256) void scale_kernel(T* __restrict__ t, int64_t n
 
 struct Plan {
   int Dp, Vp, chunk_rows, chunks, strip;
-  bool thin, thin_dw, pad;
+  bool thin[3], pad;  // thin: of each kind's tiles
   int64_t kept, idx, tgt, target_logit, row_loss, xc, w, stats, p, acc, parts, total;
 };
+
+template <typename T, int KIND, int BMT>
+struct Sizes {
+  int64_t tiles;
+  int ktiles;
+  Sizes(int64_t rows, int64_t D, int64_t V) {
+    const int64_t M = KIND == kDw ? D : rows, N = KIND == kDx ? D : V, K = KIND == kLogits ? D : KIND == kDx ? V : rows;
+    tiles = (M + BMT - 1) / BMT * ((N + Geo<BMT, T>::BN - 1) / Geo<BMT, T>::BN);
+    ktiles = (int)((K + kBKT<T> - 1) / kBKT<T>);
+  }
+  float us() const { return product_us<T, KIND, BMT>(tiles, ktiles, slices_of<T, KIND, BMT>(tiles, ktiles)); }
+  int64_t part_bytes() const {
+    return KIND == kLogits ? 0 : std::min<int64_t>(kUnits, tiles * kSlices) * BMT * Geo<BMT, T>::BN * 4;
+  }
+};
+
+// Whether a product of this many rows takes thin tiles: where they are the faster ones by product_us.
+template <typename T, int KIND>
+bool thin_of(int64_t rows, int64_t D, int64_t V) {
+  return Sizes<T, KIND, THIN>(rows, D, V).us() < Sizes<T, KIND, BM>(rows, D, V).us();
+}
+template <typename T, int KIND>
+int64_t part_bytes(bool thin, int64_t rows, int64_t D, int64_t V) {
+  return thin ? Sizes<T, KIND, THIN>(rows, D, V).part_bytes() : Sizes<T, KIND, BM>(rows, D, V).part_bytes();
+}
 
 template <typename T>
 Plan plan_of(int64_t T_, int64_t D, int64_t V, bool grad) {
@@ -678,16 +788,17 @@ Plan plan_of(int64_t T_, int64_t D, int64_t V, bool grad) {
   Plan q;
   q.Dp = (int)((D + VEC - 1) / VEC * VEC);
   q.Vp = (int)((V + VEC - 1) / VEC * VEC);
-  q.thin = T_ <= THIN;
-  q.thin_dw = D <= THIN;
   q.pad = V % VEC != 0;
-  q.strip = q.thin ? Geo<THIN, T>::WTN : Geo<BM, T>::WTN;
-  const int64_t strips = (V + q.strip - 1) / q.strip;
-  const int64_t row_bytes = grad ? (int64_t)q.Vp * (int64_t)sizeof(T) : strips * 8;
-  int64_t rows = std::max<int64_t>(BM, kChunkBytes / row_bytes / BM * BM);
-  rows = std::min(rows, T_);
+  // a strip is half a tile's columns; with gradients a row of P is in a chunk as a whole
+  const int64_t row_bytes = grad ? (int64_t)q.Vp * (int64_t)sizeof(T) : (V + 63) / 64 * 8;
+  const int64_t rows = std::min(T_, std::max<int64_t>(BM, kChunkBytes / row_bytes / BM * BM));
   q.chunk_rows = (int)rows;
   q.chunks = (int)((T_ + rows - 1) / rows);
+  q.thin[kLogits] = thin_of<T, kLogits>(rows, D, V);
+  q.thin[kDx] = thin_of<T, kDx>(rows, D, V);
+  q.thin[kDw] = thin_of<T, kDw>(rows, D, V);
+  q.strip = q.thin[kLogits] ? Geo<THIN, T>::WTN : Geo<BM, T>::WTN;
+  const int64_t strips = (V + q.strip - 1) / q.strip;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -703,14 +814,8 @@ Plan plan_of(int64_t T_, int64_t D, int64_t V, bool grad) {
   q.w = take(q.pad ? D * q.Vp * (int64_t)sizeof(T) : 0);
   q.stats = take(strips * rows * 8);
   q.p = take(grad ? rows * row_bytes : 0);
-  q.acc = take(grad && q.chunks > 1 ? D * V * 4 : 0);
-  auto parts = [&](int64_t M, int64_t N, int bm, int bn) {
-    const int64_t tiles = (M + bm - 1) / bm * ((N + bn - 1) / bn);
-    return std::min<int64_t>(kUnits, tiles * kSlices) * bm * bn * 4;
-  };
-  const int64_t dx = q.thin ? parts(rows, D, THIN, Geo<THIN, T>::BN) : parts(rows, D, BM, BN);
-  const int64_t dw = q.thin_dw ? parts(D, V, THIN, Geo<THIN, T>::BN) : parts(D, V, BM, BN);
-  q.parts = take(grad ? std::max(dx, dw) : 0);
+  q.acc = take(grad && q.chunks > 1 ? (D + BM - 1) / BM * BM * ((V + BN - 1) / BN * BN) * 4 : 0);
+  q.parts = take(grad ? std::max(part_bytes<T, kDx>(q.thin[kDx], rows, D, V), part_bytes<T, kDw>(q.thin[kDw], rows, D, V)) : 0);
   q.total = at;
   return q;
 }
@@ -725,9 +830,7 @@ int check_sizes(const char* name, int64_t T, int64_t D, int64_t V, int dtype) {
 
 template <typename T, int KIND, int BMT>
 int launch_product(const LceArgs& a, hipStream_t s) {
-  using GE = Geo<BMT, T>;
-  const int64_t M = KIND == kDw ? a.D : std::min(a.chunk_rows, a.T - a.chunk * a.chunk_rows), N = KIND == kDx ? a.D : a.V;
-  const int64_t tiles = (M + BMT - 1) / BMT * ((N + GE::BN - 1) / GE::BN);
+  const int64_t tiles = Sizes<T, KIND, BMT>(std::min(a.chunk_rows, a.T - a.chunk * a.chunk_rows), a.D, a.V).tiles;
   // a product of fewer rows (or a shorter reduction) may be cut into more slices, up to kUnits units
   int64_t units = KIND == kLogits ? tiles : std::max<int64_t>(tiles, std::min<int64_t>(kUnits, tiles * kSlices));
   units = (units + 7) / 8 * 8;
@@ -770,23 +873,23 @@ int run(LceArgs a, char* ws, int64_t ws_bytes, hipStream_t s) {
   hipLaunchKernelGGL(pack_rows_kernel<T>, dim3((a.T + rows_per - 1) / rows_per), dim3(256), rows_per * 4, s, a, rows_per);
   ABACUS_CHECK_LAUNCH("linear_cross_entropy pack");
   if (q.pad) {
-    const int64_t n = (int64_t)a.D * (q.Vp / VecTraits<T>::kN);
-    hipLaunchKernelGGL(pad_w_kernel<T>, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 16384)), dim3(256), 0, s,
-                       (const T*)a.w, n, a.V, q.Vp, (T*)(ws + q.w));
+    const dim3 grid((unsigned)((q.Vp / VecTraits<T>::kN + 255) / 256), (unsigned)((a.D + kPadRows - 1) / kPadRows));
+    hipLaunchKernelGGL(pad_w_kernel<T>, grid, dim3(256), 0, s, (const T*)a.w, a.D, a.V, q.Vp, (T*)(ws + q.w));
     ABACUS_CHECK_LAUNCH("linear_cross_entropy pad");
     a.w = ws + q.w;
     a.ldv = q.Vp;
   }
+  a.chunks = q.chunks;
   for (a.chunk = 0; a.chunk < q.chunks; ++a.chunk) {
-    if (int rc = q.thin ? launch_product<T, kLogits, THIN>(a, s) : launch_product<T, kLogits, BM>(a, s)) return rc;
+    if (int rc = q.thin[kLogits] ? launch_product<T, kLogits, THIN>(a, s) : launch_product<T, kLogits, BM>(a, s)) return rc;
     const int rows = std::min(a.chunk_rows, a.T - a.chunk * a.chunk_rows);
     hipLaunchKernelGGL(lce_rows_kernel<T>, dim3((rows + kRowsB - 1) / kRowsB), dim3(256), 0, s, a, q.strip);
     ABACUS_CHECK_LAUNCH("linear_cross_entropy rows");
     if (a.dx) {
-      if (int rc = q.thin ? launch_product<T, kDx, THIN>(a, s) : launch_product<T, kDx, BM>(a, s)) return rc;
+      if (int rc = q.thin[kDx] ? launch_product<T, kDx, THIN>(a, s) : launch_product<T, kDx, BM>(a, s)) return rc;
     }
     if (a.dw) {
-      if (int rc = q.thin_dw ? launch_product<T, kDw, THIN>(a, s) : launch_product<T, kDw, BM>(a, s)) return rc;
+      if (int rc = q.thin[kDw] ? launch_product<T, kDw, THIN>(a, s) : launch_product<T, kDw, BM>(a, s)) return rc;
     }
   }
   if (a.reduction != ABACUS_LOSS_ROWS && a.loss) {
