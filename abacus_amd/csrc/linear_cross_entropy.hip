@@ -3,9 +3,11 @@
 // trainer.py:77-85).
 //
 //   l = x W  (fp32),   lse_t = log sum_v exp l_tv,   loss_t = lse_t - l[t, target_t]
-//   P_tv = s_t (exp(l_tv - lse_t) - [v = target_t]),   dx = P W^T,   dw = x^T P
+//   P_tv = s_t (exp(l_tv - lse_t) - [v = target_t]),   dx = c P W^T,   dw = c x^T P
 //
-// s_t is 1 / kept rows (mean), 1 (sum) or a weight of each row.  Rows whose target is ignore_index are left out before
+// c is 1 / kept rows (mean), 1 (sum) or the largest weight of a row, and s_t 1 or the row's share of that: a factor common
+// to all rows stays out of P, whose rounding would be the same in each (a P of -1 / 7852 at every target:
+// 0.2% off in bf16) and would not average out.  Rows whose target is ignore_index are left out before
 // any product: the kept rows are packed (their count stays on the device) and every launch ends at that count, so a
 // batch of prompts costs what its answers cost.
 //
@@ -33,8 +35,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kCUs = 256;
 constexpr int64_t kChunkBytes = 1ll << 30;       // of P, or of the strips' statistics where there is no P
 constexpr int kUnits = 512;                       // tiles x slices of a sliced product at most
-constexpr int kSlices = 16;
-constexpr int kReduceRows = 16;                   // rows of a tile that a block of the adding pass takes
+constexpr int kSlices = 32;
+constexpr int kFewRows = 64;                      // rows up to which w streams once for each product, without tiles
+constexpr int kReduceRows = 4;                    // rows of a tile that a work-group of the adding pass takes
 
 enum Kind : int { kLogits = 0, kDx = 1, kDw = 2 };
 
@@ -48,6 +51,7 @@ struct LceArgs {
   int64_t ldv;
   int chunk, chunk_rows;  // this chunk's number, rows a chunk
   int chunks;
+  int thin;               // bit k: kind k's tiles are thin
   int reduction;          // ABACUS_LOSS_*
   int grad;               // P is wanted
   const float* row_grad;  // weights of the rows, or NULL
@@ -55,12 +59,15 @@ struct LceArgs {
   void* dx;               // NULL: not wanted
   void* dw;
   // workspace
-  int* kept;              // one int: the number of kept rows
+  int* kept;              // the number of kept rows, and
+  float* scale;           // the factor of both gradients, and
+  int* slices;            // (by Kind) of this chunk's products
   int* idx;               // kept row -> row
   int* tgt;               // kept row -> target (-1: outside the vocabulary)
   float* target_logit;    // of each kept row; NaN until its strip writes it
   float* row_loss;        // of each kept row
   void* xc;               // kept rows of x
+  void* xt;               // few rows: x transposed, (D, kFewRows)
   float2* stats;          // (strip, chunk row): maximum, sum
   void* p;                // (chunk rows, Vp)
   float* acc;             // dw over several chunks
@@ -87,12 +94,15 @@ __host__ __device__ inline float product_us(int64_t tiles, int ktiles, int slice
   const float us = rounds * ((float)((ktiles + slices - 1) / slices) * kTileUs<T, BMT> + kEndsUs<KIND, BMT>);
   return slices == 1 ? us : us + 6.f + (float)(tiles * slices) * (BMT * Geo<BMT, T>::BN * 4) * 2.f / 4.0e6f;
 }
+__host__ __device__ inline bool slices_fit(int64_t tiles, int ktiles, int s) {
+  return s == 1 || (s <= kSlices && tiles * s <= kUnits && ktiles >= 4 * s);
+}
 template <typename T, int KIND, int BMT>
 __host__ __device__ inline int slices_of(int64_t tiles, int ktiles) {
   int best = 1;
   if constexpr (KIND != kLogits) {
     float least = product_us<T, KIND, BMT>(tiles, ktiles, 1);
-    for (int s = 2; s <= kSlices && tiles * s <= kUnits && ktiles >= 4 * s; ++s) {
+    for (int s = 2; slices_fit(tiles, ktiles, s); ++s) {
       const float us = product_us<T, KIND, BMT>(tiles, ktiles, s);
       if (us < least) {
         least = us;
@@ -112,6 +122,7 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(LceArgs a, int rows_per)
   constexpr int VEC = kVec<T>;
   extern __shared__ int place_s[];  // rows_per
   __shared__ int wave_s[4];
+  __shared__ float most_s[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row0 = blockIdx.x * rows_per, rows = min(rows_per, a.T - row0);
   int before = 0;
@@ -136,7 +147,29 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(LceArgs a, int rows_per)
       }
       before += __popcll(mask);
     }
-    if (lane == 0 && row0 + rows == a.T) *a.kept = before;
+    if (lane == 0 && row0 + rows == a.T) {
+      *a.kept = before;
+      a.slices[kDx] = a.slices[kDw] = 1;
+      if (a.reduction != ABACUS_LOSS_ROWS) *a.scale = a.reduction == ABACUS_LOSS_MEAN ? 1.0f / (float)before : 1.0f;
+    }
+  }
+  if (a.row_grad && row0 + rows == a.T) {  // (the last work-group's business too)
+    float most = 0.f;
+    for (int i = tid; i < a.T; i += 256) {
+      const float g = fabsf(a.row_grad[i]);
+      most = a.targets[i] != a.ignore_index && !(g <= most) ? g : most;  // (a NaN stays)
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      const float o = __shfl_xor(most, off, 64);
+      most = !(o <= most) ? o : most;
+    }
+    if (lane == 0) most_s[wave] = most;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < 4; ++w) most = !(most_s[w] <= most) ? most_s[w] : most;
+      *a.scale = most == 0.f ? 1.0f : most;
+    }
   }
   __syncthreads();
   const bool whole = a.D == a.Dp && a.x_stride % VEC == 0 && (uintptr_t)a.x % 16 == 0;
@@ -193,6 +226,56 @@ __device__ inline Vec16 load_end(const T* row, int c, int V) {
   return o;
 }
 
+// The same for few rows: a work-group takes 64 columns of all of them, and turns them for dw.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_few_kernel(LceArgs a) {
+  __shared__ int place_s[kFewRows], kept_s;
+  __shared__ T tile_s[kFewRows][66];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = blockIdx.x * 64 + lane;
+  if (wave == 0) {
+    const int64_t t = lane < a.T ? a.targets[lane] : a.ignore_index;
+    const bool kept = lane < a.T && t != a.ignore_index;
+    const uint64_t mask = __ballot(kept);
+    const int at = __popcll(mask & ((1ull << lane) - 1)), n = __popcll(mask);
+    place_s[lane] = kept ? at : -1;
+    if (lane == 0) kept_s = n;
+    if (blockIdx.x == 0) {
+      if (kept) {
+        a.idx[at] = lane;
+        a.tgt[at] = t >= 0 && t < a.V ? (int)t : -1;
+        a.target_logit[at] = __builtin_nanf("");
+      } else if (lane < a.T && a.reduction == ABACUS_LOSS_ROWS && a.loss) {
+        a.loss[lane] = 0.f;
+      }
+      float most = a.row_grad && kept ? fabsf(a.row_grad[lane]) : 0.f;
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) {
+        const float o = __shfl_xor(most, off, 64);
+        most = !(o <= most) ? o : most;
+      }
+      if (lane == 0) {
+        *a.kept = n;
+        *a.scale = a.row_grad ? (most == 0.f ? 1.0f : most) : a.reduction == ABACUS_LOSS_MEAN ? 1.0f / (float)n : 1.0f;
+      }
+    }
+  }
+  __syncthreads();
+  for (int r = wave; r < a.T; r += 4) {
+    const int at = place_s[r];
+    if (at < 0) {
+      if (a.dx && c < a.D) ((T*)a.dx)[(int64_t)r * a.D + c] = from_f32<T>(0.f);
+    } else if (c < a.Dp) {
+      const T v = c < a.D ? ((const T*)a.x)[(int64_t)r * a.x_stride + c] : from_f32<T>(0.f);
+      ((T*)a.xc)[(int64_t)at * a.Dp + c] = v;
+      tile_s[at][lane] = v;
+    }
+  }
+  if (!a.xt) return;
+  __syncthreads();
+  for (int d = wave; d < min(64, a.D - (int)blockIdx.x * 64); d += 4)  // a lane a row, zeros past the last
+    ((T*)a.xt)[(int64_t)(blockIdx.x * 64 + d) * kFewRows + lane] = lane < kept_s ? tile_s[lane][d] : from_f32<T>(0.f);
+}
+
 // w's rows of V values at a pitch of whole vectors, zeros behind them.  A thread takes a column of kPadRows vectors, so
 // that as many loads are in flight (2048 x 50257 bf16: 110 us a vector at a time).
 constexpr int kPadRows = 8;
@@ -230,48 +313,75 @@ __device__ inline uint32_t encode2(float a, float b) {
 }
 __device__ inline float decode(uint32_t h) { return h ? bits_f32((h << 13) + (64u << 23)) : 0.f; }
 
-// acc[i][j] += A B over the k-tiles kbase .. kbase + ktiles - 1: the operands' tiles come by DMA into a ring of LDS
-// stages, the matrix instructions of one k-step cover the fragment reads of the next, and the last step's the DMA.
+// acc += A B over a range of k-tiles: the operands' tiles come by DMA into a ring of LDS stages, the matrix
+// instructions of one k-step cover the fragment reads of the next, and the last step's the DMA.  begin() starts the first
+// stages' DMA (every read of the stages has to be done), run() waits for them and does the rest.
 template <typename T, bool A_MC, bool B_NC, int BMT, bool RK>
 struct TileProduct {
   using Op = MfmaOp<T, 32>;
   using GE = Geo<BMT, T>;
-  static constexpr int FM = GE::FM, FN = GE::FN, WTM = GE::WTM, WTN = GE::WTN, ST = GE::ST;
+  static constexpr int FM = GE::FM, FN = GE::FN, WTM = GE::WTM, WTN = GE::WTN, ST = GE::ST, LOADS = GE::LOADS;
   static constexpr int MCC_A = BMT * (int)sizeof(T) / 16, MCC_B = GE::BN * (int)sizeof(T) / 16;
-  static constexpr int BKT = kBKT<T>;
+  static constexpr int BKT = kBKT<T>, NFRAG = FM + FN, MF = FM * FN;
   using Acc = typename Op::Acc;
+  static_assert(MF >= NFRAG, "one fragment read per MFMA at most");
 
-  static __device__ __attribute__((always_inline)) inline void run(Acc (&acc)[FM][FN], const T* A, int64_t lda, int row0, int a_lim, const T* B,
-                                    int64_t ldb, int n0, int b_lim, int kbase, int ktiles, int k_lim, int wave_rows,
-                                    char* lds) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave / WAVES_N, wn = wave % WAVES_N;
-    const int wave_u = __builtin_amdgcn_readfirstlane(wave);
-    DmaStream<T, A_MC, GE::DMA_A, BMT> sa;
-    DmaStream<T, B_NC, GE::DMA_B, GE::BN> sb;
+  DmaStream<T, A_MC, GE::DMA_A, BMT> sa;
+  DmaStream<T, B_NC, GE::DMA_B, GE::BN> sb;
+  int kbase, ktiles, k_lim;
+  char* lds;
+  uint32_t lds32, stage;
+  int k0, lane, wave_u;
+
+  __device__ __attribute__((always_inline)) inline void prep(int kt) {
+    stage = lds32 + (uint32_t)((kt % ST) * GE::STAGE);
+    k0 = (kt + kbase) * BKT;
+  }
+  // instruction n of the LOADS of the k-tile that prep() named
+  __device__ __attribute__((always_inline)) inline void dma(int n) {
+    if (n < GE::DMA_A) sa.template issue_one<RK>(n, stage, wave_u, k0, k_lim);
+    else sb.template issue_one<RK>(n - GE::DMA_A, stage + GE::A_BYTES, wave_u, k0, k_lim);
+  }
+  // At most the newest `later` k-tiles' loads may still be in flight.
+  static __device__ __attribute__((always_inline)) inline void wait_for(int later) {
+    if (ST >= 4 && later >= 3) wait_vmcnt<(ST >= 4 ? 3 : 0) * LOADS>();
+    else if (ST >= 3 && later >= 2) wait_vmcnt<(ST >= 3 ? 2 : 0) * LOADS>();
+    else if (later >= 1) wait_vmcnt<LOADS>();
+    else wait_vmcnt<0>();
+  }
+
+  __device__ __attribute__((always_inline)) inline void begin(const T* A, int64_t lda, int row0, int a_lim, const T* B, int64_t ldb, int n0,
+                                                              int b_lim, int kbase_, int ktiles_, int k_lim_, char* lds_) {
+    const int wave = threadIdx.x >> 6;
+    lane = threadIdx.x & 63;
+    wave_u = __builtin_amdgcn_readfirstlane(wave);
+    kbase = kbase_;
+    ktiles = ktiles_;
+    k_lim = k_lim_;
+    lds = lds_;
+    lds32 = lds_addr32(lds);
     sa.setup(A, nullptr, lda, row0, a_lim, wave, lane);
     sb.setup(B, nullptr, ldb, n0, b_lim, wave, lane);
-    const uint32_t lds32 = lds_addr32(lds);
-    uint32_t stage = lds32;
-    int k0 = 0;
-    auto prep = [&](int kt) __attribute__((always_inline)) {
-      stage = lds32 + (uint32_t)((kt % ST) * GE::STAGE);
-      k0 = (kt + kbase) * BKT;
-    };
-    auto dma = [&](int n) __attribute__((always_inline)) {
-      if (n < GE::DMA_A) sa.template issue_one<RK>(n, stage, wave_u, k0, k_lim);
-      else sb.template issue_one<RK>(n - GE::DMA_A, stage + GE::A_BYTES, wave_u, k0, k_lim);
-    };
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+    for (int p = 0; p < ST; ++p)
+      if (p < ktiles) {
+        prep(p);
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
-#pragma unroll
-        for (int q = 0; q < Op::kAcc; ++q) acc[i][j][q] = 0.f;
-    if (ktiles <= 0) return;
+        for (int n = 0; n < LOADS; ++n) dma(n);
+      }
+  }
 
-    constexpr int NFRAG = FM + FN, MF = FM * FN;
-    static_assert(MF >= NFRAG, "one fragment read per MFMA at most");
+  // The first k-tile has landed.  stores: vector memory operations that every wave has issued since begin(), at least;
+  // they may still be in flight.
+  template <int STORES>
+  __device__ __attribute__((always_inline)) inline void wait_first() {
+    if (ktiles < ST) wait_vmcnt<0>();
+    else wait_vmcnt<(STORES + LOADS * (ST - 1) < 63 ? STORES + LOADS * (ST - 1) : 63)>();
+  }
+
+  __device__ __attribute__((always_inline)) inline void run(Acc (&acc)[FM][FN], int wave_rows) {
+    if (ktiles <= 0) return;
+    const int wave = threadIdx.x >> 6, wm = wave / WAVES_N, wn = wave % WAVES_N;
     Vec16 af[2][FM], bf[2][FN];
     auto read_frag = [&](const char* st, int t, int slot, int f) __attribute__((always_inline)) {
       if (f == 0 || f > FN) {
@@ -294,38 +404,24 @@ struct TileProduct {
         if (with_read && m < NFRAG) read_frag(rd, rd_t, rd_slot, m);
         if (with_dma) {
 #pragma unroll
-          for (int n = m * GE::LOADS / MF; n < (m + 1) * GE::LOADS / MF; ++n) dma(n);
+          for (int n = m * LOADS / MF; n < (m + 1) * LOADS / MF; ++n) dma(n);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-    };
-    // at most `later` k-tiles' DMA may still be in flight
-    auto wait_for = [&](int later) __attribute__((always_inline)) {
-      if (ST >= 4 && later >= 3) wait_vmcnt<(ST >= 4 ? 3 : 0) * GE::LOADS>();
-      else if (ST >= 3 && later >= 2) wait_vmcnt<(ST >= 3 ? 2 : 0) * GE::LOADS>();
-      else if (later >= 1) wait_vmcnt<GE::LOADS>();
-      else wait_vmcnt<0>();
     };
     auto ktile = [&](auto lfc, int kt, bool next, bool dma_next) __attribute__((always_inline)) {
       const char* st = lds + (kt % ST) * GE::STAGE;
       const char* st_next = lds + ((kt + 1) % ST) * GE::STAGE;
 #pragma unroll
       for (int t = 0; t < NSTEP - 1; ++t) kstep(lfc, t & 1, true, st, t + 1, (t + 1) & 1, false);
-      wait_for(min(ST - 2, ktiles - 2 - kt));
+      wait_for(min(ST - 2, ktiles - 2 - kt));  // k-tile kt + 1 has landed
       __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's reads of the stage are back: it may be refilled
       __syncthreads();
       if (dma_next) prep(kt + ST);
       __builtin_amdgcn_sched_barrier(0);
       kstep(lfc, (NSTEP - 1) & 1, next, st_next, 0, 0, dma_next);
     };
-#pragma unroll
-    for (int p = 0; p < ST; ++p)
-      if (p < ktiles) {
-        prep(p);
-#pragma unroll
-        for (int n = 0; n < GE::LOADS; ++n) dma(n);
-      }
-    wait_for(min(ST, ktiles) - 1);
+    __builtin_amdgcn_s_waitcnt(0xc07f);
     __syncthreads();
 #pragma unroll
     for (int f = 0; f < NFRAG; ++f) read_frag(lds, 0, 0, f);
@@ -359,7 +455,9 @@ __device__ inline void store_any(T* p, const float* f, int n) {
 
 // VEC finished values of a gradient at (row, col) of dx or dw; whole: rows of it are whole vectors.
 template <typename T, int KIND>
-__device__ inline void store_grad(const LceArgs& a, int row, int col, const float* f, bool whole) {
+__device__ inline void store_grad(const LceArgs& a, float scale, int row, int col, float* f, bool whole) {
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) f[i] *= scale;
   const int N = KIND == kDx ? a.D : a.V;
   T* out = KIND == kDx ? (T*)a.dx + (int64_t)a.idx[a.chunk * a.chunk_rows + row] * N + col : (T*)a.dw + (int64_t)row * N + col;
   if (whole) {
@@ -388,13 +486,193 @@ struct Cover {
     ktiles = (K + kBKT<T> - 1) / kBKT<T>;
     mt = (M + BMT - 1) / BMT;
     nt = (N + Geo<BMT, T>::BN - 1) / Geo<BMT, T>::BN;
-    // (over several chunks dw's tiles are cut alike in each, as their sums go from one to the next)
-    const int most = KIND == kDw && a.chunks > 1 ? (a.chunk_rows + kBKT<T> - 1) / kBKT<T> : ktiles;
-    slices = slices_of<T, KIND, BMT>((int64_t)mt * nt, most);
+    slices = KIND == kLogits ? 1 : a.slices[KIND];
+  }
+  // slices_of by a wave, a number of slices a lane (over several chunks dw's tiles are cut alike in each, as their
+  // sums go from one to the next)
+  __device__ inline int cut(const LceArgs& a) const {
+    const int kt = KIND == kDw && a.chunks > 1 ? (a.chunk_rows + kBKT<T> - 1) / kBKT<T> : ktiles;
+    const int64_t tiles = (int64_t)mt * nt;
+    int best = (int)(threadIdx.x & 63) + 1;
+    float least = slices_fit(tiles, kt, best) ? product_us<T, KIND, BMT>(tiles, kt, best) : 3.0e38f;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+      const float us = __shfl_xor(least, off, 64);
+      const int s = __shfl_xor(best, off, 64);
+      if (us < least || (us == least && s < best)) {
+        least = us;
+        best = s;
+      }
+    }
+    return best;
   }
 };
 
-template <typename T, int KIND, int BMT, bool RK>
+template <typename TP>
+__device__ __attribute__((always_inline)) inline void clear(typename TP::Acc (&acc)[TP::FM][TP::FN]) {
+#pragma unroll
+  for (int i = 0; i < TP::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < TP::FN; ++j)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+}
+
+// An accumulator read where it is wanted: left to itself the compiler moves all 256 of a lane out of their registers at
+// once, to scratch memory.  (settle() before the first: the matrix instructions' results are there.)
+__device__ inline float taken(float v) {
+  float r;
+  asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(r) : "a"(v));
+  return r;
+}
+__device__ inline void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// Statistics and exponentials of a tile of logits.  Fragment (i, j): lane l has row l % 32 and columns
+// 8 g + 4 (l / 32) .. +3 for g = 0..3.  Everything goes straight from registers to memory, so that the
+// next tile's first DMA can be under way: two lanes of a row trade halves for 16 bytes of bf16 operands each.
+// WHOLE: every row and column of the tile is one of the product.
+template <typename T, int BMT, typename TP, bool WHOLE, bool GRAD>
+__device__ __attribute__((always_inline)) inline void logits_out(const LceArgs& a, typename TP::Acc (&acc)[TP::FM][TP::FN], const int (&tgt)[TP::FM],
+                                                                 int row0, int n0, int n) {
+  using GE = Geo<BMT, T>;
+  constexpr int FM = GE::FM, FN = GE::FN, WTM = GE::WTM, WTN = GE::WTN;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WAVES_N, wn = wave % WAVES_N;
+  const int rl = lane & 31, half = lane >> 5, strip = n0 / WTN + wn, first = n0 + wn * WTN;
+  settle();
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int row = row0 + wm * WTM + i * 32 + rl;
+    const bool here = WHOLE || row < n;
+    float l[FN][16];
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) l[j][q] = taken(acc[i][j][q]);
+    if (!WHOLE && n0 + GE::BN > a.V) {  // columns past the vocabulary are no logits
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+          if (first + j * 32 + 8 * (q >> 2) + 4 * half + (q & 3) >= a.V) l[j][q] = -__builtin_inff();
+    }
+    const int t = tgt[i] - first;
+    if (here && t >= 0 && t < WTN && ((t >> 2) & 1) == half) {
+      float at = 0.f;
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int q = 0; q < 16; ++q) at = t == j * 32 + 8 * (q >> 2) + 4 * half + (q & 3) ? l[j][q] : at;
+      a.target_logit[a.chunk * a.chunk_rows + row] = at;
+    }
+    float m[4];  // (four at a time: one chain would wait for itself)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      m[k] = l[0][4 * k];
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int q = 4 * k; q < 4 * k + 4; q += 2) m[k] = max3(m[k], l[j][q], l[j][q + 1]);
+    }
+    m[0] = fmaxf(max3(m[0], m[1], m[2]), m[3]);
+    m[0] = fmaxf(m[0], __shfl_xor(m[0], 32, 64));
+    const float m2 = fmaxf(m[0] * kLog2e, -3.0e38f);  // (finite in a strip of -inf, whose exponentials are 0)
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; g += 2) {
+        float e[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(l[j][4 * g + k], kLog2e, -m2));
+          s[k & 3] += e[k];
+        }
+        if constexpr (GRAD) {
+          const int col = first + j * 32 + 8 * g;
+          if constexpr (sizeof(T) == 2) {
+            const auto x = __builtin_amdgcn_permlane32_swap(encode2(e[0], e[1]), encode2(e[4], e[5]), false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(encode2(e[2], e[3]), encode2(e[6], e[7]), false, false);
+            if (WHOLE || (here && col + 8 * half < a.Vp)) {
+              Vec16 v;
+              v.w[0] = x[0];
+              v.w[1] = y[0];
+              v.w[2] = x[1];
+              v.w[3] = y[1];
+              st16((uint16_t*)a.p + (int64_t)row * a.Vp + col + 8 * half, v);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (WHOLE || (here && col + 8 * k + 4 * half < a.Vp))
+                *reinterpret_cast<float4*>((float*)a.p + (int64_t)row * a.Vp + col + 8 * k + 4 * half) =
+                    make_float4(e[4 * k], e[4 * k + 1], e[4 * k + 2], e[4 * k + 3]);
+          }
+        }
+      }
+    s[0] = (s[0] + s[1]) + (s[2] + s[3]);
+    s[0] += __shfl_xor(s[0], 32, 64);
+    if (here && lane < 32 && (WHOLE || first < a.V)) a.stats[(int64_t)strip * a.chunk_rows + row] = make_float2(m2, s[0]);
+  }
+}
+
+// The logits' tiles: a work-group on each CU walks its share of the XCD's tiles, and a tile's first DMA is under way while
+// the one before goes through its exponentials (8192 x 1024 x 32000 bf16, a work-group a tile, its exponentials
+// through LDS: 667 us).
+template <typename T, int BMT, bool RK, bool GRAD>
+__global__ __launch_bounds__(NT, 1) void lce_logits_kernel(LceArgs a) {
+  using GE = Geo<BMT, T>;
+  using TP = TileProduct<T, false, true, BMT, RK>;
+  __shared__ __attribute__((aligned(1024))) char lds[GE::ST * GE::STAGE];
+  const int n = chunk_kept(a);
+  if (n == 0) return;
+  const Cover<T, kLogits, BMT> cv(a, n);
+  const int units = cv.mt * cv.nt, per = (units + 7) / 8, xcd = blockIdx.x & 7, step = gridDim.x >> 3;
+  const int end = min(units, (xcd + 1) * per);  // an equal contiguous share for each XCD
+  const T* xc = (const T*)a.xc + (int64_t)a.chunk * a.chunk_rows * a.Dp;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WAVES_N;
+  TP tp;
+  int row0 = 0, n0 = 0;
+  auto begin = [&](int u) __attribute__((always_inline)) {
+    int mt, nt;
+    row_tile(u, cv.mt, cv.nt, mt, nt);
+    row0 = mt * BMT;
+    n0 = nt * GE::BN;
+    tp.begin(xc, a.Dp, row0, n, (const T*)a.w, a.ldv, n0, a.Vp, 0, cv.ktiles, cv.K, lds);
+  };
+  int u = xcd * per + ((int)blockIdx.x >> 3);
+  if (u >= end) return;
+  begin(u);
+  bool whole = false;  // every lane of the tile before stored all it has
+  for (;;) {
+    const int row_now = row0, n_now = n0;
+    const int wave_rows = __builtin_amdgcn_readfirstlane(n - row_now - wm * GE::WTM);
+    int tgt[GE::FM];
+#pragma unroll
+    for (int i = 0; i < GE::FM; ++i)
+      tgt[i] = a.tgt[a.chunk * a.chunk_rows + min(row_now + wm * GE::WTM + i * 32 + (lane & 31), n - 1)];
+    typename TP::Acc acc[GE::FM][GE::FN];
+    clear<TP>(acc);
+    if (whole) tp.template wait_first<GE::FM * GE::FN * 2>();
+    else tp.template wait_first<0>();
+    tp.run(acc, wave_rows);
+    u += step;
+    const bool more = u < end;
+    if (more) begin(u);  // (the stages were last read before run()'s last barrier)
+    const bool inside = row_now + BMT <= n && n_now + GE::BN <= a.V;
+    if (inside) logits_out<T, BMT, TP, true, GRAD>(a, acc, tgt, row_now, n_now, n);
+    else logits_out<T, BMT, TP, false, GRAD>(a, acc, tgt, row_now, n_now, n);
+    if (!more) break;
+    whole = GRAD && inside;
+  }
+}
+
+template <typename T, int KIND, int BMT, bool RK, bool SUMS>
 __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
   using GE = Geo<BMT, T>;
   using TP = TileProduct<T, KIND == kDw, KIND != kDx, BMT, RK>;
@@ -418,143 +696,83 @@ __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
   const int wave_rows = __builtin_amdgcn_readfirstlane(cv.M - row0 - wm * WTM);
   const T* xc = (const T*)a.xc + (int64_t)a.chunk * a.chunk_rows * a.Dp;
   const T* p = (const T*)a.p;
-  const T* w = (const T*)a.w;
   typename TP::Acc acc[FM][FN];
-  if constexpr (KIND == kLogits)
-    TP::run(acc, xc, a.Dp, row0, n, w, a.ldv, n0, a.Vp, kbase, ktiles, cv.K, wave_rows, lds);
-  else if constexpr (KIND == kDx)
-    TP::run(acc, p, a.Vp, row0, n, w, a.ldv, n0, a.D, kbase, ktiles, cv.K, wave_rows, lds);
+  clear<TP>(acc);
+  TP tp;
+  if constexpr (KIND == kDx)
+    tp.begin(p, a.Vp, row0, n, (const T*)a.w, a.ldv, n0, a.D, kbase, ktiles, a.Vp, lds);
   else
-    TP::run(acc, xc, a.Dp, row0, a.Dp, p, a.Vp, n0, a.Vp, kbase, ktiles, cv.K, wave_rows, lds);
+    tp.begin(xc, a.Dp, row0, a.Dp, p, a.Vp, n0, a.Vp, kbase, ktiles, cv.K, lds);
+  tp.template wait_first<0>();
+  tp.run(acc, wave_rows);
 
   // Fragment (i, j): lane l has row l % 32 and columns 8 g + 4 (l / 32) .. +3 for g = 0..3.
   const int rl = lane & 31, ch = 4 * (lane >> 5);
-  if constexpr (KIND == kLogits) {
-    const int strip = n0 / WTN + wn, first = n0 + wn * WTN;
-    uint16_t* tile = reinterpret_cast<uint16_t*>(lds);  // bf16: the exponentials' tile on its way out
-    constexpr int LDC = GE::LDC, CV = BN / VEC;
-    __syncthreads();  // every fragment read is done
+  __syncthreads();  // every fragment read is done: the tile goes out through the stages' LDS
+  if (cv.slices > 1) {  // a slice's fp32 tile, for lce_reduce_kernel
+    float* out = a.parts + (int64_t)u * (BMT * BN);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-      const int row = row0 + wm * WTM + i * 32 + rl;
-      float l[FN][16];
+      const int row = wm * WTM + i * 32 + rl;
+      if (row0 + row >= cv.M) continue;
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int q = 0; q < 16; ++q) l[j][q] = acc[i][j][q];
-      if (n0 + BN > a.V) {  // columns past the vocabulary are no logits
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-          for (int q = 0; q < 16; ++q)
-            if (first + j * 32 + 8 * (q >> 2) + ch + (q & 3) >= a.V) l[j][q] = -__builtin_inff();
-      }
-      if (row < n) {
-        const int t = a.tgt[a.chunk * a.chunk_rows + row] - first;
-        if (t >= 0 && t < WTN && ((t >> 2) & 1) == (lane >> 5)) {
-          float at = 0.f;
-#pragma unroll
-          for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int q = 0; q < 16; ++q) at = t == j * 32 + 8 * (q >> 2) + ch + (q & 3) ? l[j][q] : at;
-          a.target_logit[a.chunk * a.chunk_rows + row] = at;
-        }
-      }
-      float m = l[0][0];
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-#pragma unroll
-        for (int q = 0; q < 16; ++q) m = fmaxf(m, l[j][q]);
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const float m2 = fmaxf(m * kLog2e, -3.0e38f);  // (finite in a strip of -inf, whose exponentials are 0)
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float e[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(l[j][4 * g + k], kLog2e, -m2));
-            s += e[k];
-          }
-          if (!a.grad) continue;
-          if constexpr (sizeof(T) == 2) {
-            *reinterpret_cast<uint2*>(tile + (wm * WTM + i * 32 + rl) * LDC + wn * WTN + j * 32 + 8 * g + ch) =
-                make_uint2(encode2(e[0], e[1]), encode2(e[2], e[3]));
-          } else if (row < n && first + j * 32 + 8 * g + ch < a.Vp) {
-            // (fp32: 16 bytes of a row a lane; its tile is larger than LDS)
-            *reinterpret_cast<float4*>((float*)a.p + (int64_t)row * a.Vp + first + j * 32 + 8 * g + ch) =
-                make_float4(e[0], e[1], e[2], e[3]);
-          }
-        }
-      s += __shfl_xor(s, 32, 64);
-      if (row < n && lane < 32 && first < a.V) a.stats[(int64_t)strip * a.chunk_rows + row] = make_float2(m2, s);
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(out + row * BN + wn * WTN + j * 32 + 8 * g + ch) =
+              make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
     }
-    if (!a.grad) return;
-    if constexpr (sizeof(T) == 2) {
-      __syncthreads();
-#pragma unroll 8
-      for (int v = tid; v < BMT * CV; v += NT) {
-        const int row = row0 + v / CV, col = n0 + v % CV * VEC;
-        if (row < n && col < a.Vp) st16((uint16_t*)a.p + (int64_t)row * a.Vp + col, ld16(tile + v / CV * LDC + v % CV * VEC));
-      }
-    }
+    return;
   }
-
-  if constexpr (KIND != kLogits) {
-    __syncthreads();  // every fragment read is done: the tile goes out through the stages' LDS
-    if (cv.slices > 1) {  // a slice's fp32 tile, for lce_reduce_kernel
-      float* out = a.parts + (int64_t)u * (BMT * BN);
+  // fp32 bands of RB rows through LDS: whole rows of vectors go out
+  constexpr int RB = 128, LDB = BN + 4, CV = BN / VEC;
+  static_assert(BMT % RB == 0 && (WTM % RB == 0 || RB % WTM == 0) && RB * LDB * 4 <= LDS_ALLOC, "bands of wave rows");
+  float* band = reinterpret_cast<float*>(lds);
+  const float scale = kept > 0 ? *a.scale : 1.0f;
+  const bool whole = KIND == kDx ? a.D == a.Dp : a.V == a.Vp;
+#pragma unroll
+  for (int pb = 0; pb < BMT / RB; ++pb) {
+    if (wm * WTM / RB == pb) {
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
           for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<float4*>(out + (wm * WTM + i * 32 + rl) * BN + wn * WTN + j * 32 + 8 * g + ch) =
+            *reinterpret_cast<float4*>(band + (wm * WTM - pb * RB + i * 32 + rl) * LDB + wn * WTN + j * 32 + 8 * g + ch) =
                 make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
-      return;
     }
-    // dw over several chunks: the sum so far, in the fragments' own order, whole lines a wave
-    const float4* sum = nullptr;
-    if (KIND == kDw && a.chunk > 0) sum = reinterpret_cast<const float4*>(a.acc) + (int64_t)r * (BMT * BN / 4) + tid;
-    auto value = [&](int i, int j, int g) __attribute__((always_inline)) {
-      float4 v = make_float4(acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
-      if (KIND == kDw && sum) {
-        const float4 x = sum[((i * FN + j) * 4 + g) * NT];
-        v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+    __syncthreads();
+    if constexpr (SUMS) {
+      // dw over several chunks: the sum so far, a tile's rows one after the other, several of a thread's vectors in flight
+      constexpr int U = 4;
+      static_assert(RB * CV % (U * NT) == 0, "whole batches");
+      const bool last = (a.chunk + 1) * (int64_t)a.chunk_rows >= kept;
+      float* sums = a.acc + (int64_t)r * (BMT * BN) + pb * RB * BN;
+      for (int v0 = tid; v0 < RB * CV; v0 += U * NT) {
+        float4 so_far[U][VEC / 4];
+        if (a.chunk > 0) {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < VEC / 4; ++k) so_far[u][k] = *reinterpret_cast<const float4*>(sums + (v0 + u * NT) * VEC + 4 * k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int v = v0 + u * NT, row = row0 + pb * RB + v / CV, col = n0 + v % CV * VEC;
+          const float* src = band + v / CV * LDB + v % CV * VEC;
+          float f[VEC];
+#pragma unroll
+          for (int k = 0; k < VEC; k += 4) {
+            float4 x = *reinterpret_cast<const float4*>(src + k);
+            if (a.chunk > 0) x = make_float4(x.x + so_far[u][k / 4].x, x.y + so_far[u][k / 4].y, x.z + so_far[u][k / 4].z, x.w + so_far[u][k / 4].w);
+            *reinterpret_cast<float4*>(f + k) = x;
+            if (!last) *reinterpret_cast<float4*>(sums + v * VEC + k) = x;
+          }
+          if (last && row < cv.M && col < cv.N) store_grad<T, KIND>(a, scale, row, col, f, whole);
+        }
       }
-      return v;
-    };
-    if (KIND == kDw && a.chunks > 1 && (a.chunk + 1) * (int64_t)a.chunk_rows < kept) {  // more to come
-      float4* to = reinterpret_cast<float4*>(a.acc) + (int64_t)r * (BMT * BN / 4) + tid;
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) to[((i * FN + j) * 4 + g) * NT] = value(i, j, g);
-      return;
-    }
-    // fp32 bands of RB rows through LDS: whole rows of vectors go out
-    constexpr int RB = 128, LDB = BN + 4, CV = BN / VEC;
-    static_assert(BMT % RB == 0 && (WTM % RB == 0 || RB % WTM == 0) && RB * LDB * 4 <= LDS_ALLOC, "bands of wave rows");
-    float* band = reinterpret_cast<float*>(lds);
-    const bool whole = KIND == kDx ? a.D == a.Dp : a.V == a.Vp;
-#pragma unroll
-    for (int pb = 0; pb < BMT / RB; ++pb) {
-      if (wm * WTM / RB == pb) {
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-              *reinterpret_cast<float4*>(band + (wm * WTM - pb * RB + i * 32 + rl) * LDB + wn * WTN + j * 32 + 8 * g + ch) =
-                  value(i, j, g);
-      }
-      __syncthreads();
+    } else {
       for (int v = tid; v < RB * CV; v += NT) {
         const int row = row0 + pb * RB + v / CV, col = n0 + v % CV * VEC;
         const float* src = band + v / CV * LDB + v % CV * VEC;
@@ -562,10 +780,385 @@ __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
           float f[VEC];
 #pragma unroll
           for (int k = 0; k < VEC; k += 4) *reinterpret_cast<float4*>(f + k) = *reinterpret_cast<const float4*>(src + k);
-          store_grad<T, KIND>(a, row, col, f, whole);
+          store_grad<T, KIND>(a, scale, row, col, f, whole);
         }
       }
-      if (pb + 1 < BMT / RB) __syncthreads();
+    }
+    if (pb + 1 < BMT / RB) __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+
+// The logits of at most 32 RF rows: w streams once through the CUs, straight into the matrix instructions' registers, at
+// any alignment.  A wave takes 32 CW columns (CW neighbouring ones a lane, one of each of CW fragments) and an eighth
+// of the reduction; the work-group adds the eighths in wave order.  Narrower columns where the vocabulary would leave
+// CUs without work.  (24 x 2048 x 50257 bf16, through an aligned copy of w and tiles of 128 rows: 114 us.)
+constexpr int kFewWaves = 8;
+
+// CW values of each of 8 (bf16) or 4 (fp32) rows of w, and the fragments of x beside them: a k-step of 16 or 8.
+template <typename T, int CW, int RF>
+struct FewStep {
+  static constexpr int KL = sizeof(T) == 2 ? 8 : 4;  // k of a lane
+  static constexpr int WORDS = CW * (int)sizeof(T) / 4;
+  uint32_t b[KL][WORDS];
+  Vec16 a[RF];
+
+  // every value in bounds: k0 + 2 KL <= D - 1, and past a row's end the next row's first values (of columns that are no logits)
+  __device__ __attribute__((always_inline)) inline void load(const LceArgs& g, const T* const (&x)[RF], int k0, int half, int col) {
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      typedef uint32_t words_any __attribute__((ext_vector_type(WORDS > 1 ? WORDS : 2), aligned(2)));
+      typedef uint32_t word_any __attribute__((aligned(2)));
+      const T* p = (const T*)g.w + (int64_t)(k0 + KL * half + i) * g.V + col;
+      if constexpr (WORDS > 1) {
+        const words_any v = *reinterpret_cast<const words_any*>(p);
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) b[i][w] = v[w];
+      } else {
+        b[i][0] = *reinterpret_cast<const word_any*>(p);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RF; ++r) a[r] = ld16(x[r] + k0 + KL * half);
+  }
+  // the reduction's end, value by value
+  __device__ inline void load_last(const LceArgs& g, const T* const (&x)[RF], int k0, int half, int col) {
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      const int k = k0 + KL * half + i;
+      T e[CW];
+#pragma unroll
+      for (int c = 0; c < CW; ++c)
+        e[c] = k < g.D && col + c < g.V ? ((const T*)g.w)[(int64_t)k * g.V + col + c] : from_f32<T>(0.f);
+      __builtin_memcpy(b[i], e, sizeof(e));
+    }
+#pragma unroll
+    for (int r = 0; r < RF; ++r) a[r] = k0 + KL * half < g.D ? ld16(x[r] + k0 + KL * half) : zero16();
+  }
+  __device__ __attribute__((always_inline)) inline void run(f32x16_t (&acc)[RF][CW]) const {
+#pragma unroll
+    for (int c = 0; c < CW; ++c) {
+      if constexpr (sizeof(T) == 2) {
+        Vec16 f;  // column c of the 8 rows
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          f.w[w] = __builtin_amdgcn_perm(b[2 * w + 1][c >> 1], b[2 * w][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int r = 0; r < RF; ++r)
+          acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a[r]), __builtin_bit_cast(bf16x8_t, f),
+                                                              acc[r][c], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < KL; ++i)
+#pragma unroll
+          for (int r = 0; r < RF; ++r)
+            acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x2f32(bits_f32(a[r].w[i]), bits_f32(b[i][c]), acc[r][c], 0, 0, 0);
+      }
+    }
+  }
+};
+
+template <typename T, int CW, int RF>
+__global__ __launch_bounds__(kFewWaves * 64, RF == 1 ? 4 : 2) void lce_few_kernel(LceArgs a) {
+  using Step = FewStep<T, CW, RF>;
+  constexpr int KS = 2 * Step::KL, COLS = 32 * CW, ROWS = 32 * RF, LDL = COLS + 4;
+  __shared__ __attribute__((aligned(16))) float part_s[kFewWaves][64 * 16];
+  __shared__ __attribute__((aligned(16))) float logit_s[ROWS * LDL];
+  const int n = chunk_kept(a);
+  if (n == 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int n0 = blockIdx.x * COLS, col = min(n0 + (lane & 31) * CW, a.V - 1);
+  const T* x[RF];
+#pragma unroll
+  for (int r = 0; r < RF; ++r)
+    x[r] = (const T*)a.xc + ((int64_t)a.chunk * a.chunk_rows + min(32 * r + (lane & 31), n - 1)) * a.Dp;
+  f32x16_t acc[RF][CW];
+#pragma unroll
+  for (int r = 0; r < RF; ++r)
+#pragma unroll
+    for (int c = 0; c < CW; ++c)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[r][c][q] = 0.f;
+  // (whole steps end before w's last row, whose end nothing follows)
+  const int whole = max(0, (a.D - 1) / KS), steps = (a.D + KS - 1) / KS;
+  const int per = (whole + kFewWaves - 1) / kFewWaves, from = wave * per, to = min(whole, from + per);
+  if (from < to) {
+    Step s0, s1;
+    s0.load(a, x, from * KS, half, col);
+    for (int k = from; k + 1 < to; ++k) {
+      s1.load(a, x, (k + 1) * KS, half, col);
+      s0.run(acc);
+      s0 = s1;
+    }
+    s0.run(acc);
+  }
+  if (wave == kFewWaves - 1) {
+    for (int k = whole; k < steps; ++k) {
+      Step s;
+      s.load_last(a, x, k * KS, half, n0 + (lane & 31) * CW);
+      s.run(acc);
+    }
+  }
+  // the waves' sums of a fragment at a time: a lane's 16 values as it has them, added in wave order to the logits' place
+#pragma unroll
+  for (int f = 0; f < RF * CW; ++f) {
+    const int r = f / CW, c = f % CW;
+    float* mine = part_s[wave] + lane * 4;
+    if (f > 0) __syncthreads();
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(mine + g * 256) =
+          make_float4(acc[r][c][4 * g], acc[r][c][4 * g + 1], acc[r][c][4 * g + 2], acc[r][c][4 * g + 3]);
+    __syncthreads();
+#pragma unroll
+    for (int v = tid; v < 1024; v += kFewWaves * 64) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kFewWaves; ++w) sum += part_s[w][v];
+      const int g = v >> 8, l = (v >> 2) & 63, k = v & 3;  // register 4 g + k of lane l
+      logit_s[(32 * r + 8 * g + 4 * (l >> 5) + k) * LDL + (l & 31) * CW + c] = sum;
+    }
+  }
+  __syncthreads();
+  // a row is LPR lanes': its statistics and exponentials
+  constexpr int LPR = kFewWaves * 64 / ROWS, PER = COLS / LPR;
+  const int row = tid / LPR, c0 = tid % LPR * PER;
+  float l[PER], m = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    l[i] = n0 + c0 + i < a.V ? logit_s[row * LDL + c0 + i] : -__builtin_inff();
+    m = fmaxf(m, l[i]);
+  }
+#pragma unroll
+  for (int off = LPR / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+  if (row >= n) return;
+  const int at = a.tgt[a.chunk * a.chunk_rows + row] - n0 - c0;
+  if (at >= 0 && at < PER) a.target_logit[a.chunk * a.chunk_rows + row] = logit_s[row * LDL + c0 + at];
+  const float m2 = fmaxf(m * kLog2e, -3.0e38f);
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    l[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(l[i], kLog2e, -m2));
+    s += l[i];
+  }
+#pragma unroll
+  for (int off = LPR / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  if (c0 == 0) a.stats[(int64_t)blockIdx.x * a.chunk_rows + row] = make_float2(m2, s);
+  if (!a.grad) return;
+#pragma unroll
+  for (int i = 0; i < PER; i += 2) {
+    const int c = n0 + c0 + i;
+    if (c >= a.Vp) break;  // (an even number, as c is)
+    if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>((uint16_t*)a.p + (int64_t)row * a.Vp + c) = encode2(l[i], l[i + 1]);
+    else *reinterpret_cast<float2*>((float*)a.p + (int64_t)row * a.Vp + c) = make_float2(l[i], l[i + 1]);
+  }
+}
+
+// VEC values to p at any element, as many as the row has left.
+template <typename T>
+__device__ inline void store_left(T* p, const float* f, int left) {
+  if (left >= kVec<T>) {
+    u32x4_any v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+      else v[i] = f32_bits(f[i]);
+    }
+    *reinterpret_cast<u32x4_any*>(p) = v;
+  } else {
+    store_any<T>(p, f, left);
+  }
+}
+
+// dx of few rows: P W^T.  A wave takes 64 of w's rows and a slice of the vocabulary, in groups of 128 bytes of a row: eight
+// lanes load a row's at any alignment, and a part of LDS of the wave's own turns them to the matrix instructions' order, a row a
+// lane (loaded as those want them, 16 bytes of 64 rows an instruction, rows of 50257 came at 2.5 TB/s).  A work-group
+// adds its waves' slices in order and writes them to parts[blockIdx.y] (rows, Dp), which lce_few_sum_kernel adds.
+template <typename T, int RF>
+__global__ __launch_bounds__(kFewWaves * 64, 2) void lce_few_dx_kernel(LceArgs a) {
+  constexpr int VEC = kVec<T>, GROUP = 8 * VEC, PITCH = 9 * 16;  // bytes of a row in LDS
+  __shared__ __attribute__((aligned(16))) char stage_s[kFewWaves][64 * PITCH];
+  static_assert(sizeof(stage_s) >= kFewWaves * 1024 * 4, "the waves' sums go through the same place");
+  const int n = chunk_kept(a);
+  if (n == 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, d0 = blockIdx.x * 64;
+  const T* wr[8];  // row 8 i + lane / 8, chunk lane % 8
+#pragma unroll
+  for (int i = 0; i < 8; ++i) wr[i] = (const T*)a.w + (int64_t)min(d0 + 8 * i + (lane >> 3), a.D - 1) * a.V;
+  const int chunk = (lane & 7) * VEC;
+  const T* pr[RF];  // a lane's half of a group is GROUP / 2 neighbouring values
+#pragma unroll
+  for (int r = 0; r < RF; ++r) pr[r] = (const T*)a.p + (int64_t)min(32 * r + (lane & 31), n - 1) * a.Vp + half * (GROUP / 2);
+  f32x16_t acc[RF][2];
+#pragma unroll
+  for (int r = 0; r < RF; ++r)
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[r][f][q] = 0.f;
+  const int whole = a.V / GROUP, all = (a.V + GROUP - 1) / GROUP, waves = gridDim.y * kFewWaves, per = (all + waves - 1) / waves;
+  const int from = (blockIdx.y * kFewWaves + wave) * per, to = min(all, from + per);
+  Vec16 w[8], p[RF][4];
+  auto load = [&](int k) __attribute__((always_inline)) {
+    if (k < whole) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const u32x4_any v = *reinterpret_cast<const u32x4_any*>(wr[i] + (int64_t)k * GROUP + chunk);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[i].w[c] = v[c];
+      }
+    } else {  // the vocabulary's end: zeros past it
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = load_end<T>(wr[i], k * GROUP + chunk, a.V);
+    }
+#pragma unroll
+    for (int r = 0; r < RF; ++r)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int at = k * GROUP + half * (GROUP / 2) + s * VEC;
+        p[r][s] = ld16(pr[r] + min(k * GROUP + s * VEC, a.Vp - VEC - half * (GROUP / 2)));
+        if (at >= a.Vp) p[r][s] = zero16();
+      }
+  };
+  char* mine = stage_s[wave];
+  if (from < to) load(from);
+  for (int k = from; k < to; ++k) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) st16(mine + (8 * i + (lane >> 3)) * PITCH + (lane & 7) * 16, w[i]);
+    Vec16 pn[RF][4];
+#pragma unroll
+    for (int r = 0; r < RF; ++r)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) pn[r][s] = p[r][s];
+    if (k + 1 < to) load(k + 1);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const Vec16 b = ld16(mine + (32 * f + (lane & 31)) * PITCH + (half * 4 + s) * 16);
+#pragma unroll
+        for (int r = 0; r < RF; ++r) MfmaOp<T, 32>::run(acc[r][f], pn[r][s], b);
+      }
+    __builtin_amdgcn_wave_barrier();
+  }
+  float* part = reinterpret_cast<float*>(stage_s);  // (wave, 1024)
+#pragma unroll
+  for (int f = 0; f < 2 * RF; ++f) {
+    __syncthreads();
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(part + wave * 1024 + g * 256 + lane * 4) = make_float4(
+          acc[f >> 1][f & 1][4 * g], acc[f >> 1][f & 1][4 * g + 1], acc[f >> 1][f & 1][4 * g + 2], acc[f >> 1][f & 1][4 * g + 3]);
+    __syncthreads();
+#pragma unroll
+    for (int u = tid; u < 1024; u += kFewWaves * 64) {
+      // neighbouring threads neighbouring columns: register 4 g + k of lane l
+      const int l = (u & 31) + (u >> 5 & 1) * 32, k = u >> 6 & 3, g = u >> 8;
+      float sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < kFewWaves; ++v) sum += part[v * 1024 + g * 256 + l * 4 + k];
+      const int row = 32 * (f >> 1) + 8 * g + 4 * (l >> 5) + k, col = d0 + 32 * (f & 1) + (l & 31);
+      if (row < n && col < a.D) a.parts[((int64_t)blockIdx.y * kFewRows + row) * a.Dp + col] = sum;
+    }
+  }
+}
+
+// dx from the slices of lce_few_dx_kernel, added in order.
+template <typename T>
+__global__ __launch_bounds__(256) void lce_few_sum_kernel(LceArgs a, int slices) {
+  constexpr int VEC = kVec<T>;
+  const int n = chunk_kept(a), vecs = a.Dp / VEC, i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n * vecs) return;
+  const int row = i / vecs, c = i % vecs * VEC;
+  float f[VEC] = {};
+  for (int s0 = 0; s0 < slices; s0 += 4) {
+    float4 x[4][VEC / 4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int k = 0; k < VEC / 4; ++k)
+        x[s][k] = *reinterpret_cast<const float4*>(a.parts + ((int64_t)min(s0 + s, slices - 1) * kFewRows + row) * a.Dp + c + 4 * k);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      if (s0 + s < slices)
+#pragma unroll
+        for (int k = 0; k < VEC / 4; ++k) {
+          f[4 * k] += x[s][k].x;
+          f[4 * k + 1] += x[s][k].y;
+          f[4 * k + 2] += x[s][k].z;
+          f[4 * k + 3] += x[s][k].w;
+        }
+  }
+  const float scale = *a.scale;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) f[k] *= scale;
+  store_left<T>((T*)a.dx + (int64_t)a.idx[row] * a.D + c, f, a.D - c);
+}
+
+// dw of few rows: x^T P, a reduction of kFewRows at most.  P's fragments of 32 CW columns stay in a wave's registers
+// while it walks its part of dw's rows; a lane ends up with CW neighbouring columns of a row, so the 512 bytes
+// of a row go out at once, at any alignment, without LDS.  ROWS: 32 or 64.
+template <typename T, int ROWS>
+__global__ __launch_bounds__(256) void lce_few_dw_kernel(LceArgs a, int rows_per) {
+  constexpr int VEC = kVec<T>, KL = VEC, KS = 2 * KL, STEPS = ROWS / KS;
+  constexpr int CW = sizeof(T) == 2 && ROWS == 64 ? 4 : VEC, WORDS = CW * (int)sizeof(T) / 4;
+  const int kept = *a.kept, n = chunk_kept(a), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+  const int n0 = blockIdx.x * 32 * CW, col = n0 + (lane & 31) * CW;
+  Vec16 b[STEPS][CW];  // fragment of column c: its KL values of the lane's rows
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    uint32_t v[KL][WORDS];
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      const int t = s * KS + KL * half + i;
+      typedef uint32_t words __attribute__((ext_vector_type(WORDS)));
+      const words x = *reinterpret_cast<const words*>((const T*)a.p + (int64_t)max(0, min(t, n - 1)) * a.Vp + min(col, a.Vp - CW));
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) v[i][w] = t < n ? x[w] : 0u;
+    }
+#pragma unroll
+    for (int c = 0; c < CW; ++c)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if constexpr (sizeof(T) == 2)
+          b[s][c].w[w] = __builtin_amdgcn_perm(v[2 * w + 1][c >> 1], v[2 * w][c >> 1], c & 1 ? 0x07060302u : 0x05040100u);
+        else
+          b[s][c].w[w] = v[w][c];
+      }
+  }
+  const float scale = kept > 0 ? *a.scale : 1.0f;
+  const int from = (blockIdx.y * 4 + wave) * rows_per, to = min(a.D, from + rows_per);
+  for (int d0 = from; d0 < to; d0 += 32) {
+    const T* xt = (const T*)a.xt + (int64_t)min(d0 + (lane & 31), a.D - 1) * kFewRows;
+    Vec16 x[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) x[s] = ld16(xt + s * KS + KL * half);
+    f32x16_t acc[CW];
+#pragma unroll
+    for (int c = 0; c < CW; ++c)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) acc[c][q] = 0.f;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+      for (int c = 0; c < CW; ++c) MfmaOp<T, 32>::run(acc[c], x[s], b[s][c]);
+#pragma unroll
+    for (int q = 0; q < 16; ++q) {
+      const int d = d0 + 8 * (q >> 2) + 4 * half + (q & 3);
+      if (d >= to || col >= a.V) continue;
+      T* out = (T*)a.dw + (int64_t)d * a.V + col;
+      float f[VEC] = {};
+#pragma unroll
+      for (int c = 0; c < CW; ++c) f[c] = acc[c][q] * scale;
+      if constexpr (CW == VEC) {
+        store_left<T>(out, f, a.V - col);
+      } else {
+        typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+        if (col + CW <= a.V) *reinterpret_cast<u32x2_any*>(out) = u32x2_any{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
+        else store_any<T>(out, f, a.V - col);
+      }
     }
   }
 }
@@ -583,6 +1176,7 @@ __global__ __launch_bounds__(256) void lce_reduce_kernel(LceArgs a) {
   int mt, nt;
   row_tile(r, cv.mt, cv.nt, mt, nt);
   const float* tile = a.parts + (int64_t)r * cv.slices * (BMT * BN);
+  const float scale = *a.scale;
   const bool whole = KIND == kDx ? a.D == a.Dp : a.V == a.Vp;
   for (int v = threadIdx.x; v < kReduceRows * CV; v += 256) {
     const int tr = band * kReduceRows + v / CV, tc = v % CV * VEC;
@@ -591,16 +1185,23 @@ __global__ __launch_bounds__(256) void lce_reduce_kernel(LceArgs a) {
     float f[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) f[k] = 0.f;
-    for (int s = 0; s < cv.slices; ++s) {
-      const float* src = tile + (int64_t)s * (BMT * BN) + tr * BN + tc;
+    for (int s0 = 0; s0 < cv.slices; s0 += 4) {
+      float4 x[4][VEC / 4];
 #pragma unroll
-      for (int k = 0; k < VEC; k += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(src + k);
-        f[k] += x.x;
-        f[k + 1] += x.y;
-        f[k + 2] += x.z;
-        f[k + 3] += x.w;
-      }
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int k = 0; k < VEC / 4; ++k)
+          x[s][k] = *reinterpret_cast<const float4*>(tile + (int64_t)min(s0 + s, cv.slices - 1) * (BMT * BN) + tr * BN + tc + 4 * k);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (s0 + s < cv.slices)
+#pragma unroll
+          for (int k = 0; k < VEC / 4; ++k) {
+            f[4 * k] += x[s][k].x;
+            f[4 * k + 1] += x[s][k].y;
+            f[4 * k + 2] += x[s][k].z;
+            f[4 * k + 3] += x[s][k].w;
+          }
     }
     if (KIND == kDw && a.chunks > 1) {  // the sum over the chunks so far, at the tile's place
       float* sum = a.acc + (int64_t)r * (BMT * BN) + tr * BN + tc;
@@ -612,7 +1213,7 @@ __global__ __launch_bounds__(256) void lce_reduce_kernel(LceArgs a) {
       }
       if (!done) continue;
     }
-    store_grad<T, KIND>(a, row, col, f, whole);
+    store_grad<T, KIND>(a, scale, row, col, f, whole);
   }
 }
 
@@ -624,38 +1225,43 @@ constexpr int kRowsB = 8;
 constexpr int kStripsB = 512;  // strips whose factors are in LDS at a time
 constexpr int kAheadB = 4;     // vectors of a thread in flight
 
+// Few rows: the work-groups of one row group (grid.y of them) take seg strips of P each.
 template <typename T>
-__global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip) {
+__global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip, int seg) {
   constexpr int VEC = kVec<T>, G = 256 / kRowsB;
-  __shared__ float2 part_s[G][kRowsB];
+  __shared__ float2 part_s[4][kRowsB];
   __shared__ float2 row_s[kRowsB];  // maximum, 1 / sum
   __shared__ float factor_s[kStripsB];
   const int tid = threadIdx.x, n = chunk_kept(a), row0 = blockIdx.x * kRowsB, base = a.chunk * a.chunk_rows;
   if (row0 >= n) return;
   const int strips = (a.V + strip - 1) / strip;
+  auto join = [](float& m, float& s, float2 o) {
+    const float top = fmaxf(m, o.x);
+    s = s * __builtin_amdgcn_exp2f(m - top) + o.y * __builtin_amdgcn_exp2f(o.x - top);
+    m = top;
+  };
   {
     const int r = tid % kRowsB, g = tid / kRowsB, row = min(row0 + r, n - 1);
-    float m = -__builtin_inff(), s = 0.f;
-    for (int k = g; k < strips; k += G) {
-      const float2 st = a.stats[(int64_t)k * a.chunk_rows + row];
-      const float top = fmaxf(m, st.x);
-      s = s * __builtin_amdgcn_exp2f(m - top) + st.y * __builtin_amdgcn_exp2f(st.x - top);
-      m = top;
+    float m = -3.0e38f, s = 0.f;  // (no strip's maximum is less)
+    for (int k = g; k < strips; k += 4 * G) {
+      float2 st[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) st[u] = a.stats[(int64_t)min(k + u * G, strips - 1) * a.chunk_rows + row];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (k + u * G < strips) join(m, s, st[u]);
     }
-    part_s[g][r] = make_float2(m, s);
+#pragma unroll
+    for (int off = kRowsB; off < 64; off <<= 1) join(m, s, make_float2(__shfl_xor(m, off, 64), __shfl_xor(s, off, 64)));
+    if ((tid & 63) < kRowsB) part_s[tid >> 6][r] = make_float2(m, s);
   }
   __syncthreads();
   if (tid < kRowsB) {
-    float m = -__builtin_inff(), s = 0.f;
-    for (int g = 0; g < G && g < strips; ++g) {
-      const float2 st = part_s[g][tid];
-      const float top = fmaxf(m, st.x);
-      s = s * __builtin_amdgcn_exp2f(m - top) + st.y * __builtin_amdgcn_exp2f(st.x - top);
-      m = top;
-    }
+    float m = part_s[0][tid].x, s = part_s[0][tid].y;
+    for (int w = 1; w < 4; ++w) join(m, s, part_s[w][tid]);
     row_s[tid] = make_float2(m, 1.0f / s);
     const int row = row0 + tid;
-    if (row < n) {
+    if (row < n && blockIdx.y == 0) {
       // the target's distance from the maximum first: it is small where the loss is
       const float l = kLn2 * (__builtin_amdgcn_logf(s) + __builtin_fmaf(-a.target_logit[base + row], kLog2e, m));
       if (a.reduction == ABACUS_LOSS_ROWS) {
@@ -666,20 +1272,25 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip) {
     }
   }
   if (!a.grad) return;
+  if (row0 == 0 && blockIdx.y == 0 && !a.xt && tid >= 128) {  // for the products that follow, a wave each
+    const int cut = tid < 192 ? (a.thin & 1 << kDx ? Cover<T, kDx, THIN>(a, n).cut(a) : Cover<T, kDx, BM>(a, n).cut(a))
+                              : (a.thin & 1 << kDw ? Cover<T, kDw, THIN>(a, n).cut(a) : Cover<T, kDw, BM>(a, n).cut(a));
+    if (tid % 64 == 0) a.slices[tid < 192 ? kDx : kDw] = cut;
+  }
   __syncthreads();
-  const int kept = *a.kept;
+  const int first = blockIdx.y * seg, last = min(strips, first + seg);
   for (int r = 0; r < min(kRowsB, n - row0); ++r) {
     const int row = row0 + r;
     const float top = row_s[r].x, inv = row_s[r].y;
-    const float s = a.row_grad ? a.row_grad[a.idx[base + row]] : a.reduction == ABACUS_LOSS_MEAN ? 1.0f / (float)kept : 1.0f;
+    const float s = a.row_grad ? a.row_grad[a.idx[base + row]] / *a.scale : 1.0f;
     const int t = a.tgt[base + row];
     T* p = (T*)a.p + (int64_t)row * a.Vp;
-    for (int k0 = 0; k0 < strips; k0 += kStripsB) {
+    for (int k0 = first; k0 < last; k0 += kStripsB) {
       __syncthreads();
-      for (int k = tid; k < min(kStripsB, strips - k0); k += 256)
+      for (int k = tid; k < min(kStripsB, last - k0); k += 256)
         factor_s[k] = s * inv * __builtin_amdgcn_exp2f(a.stats[(int64_t)(k0 + k) * a.chunk_rows + row].x - top);
       __syncthreads();
-      const int end = min(a.Vp, (k0 + kStripsB) * strip);
+      const int end = min(a.Vp, min(last, k0 + kStripsB) * strip);
       for (int c0 = k0 * strip + tid * VEC; c0 < end; c0 += 256 * VEC * kAheadB) {
         Vec16 e[kAheadB];
 #pragma unroll
@@ -754,7 +1365,8 @@ __global__ __launch_bounds__(256) void scale_kernel(T* __restrict__ t, int64_t n
 struct Plan {
   int Dp, Vp, chunk_rows, chunks, strip;
   bool thin[3], pad;  // thin: of each kind's tiles
-  int64_t kept, idx, tgt, target_logit, row_loss, xc, w, stats, p, acc, parts, total;
+  int few;            // few rows: columns a lane of their logits; 0: tiles
+  int64_t kept, idx, tgt, target_logit, row_loss, xc, xt, w, stats, p, acc, parts, total;
 };
 
 template <typename T, int KIND, int BMT>
@@ -782,22 +1394,34 @@ int64_t part_bytes(bool thin, int64_t rows, int64_t D, int64_t V) {
   return thin ? Sizes<T, KIND, THIN>(rows, D, V).part_bytes() : Sizes<T, KIND, BM>(rows, D, V).part_bytes();
 }
 
+int few_slices(int64_t D) { return (int)std::max<int64_t>(1, 2 * kCUs / ((D + 63) / 64)); }
+
+// Columns a lane: as many (registers for two work-groups a CU) as leave work for most CUs.
+template <typename T>
+int few_columns(int64_t V) {
+  constexpr int least = sizeof(T) == 2 ? 2 : 1;
+  int cw = 4;
+  while (cw > least && (V + 32 * cw - 1) / (32 * cw) < 180) cw /= 2;
+  return cw;
+}
+
 template <typename T>
 Plan plan_of(int64_t T_, int64_t D, int64_t V, bool grad) {
   constexpr int VEC = VecTraits<T>::kN;
   Plan q;
   q.Dp = (int)((D + VEC - 1) / VEC * VEC);
   q.Vp = (int)((V + VEC - 1) / VEC * VEC);
-  q.pad = V % VEC != 0;
   // a strip is half a tile's columns; with gradients a row of P is in a chunk as a whole
-  const int64_t row_bytes = grad ? (int64_t)q.Vp * (int64_t)sizeof(T) : (V + 63) / 64 * 8;
+  const int64_t row_bytes = grad ? (int64_t)q.Vp * (int64_t)sizeof(T) : (V + 31) / 32 * 8;
   const int64_t rows = std::min(T_, std::max<int64_t>(BM, kChunkBytes / row_bytes / BM * BM));
   q.chunk_rows = (int)rows;
   q.chunks = (int)((T_ + rows - 1) / rows);
   q.thin[kLogits] = thin_of<T, kLogits>(rows, D, V);
   q.thin[kDx] = thin_of<T, kDx>(rows, D, V);
   q.thin[kDw] = thin_of<T, kDw>(rows, D, V);
-  q.strip = q.thin[kLogits] ? Geo<THIN, T>::WTN : Geo<BM, T>::WTN;
+  q.few = T_ <= kFewRows && V >= 64 ? few_columns<T>(V) : 0;
+  q.pad = V % VEC != 0 && !q.few;  // (few rows read w at any alignment)
+  q.strip = q.few ? 32 * q.few : q.thin[kLogits] ? Geo<THIN, T>::WTN : Geo<BM, T>::WTN;
   const int64_t strips = (V + q.strip - 1) / q.strip;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -805,17 +1429,19 @@ Plan plan_of(int64_t T_, int64_t D, int64_t V, bool grad) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  q.kept = take(4);
+  q.kept = take(20);
   q.idx = take(T_ * 4);
   q.tgt = take(T_ * 4);
   q.target_logit = take(T_ * 4);
   q.row_loss = take(T_ * 4);
   q.xc = take(T_ * q.Dp * (int64_t)sizeof(T));
   q.w = take(q.pad ? D * q.Vp * (int64_t)sizeof(T) : 0);
+  q.xt = take(q.few && grad ? D * kFewRows * (int64_t)sizeof(T) : 0);
   q.stats = take(strips * rows * 8);
   q.p = take(grad ? rows * row_bytes : 0);
   q.acc = take(grad && q.chunks > 1 ? (D + BM - 1) / BM * BM * ((V + BN - 1) / BN * BN) * 4 : 0);
-  q.parts = take(grad ? std::max(part_bytes<T, kDx>(q.thin[kDx], rows, D, V), part_bytes<T, kDw>(q.thin[kDw], rows, D, V)) : 0);
+  if (q.few) q.parts = take(grad ? (int64_t)few_slices(D) * kFewRows * q.Dp * 4 : 0);
+  else q.parts = take(grad ? std::max(part_bytes<T, kDx>(q.thin[kDx], rows, D, V), part_bytes<T, kDw>(q.thin[kDw], rows, D, V)) : 0);
   q.total = at;
   return q;
 }
@@ -828,23 +1454,86 @@ int check_sizes(const char* name, int64_t T, int64_t D, int64_t V, int dtype) {
   return 0;
 }
 
+template <typename T, int CW>
+int launch_few_columns(const LceArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.V + 32 * CW - 1) / (32 * CW))), block(kFewWaves * 64);
+  if (a.T <= 32) hipLaunchKernelGGL((lce_few_kernel<T, CW, 1>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((lce_few_kernel<T, CW, 2>), grid, block, 0, s, a);
+  ABACUS_CHECK_LAUNCH("linear_cross_entropy few rows");
+  return 0;
+}
+template <typename T>
+int launch_few(const LceArgs& a, int cw, hipStream_t s) {
+  if (cw == 4) return launch_few_columns<T, 4>(a, s);
+  if (cw == 2) return launch_few_columns<T, 2>(a, s);
+  if constexpr (sizeof(T) == 4) return launch_few_columns<T, 1>(a, s);
+  return 1;  // (not reached: few_columns gives bf16 two at least)
+}
+
+template <typename T>
+int launch_few_dx(const LceArgs& a, hipStream_t s) {
+  const int slices = few_slices(a.D);
+  const dim3 grid((unsigned)((a.D + 63) / 64), (unsigned)slices), block(kFewWaves * 64);
+  if (a.T <= 32) hipLaunchKernelGGL((lce_few_dx_kernel<T, 1>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((lce_few_dx_kernel<T, 2>), grid, block, 0, s, a);
+  ABACUS_CHECK_LAUNCH("linear_cross_entropy few rows' dx");
+  const int64_t vecs = (int64_t)a.T * (a.Dp / VecTraits<T>::kN);
+  hipLaunchKernelGGL(lce_few_sum_kernel<T>, dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, s, a, slices);
+  ABACUS_CHECK_LAUNCH("linear_cross_entropy few rows' dx sum");
+  return 0;
+}
+
+template <typename T>
+int launch_few_dw(const LceArgs& a, hipStream_t s) {
+  const int cols = 32 * (sizeof(T) == 2 && a.T > 32 ? 4 : VecTraits<T>::kN);
+  // rows of dw a wave walks: enough waves for every SIMD twice, and P's fragments used as often as that allows
+  const int64_t groups = (a.V + cols - 1) / cols;
+  int rows_per = 256;
+  while (rows_per > 32 && groups * ((a.D + rows_per - 1) / rows_per) < 8 * kCUs) rows_per /= 2;
+  const dim3 grid((unsigned)groups, (unsigned)((a.D + 4 * rows_per - 1) / (4 * rows_per)));
+  if (a.T <= 32) hipLaunchKernelGGL((lce_few_dw_kernel<T, 32>), grid, dim3(256), 0, s, a, rows_per);
+  else hipLaunchKernelGGL((lce_few_dw_kernel<T, 64>), grid, dim3(256), 0, s, a, rows_per);
+  ABACUS_CHECK_LAUNCH("linear_cross_entropy few rows' dw");
+  return 0;
+}
+
+template <typename T, int BMT>
+int launch_logits(const LceArgs& a, hipStream_t s) {
+  const int64_t tiles = Sizes<T, kLogits, BMT>(std::min(a.chunk_rows, a.T - a.chunk * a.chunk_rows), a.D, a.V).tiles;
+  ABACUS_CHECK_ARG(tiles < (1ll << 31) - 8, "linear_cross_entropy: %lld tiles", (long long)tiles);
+  const dim3 grid((unsigned)std::min<int64_t>(kCUs, (tiles + 7) / 8 * 8));
+#define ABACUS_GO(RK)                                                                                  \
+  do {                                                                                                 \
+    if (a.grad) hipLaunchKernelGGL((lce_logits_kernel<T, BMT, RK, true>), grid, dim3(NT), 0, s, a);    \
+    else hipLaunchKernelGGL((lce_logits_kernel<T, BMT, RK, false>), grid, dim3(NT), 0, s, a);          \
+  } while (0)
+  if (a.D % kBKT<T> != 0) ABACUS_GO(true);
+  else ABACUS_GO(false);
+#undef ABACUS_GO
+  ABACUS_CHECK_LAUNCH("linear_cross_entropy logits");
+  return 0;
+}
+
 template <typename T, int KIND, int BMT>
 int launch_product(const LceArgs& a, hipStream_t s) {
   const int64_t tiles = Sizes<T, KIND, BMT>(std::min(a.chunk_rows, a.T - a.chunk * a.chunk_rows), a.D, a.V).tiles;
   // a product of fewer rows (or a shorter reduction) may be cut into more slices, up to kUnits units
-  int64_t units = KIND == kLogits ? tiles : std::max<int64_t>(tiles, std::min<int64_t>(kUnits, tiles * kSlices));
-  units = (units + 7) / 8 * 8;
+  const int64_t units = (std::max<int64_t>(tiles, std::min<int64_t>(kUnits, tiles * kSlices)) + 7) / 8 * 8;
   ABACUS_CHECK_ARG(units < (1ll << 31), "linear_cross_entropy: %lld tiles", (long long)units);
-  const bool ragged = KIND == kDw || (KIND == kLogits ? a.D : a.Vp) % kBKT<T> != 0;
-  if (ragged) hipLaunchKernelGGL((lce_product_kernel<T, KIND, BMT, true>), dim3((unsigned)units), dim3(NT), 0, s, a);
-  else if constexpr (KIND != kDw) hipLaunchKernelGGL((lce_product_kernel<T, KIND, BMT, false>), dim3((unsigned)units), dim3(NT), 0, s, a);
+  const dim3 grid((unsigned)units);
+  if constexpr (KIND == kDw) {
+    if (a.chunks > 1) hipLaunchKernelGGL((lce_product_kernel<T, KIND, BMT, true, true>), grid, dim3(NT), 0, s, a);
+    else hipLaunchKernelGGL((lce_product_kernel<T, KIND, BMT, true, false>), grid, dim3(NT), 0, s, a);
+  } else if (a.Vp % kBKT<T> != 0) {
+    hipLaunchKernelGGL((lce_product_kernel<T, KIND, BMT, true, false>), grid, dim3(NT), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((lce_product_kernel<T, KIND, BMT, false, false>), grid, dim3(NT), 0, s, a);
+  }
   ABACUS_CHECK_LAUNCH("linear_cross_entropy product");
-  if constexpr (KIND != kLogits) {
-    if (KIND == kDx || 2 * tiles <= kUnits) {  // (two slices or more are of at most kUnits / 2 tiles)
-      const int64_t cut = std::min<int64_t>(tiles, kUnits / 2);
-      hipLaunchKernelGGL((lce_reduce_kernel<T, KIND, BMT>), dim3((unsigned)(cut * (BMT / kReduceRows))), dim3(256), 0, s, a);
-      ABACUS_CHECK_LAUNCH("linear_cross_entropy reduce");
-    }
+  if (KIND == kDx || 2 * tiles <= kUnits) {  // (two slices or more are of at most kUnits / 2 tiles)
+    const int64_t cut = std::min<int64_t>(tiles, kUnits / 2);
+    hipLaunchKernelGGL((lce_reduce_kernel<T, KIND, BMT>), dim3((unsigned)(cut * (BMT / kReduceRows))), dim3(256), 0, s, a);
+    ABACUS_CHECK_LAUNCH("linear_cross_entropy reduce");
   }
   return 0;
 }
@@ -858,19 +1547,22 @@ int run(LceArgs a, char* ws, int64_t ws_bytes, hipStream_t s) {
   a.Vp = q.Vp;
   a.chunk_rows = q.chunk_rows;
   a.kept = (int*)(ws + q.kept);
+  a.scale = (float*)(ws + q.kept) + 1;
+  a.slices = (int*)(ws + q.kept) + 2;
   a.idx = (int*)(ws + q.idx);
   a.tgt = (int*)(ws + q.tgt);
   a.target_logit = (float*)(ws + q.target_logit);
   a.row_loss = (float*)(ws + q.row_loss);
   a.xc = ws + q.xc;
+  a.xt = q.few && a.grad ? ws + q.xt : nullptr;
   a.stats = (float2*)(ws + q.stats);
   a.p = ws + q.p;
   a.acc = (float*)(ws + q.acc);
   a.parts = (float*)(ws + q.parts);
   a.ldv = a.V;
-  int rows_per = std::max(4, (a.T + 511) / 512);
-  rows_per = std::min(rows_per, 4096);
-  hipLaunchKernelGGL(pack_rows_kernel<T>, dim3((a.T + rows_per - 1) / rows_per), dim3(256), rows_per * 4, s, a, rows_per);
+  const int rows_per = std::min(4096, std::max(4, (a.T + 511) / 512));
+  if (q.few) hipLaunchKernelGGL(pack_few_kernel<T>, dim3((a.Dp + 63) / 64), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(pack_rows_kernel<T>, dim3((a.T + rows_per - 1) / rows_per), dim3(256), rows_per * 4, s, a, rows_per);
   ABACUS_CHECK_LAUNCH("linear_cross_entropy pack");
   if (q.pad) {
     const dim3 grid((unsigned)((q.Vp / VecTraits<T>::kN + 255) / 256), (unsigned)((a.D + kPadRows - 1) / kPadRows));
@@ -880,16 +1572,20 @@ int run(LceArgs a, char* ws, int64_t ws_bytes, hipStream_t s) {
     a.ldv = q.Vp;
   }
   a.chunks = q.chunks;
+  a.thin = q.thin[kDx] << kDx | q.thin[kDw] << kDw;
   for (a.chunk = 0; a.chunk < q.chunks; ++a.chunk) {
-    if (int rc = q.thin[kLogits] ? launch_product<T, kLogits, THIN>(a, s) : launch_product<T, kLogits, BM>(a, s)) return rc;
+    if (int rc = q.few ? launch_few<T>(a, q.few, s) : q.thin[kLogits] ? launch_logits<T, THIN>(a, s) : launch_logits<T, BM>(a, s)) return rc;
     const int rows = std::min(a.chunk_rows, a.T - a.chunk * a.chunk_rows);
-    hipLaunchKernelGGL(lce_rows_kernel<T>, dim3((rows + kRowsB - 1) / kRowsB), dim3(256), 0, s, a, q.strip);
+    // (work-groups enough for every CU twice, of a few strips at least)
+    const int groups = (rows + kRowsB - 1) / kRowsB, strips = (a.V + q.strip - 1) / q.strip;
+    const int segs = a.grad ? std::max(1, std::min(2 * kCUs / groups, strips / 8)) : 1, seg = (strips + segs - 1) / segs;
+    hipLaunchKernelGGL(lce_rows_kernel<T>, dim3(groups, (strips + seg - 1) / seg), dim3(256), 0, s, a, q.strip, seg);
     ABACUS_CHECK_LAUNCH("linear_cross_entropy rows");
     if (a.dx) {
-      if (int rc = q.thin[kDx] ? launch_product<T, kDx, THIN>(a, s) : launch_product<T, kDx, BM>(a, s)) return rc;
+      if (int rc = q.few ? launch_few_dx<T>(a, s) : q.thin[kDx] ? launch_product<T, kDx, THIN>(a, s) : launch_product<T, kDx, BM>(a, s)) return rc;
     }
     if (a.dw) {
-      if (int rc = q.thin[kDw] ? launch_product<T, kDw, THIN>(a, s) : launch_product<T, kDw, BM>(a, s)) return rc;
+      if (int rc = q.few ? launch_few_dw<T>(a, s) : q.thin[kDw] ? launch_product<T, kDw, THIN>(a, s) : launch_product<T, kDw, BM>(a, s)) return rc;
     }
   }
   if (a.reduction != ABACUS_LOSS_ROWS && a.loss) {
