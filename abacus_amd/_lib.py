@@ -100,7 +100,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "abacus_cross_entropy_mean_bwd": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I, _P, _P]),
     "abacus_linear_cross_entropy_ws_bytes": (_I64, [_I64, _I64, _I64, _I, _I]),
     "abacus_linear_cross_entropy": (_I, [_P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _P, _P, _P, _P, _P, _I64, _P]),
-    "abacus_scale_by": (_I, [_P, _I64, _I, _P, _P]),
+    "abacus_scale_by": (_I, [_P, _I64, _P, _I64, _I, _P, _P]),
+    "abacus_capture_id": (_I, [_P, _P]),
     "abacus_embedding_fwd": (_I, [_P, _P, _I64, _I64, _I64, _F, _I, _P, _P]),
     "abacus_embedding_bwd_ws_bytes": (_I64, [_I64, _I64, _I64]),
     "abacus_embedding_bwd": (_I, [_P, _P, _I64, _I64, _I64, _F, _I, _P, _P, _I64, _P]),

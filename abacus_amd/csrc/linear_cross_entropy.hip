@@ -1342,11 +1342,16 @@ __global__ __launch_bounds__(1024) void lce_sum_kernel(LceArgs a) {
   }
 }
 
-// t *= *g, left alone where *g is 1.
+// t *= *g (blockIdx.y 1: u), left alone where *g is 1.
 template <typename T>
-__global__ __launch_bounds__(256) void scale_kernel(T* __restrict__ t, int64_t n, const float* __restrict__ g) {
+__global__ __launch_bounds__(256) void scale_kernel(T* __restrict__ t, int64_t n, T* __restrict__ u, int64_t m,
+                                                    const float* __restrict__ g) {
   const float f = *g;
   if (f == 1.0f) return;
+  if (blockIdx.y) {
+    t = u;
+    n = m;
+  }
   constexpr int VEC = kVec<T>;
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC; i < n; i += (int64_t)gridDim.x * 256 * VEC) {
     if (i + VEC <= n) {
@@ -1618,7 +1623,7 @@ int abacus_linear_cross_entropy(const void* x_TD, int64_t x_stride, const void* 
   const bool grad = dx_TD != nullptr || dw_DV != nullptr;
   ABACUS_CHECK_ARG(reduction != ABACUS_LOSS_ROWS || grad == (row_grad_T != nullptr), "linear_cross_entropy: gradients of rows' losses need the rows' weights");
   ABACUS_CHECK_ARG(grad || loss != nullptr, "linear_cross_entropy: nothing to compute");
-  if (T == 0) return 0;
+  ABACUS_CHECK_ARG(T > 0, "linear_cross_entropy: no rows");
   LceArgs a{};
   a.x = x_TD;
   a.x_stride = x_stride;
@@ -1638,13 +1643,25 @@ int abacus_linear_cross_entropy(const void* x_TD, int64_t x_stride, const void* 
                         : run<float>(a, (char*)ws, ws_bytes, (hipStream_t)stream);
 }
 
-int abacus_scale_by(void* t, int64_t n, int dtype, const float* g, void* stream) {
+int abacus_capture_id(int64_t* id, void* stream) {
+  ABACUS_CHECK_ARG(id != nullptr, "capture_id: no place for the answer");
+  hipStreamCaptureStatus status;
+  unsigned long long at = 0;
+  const hipError_t rc = hipStreamGetCaptureInfo((hipStream_t)stream, &status, &at);
+  ABACUS_CHECK_ARG(rc == hipSuccess, "capture_id: %s", hipGetErrorString(rc));
+  *id = status == hipStreamCaptureStatusActive ? (int64_t)at : 0;
+  return 0;
+}
+
+int abacus_scale_by(void* t, int64_t n, void* u, int64_t m, int dtype, const float* g, void* stream) {
   ABACUS_CHECK_ARG(dtype == kF32 || dtype == kBF16, "scale_by: unsupported dtype code %d (0 = fp32, 1 = bf16)", dtype);
-  ABACUS_CHECK_ARG(n >= 0, "scale_by: %lld values", (long long)n);
-  if (n == 0) return 0;
-  const unsigned blocks = (unsigned)std::min<int64_t>((n + 2047) / 2048, 4096);
-  if (dtype == kBF16) hipLaunchKernelGGL(scale_kernel<uint16_t>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (uint16_t*)t, n, g);
-  else hipLaunchKernelGGL(scale_kernel<float>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (float*)t, n, g);
+  ABACUS_CHECK_ARG(n >= 0 && m >= 0, "scale_by: %lld and %lld values", (long long)n, (long long)m);
+  if (n == 0 && m == 0) return 0;
+  const dim3 grid((unsigned)std::min<int64_t>((std::max(n, m) + 2047) / 2048, 4096), 2);
+  if (dtype == kBF16)
+    hipLaunchKernelGGL(scale_kernel<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, (uint16_t*)t, n, (uint16_t*)u, m, g);
+  else
+    hipLaunchKernelGGL(scale_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, (float*)t, n, (float*)u, m, g);
   ABACUS_CHECK_LAUNCH("scale_by");
   return 0;
 }

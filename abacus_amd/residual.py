@@ -8,8 +8,10 @@ them.  CPU tensors take the same steps in torch's operations.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
+from .kv_cache import _call
 from .moe import _contig
 
 __all__ = ["residual_norm"]
@@ -42,63 +44,74 @@ def _forward(x, y, gamma, post_gamma, gate, scale: float, eps: float, keep: bool
     r, h = torch.empty_like(x), torch.empty_like(x)
     rstd = torch.empty(rows, dtype=torch.float32, device=dev) if keep else None
     y_rstd = torch.empty(rows, dtype=torch.float32, device=dev) if keep and post_gamma is not None else None
-    _lib.call("abacus_residual_norm_fwd", _lib.ptr(x), _lib.ptr(y), _lib.ptr(gamma), _lib.ptr(post_gamma), _lib.ptr(gate),
-              _gate_kind(gate), rows, D, scale, eps, _lib.dtype_code(x.dtype), _lib.ptr(r), _lib.ptr(h), _lib.ptr(rstd),
-              _lib.ptr(y_rstd), _lib.stream_of(dev))
+    _call(dev, "abacus_residual_norm_fwd", _lib.ptr(x), _lib.ptr(y), _lib.ptr(gamma), _lib.ptr(post_gamma), _lib.ptr(gate),
+          _gate_kind(gate), rows, D, scale, eps, _lib.dtype_code(x.dtype), _lib.ptr(r), _lib.ptr(h), _lib.ptr(rstd),
+          _lib.ptr(y_rstd))
     return r, h, rstd, y_rstd
 
 
+def _recorded(ctx, grads, dr, dh, y, gamma, post_gamma, gate, r):
+    """grads, tied to what they were formed from where the running backward is itself recorded: dx and dgamma to r (which
+    leads on to x and y) and gamma, the others to dx and the branch's own operands."""
+    from .transformer import _KernelGradient
+
+    dx, dy, dgamma, dpost, dgate = grads
+    d_out = torch.stack([torch.zeros_like(r) if d is None else d for d in (dr, dh)])
+    dx, dgamma = _KernelGradient.apply(lambda r, gamma: torch.stack((r, _norm(r, gamma, ctx.eps))), (dx, dgamma), d_out, r,
+                                       gamma)
+    if post_gamma is None and gate is None:
+        return dx, ctx.scale * dx, dgamma, None, None
+
+    def branch(y, *rest):
+        rest = list(rest)
+        b = y if post_gamma is None else _norm(y, rest.pop(0), ctx.eps)
+        return ctx.scale * (b if gate is None else rest.pop(0) * b)
+
+    formed = iter(_KernelGradient.apply(branch, tuple(d for d in (dy, dpost, dgate) if d is not None), dx,
+                                        *(t for t in (y, post_gamma, gate) if t is not None)))
+    return dx, next(formed), dgamma, *(None if d is None else next(formed) for d in (dpost, dgate))
+
+
 class _ResidualNorm(torch.autograd.Function):
+    """residual_norm and its gradients, one kernel each way and the sums over rows."""
+
     @staticmethod
     def forward(ctx, x, y, gamma, post_gamma, gate, scale: float, eps: float):
+        ctx.set_materialize_grads(False)
+        ctx.scale, ctx.eps = scale, eps
         c = [None if t is None else _contig(t) for t in (x, y, gamma, post_gamma, gate)]
         r, h, rstd, y_rstd = _forward(*c, scale, eps, True)
-        ctx.save_for_backward(x, y, gamma, post_gamma, gate, r, rstd, y_rstd)
-        ctx.scale, ctx.eps = scale, eps
-        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(None if post_gamma is None and gate is None else y, gamma, post_gamma, gate, r, rstd, y_rstd)
         return r, h
 
     @staticmethod
     def backward(ctx, dr, dh):
-        from .transformer import _KernelGradient
-
         if dr is None and dh is None:
             return (None,) * 7
-        x, y, gamma, post_gamma, gate, r, rstd, y_rstd = ctx.saved_tensors
+        *leaves, rstd, y_rstd = ctx.saved_tensors
+        if not torch.is_grad_enabled():
+            return (*_ResidualNorm.gradients(ctx, dr, dh, *leaves, rstd, y_rstd), None, None)
         with torch.no_grad():
-            grads = _ResidualNorm.gradients(ctx, dr, dh, y, gamma, post_gamma, gate, r, rstd, y_rstd)
-        if torch.is_grad_enabled():
-            there = [t is not None for t in (post_gamma, gate)]
-
-            def op(x, y, gamma, *rest):  # r and h side by side: one output
-                rest = list(rest)
-                post, gt = (rest.pop(0) if t else None for t in there)
-                branch = y if post is None else _norm(y, post, ctx.eps)
-                r = x + ctx.scale * (branch if gt is None else gt * branch)
-                return torch.stack((r, _norm(r, gamma, ctx.eps)))
-
-            leaves = [t for t in (x, y, gamma, post_gamma, gate) if t is not None]
-            d_out = torch.stack([torch.zeros_like(r) if d is None else d for d in (dr, dh)])
-            formed = iter(_KernelGradient.apply(op, tuple(g for g in grads if g is not None), d_out, *leaves))
-            grads = tuple(None if g is None else next(formed) for g in grads)
-        return (*grads, None, None)
+            grads = _ResidualNorm.gradients(ctx, dr, dh, *leaves, rstd, y_rstd)
+        return (*_recorded(ctx, grads, dr, dh, *leaves), None, None)
 
     @staticmethod
     def gradients(ctx, dr, dh, y, gamma, post_gamma, gate, r, rstd, y_rstd):
-        D, dev = r.shape[-1], r.device
+        D, dev, dt = r.shape[-1], r.device, _lib.dtype_code(r.dtype)
         rows = r.numel() // D
-        same = post_gamma is None and gate is None and ctx.scale == 1.0  # dy is dx
         dr, dh, y, gamma, post_gamma, gate = (None if t is None else _contig(t) for t in (dr, dh, y, gamma, post_gamma, gate))
         dx = torch.empty_like(r)
+        dgamma = torch.empty_like(gamma)
+        same = post_gamma is None and gate is None and ctx.scale == 1.0  # dy is dx
         dy = None if same else torch.empty_like(r)
-        dgamma, dpost, dgate = (None if t is None else torch.empty_like(t) for t in (gamma, post_gamma, gate))
-        kind = _gate_kind(gate)
+        dpost = None if post_gamma is None else torch.empty_like(post_gamma)
+        dgate = None if gate is None else torch.empty_like(gate)
+        kind, ptr = _gate_kind(gate), _lib.ptr
         nbytes = _lib.query("abacus_residual_norm_bwd_ws_bytes", rows, D, int(post_gamma is not None), kind)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _lib.call("abacus_residual_norm_bwd", _lib.ptr(dr), _lib.ptr(dh), _lib.ptr(r), _lib.ptr(y), _lib.ptr(gamma),
-                  _lib.ptr(post_gamma), _lib.ptr(gate), kind, _lib.ptr(rstd), _lib.ptr(y_rstd), rows, D, ctx.scale,
-                  _lib.dtype_code(r.dtype), _lib.ptr(dx), _lib.ptr(dy), _lib.ptr(dgamma), _lib.ptr(dpost), _lib.ptr(dgate),
-                  _lib.ptr(ws), nbytes, _lib.stream_of(dev))
+        _call(dev, "abacus_residual_norm_bwd", ptr(dr), ptr(dh), ptr(r), ptr(y), ptr(gamma), ptr(post_gamma), ptr(gate), kind,
+              ptr(rstd), ptr(y_rstd), rows, D, ctx.scale, dt, ptr(dx), ptr(dy), ptr(dgamma), ptr(dpost), ptr(dgate), ptr(ws),
+              nbytes)
         return dx, dx if same else dy, dgamma, dpost, dgate
 
 
@@ -118,17 +131,21 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, gamma: torch.Tensor, post_ga
             raise ValueError(f"{name} has {D} values, got {tuple(t.shape)}")
     if gate is not None and gate.shape not in ((D,), x.shape):
         raise ValueError(f"gate has {D} values or x's shape {tuple(x.shape)}, got {tuple(gate.shape)}")
-    tensors = [t for t in (y, gamma, post_gamma, gate) if t is not None]
-    if any(t.dtype != x.dtype for t in tensors):
-        raise TypeError(f"residual_norm takes tensors of one type, got {x.dtype} and {', '.join(str(t.dtype) for t in tensors)}")
-    if any(t.device != x.device for t in tensors):
-        raise ValueError("residual_norm takes tensors on one device")
+    grad = x.requires_grad
+    for name, t in (("y", y), ("gamma", gamma), ("post_gamma", post_gamma), ("gate", gate)):
+        if t is None:
+            continue
+        if t.dtype != x.dtype:
+            raise TypeError(f"residual_norm takes tensors of one type: x is {x.dtype} and {name} {t.dtype}")
+        if t.device != x.device:
+            raise ValueError(f"residual_norm takes tensors on one device: x is on {x.device} and {name} on {t.device}")
+        grad = grad or t.requires_grad
     if x.device.type == "cpu" or x.numel() == 0:
         return _plain(x, y, gamma, post_gamma, gate, scale, eps)
     least, most = (8, 8192) if _lib.dtype_code(x.dtype, x.device) == _lib.BF16 else (4, 4096)
     if not least <= D <= most:
         raise ValueError(f"residual_norm takes a dim of {least} to {most} for {x.dtype} on the GPU, got {D}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *tensors)):
+    if grad and torch.is_grad_enabled() or forward_ad._current_level >= 0:  # (which refuses a tangent)
         return _ResidualNorm.apply(x, y, gamma, post_gamma, gate, float(scale), float(eps))
     operands = [None if t is None else _contig(t) for t in (x, y, gamma, post_gamma, gate)]
     return _forward(*operands, float(scale), float(eps), False)[:2]

@@ -20,9 +20,10 @@ import os
 
 from . import _lib
 from .optim import WSD, AdamW
+from .vocabulary import linear_cross_entropy
 
-__all__ = ["Trainer", "cross_entropy", "get_device", "make_optimizer", "next_token_loss", "set_use_liger",
-           "train_step"]
+__all__ = ["Trainer", "cross_entropy", "get_device", "head_loss", "linear_cross_entropy", "make_optimizer",
+           "next_token_loss", "set_use_liger", "train_step"]
 
 
 class _CrossEntropyFunction(torch.autograd.Function):
@@ -159,12 +160,26 @@ def next_token_loss(logits_BLV: torch.Tensor, tokens_BL: torch.Tensor) -> torch.
     return F.cross_entropy(logits_NV, targets_BL.reshape(-1), ignore_index=-100)
 
 
-def train_step(model: torch.nn.Module, optimizer: AdamW, tokens_BL: torch.Tensor) -> torch.Tensor:
-    """Returns the step's (detached) loss."""
-    model.train()
+def head_loss(x_BLD: torch.Tensor, w_D_vocab: torch.Tensor, tokens_BL: torch.Tensor) -> torch.Tensor:
+    """next_token_loss of x_BLD @ w_D_vocab without its logits in memory (linear_cross_entropy), in fp32.
+
+    The same pairs and count: position l against token l + 1, -100 left out.  Nothing waits on the host, so a
+    batch without target tokens gives NaN (and no gradient), and so does a token outside the vocabulary.
+    """
+    return linear_cross_entropy(x_BLD, w_D_vocab, F.pad(tokens_BL[:, 1:], (0, 1), value=-100), ignore_index=-100)
+
+
+def _step_loss(model: torch.nn.Module, tokens_BL: torch.Tensor, fused_loss: bool) -> torch.Tensor:
     inputs_BL = tokens_BL.clamp(min=0)  # -100 is padding; the embedding has no row for it
-    logits = model(inputs_BL)  # (B, L, vocab)
-    loss = next_token_loss(logits, tokens_BL)
+    if fused_loss:
+        return head_loss(model.hidden(inputs_BL), model.w_D_vocab, tokens_BL)
+    return next_token_loss(model(inputs_BL), tokens_BL)  # of (B, L, vocab) logits
+
+
+def train_step(model: torch.nn.Module, optimizer: AdamW, tokens_BL: torch.Tensor, fused_loss: bool = False) -> torch.Tensor:
+    """Returns the step's (detached) loss.  fused_loss: by head_loss, without the logits in memory."""
+    model.train()
+    loss = _step_loss(model, tokens_BL, fused_loss)
     optimizer.zero_grad()
     loss.backward()
     optimizer.step()
@@ -183,9 +198,11 @@ def get_device() -> torch.device:
 class Trainer:
     """trainer.py:29-103, the single-process path: the model moved to the device, the
     reference's AdamW with its defaults, and the WSD schedule when total_steps is given.
-    Data, pipeline and context parallelism need several processes and are refused."""
+    Data, pipeline and context parallelism need several processes and are refused.
+    fused_loss: the loss by head_loss, without the logits in memory (no counterpart in the reference)."""
 
-    def __init__(self, model: torch.nn.Module, parallel=None, pipeline=None, total_steps: int | None = None):
+    def __init__(self, model: torch.nn.Module, parallel=None, pipeline=None, total_steps: int | None = None,
+                 fused_loss: bool = False):
         if parallel is not None and pipeline is not None:
             raise ValueError("pipeline parallel does not use DataParallel")
         if parallel is not None or pipeline is not None:
@@ -195,6 +212,7 @@ class Trainer:
         self.model = model.to(self.device)
         self.parallel = None
         self.pipeline = None
+        self.fused_loss = fused_loss
         self.optimizer = AdamW(self.model)
         self.scheduler = WSD(total_steps) if total_steps is not None else None
         if self.scheduler is not None:
@@ -204,9 +222,7 @@ class Trainer:
         """(loss, local loss), both the step's mean next-token cross-entropy on one process."""
         self.model.train()
         tokens_BL = tokens_BL.to(self.device)
-        inputs_BL = tokens_BL.clamp(min=0)  # -100 is padding; the embedding has no row for it
-        logits = self.model(inputs_BL)  # (B, L, vocab)
-        loss = next_token_loss(logits, tokens_BL)
+        loss = _step_loss(self.model, tokens_BL, self.fused_loss)
         self.optimizer.zero_grad()
         loss.backward()
         local_loss = loss.detach()

@@ -14,15 +14,15 @@ reference's:
   TransformerMoe       abacus/transformer_moe.py:17-75
 
 The MoE layer inside each block is abacus_amd.moe.MoE (the HIP path).  On
-the GPU, RMSNorm, the q/k norms fused with the rotary embedding, and causal
-attention in bf16 with head dim 64 or 128 also run on this
+the GPU, the embedding with its gradient, RMSNorm, alone and with the residual sum before it, the q/k norms
+fused with the rotary embedding, and causal attention in bf16 with head dim 64 or 128 also run on this
 library's HIP kernels; the (L, L) scores never reach HBM and stay fp32 where
 the reference rounds them to the activation dtype.  Other attention inputs go
 to torch's fused causal kernels (flash / memory-efficient), and on the CPU,
 or for inputs no fused kernel takes, attention is materialised like the
 reference's (scores, mask, softmax, weighted sum) as one autograd function
 whose batched products all take contiguous operands.  The dense projections
-and the embedding run on torch.  Tensor, sequence and context parallelism
+run on torch.  Tensor, sequence and context parallelism
 with more than one process are not implemented here (one GPU).
 
 ``forward_cached`` (of the attention, the block and the model; no reference
@@ -36,11 +36,14 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .kv_cache import BatchRows, KVPages, PagedKVCache
 from .moe import MoE, MoEExpertParallel, _contig, _rank_and_world_size
+from .residual import residual_norm
+from .vocabulary import embedding
 
 __all__ = [
     "Embedding",
@@ -60,7 +63,7 @@ def _single_process(what: str) -> None:
 
 
 class Embedding(torch.nn.Module):
-    """Token embedding table (embedding.py:8-23): w_vocab_D ~ N(0, 1)."""
+    """Token embedding table (embedding.py:8-23): w_vocab_D ~ N(0, 1).  On the GPU by abacus_amd.vocabulary.embedding."""
 
     def __init__(self, vocab_size: int, dim: int):
         super().__init__()
@@ -70,7 +73,12 @@ class Embedding(torch.nn.Module):
         torch.nn.init.normal_(self.w_vocab_D)
 
     def forward(self, tokens_BL: torch.Tensor) -> torch.Tensor:
-        return self.w_vocab_D[tokens_BL]  # (B, L, D)
+        w = self.w_vocab_D
+        # (the kernels carry no tangents and no functional transforms, indexing does)
+        if (w.is_cuda and w.dtype in (torch.float32, torch.bfloat16) and tokens_BL.dtype == torch.int64 and tokens_BL.is_cuda
+                and forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active()):
+            return embedding(tokens_BL, w)
+        return w[tokens_BL]  # (B, L, D)
 
 
 class Rotary(torch.nn.Module):
@@ -301,6 +309,22 @@ class RMSNorm(torch.nn.Module):
             return _RMSNormFunction.apply(x_BLD, self.w_gamma_D, 1e-5)
         rms_BL = torch.sqrt(x_BLD.square().mean(dim=-1, keepdim=True) + 1e-5)  # (B, L, 1)
         return self.w_gamma_D * x_BLD / rms_BL
+
+
+def _bare(module: torch.nn.Module, kind: type) -> bool:
+    """Whether calling `module` is calling kind.forward: no subclass, no hooks, no forward of its own."""
+    return (type(module) is kind and "forward" not in module.__dict__ and not torch.nn.modules.module._has_any_global_hook()
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+
+
+def _add_norm(x: torch.Tensor, y: torch.Tensor, norm: torch.nn.Module):
+    """x + y and its norm (transformer_block.py:98-100): residual_norm's one pass where the HIP norm takes x and nothing
+    looks between the two, the same bits as the two steps.  (While a KernelTimer is active the two run, each under its name.)"""
+    if (_bare(norm, RMSNorm) and norm.world_size == 1 and not _lib.timing() and x.shape == y.shape and _of_kind(x, y)
+            and x.numel() > 0 and _fused_norm_ok(x, norm.w_gamma_D)):
+        return residual_norm(x, y, norm.w_gamma_D, eps=1e-5)
+    x = x + y
+    return x, norm(x)
 
 
 class _CausalAttention(torch.autograd.Function):
@@ -780,17 +804,26 @@ class TransformerBlockMoe(torch.nn.Module):
         self.dropout = torch.nn.Dropout(dropout)
 
     def forward(self, x_BLD: torch.Tensor, rotary: torch.nn.Module | None = None) -> torch.Tensor:
-        attn_BLD = self.attention(self.norm_attention(x_BLD), rotary)
-        x_BLD = x_BLD + self.dropout(attn_BLD)
-        moe_BLD = self.moe(self.norm_mlp(x_BLD))
-        return x_BLD + self.dropout(moe_BLD)
+        x_BLD, moe_BLD = self._halves(x_BLD, self.norm_attention(x_BLD), rotary)
+        return x_BLD + moe_BLD
+
+    def _halves(self, x_BLD, normed_BLD, rotary):
+        """The stream after the attention's half, and what the MoE's adds to it; normed_BLD is norm_attention(x_BLD)."""
+        attn_BLD = self.attention(normed_BLD, rotary)
+        x_BLD, normed_BLD = _add_norm(x_BLD, self.dropout(attn_BLD), self.norm_mlp)
+        return x_BLD, self.dropout(self.moe(normed_BLD))
 
     @torch.no_grad()
     def forward_cached(self, x_TD: torch.Tensor, pages: KVPages, rows: BatchRows, cos_TK: torch.Tensor | None = None,
                        sin_TK: torch.Tensor | None = None) -> torch.Tensor:
         _check_cached(self, x_TD, "(tokens, dim)", 2)
-        x_TD = x_TD + self.attention.forward_cached(self.norm_attention(x_TD), pages, rows, cos_TK, sin_TK)
-        return x_TD + self.moe(self.norm_mlp(x_TD))
+        x_TD, moe_TD = self._halves_cached(x_TD, self.norm_attention(x_TD), pages, rows, cos_TK, sin_TK)
+        return x_TD + moe_TD
+
+    def _halves_cached(self, x_TD, normed_TD, pages, rows, cos_TK, sin_TK):
+        attn_TD = self.attention.forward_cached(normed_TD, pages, rows, cos_TK, sin_TK)
+        x_TD, normed_TD = _add_norm(x_TD, attn_TD, self.norm_mlp)
+        return x_TD, self.moe(normed_TD)
 
 
 class TransformerMoe(torch.nn.Module):
@@ -836,10 +869,24 @@ class TransformerMoe(torch.nn.Module):
         torch.nn.init.xavier_uniform_(self.w_D_vocab)
 
     def forward(self, tokens_BL: torch.Tensor) -> torch.Tensor:
+        return self.hidden(tokens_BL) @ self.w_D_vocab  # (B, L, vocab)
+
+    def hidden(self, tokens_BL: torch.Tensor) -> torch.Tensor:
+        """What the head multiplies: the blocks' output through the last norm, (B, L, D)."""
         x_BLD = self.embedding(tokens_BL)
-        for block in self.blocks:
-            x_BLD = block(x_BLD, self.rotary)
-        return self.norm(x_BLD) @ self.w_D_vocab  # (B, L, vocab)
+        if not (x_BLD.is_cuda and len(self.blocks) and all(_bare(b, TransformerBlockMoe) for b in self.blocks)):
+            for block in self.blocks:
+                x_BLD = block(x_BLD, self.rotary)
+            return self.norm(x_BLD)
+        # a block's last sum and the next one's first norm are one step
+        normed_BLD = self.blocks[0].norm_attention(x_BLD)
+        for block, norm in zip(self.blocks, self._norms_after()):
+            x_BLD, moe_BLD = block._halves(x_BLD, normed_BLD, self.rotary)
+            x_BLD, normed_BLD = _add_norm(x_BLD, moe_BLD, norm)
+        return normed_BLD
+
+    def _norms_after(self):
+        return [*(b.norm_attention for b in list(self.blocks)[1:]), self.norm]
 
     @torch.no_grad()
     def forward_cached(self, tokens_T: torch.Tensor, cache: PagedKVCache, rows: BatchRows,
@@ -852,7 +899,20 @@ class TransformerMoe(torch.nn.Module):
             raise ValueError(f"a cache of {cache.n_layers} layers for {self.n_blocks} blocks")
         x_TD = self.embedding(tokens_T)
         cos, sin = self.rotary(x_TD, positions=rows.positions(tokens_T.shape[0]))  # (1, 1, T, K)
-        for i, block in enumerate(self.blocks):
+        blocks = list(self.blocks)
+        if x_TD.is_cuda and blocks and all(_bare(b, TransformerBlockMoe) and "forward_cached" not in b.__dict__ for b in blocks):
+            # (as in hidden; the last block's sum is taken of the rows that are wanted alone)
+            for b in blocks:
+                _check_cached(b, x_TD, "(tokens, dim)", 2)
+            normed_TD = blocks[0].norm_attention(x_TD)
+            for i, (block, norm) in enumerate(zip(blocks, self._norms_after())):
+                x_TD, moe_TD = block._halves_cached(x_TD, normed_TD, cache.layer(i), rows, cos[0, 0], sin[0, 0])
+                if i + 1 < len(blocks):
+                    x_TD, normed_TD = _add_norm(x_TD, moe_TD, norm)
+            if out_rows is not None:
+                x_TD, moe_TD = x_TD[out_rows], moe_TD[out_rows]
+            return _add_norm(x_TD, moe_TD, self.norm)[1] @ self.w_D_vocab
+        for i, block in enumerate(blocks):
             x_TD = block.forward_cached(x_TD, cache.layer(i), rows, cos[0, 0], sin[0, 0])
         if out_rows is not None:
             x_TD = x_TD[out_rows]

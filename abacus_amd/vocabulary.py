@@ -12,10 +12,15 @@ CPU tensors take the same steps in torch's operations.
 
 from __future__ import annotations
 
+import ctypes
+import math
+
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import _lib
+from .kv_cache import _call
 from .moe import _contig
 
 __all__ = ["embedding", "linear_cross_entropy"]
@@ -29,6 +34,16 @@ def _plain_loss(x_TD, w_DV, targets_T, ignore_index: int, reduction: str):
     return F.cross_entropy(x_TD.to(wide) @ w_DV.to(wide), targets_T, ignore_index=ignore_index, reduction=reduction)
 
 
+def _loss_op(x_TD, w_DV, targets_T, ignore_index: int, reduction: str):
+    """The loss as the kernels have it, for its second derivatives: NaN, not an assertion, for a target outside the vocabulary."""
+    logits = x_TD @ w_DV
+    kept = targets_T != ignore_index
+    known = kept & (targets_T >= 0) & (targets_T < w_DV.shape[1])
+    rows = torch.logsumexp(logits, -1) - logits.gather(1, torch.where(known, targets_T, 0)[:, None])[:, 0]
+    rows = torch.where(kept, torch.where(known, rows, math.nan), 0.0)
+    return rows if reduction == "none" else rows.sum() / (kept.sum().clamp(min=1) if reduction == "mean" else 1)
+
+
 def _loss_call(x_TD, w_DV, targets_T, ignore_index: int, reduction: str, row_grad=None, want=(False, False), want_loss=True):
     """(loss or None, dx or None, dw or None) of one call of the kernels."""
     T, D = x_TD.shape
@@ -40,41 +55,48 @@ def _loss_call(x_TD, w_DV, targets_T, ignore_index: int, reduction: str, row_gra
     nbytes = _lib.query("abacus_linear_cross_entropy_ws_bytes", T, D, V, dt, int(any(want)))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     w = _contig(w_DV)
-    _lib.call("abacus_linear_cross_entropy", x_TD.data_ptr(), x_TD.stride(0), _lib.ptr(w), targets_T.data_ptr(), T, D, V,
-              ignore_index, dt, _REDUCTIONS[reduction], _lib.ptr(row_grad), _lib.ptr(loss), _lib.ptr(dx), _lib.ptr(dw),
-              _lib.ptr(ws), nbytes, _lib.stream_of(dev))
+    _call(dev, "abacus_linear_cross_entropy", x_TD.data_ptr(), x_TD.stride(0), _lib.ptr(w), targets_T.data_ptr(), T, D, V,
+          ignore_index, dt, _REDUCTIONS[reduction], _lib.ptr(row_grad), _lib.ptr(loss), _lib.ptr(dx), _lib.ptr(dw),
+          _lib.ptr(ws), nbytes)
     return loss, dx, dw
 
 
-def _scaled(grad: torch.Tensor | None, g: torch.Tensor):
-    """grad times the scalar g, in place; left alone (on the device) where g is 1."""
-    if grad is not None:
-        _lib.call("abacus_scale_by", _lib.ptr(grad), grad.numel(), _lib.dtype_code(grad.dtype), g.data_ptr(),
-                  _lib.stream_of(grad.device))
-    return grad
+def _capture(dev: torch.device) -> int:
+    """The number of the graph that the current stream records, 0 where it records none."""
+    if not torch.cuda.is_current_stream_capturing():
+        return 0
+    number = ctypes.c_int64()
+    _call(dev, "abacus_capture_id", ctypes.addressof(number))
+    return number.value
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     """Loss and gradients in one pass over the logits: of a mean or a sum the forward forms both gradients, and the
-    backward multiplies them by the loss's own.  The losses of rows have gradients a row that only the
-    backward knows, so it makes the pass once more; so does a second backward of a mean or a sum."""
+    backward multiplies them by the loss's own (they are left alone, on the device, where that is 1).  The losses of rows
+    have gradients a row that only the backward knows, so it makes the pass once more; so does a second
+    backward of a mean or a sum, and one that is not recorded into the graph its forward is in (each of the two may be
+    replayed without the other)."""
 
     @staticmethod
     def forward(ctx, x_TD, w_DV, targets_T, ignore_index: int, reduction: str):
         ctx.save_for_backward(x_TD, w_DV, targets_T)
         ctx.args = ignore_index, reduction
         now = ctx.needs_input_grad[:2] if reduction != "none" else (False, False)
+        ctx.capture = _capture(x_TD.device)
         loss, *ctx.grads = _loss_call(x_TD, w_DV, targets_T, ignore_index, reduction, want=now)
         return loss
 
     @staticmethod
     def backward(ctx, g):
+        x, w, targets = ctx.saved_tensors
+        if not torch.is_grad_enabled():
+            return (*_LinearCrossEntropy.gradients(ctx, g, x, w, targets), None, None, None)
         from .transformer import _by_kernel
 
-        x, w, targets = ctx.saved_tensors
-        ignore_index, reduction = ctx.args
-        op = lambda x, w: _plain_loss(x, w, targets, ignore_index, reduction)
-        return (*_by_kernel(op, lambda: _LinearCrossEntropy.gradients(ctx, g, x, w, targets), g, x, w), None, None, None)
+        op = lambda x, w: _loss_op(x, w, targets, *ctx.args)
+        wanted = lambda: tuple(torch.zeros_like(t) if d is None else d
+                               for t, d in zip((x, w), _LinearCrossEntropy.gradients(ctx, g, x, w, targets)))
+        return (*_by_kernel(op, wanted, g, x, w), None, None, None)
 
     @staticmethod
     def gradients(ctx, g, x, w, targets):
@@ -83,9 +105,12 @@ class _LinearCrossEntropy(torch.autograd.Function):
         if reduction == "none":
             return _loss_call(x, w, targets, ignore_index, reduction, g, ctx.needs_input_grad[:2], want_loss=False)[1:]
         grads, ctx.grads = ctx.grads, None
-        if grads is None:  # handed over by an earlier backward of this graph
+        if grads is None or ctx.capture != _capture(x.device):  # handed over by an earlier backward, or another's to write
             grads = _loss_call(x, w, targets, ignore_index, reduction, want=ctx.needs_input_grad[:2])[1:]
-        return tuple(_scaled(grad, g) for grad in grads)
+        sizes = [0 if t is None else t.numel() for t in grads]
+        _call(x.device, "abacus_scale_by", _lib.ptr(grads[0]), sizes[0], _lib.ptr(grads[1]), sizes[1], _lib.dtype_code(x.dtype),
+              g.data_ptr())
+        return grads
 
 
 def linear_cross_entropy(x: torch.Tensor, w_DV: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
@@ -115,7 +140,8 @@ def linear_cross_entropy(x: torch.Tensor, w_DV: torch.Tensor, targets: torch.Ten
         _lib.dtype_code(x.dtype, x.device)  # refuses other types
         if x_TD.stride(1) != 1 or x_TD.stride(0) < x_TD.shape[1]:
             x_TD = x_TD.contiguous()
-        if torch.is_grad_enabled() and (x.requires_grad or w_DV.requires_grad):
+        # (forward mode too, where torch refuses a tangent that the kernels would drop)
+        if torch.is_grad_enabled() and (x.requires_grad or w_DV.requires_grad) or forward_ad._current_level >= 0:
             loss = _LinearCrossEntropy.apply(x_TD, w_DV, targets_T, int(ignore_index), reduction)
         else:
             loss = _loss_call(x_TD, w_DV, targets_T, int(ignore_index), reduction)[0]
@@ -134,7 +160,9 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, d_out):
         (tokens,) = ctx.saved_tensors
-        return None, _EmbeddingGradient.apply(d_out, tokens, ctx.shape, ctx.scale), None
+        if torch.is_grad_enabled():  # (it is to be differentiated itself)
+            return None, _EmbeddingGradient.apply(d_out, tokens, ctx.shape, ctx.scale), None
+        return None, _embed_gradient(d_out, tokens, ctx.shape, ctx.scale), None
 
 
 class _EmbeddingGradient(torch.autograd.Function):
@@ -144,15 +172,7 @@ class _EmbeddingGradient(torch.autograd.Function):
     def forward(ctx, d_out, tokens, shape, scale: float):
         ctx.save_for_backward(tokens)
         ctx.scale = scale
-        V, D = shape
-        T, dev = tokens.numel(), d_out.device
-        dw = torch.empty(V, D, dtype=d_out.dtype, device=dev)
-        nbytes = _lib.query("abacus_embedding_bwd_ws_bytes", T, V, D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        d_out = _contig(d_out)
-        _lib.call("abacus_embedding_bwd", tokens.data_ptr(), _lib.ptr(d_out), T, V, D, scale, _lib.dtype_code(d_out.dtype),
-                  _lib.ptr(dw), _lib.ptr(ws), nbytes, _lib.stream_of(dev))
-        return dw
+        return _embed_gradient(d_out, tokens, shape, scale)
 
     @staticmethod
     def backward(ctx, d_dw):
@@ -160,12 +180,24 @@ class _EmbeddingGradient(torch.autograd.Function):
         return _Embedding.apply(tokens, d_dw, ctx.scale), None, None, None
 
 
+def _embed_gradient(d_out, tokens, shape, scale: float):
+    V, D = shape
+    T, dev = tokens.numel(), d_out.device
+    dw = torch.empty(V, D, dtype=d_out.dtype, device=dev)
+    nbytes = _lib.query("abacus_embedding_bwd_ws_bytes", T, V, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    d_out = _contig(d_out)
+    _call(dev, "abacus_embedding_bwd", tokens.data_ptr(), _lib.ptr(d_out), T, V, D, scale, _lib.dtype_code(d_out.dtype),
+          _lib.ptr(dw), _lib.ptr(ws), nbytes)
+    return dw
+
+
 def _embed_call(tokens, w_VD, scale: float):
     V, D = w_VD.shape
     w = _contig(w_VD)
     out = torch.empty(*tokens.shape, D, dtype=w.dtype, device=w.device)
-    _lib.call("abacus_embedding_fwd", tokens.data_ptr(), _lib.ptr(w), tokens.numel(), V, D, scale,
-              _lib.dtype_code(w.dtype), _lib.ptr(out), _lib.stream_of(w.device))
+    _call(w.device, "abacus_embedding_fwd", tokens.data_ptr(), _lib.ptr(w), tokens.numel(), V, D, scale,
+          _lib.dtype_code(w.dtype), _lib.ptr(out))
     return out
 
 
@@ -186,6 +218,6 @@ def embedding(tokens: torch.Tensor, w_VD: torch.Tensor, scale: float = 1.0) -> t
         return w_VD[tokens] if scale == 1.0 else w_VD[tokens] * scale
     _lib.dtype_code(w_VD.dtype, w_VD.device)  # refuses other types
     tokens = tokens.contiguous()
-    if torch.is_grad_enabled() and w_VD.requires_grad:
+    if torch.is_grad_enabled() and w_VD.requires_grad or forward_ad._current_level >= 0:  # (which refuses a tangent)
         return _Embedding.apply(tokens, w_VD, float(scale))
     return _embed_call(tokens, w_VD, float(scale))

@@ -432,7 +432,8 @@ int abacus_cross_entropy_mean_bwd(const void* logits_NV, const int64_t* targets_
  * Any D and V; x may start at any element, the other operands are 16-byte aligned.
  * ws: device workspace of abacus_linear_cross_entropy_ws_bytes bytes (grad: with gradients).
  *
- * abacus_scale_by: n values of `dtype` times *g (device memory), left as they are where it is 1. */
+ * abacus_scale_by: n values of `dtype` at t and m at u times *g (device memory), left as they are where it is 1.
+ * abacus_capture_id: *id (host memory) the number of the graph that the stream records, 0 where it records none. */
 #define ABACUS_LOSS_ROWS 0
 #define ABACUS_LOSS_SUM 1
 #define ABACUS_LOSS_MEAN 2
@@ -441,7 +442,8 @@ int abacus_linear_cross_entropy(const void* x_TD, int64_t x_stride, const void* 
                                 int64_t T, int64_t D, int64_t V, int64_t ignore_index, int dtype, int reduction,
                                 const float* row_grad_T, float* loss, void* dx_TD, void* dw_DV, void* ws,
                                 int64_t ws_bytes, void* stream);
-int abacus_scale_by(void* t, int64_t n, int dtype, const float* g, void* stream);
+int abacus_scale_by(void* t, int64_t n, void* u, int64_t m, int dtype, const float* g, void* stream);
+int abacus_capture_id(int64_t* id, void* stream);
 
 /* The embedding of tokens (embedding.py:20-23): out_TD[t] = scale * w_VD[tokens_T[t]], a
  * negative token counted from the end; a token outside [-V, V) gives NaN and has no gradient.
