@@ -260,14 +260,20 @@ __global__ __launch_bounds__(256) void pack_few_kernel(LceArgs a) {
     }
   }
   __syncthreads();
-  for (int r = wave; r < a.T; r += 4) {
-    const int at = place_s[r];
-    if (at < 0) {
-      if (a.dx && c < a.D) ((T*)a.dx)[(int64_t)r * a.D + c] = from_f32<T>(0.f);
-    } else if (c < a.Dp) {
-      const T v = c < a.D ? ((const T*)a.x)[(int64_t)r * a.x_stride + c] : from_f32<T>(0.f);
-      ((T*)a.xc)[(int64_t)at * a.Dp + c] = v;
-      tile_s[at][lane] = v;
+  for (int r0 = wave; r0 < a.T; r0 += 32) {
+    T v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = ((const T*)a.x)[(int64_t)min(r0 + 4 * u, a.T - 1) * a.x_stride + min(c, a.D - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int r = r0 + 4 * u, at = r < a.T ? place_s[r] : -1;
+      if (at >= 0 && c < a.Dp) {
+        if (c >= a.D) v[u] = from_f32<T>(0.f);
+        ((T*)a.xc)[(int64_t)at * a.Dp + c] = v[u];
+        tile_s[at][lane] = v[u];
+      } else if (r < a.T && at < 0 && a.dx && c < a.D) {
+        ((T*)a.dx)[(int64_t)r * a.D + c] = from_f32<T>(0.f);
+      }
     }
   }
   if (!a.xt) return;
@@ -796,6 +802,13 @@ __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
 // CUs without work.  (24 x 2048 x 50257 bf16, through an aligned copy of w and tiles of 128 rows: 114 us.)
 constexpr int kFewWaves = 8;
 
+// Block b of n -> the one of its place where each XCD (it runs on XCD b % 8) has neighbouring ones: they share the cache lines
+// that their columns' ends lie in.
+__device__ inline int by_xcd(int b, int n) {
+  const int x = b & 7;
+  return x * (n >> 3) + min(x, n & 7) + (b >> 3);
+}
+
 // CW values of each of 8 (bf16) or 4 (fp32) rows of w, and the fragments of x beside them: a k-step of 16 or 8.
 template <typename T, int CW, int RF>
 struct FewStep {
@@ -868,7 +881,8 @@ __global__ __launch_bounds__(kFewWaves * 64, RF == 1 ? 4 : 2) void lce_few_kerne
   const int n = chunk_kept(a);
   if (n == 0) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  const int n0 = blockIdx.x * COLS, col = min(n0 + (lane & 31) * CW, a.V - 1);
+  const int strip = by_xcd(blockIdx.x, gridDim.x);
+  const int n0 = strip * COLS, col = min(n0 + (lane & 31) * CW, a.V - 1);
   const T* x[RF];
 #pragma unroll
   for (int r = 0; r < RF; ++r)
@@ -882,12 +896,12 @@ __global__ __launch_bounds__(kFewWaves * 64, RF == 1 ? 4 : 2) void lce_few_kerne
       for (int q = 0; q < 16; ++q) acc[r][c][q] = 0.f;
   // (whole steps end before w's last row, whose end nothing follows)
   const int whole = max(0, (a.D - 1) / KS), steps = (a.D + KS - 1) / KS;
-  const int per = (whole + kFewWaves - 1) / kFewWaves, from = wave * per, to = min(whole, from + per);
-  if (from < to) {
+  // a step of each wave in turn: together they read 128 neighbouring rows of w
+  if (wave < whole) {
     Step s0, s1;
-    s0.load(a, x, from * KS, half, col);
-    for (int k = from; k + 1 < to; ++k) {
-      s1.load(a, x, (k + 1) * KS, half, col);
+    s0.load(a, x, wave * KS, half, col);
+    for (int k = wave; k + kFewWaves < whole; k += kFewWaves) {
+      s1.load(a, x, (k + kFewWaves) * KS, half, col);
       s0.run(acc);
       s0 = s1;
     }
@@ -944,7 +958,7 @@ __global__ __launch_bounds__(kFewWaves * 64, RF == 1 ? 4 : 2) void lce_few_kerne
   }
 #pragma unroll
   for (int off = LPR / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-  if (c0 == 0) a.stats[(int64_t)blockIdx.x * a.chunk_rows + row] = make_float2(m2, s);
+  if (c0 == 0) a.stats[(int64_t)strip * a.chunk_rows + row] = make_float2(m2, s);
   if (!a.grad) return;
 #pragma unroll
   for (int i = 0; i < PER; i += 2) {
@@ -1069,20 +1083,22 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void lce_few_dx_kernel(LceArgs a
 template <typename T>
 __global__ __launch_bounds__(256) void lce_few_sum_kernel(LceArgs a, int slices) {
   constexpr int VEC = kVec<T>;
-  const int n = chunk_kept(a), vecs = a.Dp / VEC, i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= n * vecs) return;
-  const int row = i / vecs, c = i % vecs * VEC;
+  __shared__ float part_s[3][VEC][64];
+  const int n = chunk_kept(a), vecs = a.Dp / VEC, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
+  if (blockIdx.x * 64 >= n * vecs) return;
+  const int row = min(i, n * vecs - 1) / vecs, c = min(i, n * vecs - 1) % vecs * VEC;
+  const int each = (slices + 3) / 4, last = min(slices, (wave + 1) * each);
   float f[VEC] = {};
-  for (int s0 = 0; s0 < slices; s0 += 4) {
+  for (int s0 = wave * each; s0 < last; s0 += 4) {
     float4 x[4][VEC / 4];
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
       for (int k = 0; k < VEC / 4; ++k)
-        x[s][k] = *reinterpret_cast<const float4*>(a.parts + ((int64_t)min(s0 + s, slices - 1) * kFewRows + row) * a.Dp + c + 4 * k);
+        x[s][k] = *reinterpret_cast<const float4*>(a.parts + ((int64_t)min(s0 + s, last - 1) * kFewRows + row) * a.Dp + c + 4 * k);
 #pragma unroll
     for (int s = 0; s < 4; ++s)
-      if (s0 + s < slices)
+      if (s0 + s < last)
 #pragma unroll
         for (int k = 0; k < VEC / 4; ++k) {
           f[4 * k] += x[s][k].x;
@@ -1091,6 +1107,16 @@ __global__ __launch_bounds__(256) void lce_few_sum_kernel(LceArgs a, int slices)
           f[4 * k + 3] += x[s][k].w;
         }
   }
+  if (wave > 0) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) part_s[wave - 1][k][lane] = f[k];
+  }
+  __syncthreads();
+  if (wave > 0 || i >= n * vecs) return;
+#pragma unroll
+  for (int w = 0; w < 3; ++w)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) f[k] += part_s[w][k][lane];
   const float scale = *a.scale;
 #pragma unroll
   for (int k = 0; k < VEC; ++k) f[k] *= scale;
@@ -1105,7 +1131,8 @@ __global__ __launch_bounds__(256) void lce_few_dw_kernel(LceArgs a, int rows_per
   constexpr int VEC = kVec<T>, KL = VEC, KS = 2 * KL, STEPS = ROWS / KS;
   constexpr int CW = sizeof(T) == 2 && ROWS == 64 ? 4 : VEC, WORDS = CW * (int)sizeof(T) / 4;
   const int kept = *a.kept, n = chunk_kept(a), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int n0 = blockIdx.x * 32 * CW, col = n0 + (lane & 31) * CW;
+  const int at = by_xcd(blockIdx.x + blockIdx.y * gridDim.x, gridDim.x * gridDim.y), band = at / gridDim.x;
+  const int n0 = (at - band * gridDim.x) * 32 * CW, col = n0 + (lane & 31) * CW;
   Vec16 b[STEPS][CW];  // fragment of column c: its KL values of the lane's rows
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
@@ -1129,7 +1156,7 @@ __global__ __launch_bounds__(256) void lce_few_dw_kernel(LceArgs a, int rows_per
       }
   }
   const float scale = kept > 0 ? *a.scale : 1.0f;
-  const int from = (blockIdx.y * 4 + wave) * rows_per, to = min(a.D, from + rows_per);
+  const int from = (band * 4 + wave) * rows_per, to = min(a.D, from + rows_per);
   for (int d0 = from; d0 < to; d0 += 32) {
     const T* xt = (const T*)a.xt + (int64_t)min(d0 + (lane & 31), a.D - 1) * kFewRows;
     Vec16 x[STEPS];
@@ -1261,7 +1288,7 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip, int
     for (int w = 1; w < 4; ++w) join(m, s, part_s[w][tid]);
     row_s[tid] = make_float2(m, 1.0f / s);
     const int row = row0 + tid;
-    if (row < n && blockIdx.y == 0) {
+    if (row < n && blockIdx.y == 0 && blockIdx.z == 0) {
       // the target's distance from the maximum first: it is small where the loss is
       const float l = kLn2 * (__builtin_amdgcn_logf(s) + __builtin_fmaf(-a.target_logit[base + row], kLog2e, m));
       if (a.reduction == ABACUS_LOSS_ROWS) {
@@ -1272,14 +1299,14 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip, int
     }
   }
   if (!a.grad) return;
-  if (row0 == 0 && blockIdx.y == 0 && !a.xt && tid >= 128) {  // for the products that follow, a wave each
+  if (row0 == 0 && blockIdx.y == 0 && blockIdx.z == 0 && !a.xt && tid >= 128) {  // for the products that follow, a wave each
     const int cut = tid < 192 ? (a.thin & 1 << kDx ? Cover<T, kDx, THIN>(a, n).cut(a) : Cover<T, kDx, BM>(a, n).cut(a))
                               : (a.thin & 1 << kDw ? Cover<T, kDw, THIN>(a, n).cut(a) : Cover<T, kDw, BM>(a, n).cut(a));
     if (tid % 64 == 0) a.slices[tid < 192 ? kDx : kDw] = cut;
   }
   __syncthreads();
   const int first = blockIdx.y * seg, last = min(strips, first + seg);
-  for (int r = 0; r < min(kRowsB, n - row0); ++r) {
+  for (int r = blockIdx.z; r < min(kRowsB, n - row0); r += gridDim.z) {
     const int row = row0 + r;
     const float top = row_s[r].x, inv = row_s[r].y;
     const float s = a.row_grad ? a.row_grad[a.idx[base + row]] / *a.scale : 1.0f;
@@ -1401,7 +1428,8 @@ int64_t part_bytes(bool thin, int64_t rows, int64_t D, int64_t V) {
 
 int few_slices(int64_t D) { return (int)std::max<int64_t>(1, 2 * kCUs / ((D + 63) / 64)); }
 
-// Columns a lane: as many (registers for two work-groups a CU) as leave work for most CUs.
+// Columns a lane: as many (registers for two work-groups a CU) as leave work for most CUs.  (24 x 2048 x 32000 bf16: 4 columns
+// 250 work-groups, 39 us, 2 columns 500, 44 us.)
 template <typename T>
 int few_columns(int64_t V) {
   constexpr int least = sizeof(T) == 2 ? 2 : 1;
@@ -1483,7 +1511,7 @@ int launch_few_dx(const LceArgs& a, hipStream_t s) {
   else hipLaunchKernelGGL((lce_few_dx_kernel<T, 2>), grid, block, 0, s, a);
   ABACUS_CHECK_LAUNCH("linear_cross_entropy few rows' dx");
   const int64_t vecs = (int64_t)a.T * (a.Dp / VecTraits<T>::kN);
-  hipLaunchKernelGGL(lce_few_sum_kernel<T>, dim3((unsigned)((vecs + 255) / 256)), dim3(256), 0, s, a, slices);
+  hipLaunchKernelGGL(lce_few_sum_kernel<T>, dim3((unsigned)((vecs + 63) / 64)), dim3(256), 0, s, a, slices);
   ABACUS_CHECK_LAUNCH("linear_cross_entropy few rows' dx sum");
   return 0;
 }
@@ -1584,7 +1612,8 @@ int run(LceArgs a, char* ws, int64_t ws_bytes, hipStream_t s) {
     // (work-groups enough for every CU twice, of a few strips at least)
     const int groups = (rows + kRowsB - 1) / kRowsB, strips = (a.V + q.strip - 1) / q.strip;
     const int segs = a.grad ? std::max(1, std::min(2 * kCUs / groups, strips / 8)) : 1, seg = (strips + segs - 1) / segs;
-    hipLaunchKernelGGL(lce_rows_kernel<T>, dim3(groups, (strips + seg - 1) / seg), dim3(256), 0, s, a, q.strip, seg);
+    const int pieces = (strips + seg - 1) / seg, turns = a.grad ? std::max(1, std::min(kRowsB, 4 * kCUs / (groups * pieces))) : 1;
+    hipLaunchKernelGGL(lce_rows_kernel<T>, dim3(groups, pieces, turns), dim3(256), 0, s, a, q.strip, seg);
     ABACUS_CHECK_LAUNCH("linear_cross_entropy rows");
     if (a.dx) {
       if (int rc = q.few ? launch_few_dx<T>(a, s) : q.thin[kDx] ? launch_product<T, kDx, THIN>(a, s) : launch_product<T, kDx, BM>(a, s)) return rc;
