@@ -20,6 +20,12 @@
 //   3. dx and dw: two products on P.  Where their tiles are fewer than the CUs, slices of the reduction in fp32,
 //      added in slice order.  Over several chunks dw adds up in fp32.
 // So 6 n D V operations of matrix products in all: the logits are not computed again for the gradient.
+//
+// Up to kFewRows rows are bound by w's bytes instead, and three kernels of their own read or write w and dw once each, at any
+// alignment, where the tiles need w's rows at whole vectors: a copy where the vocabulary is not.
+//
+// 8188 x 1024 x 32000 bf16 takes 1.75 ms (1.42 at the rate of a large product alone), 16384 x 4096 x 65536 22.8 ms, the
+// losses of 24 x 2048 x 50257 59 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -33,10 +39,14 @@ using namespace pipe;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kCUs = 256;
-constexpr int64_t kChunkBytes = 1ll << 30;       // of P, or of the strips' statistics where there is no P
+// Of P, or of the strips' statistics where there is no P: 16384 x 4096 x 65536 bf16 in two pieces takes 22.6 ms, as in one
+// (2 GiB), in four 23.5, as each adds to dw's fp32 sums.
+constexpr int64_t kChunkBytes = 1ll << 30;
 constexpr int kUnits = 512;                       // tiles x slices of a sliced product at most
 constexpr int kSlices = 32;
-constexpr int kFewRows = 64;                      // rows up to which w streams once for each product, without tiles
+// Rows up to which w streams once for each product, without tiles: 64 x 2048 x 32000 bf16 both ways 145 us, by tiles 159;
+// of 50257 columns 249 and, with w's copy, 308; 32 x 512 x 8000 48 and 62.  More rows would need more than a wave's registers.
+constexpr int kFewRows = 64;
 constexpr int kReduceRows = 4;                    // rows of a tile that a work-group of the adding pass takes
 
 enum Kind : int { kLogits = 0, kDx = 1, kDw = 2 };
@@ -116,7 +126,8 @@ __host__ __device__ inline int slices_of(int64_t tiles, int ktiles) {
 // ---------------------------------------------------------------- packing the kept rows
 
 // A block takes rows_per rows: it counts the kept rows before them, so that no block waits for another, and copies
-// its kept rows to their places; the rows left out get a gradient of 0.
+// its kept rows to their places; the rows left out get a gradient of 0.  (8192 x 1024 bf16: 23 us, half of them the reading
+// of the targets; 16384 x 4096: 83 us, 3.2 TB/s.)
 template <typename T>
 __global__ __launch_bounds__(256) void pack_rows_kernel(LceArgs a, int rows_per) {
   constexpr int VEC = kVec<T>;
@@ -226,7 +237,8 @@ __device__ inline Vec16 load_end(const T* row, int c, int V) {
   return o;
 }
 
-// The same for few rows: a work-group takes 64 columns of all of them, and turns them for dw.
+// The same for few rows: a work-group takes 64 columns of all of them, and turns them for dw.  (Bound by latency: 24 x 2048
+// bf16 4.8 us, with a row a wave at a time 8.4 for 40.)
 template <typename T>
 __global__ __launch_bounds__(256) void pack_few_kernel(LceArgs a) {
   __shared__ int place_s[kFewRows], kept_s;
@@ -283,7 +295,7 @@ __global__ __launch_bounds__(256) void pack_few_kernel(LceArgs a) {
 }
 
 // w's rows of V values at a pitch of whole vectors, zeros behind them.  A thread takes a column of kPadRows vectors, so
-// that as many loads are in flight (2048 x 50257 bf16: 110 us a vector at a time).
+// that as many loads are in flight.  (2048 x 50257 bf16: 81 us, 5.1 TB/s; a vector at a time 110.)
 constexpr int kPadRows = 8;
 template <typename T>
 __global__ __launch_bounds__(256) void pad_w_kernel(const T* __restrict__ w, int D, int V, int Vp, T* __restrict__ out) {
@@ -318,6 +330,12 @@ __device__ inline uint32_t encode2(float a, float b) {
   return (x >> 13) | (y >> 13 << 16);
 }
 __device__ inline float decode(uint32_t h) { return h ? bits_f32((h << 13) + (64u << 23)) : 0.f; }
+
+// exp(l - m).  The difference comes first: it is never above 0, and as exact as l is, however large the logits are (one
+// multiply-add of l log2(e) and m log2(e) would save an instruction and be off by the rounding of the second: above 1 for some m).
+__device__ inline float exp_from(float l, float m) { return __builtin_amdgcn_exp2f((l - m) * kLog2e); }
+// Finite in a strip of -inf, whose exponentials are 0.
+__device__ inline float top_of(float m) { return fmaxf(m, -3.0e38f); }
 
 // acc += A B over a range of k-tiles: the operands' tiles come by DMA into a ring of LDS stages, the matrix
 // instructions of one k-step cover the fragment reads of the next, and the last step's the DMA.  begin() starts the first
@@ -587,7 +605,7 @@ __device__ __attribute__((always_inline)) inline void logits_out(const LceArgs& 
     }
     m[0] = fmaxf(max3(m[0], m[1], m[2]), m[3]);
     m[0] = fmaxf(m[0], __shfl_xor(m[0], 32, 64));
-    const float m2 = fmaxf(m[0] * kLog2e, -3.0e38f);  // (finite in a strip of -inf, whose exponentials are 0)
+    const float top = top_of(m[0]);
     float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < FN; ++j)
@@ -596,7 +614,7 @@ __device__ __attribute__((always_inline)) inline void logits_out(const LceArgs& 
         float e[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(l[j][4 * g + k], kLog2e, -m2));
+          e[k] = exp_from(l[j][4 * g + k], top);
           s[k & 3] += e[k];
         }
         if constexpr (GRAD) {
@@ -623,13 +641,15 @@ __device__ __attribute__((always_inline)) inline void logits_out(const LceArgs& 
       }
     s[0] = (s[0] + s[1]) + (s[2] + s[3]);
     s[0] += __shfl_xor(s[0], 32, 64);
-    if (here && lane < 32 && (WHOLE || first < a.V)) a.stats[(int64_t)strip * a.chunk_rows + row] = make_float2(m2, s[0]);
+    if (here && lane < 32 && (WHOLE || first < a.V)) a.stats[(int64_t)strip * a.chunk_rows + row] = make_float2(top, s[0]);
   }
 }
 
 // The logits' tiles: a work-group on each CU walks its share of the XCD's tiles, and a tile's first DMA is under way while
-// the one before goes through its exponentials (8192 x 1024 x 32000 bf16, a work-group a tile, its exponentials
-// through LDS: 667 us).
+// the one before goes through its exponentials.  Bound by the matrix instructions and, in short reductions, by the exponentials
+// and their rounding after them (about 8 us a tile of 256 x 256, in which the matrix unit rests): 16384 x 4096 x 65536
+// bf16 7.3 ms, 1200 TF/s; 8188 x 1024 x 32000 593 to 655 us, 820 to 900 TF/s (a work-group a tile, its exponentials
+// through LDS: 667 where this takes 593); 900 x 512 x 8000 fp32 84 us.
 template <typename T, int BMT, bool RK, bool GRAD>
 __global__ __launch_bounds__(NT, 1) void lce_logits_kernel(LceArgs a) {
   using GE = Geo<BMT, T>;
@@ -678,6 +698,9 @@ __global__ __launch_bounds__(NT, 1) void lce_logits_kernel(LceArgs a) {
   }
 }
 
+// A tile, or a slice of its reduction, of dx = P W^T (kDx) or dw = x^T P (kDw) a work-group: bound by the matrix
+// instructions, at large sizes by the clock that their power leaves.  8188 x 1024 x 32000 bf16: 478 and 470 us, 1120 and 1140
+// TF/s; 16384 x 4096 x 65536: 7.0 and 7.4 ms, 1250 and 1180; 900 x 512 x 8000 fp32, thin tiles: 82 and 79 us.
 template <typename T, int KIND, int BMT, bool RK, bool SUMS>
 __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
   using GE = Geo<BMT, T>;
@@ -798,8 +821,10 @@ __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
 
 // The logits of at most 32 RF rows: w streams once through the CUs, straight into the matrix instructions' registers, at
 // any alignment.  A wave takes 32 CW columns (CW neighbouring ones a lane, one of each of CW fragments) and an eighth
-// of the reduction; the work-group adds the eighths in wave order.  Narrower columns where the vocabulary would leave
-// CUs without work.  (24 x 2048 x 50257 bf16, through an aligned copy of w and tiles of 128 rows: 114 us.)
+// of the reduction, a step of 16 (bf16) or 8 rows of w in turn; the work-group adds the eighths in wave order.  Narrower
+// columns where the vocabulary would leave CUs without work.  Bound by w's bytes: 24 x 2048 x 50257 bf16 50 us, 4.1 TB/s
+// (55 with an eighth in one run of rows, 57 without by_xcd too, 114 through an aligned copy of w and tiles of 128 rows);
+// 40 rows 76 us, as the registers leave one work-group a CU.
 constexpr int kFewWaves = 8;
 
 // Block b of n -> the one of its place where each XCD (it runs on XCD b % 8) has neighbouring ones: they share the cache lines
@@ -949,16 +974,16 @@ __global__ __launch_bounds__(kFewWaves * 64, RF == 1 ? 4 : 2) void lce_few_kerne
   if (row >= n) return;
   const int at = a.tgt[a.chunk * a.chunk_rows + row] - n0 - c0;
   if (at >= 0 && at < PER) a.target_logit[a.chunk * a.chunk_rows + row] = logit_s[row * LDL + c0 + at];
-  const float m2 = fmaxf(m * kLog2e, -3.0e38f);
+  const float top = top_of(m);
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    l[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(l[i], kLog2e, -m2));
+    l[i] = exp_from(l[i], top);
     s += l[i];
   }
 #pragma unroll
   for (int off = LPR / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-  if (c0 == 0) a.stats[(int64_t)strip * a.chunk_rows + row] = make_float2(m2, s);
+  if (c0 == 0) a.stats[(int64_t)strip * a.chunk_rows + row] = make_float2(top, s);
   if (!a.grad) return;
 #pragma unroll
   for (int i = 0; i < PER; i += 2) {
@@ -989,6 +1014,8 @@ __device__ inline void store_left(T* p, const float* f, int left) {
 // lanes load a row's at any alignment, and a part of LDS of the wave's own turns them to the matrix instructions' order, a row a
 // lane (loaded as those want them, 16 bytes of 64 rows an instruction, rows of 50257 came at 2.5 TB/s).  A work-group
 // adds its waves' slices in order and writes them to parts[blockIdx.y] (rows, Dp), which lce_few_sum_kernel adds.
+// (24 x 2048 x 32000 bf16: 27 us, 40 x 2048 x 50257 63: 4.9 and 3.3 TB/s, part of w from the memory-side cache, where the
+// logits' pass has left it.)
 template <typename T, int RF>
 __global__ __launch_bounds__(kFewWaves * 64, 2) void lce_few_dx_kernel(LceArgs a) {
   constexpr int VEC = kVec<T>, GROUP = 8 * VEC, PITCH = 9 * 16;  // bytes of a row in LDS
@@ -1079,7 +1106,8 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void lce_few_dx_kernel(LceArgs a
   }
 }
 
-// dx from the slices of lce_few_dx_kernel, added in order.
+// dx from the slices of lce_few_dx_kernel: a wave adds a quarter of them in order, and one the quarters.  (Latency: 24 x 1024
+// of 32 slices under 6 us, a thread all slices 8.5.)
 template <typename T>
 __global__ __launch_bounds__(256) void lce_few_sum_kernel(LceArgs a, int slices) {
   constexpr int VEC = kVec<T>;
@@ -1125,7 +1153,9 @@ __global__ __launch_bounds__(256) void lce_few_sum_kernel(LceArgs a, int slices)
 
 // dw of few rows: x^T P, a reduction of kFewRows at most.  P's fragments of 32 CW columns stay in a wave's registers
 // while it walks its part of dw's rows; a lane ends up with CW neighbouring columns of a row, so the 512 bytes
-// of a row go out at once, at any alignment, without LDS.  ROWS: 32 or 64.
+// of a row go out at once, at any alignment, without LDS.  ROWS: 32 or 64.  Bound by dw's bytes: 24 x 2048 x 32000 bf16
+// 28 us, 4.7 TB/s; 40 x 2048 x 50257 55 us, 3.7 (63 with neighbouring columns on different XCDs: rows of an odd length share
+// cache lines there).
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void lce_few_dw_kernel(LceArgs a, int rows_per) {
   constexpr int VEC = kVec<T>, KL = VEC, KS = 2 * KL, STEPS = ROWS / KS;
@@ -1190,7 +1220,7 @@ __global__ __launch_bounds__(256) void lce_few_dw_kernel(LceArgs a, int rows_per
   }
 }
 
-// The slices of a product's tiles added in slice order.
+// The slices of a product's tiles added in slice order, bound by their bytes: of 8192 x 1024 in 32 x 4 tiles 14.5 us.
 template <typename T, int KIND, int BMT>
 __global__ __launch_bounds__(256) void lce_reduce_kernel(LceArgs a) {
   constexpr int BN = Geo<BMT, T>::BN, VEC = kVec<T>, CV = BN / VEC;
@@ -1252,7 +1282,9 @@ constexpr int kRowsB = 8;
 constexpr int kStripsB = 512;  // strips whose factors are in LDS at a time
 constexpr int kAheadB = 4;     // vectors of a thread in flight
 
-// Few rows: the work-groups of one row group (grid.y of them) take seg strips of P each.
+// A row group's work-groups take seg strips each (grid.y) and, where that leaves CUs without work, every grid.z-th row of it:
+// 24 x 16000 bf16 11 us with all 8 rows in turn, under 6 so.  Bound by P's bytes, there and back: 8188 x 32000 bf16 210 us,
+// 5.0 TB/s; 1793 x 50257 79 us.
 template <typename T>
 __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip, int seg) {
   constexpr int VEC = kVec<T>, G = 256 / kRowsB;
@@ -1264,7 +1296,7 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip, int
   const int strips = (a.V + strip - 1) / strip;
   auto join = [](float& m, float& s, float2 o) {
     const float top = fmaxf(m, o.x);
-    s = s * __builtin_amdgcn_exp2f(m - top) + o.y * __builtin_amdgcn_exp2f(o.x - top);
+    s = s * exp_from(m, top) + o.y * exp_from(o.x, top);
     m = top;
   };
   {
@@ -1290,7 +1322,7 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip, int
     const int row = row0 + tid;
     if (row < n && blockIdx.y == 0 && blockIdx.z == 0) {
       // the target's distance from the maximum first: it is small where the loss is
-      const float l = kLn2 * (__builtin_amdgcn_logf(s) + __builtin_fmaf(-a.target_logit[base + row], kLog2e, m));
+      const float l = __builtin_fmaf(kLn2, __builtin_amdgcn_logf(s), m - a.target_logit[base + row]);
       if (a.reduction == ABACUS_LOSS_ROWS) {
         if (a.loss) a.loss[a.idx[base + row]] = l;
       } else {
@@ -1315,7 +1347,7 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip, int
     for (int k0 = first; k0 < last; k0 += kStripsB) {
       __syncthreads();
       for (int k = tid; k < min(kStripsB, last - k0); k += 256)
-        factor_s[k] = s * inv * __builtin_amdgcn_exp2f(a.stats[(int64_t)(k0 + k) * a.chunk_rows + row].x - top);
+        factor_s[k] = s * inv * exp_from(a.stats[(int64_t)(k0 + k) * a.chunk_rows + row].x, top);
       __syncthreads();
       const int end = min(a.Vp, min(last, k0 + kStripsB) * strip);
       for (int c0 = k0 * strip + tid * VEC; c0 < end; c0 += 256 * VEC * kAheadB) {
@@ -1334,7 +1366,7 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip, int
             else o[k] = f * bits_f32(e[u].w[k]);
           }
           if (t >= c && t < c + VEC) {
-            const float pt = inv * __builtin_amdgcn_exp2f(__builtin_fmaf(a.target_logit[base + row], kLog2e, -top));
+            const float pt = inv * exp_from(a.target_logit[base + row], top);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) o[k] = t == c + k ? s * (pt - 1.0f) : o[k];
           }
@@ -1353,7 +1385,7 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip, int
   }
 }
 
-// The kept rows' losses added in a fixed order, in fp64.
+// The kept rows' losses added in a fixed order, in fp64 (4 us, 16384 rows 10).
 __global__ __launch_bounds__(1024) void lce_sum_kernel(LceArgs a) {
   __shared__ double sum_s[16];
   const int kept = *a.kept, tid = threadIdx.x;
@@ -1369,7 +1401,7 @@ __global__ __launch_bounds__(1024) void lce_sum_kernel(LceArgs a) {
   }
 }
 
-// t *= *g (blockIdx.y 1: u), left alone where *g is 1.
+// t *= *g (blockIdx.y 1: u), left alone where *g is 1 (a launch, 4 us).
 template <typename T>
 __global__ __launch_bounds__(256) void scale_kernel(T* __restrict__ t, int64_t n, T* __restrict__ u, int64_t m,
                                                     const float* __restrict__ g) {
@@ -1453,7 +1485,8 @@ Plan plan_of(int64_t T_, int64_t D, int64_t V, bool grad) {
   q.thin[kDx] = thin_of<T, kDx>(rows, D, V);
   q.thin[kDw] = thin_of<T, kDw>(rows, D, V);
   q.few = T_ <= kFewRows && V >= 64 ? few_columns<T>(V) : 0;
-  q.pad = V % VEC != 0 && !q.few;  // (few rows read w at any alignment)
+  // (few rows read w at any alignment, and at least 64 of its columns at a time)
+  q.pad = V % VEC != 0 && !q.few;
   q.strip = q.few ? 32 * q.few : q.thin[kLogits] ? Geo<THIN, T>::WTN : Geo<BM, T>::WTN;
   const int64_t strips = (V + q.strip - 1) / q.strip;
   int64_t at = 0;

@@ -234,6 +234,25 @@ def test_linear_cross_entropy_of_odd_values(T, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("T", [30, 60, 200])
+def test_linear_cross_entropy_of_the_largest_logits(T, dtype):
+    """Logits of up to 10^8, 2^18 and more apart: probabilities are 0 and 1, every product and sum below is exact, and the gradients
+    are 64 bits' rounded once."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.randint(-2, 3, (T, 8), device="cuda", generator=g).to(dtype)
+    x[:, 0] = torch.tensor([-2, -1, 1, 2], device="cuda").repeat(T // 4 + 1)[:T].to(dtype)
+    w = torch.randint(-4, 5, (8, 200), device="cuda", generator=g).to(dtype)
+    w[0] = (torch.randperm(200, device="cuda", generator=g) * 2.0 ** 18).to(dtype)
+    t = torch.randint(0, 200, (T,), device="cuda", generator=g)
+    x, w = x.requires_grad_(), w.requires_grad_()
+    got = torch.autograd.grad(linear_cross_entropy(x, w, t, reduction="sum"), (x, w))
+    a, b = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    want = torch.autograd.grad(F.cross_entropy(a @ b, t, reduction="sum"), (a, b))
+    assert all(torch.equal(v, d.to(dtype)) for v, d in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_linear_cross_entropy_of_no_rows():
     w = torch.randn(8, 16, device="cuda", requires_grad=True)
     x = torch.randn(0, 8, device="cuda", requires_grad=True)
