@@ -554,6 +554,11 @@ int abacus_residual_norm_bwd(const void* dr, const void* dh, const void* r, cons
   ABACUS_CHECK_ARG((post_gamma != nullptr) == (dpost != nullptr) && (gate != nullptr) == (dgate != nullptr),
                    "residual_norm_bwd: the post norm's and the gate's gradients come with them");
   ABACUS_CHECK_ARG(rows >= 1, "residual_norm_bwd: no rows");
+  const bool plain = !post_gamma && gate_kind == kNoGate && scale == 1.0f;
+  ABACUS_CHECK_ARG(plain ? !dy || dy == dx : dy && dy != dx,
+                   "residual_norm_bwd: dy is dx's memory or NULL without post_gamma, gate and scale, and its own with one");
+  ABACUS_CHECK_ARG(rstd && (!post_gamma || y_rstd) && (y || (!post_gamma && gate_kind == kNoGate)),
+                   "residual_norm_bwd: the forward's rstd, and with post_gamma y_rstd, and with it or a gate y");
   const int64_t need = abacus_residual_norm_bwd_ws_bytes(rows, D, post_gamma != nullptr, gate_kind);
   ABACUS_CHECK_ARG(ws != nullptr && ws_bytes >= need, "residual_norm_bwd: workspace of %lld bytes, %lld needed",
                    (long long)ws_bytes, (long long)need);
@@ -577,7 +582,6 @@ int abacus_residual_norm_bwd(const void* dr, const void* dh, const void* r, cons
   a.partial = (float*)ws;
   const Shape sh = shape_of(D, dtype == kBF16 ? 8 : 4, kBwdVectors);
   a.lpr = sh.lpr;
-  const bool plain = !post_gamma && gate_kind == kNoGate && scale == 1.0f;
   const int at_once = std::max(1, (plain ? kBwdWavesPlain : kBwdWaves) / (sh.threads / 64));
   const int64_t blocks = sh.blocks(rows, std::min(kBwdBlocks, 256 * at_once));
   const hipStream_t s = (hipStream_t)stream;

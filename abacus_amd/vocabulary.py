@@ -121,6 +121,11 @@ def linear_cross_entropy(x: torch.Tensor, w_DV: torch.Tensor, targets: torch.Ten
     ("none", 0 where ignored).  A mean of no rows is NaN and its gradients are 0.  A target outside [0, V) other than
     ignore_index makes its row's loss NaN, as train.cross_entropy on the GPU has it (on the CPU torch raises); nothing
     waits on the host.  Logits and sums are fp32, whatever the operands' type; ignored rows cost no products.
+
+    Where a gradient is recorded, a mean's or sum's forward forms both and the backward hands them over (times the loss's
+    own, rounded once more where that is not 1).  Besides them a call holds the kept rows of x, and with gradients a piece of the
+    probabilities of at most 1 GiB in w's type, of the rows one after the other; a w of other strides than a contiguous one's,
+    or of an odd vocabulary for over 64 rows, is copied.
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction is one of {', '.join(_REDUCTIONS)}, got {reduction!r}")

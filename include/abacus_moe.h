@@ -429,7 +429,7 @@ int abacus_cross_entropy_mean_bwd(const void* logits_NV, const int64_t* targets_
  * sum or mean, or with ABACUS_LOSS_ROWS of the sum of row_grad_T[t] (fp32) times each
  * row's loss (NULL without gradients, and for the others).  Logits, sums and
  * gradients are fp32; P = s (softmax - onehot) is rounded to `dtype` for the products, the gradients once.
- * Any D and V; x may start at any element, the other operands are 16-byte aligned.
+ * T, D and V from 1 on; x may start at any element, the other operands are 16-byte aligned.
  * ws: device workspace of abacus_linear_cross_entropy_ws_bytes bytes (grad: with gradients).
  *
  * abacus_scale_by: n values of `dtype` at t and m at u times *g (device memory), left as they are where it is 1.

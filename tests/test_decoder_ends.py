@@ -63,6 +63,14 @@ def test_head_loss_is_next_token_loss_on_cpu():
     ("abacus_residual_norm_fwd", (16, 16, 16, None, None, 0, 4, 7, 1.0, 1e-5, 1, 16, 16, None, None, None), "dim 7"),
     ("abacus_residual_norm_bwd", (16, 16, 16, 16, 16, None, None, 0, 16, None, 4, 64, 1.0, 1, 16, 16, 16, 16, None, 16, 1 << 30, None),
      "gradients"),
+    ("abacus_residual_norm_bwd", (16, 16, 16, None, 16, None, None, 0, 16, None, 4, 64, 1.0, 1, 16, 32, 16, None, None, 16, 1 << 30, None),
+     "dx's memory"),
+    ("abacus_residual_norm_bwd", (16, 16, 16, None, 16, None, None, 0, 16, None, 4, 64, 0.5, 1, 16, None, 16, None, None, 16, 1 << 30, None),
+     "its own"),
+    ("abacus_residual_norm_bwd", (16, 16, 16, 16, 16, 16, None, 0, 16, None, 4, 64, 1.0, 1, 16, 32, 16, 16, None, 16, 1 << 30, None),
+     "y_rstd"),
+    ("abacus_residual_norm_bwd", (16, 16, 16, None, 16, None, 16, 1, 16, None, 4, 64, 1.0, 1, 16, 32, 16, None, 16, 16, 1 << 30, None),
+     "a gate y"),
     ("abacus_residual_norm_bwd", (16, 16, 16, 16, 16, None, None, 0, 16, None, 4, 64, 1.0, 1, 16, 16, 16, None, None, 16, 0, None),
      "workspace"),
 ])

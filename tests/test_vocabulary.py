@@ -136,6 +136,29 @@ def test_linear_cross_entropy_matches_64_bits(T, D, V, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_linear_cross_entropy_of_many_rows_and_few_classes(dtype):
+    x, w, t = _loss_case(20011, 12, 3, dtype, 0.1)
+    x, w = x.requires_grad_(), w.requires_grad_()
+    got = linear_cross_entropy(x, w, t)
+    _check_loss(x, w, t, "mean", got.detach(), torch.autograd.grad(got, (x, w)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [40, 150])
+def test_linear_cross_entropy_ignores_any_index(T):
+    """A class as the ignored one, and a number outside int32: the bits of the same rows ignored by -100."""
+    x, w, t = _loss_case(T, 64, 300, torch.bfloat16, 0.3)
+    x, w = x.requires_grad_(), w.requires_grad_()
+    for index in (0, 299, -(1 << 40)):
+        kept = torch.where(t == index, -100, t)
+        want = linear_cross_entropy(x, w, kept)
+        got = linear_cross_entropy(x, w, torch.where(kept == -100, index, kept), ignore_index=index)
+        assert torch.equal(got, want)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, (x, w)), torch.autograd.grad(want, (x, w))))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 40001), (torch.float32, 20000)], ids=IDS)
 @pytest.mark.parametrize("ignored", [0.0, 0.3, 1.0])
 def test_linear_cross_entropy_over_chunks(dtype, V, ignored):
@@ -283,7 +306,7 @@ def test_linear_cross_entropy_past_32_bits(T):
     l = xd @ tail
     want = (lse - l.gather(1, (t - (V - 64))[:, None])[:, 0]).sum()
     far = 2 * _adds(D, torch.bfloat16) * (xd.abs() @ tail.abs()).amax() + 2.0 ** -22 * (4 + 12)
-    assert abs(float(loss) - float(want)) <= T * float(far)
+    assert abs(float(loss.detach()) - float(want)) <= T * float(far)
     p = torch.exp(l - lse[:, None])
     P = p.clone().scatter_add_(1, (t - (V - 64))[:, None], -torch.ones(T, 1, dtype=torch.float64, device="cuda"))
     off = 2.0 ** -8 * P.abs() + p * (float(far) + 2.0 ** -11)
