@@ -64,6 +64,7 @@ struct LceArgs {
   int thin;               // bit k: kind k's tiles are thin
   int reduction;          // ABACUS_LOSS_*
   int grad;               // P is wanted
+  int add;                // the launch's last work-group adds the losses
   const float* row_grad;  // weights of the rows, or NULL
   float* loss;
   void* dx;               // NULL: not wanted
@@ -1106,12 +1107,41 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void lce_few_dx_kernel(LceArgs a
   }
 }
 
+// The kept rows' losses added in a fixed order, in fp64, by the 256 threads of a work-group beside dx's slices' (a launch of its own
+// costs 4 to 10 us and the host 3), or alone.
+__device__ inline void add_losses(const LceArgs& a) {
+  __shared__ double sum_s[4];
+  constexpr int U = 8;
+  const int kept = *a.kept, tid = threadIdx.x;
+  double s = 0.0;
+  for (int i = tid; i < kept; i += 256 * U) {
+    float l[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) l[u] = a.row_loss[min(i + 256 * u, kept - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) s += i + 256 * u < kept ? (double)l[u] : 0.0;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  if ((tid & 63) == 0) sum_s[tid >> 6] = s;
+  __syncthreads();
+  if (tid == 0) {
+    s = ((s + sum_s[1]) + sum_s[2]) + sum_s[3];
+    a.loss[0] = (float)(a.reduction == ABACUS_LOSS_MEAN ? s / (double)kept : s);
+  }
+}
+__global__ __launch_bounds__(256) void lce_sum_kernel(LceArgs a) { add_losses(a); }
+
 // dx from the slices of lce_few_dx_kernel: a wave adds a quarter of them in order, and one the quarters.  (Latency: 24 x 1024
 // of 32 slices under 6 us, a thread all slices 8.5.)
 template <typename T>
 __global__ __launch_bounds__(256) void lce_few_sum_kernel(LceArgs a, int slices) {
   constexpr int VEC = kVec<T>;
   __shared__ float part_s[3][VEC][64];
+  if (a.add && blockIdx.x + 1 == gridDim.x) {
+    add_losses(a);
+    return;
+  }
   const int n = chunk_kept(a), vecs = a.Dp / VEC, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
   if (blockIdx.x * 64 >= n * vecs) return;
   const int row = min(i, n * vecs - 1) / vecs, c = min(i, n * vecs - 1) % vecs * VEC;
@@ -1224,6 +1254,10 @@ __global__ __launch_bounds__(256) void lce_few_dw_kernel(LceArgs a, int rows_per
 template <typename T, int KIND, int BMT>
 __global__ __launch_bounds__(256) void lce_reduce_kernel(LceArgs a) {
   constexpr int BN = Geo<BMT, T>::BN, VEC = kVec<T>, CV = BN / VEC;
+  if (KIND == kDx && a.add && blockIdx.x + 1 == gridDim.x) {
+    add_losses(a);
+    return;
+  }
   const int kept = *a.kept, n = chunk_kept(a);
   if (n == 0) return;
   const Cover<T, KIND, BMT> cv(a, n);
@@ -1385,22 +1419,6 @@ __global__ __launch_bounds__(256) void lce_rows_kernel(LceArgs a, int strip, int
   }
 }
 
-// The kept rows' losses added in a fixed order, in fp64 (4 us, 16384 rows 10).
-__global__ __launch_bounds__(1024) void lce_sum_kernel(LceArgs a) {
-  __shared__ double sum_s[16];
-  const int kept = *a.kept, tid = threadIdx.x;
-  double s = 0.0;
-  for (int i = tid; i < kept; i += 1024) s += (double)a.row_loss[i];
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-  if ((tid & 63) == 0) sum_s[tid >> 6] = s;
-  __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < 16; ++i) s += sum_s[i];
-    a.loss[0] = (float)(a.reduction == ABACUS_LOSS_MEAN ? s / (double)kept : s);
-  }
-}
-
 // t *= *g (blockIdx.y 1: u), left alone where *g is 1 (a launch, 4 us).
 template <typename T>
 __global__ __launch_bounds__(256) void scale_kernel(T* __restrict__ t, int64_t n, T* __restrict__ u, int64_t m,
@@ -1544,7 +1562,7 @@ int launch_few_dx(const LceArgs& a, hipStream_t s) {
   else hipLaunchKernelGGL((lce_few_dx_kernel<T, 2>), grid, block, 0, s, a);
   ABACUS_CHECK_LAUNCH("linear_cross_entropy few rows' dx");
   const int64_t vecs = (int64_t)a.T * (a.Dp / VecTraits<T>::kN);
-  hipLaunchKernelGGL(lce_few_sum_kernel<T>, dim3((unsigned)((vecs + 63) / 64)), dim3(256), 0, s, a, slices);
+  hipLaunchKernelGGL(lce_few_sum_kernel<T>, dim3((unsigned)((vecs + 63) / 64 + a.add)), dim3(256), 0, s, a, slices);
   ABACUS_CHECK_LAUNCH("linear_cross_entropy few rows' dx sum");
   return 0;
 }
@@ -1598,7 +1616,7 @@ int launch_product(const LceArgs& a, hipStream_t s) {
   ABACUS_CHECK_LAUNCH("linear_cross_entropy product");
   if (KIND == kDx || 2 * tiles <= kUnits) {  // (two slices or more are of at most kUnits / 2 tiles)
     const int64_t cut = std::min<int64_t>(tiles, kUnits / 2);
-    hipLaunchKernelGGL((lce_reduce_kernel<T, KIND, BMT>), dim3((unsigned)(cut * (BMT / kReduceRows))), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((lce_reduce_kernel<T, KIND, BMT>), dim3((unsigned)(cut * (BMT / kReduceRows) + (KIND == kDx ? a.add : 0))), dim3(256), 0, s, a);
     ABACUS_CHECK_LAUNCH("linear_cross_entropy reduce");
   }
   return 0;
@@ -1639,7 +1657,9 @@ int run(LceArgs a, char* ws, int64_t ws_bytes, hipStream_t s) {
   }
   a.chunks = q.chunks;
   a.thin = q.thin[kDx] << kDx | q.thin[kDw] << kDw;
+  const bool one_loss = a.reduction != ABACUS_LOSS_ROWS && a.loss;
   for (a.chunk = 0; a.chunk < q.chunks; ++a.chunk) {
+    a.add = one_loss && a.dx && a.chunk + 1 == q.chunks;
     if (int rc = q.few ? launch_few<T>(a, q.few, s) : q.thin[kLogits] ? launch_logits<T, THIN>(a, s) : launch_logits<T, BM>(a, s)) return rc;
     const int rows = std::min(a.chunk_rows, a.T - a.chunk * a.chunk_rows);
     // (work-groups enough for every CU twice, of a few strips at least)
@@ -1655,8 +1675,8 @@ int run(LceArgs a, char* ws, int64_t ws_bytes, hipStream_t s) {
       if (int rc = q.few ? launch_few_dw<T>(a, s) : q.thin[kDw] ? launch_product<T, kDw, THIN>(a, s) : launch_product<T, kDw, BM>(a, s)) return rc;
     }
   }
-  if (a.reduction != ABACUS_LOSS_ROWS && a.loss) {
-    hipLaunchKernelGGL(lce_sum_kernel, dim3(1), dim3(1024), 0, s, a);
+  if (one_loss && !a.dx) {
+    hipLaunchKernelGGL(lce_sum_kernel, dim3(1), dim3(256), 0, s, a);
     ABACUS_CHECK_LAUNCH("linear_cross_entropy sum");
   }
   return 0;
