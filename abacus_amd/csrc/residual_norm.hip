@@ -436,12 +436,13 @@ __global__ __launch_bounds__(1024) void residual_norm_sum_kernel(const float* __
 
 // ---------------------------------------------------------------- host
 
-constexpr int kBwdBlocks = 768;  // at most: a row of partials each
+// Work-groups of the backward at most, a row of partials each.  Those of two waves may be more: 16384 x 1024 bf16 with post and a
+// gate 53 + 9 us by 1280, 68 + 6 by 768; of more waves, more of them only cost the sums (plain 57 to 64 us of 16384 x 1024).
+constexpr int kBwdBlocks = 768, kBwdSmallBlocks = 1280;
 constexpr int kFwdBlocks = 4096;
 // Waves of the backward that a CU holds at once, by its registers: a work-group more would wait for a place and
 // then work alone.  (With post and a gate 8, 16 and 24: 56, 43 and 58 us of 4095 x 2568 bf16; plain 16, 24 and 32 alike.)
 constexpr int kBwdWavesPlain = 24, kBwdWaves = 16;
-constexpr int kWaveVectors = 2;   // of a lane in kWave; one in kGroup
 
 struct Shape {
   int layout, lpr, vpl, threads;
@@ -451,20 +452,28 @@ struct Shape {
   }
 };
 
-// kEven where the RMSNorm kernels take D and a lane would hold at most `most` vectors; else kWave with up to two, else kGroup.
+// Vectors of a lane in kEven.  Plain forwards have the RMSNorm kernels' (a work-group a row of 4096 bf16 91 us, not 95, but other
+// sums); otherwise what a lane's registers hold beside the sums over rows.  With post and a gate, one vector more or less (the
+// rows go to kGroup then): forwards of 8192 x 4096 bf16 57 us of one, 69 of eight, of 16384 x 1024 32 of one, 29 of two;
+// backwards of 16384 x 1024 bf16 53 of one, 80 of two, of 32768 x 512 fp32 (half the values) 87 of one, 76 of two; plain
+// backwards of 16384 x 1024 bf16 34 of one, 27 of two.
+constexpr int kPlainFwdVectors = 8, kVectors = 2, kBf16BwdVectors = 1;
+int most_vectors(bool bwd, bool plain, int dtype) {
+  if (!bwd) return plain ? kPlainFwdVectors : kVectors;
+  return plain || dtype != kBF16 ? kVectors : kBf16BwdVectors;
+}
+
+// kEven where the RMSNorm kernels take D and a lane would hold at most `most` vectors; else kWave with up to two of them,
+// else kGroup with one.
 Shape shape_of(int64_t D, int epv, int most) {
   const int64_t nvec = (D + epv - 1) / epv;
   int lpr = 64;
   while (lpr > 1 && nvec % lpr != 0) lpr >>= 1;
   const int64_t each = nvec / lpr;
   if (D % epv == 0 && each <= most && (each & (each - 1)) == 0) return {kEven, lpr, (int)each, 256};
-  if (nvec <= 64 * kWaveVectors) return {kWave, 64, nvec <= 64 ? 1 : 2, 256};
+  if (nvec <= 64 * std::min(most, kVectors)) return {kWave, 64, nvec <= 64 ? 1 : 2, 256};
   return {kGroup, 64, 1, (int)((nvec + 63) / 64) * 64};
 }
-
-// Of a lane in kEven.  The forward's are what the RMSNorm kernels have (a work-group a row of 4096 bf16 91 us, not 95, but other
-// sums); the backward's what its registers hold beside the sums.
-constexpr int kFwdVectors = 8, kBwdVectors = 2;
 
 int check(const char* name, int64_t rows, int64_t D, int gate_kind, bool gate, int dtype) {
   ABACUS_CHECK_ARG(dtype == kF32 || dtype == kBF16, "%s: unsupported dtype code %d (0 = fp32, 1 = bf16)", name, dtype);
@@ -489,15 +498,15 @@ int launch(const NormArgs& a, const Shape& sh, int64_t blocks, hipStream_t s) {
 template <typename T, bool PLAIN, bool BWD>
 int by_shape(const NormArgs& a, const Shape& sh, int64_t blocks, hipStream_t s) {
   if (sh.layout == kGroup) return launch<T, 1, kGroup, PLAIN, BWD>(a, sh, blocks, s);
-  if (sh.layout == kWave)
-    return sh.vpl == 1 ? launch<T, 1, kWave, PLAIN, BWD>(a, sh, blocks, s) : launch<T, 2, kWave, PLAIN, BWD>(a, sh, blocks, s);
-  if (sh.vpl == 1) return launch<T, 1, kEven, PLAIN, BWD>(a, sh, blocks, s);
-  if (sh.vpl == 2) return launch<T, 2, kEven, PLAIN, BWD>(a, sh, blocks, s);
-  if constexpr (!BWD) {
-    if (sh.vpl == 4) return launch<T, 4, kEven, PLAIN, BWD>(a, sh, blocks, s);
-    return launch<T, 8, kEven, PLAIN, BWD>(a, sh, blocks, s);
+  if (sh.vpl == 1)
+    return sh.layout == kWave ? launch<T, 1, kWave, PLAIN, BWD>(a, sh, blocks, s) : launch<T, 1, kEven, PLAIN, BWD>(a, sh, blocks, s);
+  if constexpr (!BWD || PLAIN || sizeof(T) == 4) {
+    if (sh.vpl == 2)
+      return sh.layout == kWave ? launch<T, 2, kWave, PLAIN, BWD>(a, sh, blocks, s) : launch<T, 2, kEven, PLAIN, BWD>(a, sh, blocks, s);
   }
-  return 1;  // (not reached: kBwdVectors is 2)
+  if constexpr (!BWD && PLAIN)
+    return sh.vpl == 4 ? launch<T, 4, kEven, PLAIN, BWD>(a, sh, blocks, s) : launch<T, 8, kEven, PLAIN, BWD>(a, sh, blocks, s);
+  return 1;  // (not reached: most_vectors)
 }
 
 template <bool BWD>
@@ -536,14 +545,15 @@ int abacus_residual_norm_fwd(const void* x, const void* y, const void* gamma, co
   a.h = h;
   a.rstd = rstd;
   a.y_rstd = y_rstd;
-  const Shape sh = shape_of(D, dtype == kBF16 ? 8 : 4, kFwdVectors);
+  const bool plain = !post_gamma && gate_kind == kNoGate && scale == 1.0f;
+  const Shape sh = shape_of(D, dtype == kBF16 ? 8 : 4, most_vectors(false, plain, dtype));
   a.lpr = sh.lpr;
   return dispatch<false>(a, sh, sh.blocks(rows, kFwdBlocks), dtype, (hipStream_t)stream);
 }
 
 int64_t abacus_residual_norm_bwd_ws_bytes(int64_t rows, int64_t D, int post, int gate_kind) {
   if (rows <= 0 || D <= 0) return 0;
-  return (int64_t)kBwdBlocks * sums_of(post != 0, gate_kind) * D * 4;
+  return (int64_t)kBwdSmallBlocks * sums_of(post != 0, gate_kind) * D * 4;
 }
 
 int abacus_residual_norm_bwd(const void* dr, const void* dh, const void* r, const void* y, const void* gamma,
@@ -580,10 +590,10 @@ int abacus_residual_norm_bwd(const void* dr, const void* dh, const void* r, cons
   a.dy = dy;
   a.dgate = dgate;
   a.partial = (float*)ws;
-  const Shape sh = shape_of(D, dtype == kBF16 ? 8 : 4, kBwdVectors);
+  const Shape sh = shape_of(D, dtype == kBF16 ? 8 : 4, most_vectors(true, plain, dtype));
   a.lpr = sh.lpr;
   const int at_once = std::max(1, (plain ? kBwdWavesPlain : kBwdWaves) / (sh.threads / 64));
-  const int64_t blocks = sh.blocks(rows, std::min(kBwdBlocks, 256 * at_once));
+  const int64_t blocks = sh.blocks(rows, std::min(sh.threads <= 128 ? kBwdSmallBlocks : kBwdBlocks, 256 * at_once));
   const hipStream_t s = (hipStream_t)stream;
   if (int rc = dispatch<true>(a, sh, blocks, dtype, s)) return rc;
   SumOut o{{dgamma, dgate, nullptr}};
