@@ -700,7 +700,7 @@ __global__ __launch_bounds__(NT, 1) void lce_logits_kernel(LceArgs a) {
 }
 
 // A tile, or a slice of its reduction, of dx = P W^T (kDx) or dw = x^T P (kDw) a work-group: bound by the matrix
-// instructions, at large sizes by the clock that their power leaves.  8188 x 1024 x 32000 bf16: 478 and 470 us, 1120 and 1140
+// instructions, at large sizes by the clock that their power leaves.  8188 x 1024 x 32000 bf16: 468 and 460 us, 1150 and 1170
 // TF/s; 16384 x 4096 x 65536: 7.0 and 7.4 ms, 1250 and 1180; 900 x 512 x 8000 fp32, thin tiles: 82 and 79 us.
 template <typename T, int KIND, int BMT, bool RK, bool SUMS>
 __global__ __launch_bounds__(NT, 1) void lce_product_kernel(LceArgs a) {
@@ -1250,7 +1250,8 @@ __global__ __launch_bounds__(256) void lce_few_dw_kernel(LceArgs a, int rows_per
   }
 }
 
-// The slices of a product's tiles added in slice order, bound by their bytes: of 8192 x 1024 in 32 x 4 tiles 14.5 us.
+// The slices of a product's tiles added in slice order, bound by their bytes: of 8192 x 1024 in 32 x 4 tiles 14 us, 18 with the
+// losses' sum beside them.
 template <typename T, int KIND, int BMT>
 __global__ __launch_bounds__(256) void lce_reduce_kernel(LceArgs a) {
   constexpr int BN = Geo<BMT, T>::BN, VEC = kVec<T>, CV = BN / VEC;
