@@ -139,6 +139,30 @@ def test_gradients_agree_with_differences(T):
         _agrees(by_kernel, both, [rand(T, 40), rand(T, 40), rand(40), rand(40), *(() if gate is None else (gate,))])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [20, 150])
+def test_shared_and_broadcast_operands(T):
+    """A table that is the head too, and a gate and a weight that are one value a row and one in all: their gradients are the
+    sums of what each use has, in fp32 the separate operands' up to the order of those sums."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    t = torch.randint(0, 70, (2, T), device="cuda", generator=g)
+    table, post, gate, gamma = (v.requires_grad_() for v in (rand(70, 24), rand(24), rand(T, 1), rand(1)))
+
+    def run(first, second, gate, gamma):
+        x = embedding(t[0], first)
+        r, h = residual_norm(x, x, gamma, post, gate)
+        return linear_cross_entropy(h + 0.1 * r, second, t[1])
+
+    shared = torch.autograd.grad(run(table, table.t(), gate.expand(T, 24), gamma.expand(24)), (table, gate, gamma))
+    apart = [v.detach().clone().requires_grad_() for v in (table, table.t().contiguous(), gate.expand(T, 24).contiguous(),
+                                                           gamma.expand(24).contiguous())]
+    one, two, dgate, dgamma = torch.autograd.grad(run(*apart), apart)
+    for got, want, terms in ((shared[0], one + two.t(), one.abs() + two.t().abs()), (shared[1], dgate.sum(1, True), dgate.abs().sum(1, True)),
+                             (shared[2], dgamma.sum(0, True), dgamma.abs().sum(0, True))):
+        assert torch.all((got - want).abs() <= 26 * 2.0 ** -24 * terms)
+
+
 # ---------------------------------------------------------------- the decoder
 
 
