@@ -86,8 +86,6 @@ struct LceArgs {
 };
 
 template <typename T> constexpr int kVec = VecTraits<T>::kN;
-// columns of one wave: a row's statistics go by these strips
-template <typename T, int BMT> constexpr int kStrip = Geo<BMT, T>::WTN;
 
 __device__ inline int chunk_kept(const LceArgs& a) {
   return max(0, min(a.chunk_rows, *a.kept - a.chunk * a.chunk_rows));
@@ -463,18 +461,23 @@ struct TileProduct {
   }
 };
 
-// n (at most VEC) values to p at any alignment of T.
+// VEC values to p at any element, as many as the row has left.
 template <typename T>
-__device__ inline void store_any(T* p, const float* f, int n) {
-  if constexpr (sizeof(T) == 2) {
-    Vec16 v;
+__device__ inline void store_left(T* p, const float* f, int left) {
+  if (left >= kVec<T>) {
+    u32x4_any v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v.w[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-    st8_any(p, v, n);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+      else v[i] = f32_bits(f[i]);
+    }
+    *reinterpret_cast<u32x4_any*>(p) = v;
+  } else if constexpr (sizeof(T) == 2) {
+    st8_any(p, Vec16{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])}, left);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) p[i] = f[i];
+    for (int i = 0; i < 3; ++i)
+      if (i < left) p[i] = f[i];
   }
 }
 
@@ -496,7 +499,7 @@ __device__ inline void store_grad(const LceArgs& a, float scale, int row, int co
     }
     st16(out, v);
   } else {
-    store_any<T>(out, f, N - col);
+    store_left<T>(out, f, N - col);
   }
 }
 
@@ -995,22 +998,6 @@ __global__ __launch_bounds__(kFewWaves * 64, RF == 1 ? 4 : 2) void lce_few_kerne
   }
 }
 
-// VEC values to p at any element, as many as the row has left.
-template <typename T>
-__device__ inline void store_left(T* p, const float* f, int left) {
-  if (left >= kVec<T>) {
-    u32x4_any v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 2) v[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-      else v[i] = f32_bits(f[i]);
-    }
-    *reinterpret_cast<u32x4_any*>(p) = v;
-  } else {
-    store_any<T>(p, f, left);
-  }
-}
-
 // dx of few rows: P W^T.  A wave takes 64 of w's rows and a slice of the vocabulary, in groups of 128 bytes of a row: eight
 // lanes load a row's at any alignment, and a part of LDS of the wave's own turns them to the matrix instructions' order, a row a
 // lane (loaded as those want them, 16 bytes of 64 rows an instruction, rows of 50257 came at 2.5 TB/s).  A work-group
@@ -1244,7 +1231,7 @@ __global__ __launch_bounds__(256) void lce_few_dw_kernel(LceArgs a, int rows_per
       } else {
         typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
         if (col + CW <= a.V) *reinterpret_cast<u32x2_any*>(out) = u32x2_any{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
-        else store_any<T>(out, f, a.V - col);
+        else st8_any(out, Vec16{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])}, a.V - col);
       }
     }
   }
