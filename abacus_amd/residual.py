@@ -7,6 +7,8 @@ them.  CPU tensors take the same steps in torch's operations.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 from torch.autograd import forward_ad
 
@@ -145,7 +147,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, gamma: torch.Tensor, post_ga
     least, most = (8, 8192) if _lib.dtype_code(x.dtype, x.device) == _lib.BF16 else (4, 4096)
     if not least <= D <= most:
         raise ValueError(f"residual_norm takes a dim of {least} to {most} for {x.dtype} on the GPU, got {D}")
+    scale = ctypes.c_float(scale).value  # as the kernels have it: whether it is 1 is asked on both sides
     if grad and torch.is_grad_enabled() or forward_ad._current_level >= 0:  # (which refuses a tangent)
-        return _ResidualNorm.apply(x, y, gamma, post_gamma, gate, float(scale), float(eps))
+        return _ResidualNorm.apply(x, y, gamma, post_gamma, gate, scale, float(eps))
     operands = [None if t is None else _contig(t) for t in (x, y, gamma, post_gamma, gate)]
-    return _forward(*operands, float(scale), float(eps), False)[:2]
+    return _forward(*operands, scale, float(eps), False)[:2]

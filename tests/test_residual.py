@@ -174,6 +174,16 @@ def test_layouts_and_odd_values(dtype):
 
 
 @pytest.mark.gpu
+def test_a_scale_that_rounds_to_one():
+    """1 + 2^-30 is 1 in fp32: the bits of no scale, both ways."""
+    d = _leaves(9, 40, torch.float32, False, "none")
+    leaves = [d[n].requires_grad_() for n in ("x", "y", "gamma")]
+    dr, dh = torch.randn_like(d["x"]), torch.randn_like(d["x"])
+    got, want = (torch.autograd.grad(residual_norm(*leaves, scale=s), leaves, (dr, dh)) for s in (1 + 2.0 ** -30, 1.0))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_no_rows_and_refusals_on_gpu():
     d = _leaves(0, 16, torch.float32, False, "channel")
     r, h = residual_norm(**d)
