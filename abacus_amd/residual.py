@@ -39,6 +39,11 @@ def _gate_kind(gate: torch.Tensor | None) -> int:
     return 0 if gate is None else 1 if gate.dim() == 1 else 2
 
 
+def _at(t: torch.Tensor | None) -> int | None:
+    """The address of an operand that _contig has seen, or of a new tensor."""
+    return None if t is None else t.data_ptr()
+
+
 def _forward(x, y, gamma, post_gamma, gate, scale: float, eps: float, keep: bool):
     """(r, h, rstd, y_rstd) of contiguous tensors; the last two None where they are not kept."""
     D, dev = x.shape[-1], x.device
@@ -46,9 +51,8 @@ def _forward(x, y, gamma, post_gamma, gate, scale: float, eps: float, keep: bool
     r, h = torch.empty_like(x), torch.empty_like(x)
     rstd = torch.empty(rows, dtype=torch.float32, device=dev) if keep else None
     y_rstd = torch.empty(rows, dtype=torch.float32, device=dev) if keep and post_gamma is not None else None
-    _call(dev, "abacus_residual_norm_fwd", _lib.ptr(x), _lib.ptr(y), _lib.ptr(gamma), _lib.ptr(post_gamma), _lib.ptr(gate),
-          _gate_kind(gate), rows, D, scale, eps, _lib.dtype_code(x.dtype), _lib.ptr(r), _lib.ptr(h), _lib.ptr(rstd),
-          _lib.ptr(y_rstd))
+    _call(dev, "abacus_residual_norm_fwd", x.data_ptr(), y.data_ptr(), gamma.data_ptr(), _at(post_gamma), _at(gate),
+          _gate_kind(gate), rows, D, scale, eps, _lib.dtype_code(x.dtype), r.data_ptr(), h.data_ptr(), _at(rstd), _at(y_rstd))
     return r, h, rstd, y_rstd
 
 
@@ -101,19 +105,19 @@ class _ResidualNorm(torch.autograd.Function):
     def gradients(ctx, dr, dh, y, gamma, post_gamma, gate, r, rstd, y_rstd):
         D, dev, dt = r.shape[-1], r.device, _lib.dtype_code(r.dtype)
         rows = r.numel() // D
-        dr, dh, y, gamma, post_gamma, gate = (None if t is None else _contig(t) for t in (dr, dh, y, gamma, post_gamma, gate))
+        dr, dh, y, gamma, post_gamma, gate = [None if t is None else _contig(t) for t in (dr, dh, y, gamma, post_gamma, gate)]
         dx = torch.empty_like(r)
         dgamma = torch.empty_like(gamma)
         same = post_gamma is None and gate is None and ctx.scale == 1.0  # dy is dx
         dy = None if same else torch.empty_like(r)
         dpost = None if post_gamma is None else torch.empty_like(post_gamma)
         dgate = None if gate is None else torch.empty_like(gate)
-        kind, ptr = _gate_kind(gate), _lib.ptr
+        kind = _gate_kind(gate)
         nbytes = _lib.query("abacus_residual_norm_bwd_ws_bytes", rows, D, int(post_gamma is not None), kind)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        _call(dev, "abacus_residual_norm_bwd", ptr(dr), ptr(dh), ptr(r), ptr(y), ptr(gamma), ptr(post_gamma), ptr(gate), kind,
-              ptr(rstd), ptr(y_rstd), rows, D, ctx.scale, dt, ptr(dx), ptr(dy), ptr(dgamma), ptr(dpost), ptr(dgate), ptr(ws),
-              nbytes)
+        _call(dev, "abacus_residual_norm_bwd", _at(dr), _at(dh), r.data_ptr(), _at(y), gamma.data_ptr(), _at(post_gamma),
+              _at(gate), kind, rstd.data_ptr(), _at(y_rstd), rows, D, ctx.scale, dt, dx.data_ptr(), _at(dy), dgamma.data_ptr(),
+              _at(dpost), _at(dgate), ws.data_ptr(), nbytes)
         return dx, dx if same else dy, dgamma, dpost, dgate
 
 

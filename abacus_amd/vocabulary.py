@@ -192,8 +192,8 @@ def _embed_gradient(d_out, tokens, shape, scale: float):
     nbytes = _lib.query("abacus_embedding_bwd_ws_bytes", T, V, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     d_out = _contig(d_out)
-    _call(dev, "abacus_embedding_bwd", tokens.data_ptr(), _lib.ptr(d_out), T, V, D, scale, _lib.dtype_code(d_out.dtype),
-          _lib.ptr(dw), _lib.ptr(ws), nbytes)
+    _call(dev, "abacus_embedding_bwd", tokens.data_ptr(), d_out.data_ptr(), T, V, D, scale, _lib.dtype_code(d_out.dtype),
+          dw.data_ptr(), ws.data_ptr(), nbytes)
     return dw
 
 
@@ -201,8 +201,8 @@ def _embed_call(tokens, w_VD, scale: float):
     V, D = w_VD.shape
     w = _contig(w_VD)
     out = torch.empty(*tokens.shape, D, dtype=w.dtype, device=w.device)
-    _call(w.device, "abacus_embedding_fwd", tokens.data_ptr(), _lib.ptr(w), tokens.numel(), V, D, scale,
-          _lib.dtype_code(w.dtype), _lib.ptr(out))
+    _call(w.device, "abacus_embedding_fwd", tokens.data_ptr(), w.data_ptr(), tokens.numel(), V, D, scale,
+          _lib.dtype_code(w.dtype), out.data_ptr())
     return out
 
 
