@@ -5,7 +5,7 @@
 //   l = x W  (fp32),   lse_t = log sum_v exp l_tv,   loss_t = lse_t - l[t, target_t]
 //   P_tv = s_t (exp(l_tv - lse_t) - [v = target_t]),   dx = c P W^T,   dw = c x^T P
 //
-// c is 1 / kept rows (mean), 1 (sum) or the largest weight of a row, and s_t 1 or the row's share of that: a factor common
+// c is 1 / kept rows (mean), 1 (sum) or the largest finite weight of a row, and s_t 1 or the row's share of that: a factor common
 // to all rows stays out of P, whose rounding would be the same in each (a P of -1 / 7852 at every target:
 // 0.2% off in bf16) and would not average out.  Rows whose target is ignore_index are left out before
 // any product: the kept rows are packed (their count stays on the device) and every launch ends at that count, so a
@@ -124,6 +124,10 @@ __host__ __device__ inline int slices_of(int64_t tiles, int ktiles) {
 
 // ---------------------------------------------------------------- packing the kept rows
 
+// What a row's weight is worth to the factor of all rows: a NaN or an infinity nothing, as in that factor it would reach
+// every row (its own has it by its share of the factor).
+__device__ inline float weight_of(float g) { return fabsf(g) < __builtin_inff() ? fabsf(g) : 0.f; }
+
 // A block takes rows_per rows: it counts the kept rows before them, so that no block waits for another, and copies
 // its kept rows to their places; the rows left out get a gradient of 0.  (8192 x 1024 bf16: 23 us, half of them the reading
 // of the targets; 16384 x 4096: 83 us, 3.2 TB/s.)
@@ -166,18 +170,14 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(LceArgs a, int rows_per)
   if (a.row_grad && row0 + rows == a.T) {  // (the last work-group's business too)
     float most = 0.f;
     for (int i = tid; i < a.T; i += 256) {
-      const float g = fabsf(a.row_grad[i]);
-      most = a.targets[i] != a.ignore_index && !(g <= most) ? g : most;  // (a NaN stays)
+      if (a.targets[i] != a.ignore_index) most = fmaxf(most, weight_of(a.row_grad[i]));
     }
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const float o = __shfl_xor(most, off, 64);
-      most = !(o <= most) ? o : most;
-    }
+    for (int off = 32; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
     if (lane == 0) most_s[wave] = most;
     __syncthreads();
     if (tid == 0) {
-      for (int w = 1; w < 4; ++w) most = !(most_s[w] <= most) ? most_s[w] : most;
+      for (int w = 1; w < 4; ++w) most = fmaxf(most, most_s[w]);
       *a.scale = most == 0.f ? 1.0f : most;
     }
   }
@@ -258,12 +258,9 @@ __global__ __launch_bounds__(256) void pack_few_kernel(LceArgs a) {
       } else if (lane < a.T && a.reduction == ABACUS_LOSS_ROWS && a.loss) {
         a.loss[lane] = 0.f;
       }
-      float most = a.row_grad && kept ? fabsf(a.row_grad[lane]) : 0.f;
+      float most = a.row_grad && kept ? weight_of(a.row_grad[lane]) : 0.f;
 #pragma unroll
-      for (int off = 32; off > 0; off >>= 1) {
-        const float o = __shfl_xor(most, off, 64);
-        most = !(o <= most) ? o : most;
-      }
+      for (int off = 32; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
       if (lane == 0) {
         *a.kept = n;
         *a.scale = a.row_grad ? (most == 0.f ? 1.0f : most) : a.reduction == ABACUS_LOSS_MEAN ? 1.0f / (float)n : 1.0f;

@@ -532,3 +532,29 @@ def test_two_streams_at_once():
                 got.append(run(*case))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("T", [20, 64, 150])
+@pytest.mark.parametrize("odd", [float("nan"), float("inf"), -float("inf"), 0.0])
+def test_weights_of_rows_that_are_no_numbers_or_zero(T, odd, dtype):
+    """One spoils its own row's dx, and dw, wherever the row stands; a weight of 0 is a row without a gradient."""
+    x, w, t = _loss_case(T, 64, 300, dtype, 0.2)
+    rows = linear_cross_entropy(x, w, t, reduction="none")
+    x, w = x.requires_grad_(), w.requires_grad_()
+    g = torch.rand(T, device="cuda") + 0.2
+    kept = (t != -100).nonzero()[:, 0]
+    for at in (kept[:1], kept[len(kept) // 2:][:1], kept[-1:], kept[1::3], kept):
+        weights = g.clone()
+        weights[at] = odd
+        dx, dw = torch.autograd.grad(linear_cross_entropy(x, w, t, reduction="none"), (x, w), weights)
+        others = torch.ones(T, dtype=torch.bool, device="cuda")
+        others[at] = False
+        _check_loss(x.detach()[others], w, t[others], "none", rows[others], (dx[others], None), weights[others])
+        assert torch.all(dx[t == -100] == 0)
+        if odd == 0.0:
+            assert torch.all(dx[at] == 0)
+            _check_loss(x.detach(), w, t, "none", rows, (None, dw), weights)
+        else:
+            assert not torch.isfinite(dx[at]).any() and not torch.isfinite(dw).any()
