@@ -13,7 +13,6 @@ CPU tensors take the same steps in torch's operations.
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 import torch.nn.functional as F
@@ -35,12 +34,13 @@ def _plain_loss(x_TD, w_DV, targets_T, ignore_index: int, reduction: str):
 
 
 def _loss_op(x_TD, w_DV, targets_T, ignore_index: int, reduction: str):
-    """The loss as the kernels have it, for its second derivatives: NaN, not an assertion, for a target outside the vocabulary."""
-    logits = x_TD @ w_DV
+    """What the kernels' gradients are the gradients of, for second derivatives: ignored rows are left out before the product,
+    whatever they hold, and a target outside the vocabulary (whose loss is NaN) is none."""
     kept = targets_T != ignore_index
     known = kept & (targets_T >= 0) & (targets_T < w_DV.shape[1])
-    rows = torch.logsumexp(logits, -1) - logits.gather(1, torch.where(known, targets_T, 0)[:, None])[:, 0]
-    rows = torch.where(kept, torch.where(known, rows, math.nan), 0.0)
+    logits = torch.where(kept[:, None], x_TD, 0.0) @ w_DV
+    picked = logits.gather(1, torch.where(known, targets_T, 0)[:, None])[:, 0]
+    rows = torch.where(kept, torch.logsumexp(logits, -1) - torch.where(known, picked, 0.0), 0.0)
     return rows if reduction == "none" else rows.sum() / (kept.sum().clamp(min=1) if reduction == "mean" else 1)
 
 

@@ -12,6 +12,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
+from abacus_amd import vocabulary
 from abacus_amd.vocabulary import embedding, linear_cross_entropy
 
 DTYPES = [torch.bfloat16, torch.float32]
@@ -558,3 +559,51 @@ def test_weights_of_rows_that_are_no_numbers_or_zero(T, odd, dtype):
             _check_loss(x.detach(), w, t, "none", rows, (None, dw), weights)
         else:
             assert not torch.isfinite(dx[at]).any() and not torch.isfinite(dw).any()
+
+
+def _with_unknown_targets(x, w, t, reduction):
+    """The loss that the kernels' gradients are of: of the rows not ignored alone, without a target where it is outside the
+    vocabulary."""
+    kept = t != -100
+    l = x[kept] @ w
+    known = (t[kept] >= 0) & (t[kept] < w.shape[1])
+    rows = torch.logsumexp(l, -1) - torch.where(known, l.gather(1, torch.where(known, t[kept], 0)[:, None])[:, 0], 0.0)
+    return rows.mean() if reduction == "mean" else torch.zeros(len(t), dtype=l.dtype, device=l.device).index_put((kept.nonzero()[:, 0],), rows)
+
+
+def _odd_rows(device):
+    x, w, t = _loss_case(9, 16, 40, torch.float32, device=device)
+    t[1], t[4], t[6], t[7] = -100, 40, -1, -100
+    x[1], x[7, 3] = float("nan"), float("inf")
+    return x, w, t
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_second_derivatives_are_of_the_kernels_gradient(reduction):
+    """Rows that are ignored reach nothing, whatever they hold, and a target outside the vocabulary is none."""
+    x, w, t = _odd_rows("cpu")
+    g = torch.rand(9) if reduction == "none" else torch.tensor(1.5)
+    grads = []
+    for f in (vocabulary._loss_op, lambda x, w, t, _, reduction: _with_unknown_targets(x, w, t, reduction)):
+        a, b = (v.double().requires_grad_() for v in (x, w))
+        grads.append(torch.autograd.grad(f(a, b, t, -100, reduction), (a, b), g.double()))
+    assert all(torch.allclose(a, b, rtol=1e-12, atol=1e-15) for a, b in zip(*grads))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_second_derivatives_beside_odd_rows(reduction):
+    """As test_linear_cross_entropy_second_derivatives, with NaN and infinities in ignored rows and targets outside the vocabulary."""
+    x, w, t = _odd_rows("cuda")
+    g = torch.rand(9, device="cuda") if reduction == "none" else torch.tensor(1.5, device="cuda")
+
+    def second(loss, x, w, g):
+        x, w, g = (v.detach().clone().requires_grad_() for v in (x, w, g))
+        first = torch.autograd.grad(loss(x, w), (x, w), g, create_graph=True)
+        return [*first, *torch.autograd.grad(sum((f * f.detach().cos()).sum() for f in first), (x, w, g))]
+
+    got = second(lambda x, w: linear_cross_entropy(x, w, t, reduction=reduction), x, w, g)
+    want = second(lambda x, w: _with_unknown_targets(x, w, t, reduction), x.double(), w.double(), g.double())
+    for a, b in zip(got, want):
+        size = b.norm() if b.dim() else sum((f * f.cos()).abs().sum() for f in want[:2]) / g
+        assert float((a.double() - b).detach().norm()) <= 1e-5 * float(size)
