@@ -62,8 +62,8 @@ def _loss_call(x_TD, w_DV, targets_T, ignore_index: int, reduction: str, row_gra
 
 
 def _capture(dev: torch.device) -> int:
-    """The number of the graph that the current stream records, 0 where it records none."""
-    if not torch.cuda.is_current_stream_capturing():
+    """The number of the graph that dev's current stream records, 0 where it records none."""
+    if dev.index == torch._C._cuda_getDevice() and not torch.cuda.is_current_stream_capturing():  # (the current device's)
         return 0
     number = ctypes.c_int64()
     _call(dev, "abacus_capture_id", ctypes.addressof(number))

@@ -8,6 +8,8 @@ exponentials of numbers up to the largest logit lose in fp32; P by its rounding,
 in bf16 half a step of the 10-bit exponentials (2^-11); a gradient by its rounding, its products' P and its sum.
 """
 
+import ctypes
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -607,3 +609,16 @@ def test_second_derivatives_beside_odd_rows(reduction):
     for a, b in zip(got, want):
         size = b.norm() if b.dim() else sum((f * f.cos()).abs().sum() for f in want[:2]) / g
         assert float((a.double() - b).detach().norm()) <= 1e-5 * float(size)
+
+
+def test_the_graph_of_another_device_is_asked_for(monkeypatch):
+    """A call on a device that is not the current one is in the graph that its own device's stream records."""
+    def call(device, name, address):
+        assert name == "abacus_capture_id" and device.index == 1
+        ctypes.c_int64.from_address(address).value = 7
+
+    monkeypatch.setattr(vocabulary, "_call", call)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    assert vocabulary._capture(torch.device("cuda", 0)) == 0
+    assert vocabulary._capture(torch.device("cuda", 1)) == 7
