@@ -62,6 +62,18 @@ def _single_process(what: str) -> None:
         raise NotImplementedError(f"{what} across processes is not part of this single-GPU build")
 
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _eager(*tensors) -> bool:
+    """Whether torch's operations on the tensors would run now and as they are, so that a kernel may run in their place: what
+    records, compiles or transforms operations (torch.fx, a trace, a compiler, fake tensors and other dispatch modes, functorch,
+    forward mode) would not see it."""
+    return (not torch.compiler.is_compiling() and all(type(t) in _PLAIN for t in tensors) and forward_ad._current_level < 0
+            and not torch._C._are_functorch_transforms_active() and not torch._C._len_torch_dispatch_stack()
+            and torch._C._get_tracing_state() is None)
+
+
 class Embedding(torch.nn.Module):
     """Token embedding table (embedding.py:8-23): w_vocab_D ~ N(0, 1).  On the GPU by abacus_amd.vocabulary.embedding."""
 
@@ -73,12 +85,12 @@ class Embedding(torch.nn.Module):
         torch.nn.init.normal_(self.w_vocab_D)
 
     def forward(self, tokens_BL: torch.Tensor) -> torch.Tensor:
-        w = self.w_vocab_D
-        # (the kernels carry no tangents and no functional transforms, indexing does)
-        if (w.is_cuda and w.dtype in (torch.float32, torch.bfloat16) and tokens_BL.dtype == torch.int64 and tokens_BL.is_cuda
-                and forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active()):
-            return embedding(tokens_BL, w)
-        return w[tokens_BL]  # (B, L, D)
+        if not torch.jit.is_scripting():  # (a script compiles the indexing alone)
+            w = self.w_vocab_D
+            if (_eager(w, tokens_BL) and w.is_cuda and w.dtype in (torch.float32, torch.bfloat16)
+                    and tokens_BL.dtype == torch.int64 and tokens_BL.is_cuda):
+                return embedding(tokens_BL, w)
+        return self.w_vocab_D[tokens_BL]  # (B, L, D)
 
 
 class Rotary(torch.nn.Module):
@@ -320,8 +332,8 @@ def _bare(module: torch.nn.Module, kind: type) -> bool:
 def _add_norm(x: torch.Tensor, y: torch.Tensor, norm: torch.nn.Module):
     """x + y and its norm (transformer_block.py:98-100): residual_norm's one pass where the HIP norm takes x and nothing
     looks between the two, the same bits as the two steps.  (While a KernelTimer is active the two run, each under its name.)"""
-    if (_bare(norm, RMSNorm) and norm.world_size == 1 and not _lib.timing() and x.shape == y.shape and _of_kind(x, y)
-            and x.numel() > 0 and _fused_norm_ok(x, norm.w_gamma_D)):
+    if (type(x) in _PLAIN and x.is_cuda and _bare(norm, RMSNorm) and norm.world_size == 1 and not _lib.timing()
+            and x.shape == y.shape and _of_kind(x, y) and x.numel() > 0 and _fused_norm_ok(x, norm.w_gamma_D)):
         return residual_norm(x, y, norm.w_gamma_D, eps=1e-5)
     x = x + y
     return x, norm(x)
@@ -874,7 +886,7 @@ class TransformerMoe(torch.nn.Module):
     def hidden(self, tokens_BL: torch.Tensor) -> torch.Tensor:
         """What the head multiplies: the blocks' output through the last norm, (B, L, D)."""
         x_BLD = self.embedding(tokens_BL)
-        if not (x_BLD.is_cuda and len(self.blocks) and all(_bare(b, TransformerBlockMoe) for b in self.blocks)):
+        if not (type(x_BLD) in _PLAIN and x_BLD.is_cuda and len(self.blocks) and all(_bare(b, TransformerBlockMoe) for b in self.blocks)):
             for block in self.blocks:
                 x_BLD = block(x_BLD, self.rotary)
             return self.norm(x_BLD)

@@ -277,3 +277,43 @@ def test_transforms_of_the_embedding_and_refused_tangents():
         for f in (lambda: embedding(t, w), lambda: linear_cross_entropy(x, w, t), lambda: residual_norm(w, w, w[0])):
             with pytest.raises(RuntimeError):
                 f()
+
+
+class _WholeModules(torch.fx.Tracer):
+    def __init__(self, *opened):
+        super().__init__()
+        self.opened = opened
+
+    def is_leaf_module(self, m, name):
+        return not isinstance(m, self.opened)
+
+
+def test_modules_are_traced_and_scripted():
+    """torch.fx of the embedding, of a block and of the model around their parts, and torch.jit.script of the embedding."""
+    emb = tr.Embedding(7, 8)
+    t = torch.tensor([[1, 6, 1]])
+    other = torch.tensor([[0, 3], [2, 2]])
+    for made in (torch.fx.symbolic_trace(emb), torch.jit.script(emb), torch.jit.trace(emb, t)):
+        assert torch.equal(made(other), emb.w_vocab_D[other])
+    model = _model(torch.float32, "cpu")
+    calls = lambda tracer, m: [n.target for n in tracer.trace(m).nodes if n.op == "call_module"]
+    assert calls(_WholeModules(), model) == ["embedding", "blocks.0", "blocks.1", "norm"]
+    assert calls(_WholeModules(), model.blocks[0]) == ["norm_attention", "attention", "dropout", "norm_mlp", "moe", "dropout"]
+    parts = calls(_WholeModules(tr.TransformerBlockMoe), model)
+    assert len(parts) == 2 + 2 * 6 and parts[-1] == "norm"
+
+
+@pytest.mark.gpu
+def test_embedding_is_recorded_on_the_gpu():
+    """Programs that record torch's operations record the module's: a trace, a graph of them, fake tensors, a compiled whole."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    emb = tr.Embedding(700, 8).cuda()
+    t = torch.randint(0, 700, (40, 30), device="cuda")
+    other = torch.randint(0, 700, (40, 30), device="cuda")
+    for made in (torch.fx.symbolic_trace(emb), torch.jit.script(emb), torch.jit.trace(emb, t), make_fx(emb)(t),
+                 torch.compile(emb, backend="eager", fullgraph=True)):
+        assert torch.equal(made(other), emb.w_vocab_D[other])
+    with FakeTensorMode(), torch.device("cuda"):
+        assert tr.Embedding(700, 8)(torch.zeros(40, 30, dtype=torch.int64)).shape == (40, 30, 8)
