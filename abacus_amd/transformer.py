@@ -323,9 +323,11 @@ class RMSNorm(torch.nn.Module):
         return self.w_gamma_D * x_BLD / rms_BL
 
 
-def _bare(module: torch.nn.Module, kind: type) -> bool:
-    """Whether calling `module` is calling kind.forward: no subclass, no hooks, no forward of its own."""
-    return (type(module) is kind and "forward" not in module.__dict__ and not torch.nn.modules.module._has_any_global_hook()
+def _bare(module: torch.nn.Module, kind: type, method: str = "forward") -> bool:
+    """Whether calling `module` (or its `method`) is calling this file's kind.method: no subclass, no hooks, no other method (its
+    own or its class's), nothing that Module.compile has put in its call's place."""
+    return (type(module) is kind and getattr(kind, method) is _METHODS[kind, method] and method not in module.__dict__
+            and module._compiled_call_impl is None and not torch.nn.modules.module._has_any_global_hook()
             and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
 
 
@@ -912,7 +914,7 @@ class TransformerMoe(torch.nn.Module):
         x_TD = self.embedding(tokens_T)
         cos, sin = self.rotary(x_TD, positions=rows.positions(tokens_T.shape[0]))  # (1, 1, T, K)
         blocks = list(self.blocks)
-        if x_TD.is_cuda and blocks and all(_bare(b, TransformerBlockMoe) and "forward_cached" not in b.__dict__ for b in blocks):
+        if x_TD.is_cuda and blocks and all(_bare(b, TransformerBlockMoe, "forward_cached") for b in blocks):
             # (as in hidden; the last block's sum is taken of the rows that are wanted alone)
             for b in blocks:
                 _check_cached(b, x_TD, "(tokens, dim)", 2)
@@ -929,3 +931,7 @@ class TransformerMoe(torch.nn.Module):
         if out_rows is not None:
             x_TD = x_TD[out_rows]
         return self.norm(x_TD) @ self.w_D_vocab
+
+
+_METHODS = {(kind, name): getattr(kind, name)  # (for _bare)
+            for kind, name in ((RMSNorm, "forward"), (TransformerBlockMoe, "forward"), (TransformerBlockMoe, "forward_cached"))}

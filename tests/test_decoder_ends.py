@@ -317,3 +317,42 @@ def test_embedding_is_recorded_on_the_gpu():
         assert torch.equal(made(other), emb.w_vocab_D[other])
     with FakeTensorMode(), torch.device("cuda"):
         assert tr.Embedding(700, 8)(torch.zeros(40, 30, dtype=torch.int64)).shape == (40, 30, 8)
+
+
+def test_what_stands_in_for_a_call_is_seen(monkeypatch):
+    """Module.compile's replacement of a module's call, and another forward of the class."""
+    norm, block = tr.RMSNorm(8), _model(torch.float32, "cpu").blocks[0]
+    assert tr._bare(norm, tr.RMSNorm) and tr._bare(block, tr.TransformerBlockMoe)
+    norm.compile(backend="eager")
+    block.compile(backend="eager")
+    assert not tr._bare(norm, tr.RMSNorm) and not tr._bare(block, tr.TransformerBlockMoe)
+    for kind, module in ((tr.RMSNorm, tr.RMSNorm(8)), (tr.TransformerBlockMoe, _model(torch.float32, "cpu").blocks[0])):
+        assert tr._bare(module, kind)
+        forward = kind.forward
+        monkeypatch.setattr(kind, "forward", lambda self, *a: forward(self, *a))
+        assert not tr._bare(module, kind)
+    assert tr._bare(module, kind, "forward_cached")
+    monkeypatch.setattr(kind, "forward_cached", lambda self, *a: None)
+    assert not tr._bare(module, kind, "forward_cached")
+
+
+@pytest.mark.gpu
+def test_compiled_parts_are_called():
+    """hidden, forward and forward_cached call a block or norm through what Module.compile has put in its place."""
+    model = _model().eval()
+    tokens = _tokens().clamp(min=0)
+    with torch.no_grad():
+        want = model(tokens)
+        for part, times in ((model.blocks[1], 1), (model.blocks[1].norm_attention, 2), (model.blocks[0].norm_mlp, 2), (model.norm, 2)):
+            seen = []
+
+            def call(*a, impl=part._call_impl):
+                seen.append(a)
+                return impl(*a)
+
+            part._compiled_call_impl = call
+            assert torch.equal(model(tokens), want)
+            cache = PagedKVCache(2, 12, 16, 4, 16, dtype=torch.bfloat16, device="cuda")
+            model.forward_cached(tokens[0], cache, cache.extend({cache.add(): 24}))
+            part._compiled_call_impl = None
+            assert len(seen) == times
