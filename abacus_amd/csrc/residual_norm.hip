@@ -37,7 +37,7 @@ struct NormArgs {
   void *r, *h;
   float *rstd, *y_rstd;  // NULL: not kept
   const void *dr, *dh;   // NULL: zeros
-  void *dx, *dy, *dgate;
+  void *dx, *dy, *dgamma, *dpost, *dgate;  // (the last three NULL: not wanted)
   float* partial;        // (blocks, sums, D)
   int64_t rows;
   int D, lpr, gate_kind;
@@ -252,7 +252,7 @@ struct RowIn {
   }
 };
 
-// sums: dgamma, and where they are wanted dpost and the channel gate's, in that order: a lane's own in registers over all
+// sums: of dgamma, dpost and the channel gate's those that are wanted, in that order: a lane's own in registers over all
 // its rows.  (16384 x 4096 bf16 121 us; with a row in one wave's registers, which spilled, 169.)
 template <typename T, int VPL, int LAYOUT, bool PLAIN>
 __global__ __launch_bounds__(threads_of(LAYOUT)) void residual_norm_bwd_kernel(NormArgs a) {
@@ -345,7 +345,7 @@ __global__ __launch_bounds__(threads_of(LAYOUT)) void residual_norm_bwd_kernel(N
         hold(y[v]);
         hold(post[v]);
         hold(gate[v]);
-        if (a.gate_kind == kTokenGate && act) store_vec((T*)a.dgate + o, c, pack<T>(dg));
+        if (a.gate_kind == kTokenGate && a.dgate && act) store_vec((T*)a.dgate + o, c, pack<T>(dg));
       }
     }
     if constexpr (!PLAIN) {
@@ -365,8 +365,8 @@ __global__ __launch_bounds__(threads_of(LAYOUT)) void residual_norm_bwd_kernel(N
     }
   }
   // the work-group's sums, one row of the partials each
-  const bool wanted[3] = {true, !PLAIN && a.post, !PLAIN && a.gate_kind == kChannelGate};
-  const int count = 1 + (int)wanted[1] + (int)wanted[2];
+  const bool wanted[3] = {a.dgamma != nullptr, !PLAIN && a.dpost, !PLAIN && a.gate_kind == kChannelGate && a.dgate};
+  const int count = (int)wanted[0] + (int)wanted[1] + (int)wanted[2];
   int place = 0;
 #pragma unroll
   for (int k = 0; k < SUMS; ++k) {
@@ -553,7 +553,7 @@ int abacus_residual_norm_fwd(const void* x, const void* y, const void* gamma, co
 
 int64_t abacus_residual_norm_bwd_ws_bytes(int64_t rows, int64_t D, int post, int gate_kind) {
   if (rows <= 0 || D <= 0) return 0;
-  return (int64_t)kBwdSmallBlocks * sums_of(post != 0, gate_kind) * D * 4;
+  return std::min<int64_t>(kBwdSmallBlocks, rows) * sums_of(post != 0, gate_kind) * D * 4;
 }
 
 int abacus_residual_norm_bwd(const void* dr, const void* dh, const void* r, const void* y, const void* gamma,
@@ -561,8 +561,7 @@ int abacus_residual_norm_bwd(const void* dr, const void* dh, const void* r, cons
                              const float* y_rstd, int64_t rows, int64_t D, float scale, int dtype, void* dx, void* dy,
                              void* dgamma, void* dpost, void* dgate, void* ws, int64_t ws_bytes, void* stream) {
   if (int rc = check("residual_norm_bwd", rows, D, gate_kind, gate != nullptr, dtype)) return rc;
-  ABACUS_CHECK_ARG((post_gamma != nullptr) == (dpost != nullptr) && (gate != nullptr) == (dgate != nullptr),
-                   "residual_norm_bwd: the post norm's and the gate's gradients come with them");
+  ABACUS_CHECK_ARG((post_gamma || !dpost) && (gate || !dgate), "residual_norm_bwd: the post norm's and the gate's gradients come with them");
   ABACUS_CHECK_ARG(rows >= 1, "residual_norm_bwd: no rows");
   const bool plain = !post_gamma && gate_kind == kNoGate && scale == 1.0f;
   ABACUS_CHECK_ARG(plain ? !dy || dy == dx : dy && dy != dx,
@@ -588,6 +587,8 @@ int abacus_residual_norm_bwd(const void* dr, const void* dh, const void* r, cons
   a.scale = scale;
   a.dx = dx;
   a.dy = dy;
+  a.dgamma = dgamma;
+  a.dpost = dpost;
   a.dgate = dgate;
   a.partial = (float*)ws;
   const Shape sh = shape_of(D, dtype == kBF16 ? 8 : 4, most_vectors(true, plain, dtype));
@@ -596,9 +597,11 @@ int abacus_residual_norm_bwd(const void* dr, const void* dh, const void* r, cons
   const int64_t blocks = sh.blocks(rows, std::min(sh.threads <= 128 ? kBwdSmallBlocks : kBwdBlocks, 256 * at_once));
   const hipStream_t s = (hipStream_t)stream;
   if (int rc = dispatch<true>(a, sh, blocks, dtype, s)) return rc;
-  SumOut o{{dgamma, dgate, nullptr}};
-  if (post_gamma) o.out[1] = dpost, o.out[2] = dgate;
-  const int count = sums_of(post_gamma != nullptr, gate_kind);
+  SumOut o{};
+  int count = 0;
+  for (void* sum : {dgamma, dpost, gate_kind == kChannelGate ? dgate : nullptr})
+    if (sum) o.out[count++] = sum;
+  if (count == 0) return 0;
   const dim3 grid((unsigned)((D + 63) / 64), (unsigned)count);
   if (dtype == kBF16)
     hipLaunchKernelGGL(residual_norm_sum_kernel<uint16_t>, grid, dim3(1024), 0, s, a.partial, (int)blocks, count, (int)D, o);

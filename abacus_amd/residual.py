@@ -96,27 +96,26 @@ class _ResidualNorm(torch.autograd.Function):
             return (None,) * 7
         *leaves, rstd, y_rstd = ctx.saved_tensors
         if not torch.is_grad_enabled():
-            return (*_ResidualNorm.gradients(ctx, dr, dh, *leaves, rstd, y_rstd), None, None)
+            return (*_ResidualNorm.gradients(ctx, dr, dh, *leaves, rstd, y_rstd, ctx.needs_input_grad[2:5]), None, None)
         with torch.no_grad():
             grads = _ResidualNorm.gradients(ctx, dr, dh, *leaves, rstd, y_rstd)
         return (*_recorded(ctx, grads, dr, dh, *leaves), None, None)
 
     @staticmethod
-    def gradients(ctx, dr, dh, y, gamma, post_gamma, gate, r, rstd, y_rstd):
+    def gradients(ctx, dr, dh, y, gamma, post_gamma, gate, r, rstd, y_rstd, want=(True, True, True)):
+        """(dx, dy, dgamma, dpost, dgate); want: which of the last three are formed, where there is one."""
         D, dev, dt = r.shape[-1], r.device, _lib.dtype_code(r.dtype)
         rows = r.numel() // D
         dr, dh, y, gamma, post_gamma, gate = [None if t is None else _contig(t) for t in (dr, dh, y, gamma, post_gamma, gate)]
         dx = torch.empty_like(r)
-        dgamma = torch.empty_like(gamma)
         same = post_gamma is None and gate is None and ctx.scale == 1.0  # dy is dx
         dy = None if same else torch.empty_like(r)
-        dpost = None if post_gamma is None else torch.empty_like(post_gamma)
-        dgate = None if gate is None else torch.empty_like(gate)
+        dgamma, dpost, dgate = (torch.empty_like(t) if t is not None and w else None for t, w in zip((gamma, post_gamma, gate), want))
         kind = _gate_kind(gate)
         nbytes = _lib.query("abacus_residual_norm_bwd_ws_bytes", rows, D, int(post_gamma is not None), kind)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         _call(dev, "abacus_residual_norm_bwd", _at(dr), _at(dh), r.data_ptr(), _at(y), gamma.data_ptr(), _at(post_gamma),
-              _at(gate), kind, rstd.data_ptr(), _at(y_rstd), rows, D, ctx.scale, dt, dx.data_ptr(), _at(dy), dgamma.data_ptr(),
+              _at(gate), kind, rstd.data_ptr(), _at(y_rstd), rows, D, ctx.scale, dt, dx.data_ptr(), _at(dy), _at(dgamma),
               _at(dpost), _at(dgate), ws.data_ptr(), nbytes)
         return dx, dx if same else dy, dgamma, dpost, dgate
 

@@ -461,8 +461,8 @@ int abacus_embedding_bwd(const int64_t* tokens_T, const void* d_out_TD, int64_t 
  * gate_kind 0: no gate, 1: gate has D values, 2: (rows, D).  rstd and y_rstd (one fp32 a
  * row, NULL where not wanted): the two inverse roots, for the backward.
  * Backward, of dr and dh (NULL: zeros): dx, dy (may be dx's own memory or NULL where b is y and
- * scale 1 without a gate: they are the same), dgamma, and dpost and dgate with post_gamma and gate; sums over rows in
- * fp32, in a fixed order.  y is read with a gate or post_gamma only.
+ * scale 1 without a gate: they are the same), dgamma, and dpost and dgate with post_gamma and gate (each of these three
+ * NULL: not formed); sums over rows in fp32, in a fixed order.  y is read with a gate or post_gamma only.
  * ws: abacus_residual_norm_bwd_ws_bytes bytes.  D: 8 to 8192 (bf16), 4 to 4096 (fp32). */
 int abacus_residual_norm_fwd(const void* x, const void* y, const void* gamma, const void* post_gamma, const void* gate,
                              int gate_kind, int64_t rows, int64_t D, float scale, float eps, int dtype, void* r,

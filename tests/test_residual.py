@@ -9,6 +9,7 @@ over the waves, so what they are in is off by 100 * 2^-24 of the sum of magnitud
 import pytest
 import torch
 
+from abacus_amd import _lib
 from abacus_amd import transformer as tr
 from abacus_amd.residual import residual_norm
 
@@ -256,3 +257,62 @@ def test_captured_and_on_two_streams():
         want = run(twins[0])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["none", "channel", "token"])
+def test_frozen_operands_have_no_gradient_formed(gate):
+    """The norms' weights and the gate that ask for none: the others' gradients are the same bits, and nothing of a frozen gate's size
+    is allocated."""
+    rows, D = 2048, 1024
+    d = _leaves(rows, D, torch.float32, True, gate)
+    dr, dh = torch.randn_like(d["x"]), torch.randn_like(d["x"])
+    there = [n for n, t in d.items() if t is not None]
+
+    def run(asked):
+        leaves = {n: None if t is None else t.detach().requires_grad_(n in asked) for n, t in d.items()}
+        r, h = residual_norm(**leaves, scale=0.5)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        torch.autograd.backward((r, h), (dr, dh))
+        peak = torch.cuda.max_memory_allocated() - before
+        assert all(leaves[n].grad is None for n in there if n not in asked)
+        return {n: leaves[n].grad for n in asked}, peak
+
+    whole, _ = run(there)
+    for asked in (["x", "y"], ["x", "y", "gamma"], ["x", "y", "post_gamma"], [n for n in there if n != "post_gamma"],
+                  [n for n in there if n != "gate"]):
+        got, peak = run(asked)
+        assert all(torch.equal(got[n], whole[n]) for n in asked)
+        big = 2 + (gate == "token" and "gate" in asked)
+        sums = _lib.query("abacus_residual_norm_bwd_ws_bytes", rows, D, 1, int(gate == "channel"))
+        # (each large allocation may hold up to 1 MiB more of its block, and the small ones are some KiB; one tensor more is 8 MiB)
+        assert peak < big * rows * D * 4 + sums + (big + 2 << 20)
+
+
+def test_workspaces_of_few_rows_are_small():
+    """Partial sums of as many work-groups as there are rows at most."""
+    for rows in (1, 5, 200):
+        for gate_kind, sums in ((0, 2), (1, 3), (2, 2)):
+            assert 0 < _lib.query("abacus_residual_norm_bwd_ws_bytes", rows, 4096, 1, gate_kind) <= rows * sums * 4096 * 4
+
+
+@pytest.mark.gpu
+def test_second_derivatives_beside_frozen_operands():
+    """Of gradients that are recorded, with the post norm's weight and the gate frozen."""
+    d = _leaves(5, 16, torch.float32, True, "channel")
+    dr, dh = (torch.randn(5, 16, device="cuda") for _ in range(2))
+
+    def second(f, wide):
+        x, y, gamma = (d[n].detach().to(wide).requires_grad_() for n in ("x", "y", "gamma"))
+        first = torch.autograd.grad(f(x, y, gamma, d["post_gamma"].to(wide), d["gate"].to(wide)), (x, y, gamma),
+                                    (dr.to(wide), dh.to(wide)), create_graph=True)
+        return [*first, *torch.autograd.grad(sum((v * v.detach().cos()).sum() for v in first), (x, y, gamma))]
+
+    def plain(x, y, gamma, post, gate):
+        r = x + 0.5 * gate * tr._norm_op(y, post, EPS)
+        return r, tr._norm_op(r, gamma, EPS)
+
+    for a, b in zip(second(lambda *a: residual_norm(*a, scale=0.5), torch.float32), second(plain, torch.float64)):
+        assert float((a.double() - b).detach().norm()) <= 2e-5 * float(b.norm())
