@@ -72,45 +72,49 @@ def _capture(dev: torch.device) -> int:
 
 class _LinearCrossEntropy(torch.autograd.Function):
     """Loss and gradients in one pass over the logits: of a mean or a sum the forward forms both gradients, and the
-    backward multiplies them by the loss's own (they are left alone, on the device, where that is 1).  The losses of rows
+    backward multiplies them by the loss's own (they are left alone, on the device, where that is 1).  In between they are
+    saved tensors, which hooks may move and checkpointing drops.  The losses of rows
     have gradients a row that only the backward knows, so it makes the pass once more; so does a second
     backward of a mean or a sum, and one that is not recorded into the graph its forward is in (each of the two may be
     replayed without the other)."""
 
     @staticmethod
     def forward(ctx, x_TD, w_DV, targets_T, ignore_index: int, reduction: str):
-        ctx.save_for_backward(x_TD, w_DV, targets_T)
         ctx.args = ignore_index, reduction
         now = ctx.needs_input_grad[:2] if reduction != "none" else (False, False)
         ctx.capture = _capture(x_TD.device)
-        loss, *ctx.grads = _loss_call(x_TD, w_DV, targets_T, ignore_index, reduction, want=now)
+        loss, *grads = _loss_call(x_TD, w_DV, targets_T, ignore_index, reduction, want=now)
+        ctx.formed = any(now)
+        ctx.save_for_backward(x_TD, w_DV, targets_T, *grads)
         return loss
 
     @staticmethod
     def backward(ctx, g):
-        x, w, targets = ctx.saved_tensors
+        x, w, targets, *grads = ctx.saved_tensors
         if not torch.is_grad_enabled():
-            return (*_LinearCrossEntropy.gradients(ctx, g, x, w, targets), None, None, None)
+            return (*_LinearCrossEntropy.gradients(ctx, g, x, w, targets, grads), None, None, None)
         from .transformer import _by_kernel
 
         op = lambda x, w: _loss_op(x, w, targets, *ctx.args)
         wanted = lambda: tuple(torch.zeros_like(t) if d is None else d
-                               for t, d in zip((x, w), _LinearCrossEntropy.gradients(ctx, g, x, w, targets)))
+                               for t, d in zip((x, w), _LinearCrossEntropy.gradients(ctx, g, x, w, targets, grads)))
         return (*_by_kernel(op, wanted, g, x, w), None, None, None)
 
     @staticmethod
-    def gradients(ctx, g, x, w, targets):
+    def gradients(ctx, g, x, w, targets, grads):
         ignore_index, reduction = ctx.args
         g = g.contiguous()
         if reduction == "none":
             return _loss_call(x, w, targets, ignore_index, reduction, g, ctx.needs_input_grad[:2], want_loss=False)[1:]
-        grads, ctx.grads = ctx.grads, None
-        if grads is None or ctx.capture != _capture(x.device):  # handed over by an earlier backward, or another's to write
+        formed, ctx.formed = ctx.formed, False
+        if not formed or ctx.capture != _capture(x.device):  # handed over by an earlier backward, or another's to write
             grads = _loss_call(x, w, targets, ignore_index, reduction, want=ctx.needs_input_grad[:2])[1:]
+        else:  # (what becomes of them is the caller's: versions of their own, so that a retained graph does not mind)
+            grads = [None if d is None else d.data for d in grads]
         sizes = [0 if t is None else t.numel() for t in grads]
         _call(x.device, "abacus_scale_by", _lib.ptr(grads[0]), sizes[0], _lib.ptr(grads[1]), sizes[1], _lib.dtype_code(x.dtype),
               g.data_ptr())
-        return grads
+        return tuple(grads)
 
 
 def linear_cross_entropy(x: torch.Tensor, w_DV: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,

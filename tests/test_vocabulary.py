@@ -13,6 +13,7 @@ import ctypes
 import pytest
 import torch
 import torch.nn.functional as F
+import torch.utils.checkpoint
 
 from abacus_amd import vocabulary
 from abacus_amd.vocabulary import embedding, linear_cross_entropy
@@ -622,3 +623,36 @@ def test_the_graph_of_another_device_is_asked_for(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     assert vocabulary._capture(torch.device("cuda", 0)) == 0
     assert vocabulary._capture(torch.device("cuda", 1)) == 7
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_gradients_between_forward_and_backward_are_saved_tensors(reduction):
+    """Hooks on saved tensors see the gradients that the forward has formed, may move them, and checkpointing drops them; a
+    backward that is made again has them too."""
+    x, w, t = _loss_case(150, 512, 4000, torch.bfloat16, 0.2)
+    leaves = x.requires_grad_(), w.requires_grad_()
+    want = torch.autograd.grad(linear_cross_entropy(x, w, t, reduction=reduction) * 0.5, leaves)
+    shapes = []
+
+    def pack(v):
+        shapes.append(tuple(v.shape))
+        return v.cpu()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda v: v.cuda()):
+        loss = linear_cross_entropy(x, w, t, reduction=reduction) * 0.5
+    assert shapes.count((150, 512)) == 2 and shapes.count((512, 4000)) == 2
+    plain = linear_cross_entropy(x, w, t, reduction=reduction) * 0.5
+    for again in (loss, plain):
+        for _ in range(2):
+            got = torch.autograd.grad(again, leaves, retain_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            for d in got:
+                d.zero_()
+    del again, plain, got
+    del loss
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    loss = torch.utils.checkpoint.checkpoint(lambda x, w: linear_cross_entropy(x, w, t, reduction=reduction), x, w, use_reentrant=False) * 0.5
+    assert torch.cuda.memory_allocated() - before < 512 * 4000
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, leaves), want))
