@@ -656,3 +656,54 @@ def test_gradients_between_forward_and_backward_are_saved_tensors(reduction):
     loss = torch.utils.checkpoint.checkpoint(lambda x, w: linear_cross_entropy(x, w, t, reduction=reduction), x, w, use_reentrant=False) * 0.5
     assert torch.cuda.memory_allocated() - before < 512 * 4000
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, leaves), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_one_row_of_any_stride(dtype):
+    """A single row has no stride to speak of: a column that is turned to one, and one that is expanded."""
+    w = torch.randn(24, 90, device="cuda").to(dtype).requires_grad_()
+    t = torch.tensor([7], device="cuda")
+    column = torch.randn(24, 1, device="cuda").to(dtype)
+    row = column.reshape(1, 24).clone().requires_grad_()
+    want = linear_cross_entropy(row, w, t)
+    for x in (column.t(), column[:, 0].as_strided((1, 24), (0, 1)), column.t().expand(1, 24)):
+        assert x.stride(0) < 24
+        x = x.detach().requires_grad_()
+        got = linear_cross_entropy(x, w, t)
+        assert torch.equal(got, want)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(got, (x, w)), torch.autograd.grad(want, (row, w), retain_graph=True)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [10, 70])
+def test_gradient_of_rows_past_32_bits(T):
+    """dx of a w of more than 2^31 values, against 64 bits: targets and the likeliest columns lie past the 2^31st value."""
+    D, V, piece = 2048, 1_050_000, 50_000
+    x, _, t = _loss_case(T, D, 8, torch.bfloat16)
+    w = torch.empty(D, V, dtype=torch.bfloat16, device="cuda").normal_(0.0, 0.04, generator=torch.Generator(device="cuda").manual_seed(5))
+    t = V - 1 - t * 1000
+    dx, = torch.autograd.grad(linear_cross_entropy(x.requires_grad_(), w, t, reduction="sum"), x)
+    xd = x.detach().double()
+    lse, top, most = torch.full((T,), -float("inf"), dtype=torch.float64, device="cuda"), 0.0, 0.0
+    for a in range(0, V, piece):
+        l = xd @ w[:, a:a + piece].double()
+        lse = torch.logaddexp(lse, torch.logsumexp(l, -1))
+        top = max(top, float(l.abs().max()))
+        most = max(most, float((xd.abs() @ w[:, a:a + piece].double().abs()).max()))
+    far = 2 * _adds(D, torch.bfloat16) * most + 2.0 ** -22 * (4 + top)
+    want, size, off = (torch.zeros(T, D, dtype=torch.float64, device="cuda") for _ in range(3))
+    for a in range(0, V, piece):
+        wd = w[:, a:a + piece].double()
+        p = torch.exp(xd @ wd - lse[:, None])
+        here = (t >= a) & (t < a + piece)
+        P = p.clone()
+        P[here, t[here] - a] -= 1.0
+        turned = wd.t().contiguous()
+        want += P @ turned
+        size += P.abs() @ turned.abs()
+        off += (_u(torch.bfloat16) * P.abs() + p * (far + 2.0 ** -11)) @ turned.abs()
+    bound = 1.01 * (_u(torch.bfloat16) * want.abs() + off + (_adds(V, torch.bfloat16) + 2.0 ** -22) * size)
+    assert torch.all((dx.double() - want).abs() <= bound)
+    # the bound tells the target's column from the one that 32 bits would reach
+    assert float(bound.max()) < 0.25 * float(w[:, -1].float().abs().max())
