@@ -42,6 +42,7 @@ constexpr int kCUs = 256;
 // Of P, or of the strips' statistics where there is no P: 16384 x 4096 x 65536 bf16 in two pieces takes 22.6 ms, as in one
 // (2 GiB), in four 23.5, as each adds to dw's fp32 sums.
 constexpr int64_t kChunkBytes = 1ll << 30;
+constexpr int64_t kChunkRows = 1ll << 26;         // 2^31 threads of the rows' launch, which holds fewer than 2^32
 constexpr int kUnits = 512;                       // tiles x slices of a sliced product at most
 constexpr int kSlices = 32;
 // Rows up to which w streams once for each product, without tiles: 64 x 2048 x 32000 bf16 both ways 145 us, by tiles 159;
@@ -1481,7 +1482,7 @@ Plan plan_of(int64_t T_, int64_t D, int64_t V, bool grad) {
   q.Vp = (int)((V + VEC - 1) / VEC * VEC);
   // a strip is half a tile's columns; with gradients a row of P is in a chunk as a whole
   const int64_t row_bytes = grad ? (int64_t)q.Vp * (int64_t)sizeof(T) : (V + 31) / 32 * 8;
-  const int64_t rows = std::min(T_, std::max<int64_t>(BM, kChunkBytes / row_bytes / BM * BM));
+  const int64_t rows = std::min(T_, std::max<int64_t>(BM, std::min(kChunkBytes / row_bytes, kChunkRows) / BM * BM));
   q.chunk_rows = (int)rows;
   q.chunks = (int)((T_ + rows - 1) / rows);
   q.thin[kLogits] = thin_of<T, kLogits>(rows, D, V);

@@ -356,3 +356,9 @@ def test_compiled_parts_are_called():
             model.forward_cached(tokens[0], cache, cache.extend({cache.add(): 24}))
             part._compiled_call_impl = None
             assert len(seen) == times
+
+
+def test_chunks_of_rows_are_what_a_launch_holds():
+    """Past 2^26 rows the statistics of a chunk are those of 2^26 (4 numbers of 4 bytes and 8 values of 2 a row beside them)."""
+    of = lambda T: _lib.query("abacus_linear_cross_entropy_ws_bytes", T, 8, 8, _lib.BF16, 0)
+    assert of(1 << 27) - of(1 << 26) == (1 << 26) * (4 * 4 + 8 * 2)
