@@ -322,14 +322,15 @@ int backward(const int64_t* tokens, const void* dy, int64_t n, int64_t V, int64_
   int* order = (int*)(ws + sp.order);
   int* joins = (int*)(ws + sp.joins);
   float* parts = (float*)(ws + sp.parts);
+  const int pieces = n > kHot ? (int)((n + kPiece - 1) / kPiece) : 0;
+  const int slabs = (int)((D + 64 * VecTraits<T>::kN - 1) / (64 * VecTraits<T>::kN));
+  const int64_t tasks = (V + kIds - 1) / kIds * slabs, blocks = 2 * pieces + (tasks + 3) / 4;
+  // (a launch has fewer than 2^32 threads a dimension)
+  ABACUS_CHECK_ARG(blocks < (1ll << 24), "embedding_bwd: %lld tokens of a table of %lld x %lld", (long long)n, (long long)V, (long long)D);
   const int ids = (int)std::min<int64_t>(kMaxIds, (V + 255) / 256);
   hipLaunchKernelGGL(embedding_sort_kernel, dim3((unsigned)((V + ids - 1) / ids)), dim3(kSortWaves * 64),
                      kSortWaves * ids * 4, s, tokens, (int)n, (int)V, ids, start, order);
   ABACUS_CHECK_LAUNCH("embedding_bwd sort");
-  const int pieces = n > kHot ? (int)((n + kPiece - 1) / kPiece) : 0;
-  const int slabs = (int)((D + 64 * VecTraits<T>::kN - 1) / (64 * VecTraits<T>::kN));
-  const int64_t tasks = (V + kIds - 1) / kIds * slabs, blocks = 2 * pieces + (tasks + 3) / 4;
-  ABACUS_CHECK_ARG(blocks < (1ll << 31), "embedding_bwd: a table of %lld x %lld", (long long)V, (long long)D);
   hipLaunchKernelGGL(embedding_rows_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, tokens, (const T*)dy, start, order, (int)V,
                      (int)D, slabs, scale, pieces, joins, parts, (T*)dw);
   ABACUS_CHECK_LAUNCH("embedding_bwd rows");

@@ -362,3 +362,11 @@ def test_chunks_of_rows_are_what_a_launch_holds():
     """Past 2^26 rows the statistics of a chunk are those of 2^26 (4 numbers of 4 bytes and 8 values of 2 a row beside them)."""
     of = lambda T: _lib.query("abacus_linear_cross_entropy_ws_bytes", T, 8, 8, _lib.BF16, 0)
     assert of(1 << 27) - of(1 << 26) == (1 << 26) * (4 * 4 + 8 * 2)
+
+
+@pytest.mark.parametrize("name,args,msg", [
+    ("abacus_embedding_bwd", (16, 16, 4, 1 << 29, 8, 1.0, 1, 16, 16, 1 << 40, None), "tokens of a table of 536870912 x 8"),
+])
+def test_entry_points_refuse_what_no_launch_holds(name, args, msg):
+    with pytest.raises(RuntimeError, match=msg):
+        _lib.call(name, *args)
