@@ -74,6 +74,10 @@ def _eager(*tensors) -> bool:
             and torch._C._get_tracing_state() is None)
 
 
+# What the embedding's kernels hold both ways: rows and columns of a table, tokens of a call.
+_EMBEDDING_MOST = (1 << 27, 1 << 21, 1 << 26)
+
+
 class Embedding(torch.nn.Module):
     """Token embedding table (embedding.py:8-23): w_vocab_D ~ N(0, 1).  On the GPU by abacus_amd.vocabulary.embedding."""
 
@@ -89,7 +93,9 @@ class Embedding(torch.nn.Module):
             w = self.w_vocab_D
             if (_eager(w, tokens_BL) and w.is_cuda and w.dtype in (torch.float32, torch.bfloat16)
                     and tokens_BL.dtype == torch.int64 and tokens_BL.is_cuda):
-                return embedding(tokens_BL, w)
+                rows, dim, tokens = _EMBEDDING_MOST
+                if w.shape[0] <= rows and w.shape[1] <= dim and tokens_BL.numel() <= tokens:
+                    return embedding(tokens_BL, w)
         return self.w_vocab_D[tokens_BL]  # (B, L, D)
 
 

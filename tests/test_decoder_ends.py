@@ -370,3 +370,28 @@ def test_chunks_of_rows_are_what_a_launch_holds():
 def test_entry_points_refuse_what_no_launch_holds(name, args, msg):
     with pytest.raises(RuntimeError, match=msg):
         _lib.call(name, *args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,D", [((1 << 30) + 8, 1), ((1 << 28) + 8, 2), (3, (1 << 22) + 8)])
+def test_embedding_of_tables_past_the_kernels(V, D):
+    """Rows, columns and tokens past what the kernels hold go by indexing, as all did, both ways."""
+    emb = torch.nn.Module.__new__(tr.Embedding)
+    torch.nn.Module.__init__(emb)
+    emb.w_vocab_D = torch.nn.Parameter(torch.zeros(V, D, device="cuda", dtype=torch.bfloat16))
+    with torch.no_grad():
+        emb.w_vocab_D[-2:] = torch.arange(1, 3, device="cuda")[:, None].bfloat16()
+    t = torch.tensor([[0, V - 1], [V - 1, V - 2]], device="cuda")
+    out = emb(t)
+    assert torch.equal(out[..., -1].float(), torch.tensor([[0.0, 2.0], [2.0, 1.0]], device="cuda"))
+    dw, = torch.autograd.grad(out, emb.w_vocab_D, torch.ones_like(out))
+    assert torch.equal(dw[[0, 1, V - 2, V - 1], 0].float().cpu(), torch.tensor([1.0, 1.0 if V == 3 else 0.0, 1.0, 2.0]))
+
+
+@pytest.mark.gpu
+def test_embedding_of_more_tokens_than_the_kernels_hold(monkeypatch):
+    emb = tr.Embedding(50, 8).cuda()
+    t = torch.randint(0, 50, (9, 4), device="cuda")
+    monkeypatch.setattr(tr, "_EMBEDDING_MOST", (50, 8, 36))
+    monkeypatch.setattr(tr, "embedding", lambda t, w: torch.zeros(0))
+    assert emb(t).numel() == 0 and torch.equal(emb(t.repeat(2, 1)), emb.w_vocab_D[t.repeat(2, 1)])
