@@ -353,6 +353,7 @@ int abacus_embedding_fwd(const int64_t* tokens_T, const void* w_VD, int64_t T, i
                          void* out_TD, void* stream) {
   if (int rc = check("embedding_fwd", T, V, D, dtype)) return rc;
   if (T == 0) return 0;
+  ABACUS_CHECK_ARG(tokens_T && w_VD && out_TD, "embedding_fwd: null pointer");
   const int epv = dtype == kBF16 ? 8 : 4, vecs = (int)((D + epv - 1) / epv);
   const int64_t n = T * vecs;
   const unsigned blocks = (unsigned)std::min<int64_t>((n + 255) / 256, 1 << 16);
@@ -374,9 +375,10 @@ int64_t abacus_embedding_bwd_ws_bytes(int64_t T, int64_t V, int64_t D) {
 int abacus_embedding_bwd(const int64_t* tokens_T, const void* d_out_TD, int64_t T, int64_t V, int64_t D, float scale,
                          int dtype, void* dw_VD, void* ws, int64_t ws_bytes, void* stream) {
   if (int rc = check("embedding_bwd", T, V, D, dtype)) return rc;
+  ABACUS_CHECK_ARG(dw_VD && (T == 0 || (tokens_T && d_out_TD)), "embedding_bwd: null pointer");
   const int64_t need = Space(T, V, D).total;
-  ABACUS_CHECK_ARG(ws != nullptr && ws_bytes >= need, "embedding_bwd: workspace of %lld bytes, %lld needed",
-                   (long long)ws_bytes, (long long)need);
+  ABACUS_CHECK_ARG(ws != nullptr && (uintptr_t)ws % 16 == 0 && ws_bytes >= need,
+                   "embedding_bwd: workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)ws_bytes, (long long)need);
   return dtype == kBF16 ? backward<uint16_t>(tokens_T, d_out_TD, T, V, D, scale, dw_VD, (char*)ws, (hipStream_t)stream)
                         : backward<float>(tokens_T, d_out_TD, T, V, D, scale, dw_VD, (char*)ws, (hipStream_t)stream);
 }

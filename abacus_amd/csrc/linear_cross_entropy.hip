@@ -1692,6 +1692,9 @@ int abacus_linear_cross_entropy(const void* x_TD, int64_t x_stride, const void* 
   ABACUS_CHECK_ARG(reduction != ABACUS_LOSS_ROWS || grad == (row_grad_T != nullptr), "linear_cross_entropy: gradients of rows' losses need the rows' weights");
   ABACUS_CHECK_ARG(grad || loss != nullptr, "linear_cross_entropy: nothing to compute");
   ABACUS_CHECK_ARG(T > 0, "linear_cross_entropy: no rows");
+  ABACUS_CHECK_ARG(x_TD && w_DV && targets_T, "linear_cross_entropy: null pointer");
+  ABACUS_CHECK_ARG(((uintptr_t)w_DV | (uintptr_t)dx_TD | (uintptr_t)dw_DV | (uintptr_t)ws) % 16 == 0,
+                   "linear_cross_entropy: w, the gradients and the workspace must be 16-byte aligned");
   LceArgs a{};
   a.x = x_TD;
   a.x_stride = x_stride;
@@ -1725,6 +1728,8 @@ int abacus_scale_by(void* t, int64_t n, void* u, int64_t m, int dtype, const flo
   ABACUS_CHECK_ARG(dtype == kF32 || dtype == kBF16, "scale_by: unsupported dtype code %d (0 = fp32, 1 = bf16)", dtype);
   ABACUS_CHECK_ARG(n >= 0 && m >= 0, "scale_by: %lld and %lld values", (long long)n, (long long)m);
   if (n == 0 && m == 0) return 0;
+  ABACUS_CHECK_ARG(g && (t || n == 0) && (u || m == 0), "scale_by: null pointer");
+  ABACUS_CHECK_ARG(((uintptr_t)t | (uintptr_t)u) % 16 == 0, "scale_by: values must be 16-byte aligned");
   const dim3 grid((unsigned)std::min<int64_t>((std::max(n, m) + 2047) / 2048, 4096), 2);
   if (dtype == kBF16)
     hipLaunchKernelGGL(scale_kernel<uint16_t>, grid, dim3(256), 0, (hipStream_t)stream, (uint16_t*)t, n, (uint16_t*)u, m, g);

@@ -530,6 +530,7 @@ int abacus_residual_norm_fwd(const void* x, const void* y, const void* gamma, co
                              float* rstd, float* y_rstd, void* stream) {
   if (int rc = check("residual_norm_fwd", rows, D, gate_kind, gate != nullptr, dtype)) return rc;
   if (rows == 0) return 0;
+  ABACUS_CHECK_ARG(x && y && gamma && r && h, "residual_norm_fwd: null pointer");
   NormArgs a{};
   a.x = x;
   a.y = y;
@@ -563,14 +564,15 @@ int abacus_residual_norm_bwd(const void* dr, const void* dh, const void* r, cons
   if (int rc = check("residual_norm_bwd", rows, D, gate_kind, gate != nullptr, dtype)) return rc;
   ABACUS_CHECK_ARG((post_gamma || !dpost) && (gate || !dgate), "residual_norm_bwd: the post norm's and the gate's gradients come with them");
   ABACUS_CHECK_ARG(rows >= 1, "residual_norm_bwd: no rows");
+  ABACUS_CHECK_ARG(r && gamma && dx, "residual_norm_bwd: null pointer");
   const bool plain = !post_gamma && gate_kind == kNoGate && scale == 1.0f;
   ABACUS_CHECK_ARG(plain ? !dy || dy == dx : dy && dy != dx,
                    "residual_norm_bwd: dy is dx's memory or NULL without post_gamma, gate and scale, and its own with one");
   ABACUS_CHECK_ARG(rstd && (!post_gamma || y_rstd) && (y || (!post_gamma && gate_kind == kNoGate)),
                    "residual_norm_bwd: the forward's rstd, and with post_gamma y_rstd, and with it or a gate y");
   const int64_t need = abacus_residual_norm_bwd_ws_bytes(rows, D, post_gamma != nullptr, gate_kind);
-  ABACUS_CHECK_ARG(ws != nullptr && ws_bytes >= need, "residual_norm_bwd: workspace of %lld bytes, %lld needed",
-                   (long long)ws_bytes, (long long)need);
+  ABACUS_CHECK_ARG(ws != nullptr && (uintptr_t)ws % 16 == 0 && ws_bytes >= need,
+                   "residual_norm_bwd: workspace of %lld bytes, %lld needed, 16-byte aligned", (long long)ws_bytes, (long long)need);
   NormArgs a{};
   a.dr = dr;
   a.dh = dh;

@@ -432,7 +432,7 @@ int abacus_cross_entropy_mean_bwd(const void* logits_NV, const int64_t* targets_
  * T, D and V from 1 on; x may start at any element, the other operands are 16-byte aligned.
  * ws: device workspace of abacus_linear_cross_entropy_ws_bytes bytes (grad: with gradients).
  *
- * abacus_scale_by: n values of `dtype` at t and m at u times *g (device memory), left as they are where it is 1.
+ * abacus_scale_by: n values of `dtype` at t and m at u (16-byte aligned) times *g (device memory), left as they are where it is 1.
  * abacus_capture_id: *id (host memory) the number of the graph that the stream records, 0 where it records none. */
 #define ABACUS_LOSS_ROWS 0
 #define ABACUS_LOSS_SUM 1

@@ -395,3 +395,25 @@ def test_embedding_of_more_tokens_than_the_kernels_hold(monkeypatch):
     monkeypatch.setattr(tr, "_EMBEDDING_MOST", (50, 8, 36))
     monkeypatch.setattr(tr, "embedding", lambda t, w: torch.zeros(0))
     assert emb(t).numel() == 0 and torch.equal(emb(t.repeat(2, 1)), emb.w_vocab_D[t.repeat(2, 1)])
+
+
+_LOSS = ("abacus_linear_cross_entropy", (16, 8, 16, 16, 4, 8, 10, -100, 1, 2, None, 16, 16, 16, 16, 1 << 20, None))
+_SCALE = ("abacus_scale_by", (16, 4, 16, 4, 1, 16, None))
+_EMBED = ("abacus_embedding_fwd", (16, 16, 4, 8, 8, 1.0, 1, 16, None))
+_EMBED_BWD = ("abacus_embedding_bwd", (16, 16, 4, 8, 8, 1.0, 1, 16, 16, 1 << 20, None))
+_NORM = ("abacus_residual_norm_fwd", (16, 16, 16, None, None, 0, 4, 64, 1.0, 1e-5, 1, 16, 16, None, None, None))
+_NORM_BWD = ("abacus_residual_norm_bwd", (16, 16, 16, None, 16, None, None, 0, 16, None, 4, 64, 1.0, 1, 16, None, 16, None, None, 16, 1 << 20, None))
+
+
+@pytest.mark.parametrize("call,at,value,msg", [
+    *((_LOSS, at, None, "null") for at in (0, 2, 3)), *((_LOSS, at, 8, "aligned") for at in (2, 12, 13, 14)),
+    *((_SCALE, at, None, "null") for at in (0, 2, 5)), *((_SCALE, at, 24, "aligned") for at in (0, 2)),
+    *((_EMBED, at, None, "null") for at in (0, 1, 7)),
+    *((_EMBED_BWD, at, None, "null") for at in (0, 1, 7)), (_EMBED_BWD, 8, 20, "aligned"),
+    *((_NORM, at, None, "null") for at in (0, 1, 2, 11, 12)),
+    *((_NORM_BWD, at, None, "null") for at in (2, 4, 14)), (_NORM_BWD, 19, 24, "aligned"),
+], ids=lambda v: v[0] if isinstance(v, tuple) else str(v))
+def test_entry_points_refuse_missing_and_unaligned_operands(call, at, value, msg):
+    name, args = call
+    with pytest.raises(RuntimeError, match=msg):
+        _lib.call(name, *args[:at], value, *args[at + 1:])
