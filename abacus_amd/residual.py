@@ -106,6 +106,8 @@ class _ResidualNorm(torch.autograd.Function):
         """(dx, dy, dgamma, dpost, dgate); want: which of the last three are formed, where there is one."""
         D, dev, dt = r.shape[-1], r.device, _lib.dtype_code(r.dtype)
         rows = r.numel() // D
+        r, rstd = _contig(r), rstd.contiguous()
+        y_rstd = None if y_rstd is None else y_rstd.contiguous()
         dr, dh, y, gamma, post_gamma, gate = [None if t is None else _contig(t) for t in (dr, dh, y, gamma, post_gamma, gate)]
         dx = torch.empty_like(r)
         same = post_gamma is None and gate is None and ctx.scale == 1.0  # dy is dx

@@ -45,8 +45,11 @@ def _loss_op(x_TD, w_DV, targets_T, ignore_index: int, reduction: str):
 
 
 def _loss_call(x_TD, w_DV, targets_T, ignore_index: int, reduction: str, row_grad=None, want=(False, False), want_loss=True):
-    """(loss or None, dx or None, dw or None) of one call of the kernels."""
+    """(loss or None, dx or None, dw or None) of one call of the kernels, of operands of any strides."""
     T, D = x_TD.shape
+    if x_TD.stride(1) != 1 or x_TD.stride(0) < D:
+        x_TD = x_TD.contiguous()
+    targets_T = targets_T.contiguous()
     V = w_DV.shape[1]
     dev, dt = x_TD.device, _lib.dtype_code(x_TD.dtype, x_TD.device)
     loss = torch.empty((T,) if reduction == "none" else (), dtype=torch.float32, device=dev) if want_loss else None
@@ -110,7 +113,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         if not formed or ctx.capture != _capture(x.device):  # handed over by an earlier backward, or another's to write
             grads = _loss_call(x, w, targets, ignore_index, reduction, want=ctx.needs_input_grad[:2])[1:]
         else:  # (what becomes of them is the caller's: versions of their own, so that a retained graph does not mind)
-            grads = [None if d is None else d.data for d in grads]
+            grads = [None if d is None else _contig(d.data) for d in grads]
         sizes = [0 if t is None else t.numel() for t in grads]
         _call(x.device, "abacus_scale_by", _lib.ptr(grads[0]), sizes[0], _lib.ptr(grads[1]), sizes[1], _lib.dtype_code(x.dtype),
               g.data_ptr())
@@ -142,13 +145,11 @@ def linear_cross_entropy(x: torch.Tensor, w_DV: torch.Tensor, targets: torch.Ten
         raise TypeError(f"x is {x.dtype} and w is {w_DV.dtype}")
     if not x.device == w_DV.device == targets.device:
         raise ValueError(f"x, w and targets are on {x.device}, {w_DV.device} and {targets.device}")
-    x_TD, targets_T = x.reshape(-1, x.shape[-1]), targets.reshape(-1).contiguous()
+    x_TD, targets_T = x.reshape(-1, x.shape[-1]), targets.reshape(-1)
     if x.device.type == "cpu" or x_TD.shape[0] == 0:
         loss = _plain_loss(x_TD, w_DV, targets_T, ignore_index, reduction)
     else:
         _lib.dtype_code(x.dtype, x.device)  # refuses other types
-        if x_TD.stride(1) != 1 or x_TD.stride(0) < x_TD.shape[1]:
-            x_TD = x_TD.contiguous()
         # (forward mode too, where torch refuses a tangent that the kernels would drop)
         if torch.is_grad_enabled() and (x.requires_grad or w_DV.requires_grad) or forward_ad._current_level >= 0:
             loss = _LinearCrossEntropy.apply(x_TD, w_DV, targets_T, int(ignore_index), reduction)
@@ -195,7 +196,7 @@ def _embed_gradient(d_out, tokens, shape, scale: float):
     dw = torch.empty(V, D, dtype=d_out.dtype, device=dev)
     nbytes = _lib.query("abacus_embedding_bwd_ws_bytes", T, V, D)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    d_out = _contig(d_out)
+    tokens, d_out = tokens.contiguous(), _contig(d_out)
     _call(dev, "abacus_embedding_bwd", tokens.data_ptr(), d_out.data_ptr(), T, V, D, scale, _lib.dtype_code(d_out.dtype),
           dw.data_ptr(), ws.data_ptr(), nbytes)
     return dw
@@ -203,7 +204,7 @@ def _embed_gradient(d_out, tokens, shape, scale: float):
 
 def _embed_call(tokens, w_VD, scale: float):
     V, D = w_VD.shape
-    w = _contig(w_VD)
+    tokens, w = tokens.contiguous(), _contig(w_VD)
     out = torch.empty(*tokens.shape, D, dtype=w.dtype, device=w.device)
     _call(w.device, "abacus_embedding_fwd", tokens.data_ptr(), w.data_ptr(), tokens.numel(), V, D, scale,
           _lib.dtype_code(w.dtype), out.data_ptr())
@@ -226,7 +227,6 @@ def embedding(tokens: torch.Tensor, w_VD: torch.Tensor, scale: float = 1.0) -> t
     if w_VD.device.type == "cpu":
         return w_VD[tokens] if scale == 1.0 else w_VD[tokens] * scale
     _lib.dtype_code(w_VD.dtype, w_VD.device)  # refuses other types
-    tokens = tokens.contiguous()
     if torch.is_grad_enabled() and w_VD.requires_grad or forward_ad._current_level >= 0:  # (which refuses a tangent)
         return _Embedding.apply(tokens, w_VD, float(scale))
     return _embed_call(tokens, w_VD, float(scale))

@@ -417,3 +417,32 @@ def test_entry_points_refuse_missing_and_unaligned_operands(call, at, value, msg
     name, args = call
     with pytest.raises(RuntimeError, match=msg):
         _lib.call(name, *args[:at], value, *args[at + 1:])
+
+
+def _elsewhere(v):
+    """v's values at another place: rows with gaps between them, no vector aligned."""
+    if v.dim() < 2:
+        return torch.zeros(2 * v.numel() + 1, dtype=v.dtype, device=v.device)[1::2].copy_(v)
+    return torch.zeros(v.shape[0], v.shape[1] + 3, dtype=v.dtype, device=v.device)[:, 1:-2].copy_(v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [20, 150])
+def test_saved_tensors_of_other_strides(T):
+    """Hooks on saved tensors may bring them back at other places, with other strides: the same gradients."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16().requires_grad_()
+    t = torch.randint(0, 70, (2, T), device="cuda", generator=g)
+    table, w, y, gamma, post, gate = rand(70, 40), rand(40, 70), rand(T, 40), rand(40), rand(40), rand(T, 40)
+    leaves = table, w, y, gamma, post, gate
+
+    def run(reduction):
+        x = embedding(t[0], table)
+        r, h = residual_norm(x, y, gamma, post, gate, scale=0.5)
+        return linear_cross_entropy(h + r, w, t[1], reduction=reduction).sum()
+
+    for reduction in ("mean", "none"):
+        want = torch.autograd.grad(run(reduction), leaves)
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: v, _elsewhere):
+            got = torch.autograd.grad(run(reduction), leaves)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
