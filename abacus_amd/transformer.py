@@ -94,7 +94,7 @@ class Embedding(torch.nn.Module):
             if (_eager(w, tokens_BL) and w.is_cuda and w.dtype in (torch.float32, torch.bfloat16)
                     and tokens_BL.dtype == torch.int64 and tokens_BL.is_cuda):
                 rows, dim, tokens = _EMBEDDING_MOST
-                if w.shape[0] <= rows and w.shape[1] <= dim and tokens_BL.numel() <= tokens:
+                if 0 < w.shape[0] <= rows and 0 < w.shape[1] <= dim and tokens_BL.numel() <= tokens:
                     return embedding(tokens_BL, w)
         return self.w_vocab_D[tokens_BL]  # (B, L, D)
 

@@ -446,3 +446,12 @@ def test_saved_tensors_of_other_strides(T):
         with torch.autograd.graph.saved_tensors_hooks(lambda v: v, _elsewhere):
             got = torch.autograd.grad(run(reduction), leaves)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_embedding_of_empty_tables():
+    """Nothing to look up, or rows of nothing: indexing's results, as before."""
+    assert tr.Embedding(0, 8).cuda()(torch.zeros(0, 3, dtype=torch.int64, device="cuda")).shape == (0, 3, 8)
+    emb = tr.Embedding(5, 0).cuda()
+    out = emb(torch.tensor([4, 0], device="cuda"))
+    assert out.shape == (2, 0) and torch.autograd.grad(out.sum(), emb.w_vocab_D)[0].shape == (5, 0)
