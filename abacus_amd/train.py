@@ -164,23 +164,28 @@ def head_loss(x_BLD: torch.Tensor, w_D_vocab: torch.Tensor, tokens_BL: torch.Ten
     """next_token_loss of x_BLD @ w_D_vocab without its logits in memory (linear_cross_entropy), in fp32.
 
     The same pairs and count: position l against token l + 1, -100 left out.  Nothing waits on the host, so a
-    batch without target tokens gives NaN (and no gradient), and so does a token outside the vocabulary.
+    batch without target tokens gives NaN (and gradients of 0), and a target outside the vocabulary NaN, with the gradients of
+    a row that has no target: softmax alone.
     """
     return linear_cross_entropy(x_BLD, w_D_vocab, F.pad(tokens_BL[:, 1:], (0, 1), value=-100), ignore_index=-100)
 
 
-def _step_loss(model: torch.nn.Module, tokens_BL: torch.Tensor, fused_loss: bool) -> torch.Tensor:
+def _step_loss(model: torch.nn.Module, optimizer: AdamW, tokens_BL: torch.Tensor, fused_loss: bool) -> torch.Tensor:
+    """The step's loss; the last step's gradients are gone."""
     inputs_BL = tokens_BL.clamp(min=0)  # -100 is padding; the embedding has no row for it
     if fused_loss:
-        return head_loss(model.hidden(inputs_BL), model.w_D_vocab, tokens_BL)
-    return next_token_loss(model(inputs_BL), tokens_BL)  # of (B, L, vocab) logits
+        x_BLD = model.hidden(inputs_BL)
+        optimizer.zero_grad()  # (not beside the head's gradients and workspace, which its forward has)
+        return head_loss(x_BLD, model.w_D_vocab, tokens_BL)
+    loss = next_token_loss(model(inputs_BL), tokens_BL)  # of (B, L, vocab) logits
+    optimizer.zero_grad()
+    return loss
 
 
 def train_step(model: torch.nn.Module, optimizer: AdamW, tokens_BL: torch.Tensor, fused_loss: bool = False) -> torch.Tensor:
     """Returns the step's (detached) loss.  fused_loss: by head_loss, without the logits in memory."""
     model.train()
-    loss = _step_loss(model, tokens_BL, fused_loss)
-    optimizer.zero_grad()
+    loss = _step_loss(model, optimizer, tokens_BL, fused_loss)
     loss.backward()
     optimizer.step()
     return loss.detach()
@@ -222,8 +227,7 @@ class Trainer:
         """(loss, local loss), both the step's mean next-token cross-entropy on one process."""
         self.model.train()
         tokens_BL = tokens_BL.to(self.device)
-        loss = _step_loss(self.model, tokens_BL, self.fused_loss)
-        self.optimizer.zero_grad()
+        loss = _step_loss(self.model, self.optimizer, tokens_BL, self.fused_loss)
         loss.backward()
         local_loss = loss.detach()
         self._optimizer_step()

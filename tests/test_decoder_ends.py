@@ -455,3 +455,23 @@ def test_embedding_of_empty_tables():
     emb = tr.Embedding(5, 0).cuda()
     out = emb(torch.tensor([4, 0], device="cuda"))
     assert out.shape == (2, 0) and torch.autograd.grad(out.sum(), emb.w_vocab_D)[0].shape == (5, 0)
+
+
+@pytest.mark.gpu
+def test_step_without_logits_holds_no_more_than_with_them():
+    """The most that a step allocates, with gradients (200 MiB) of more than what the head's loss holds (its 16 MiB of probabilities and
+    up to 128 MiB of partial sums): the last step's are gone by then."""
+    peaks = []
+    for fused_loss in (False, True):
+        model = _model(vocab_size=8000, dim=256, n_heads=4, head_dim=64, n_experts=16, hidden_dim=4096)
+        opt = make_optimizer(model)
+        tokens = torch.randint(0, 8000, (4, 256), device="cuda")
+        for step in range(3):
+            if step == 1:
+                torch.cuda.synchronize()
+                torch.cuda.reset_peak_memory_stats()
+            train_step(model, opt, tokens, fused_loss=fused_loss)
+        torch.cuda.synchronize()
+        peaks.append(torch.cuda.max_memory_allocated())
+        del model, opt
+    assert peaks[1] <= peaks[0]
