@@ -1,16 +1,16 @@
 // The embedding of tokens and its gradient.  Reference: abacus/embedding.py:20-23, w[tokens], and its derivative.
 //
 //   out[t] = scale * w[token_t]                      a negative token counts from the end, as torch's indexing has it
-//   dw[v]  = scale * sum over t with token_t = v of dy[t]     in fp32, in the order of t
+//   dw[v]  = scale * sum over t with token_t = v of dy[t]     in fp32, in a fixed order
 //
 // Forward: a row is read and written once.  Backward: the tokens are sorted by id without a sort's passes:
 //   1. sort: a work-group owns a range of ids.  It reads all tokens, counts its own (a counter for each wave's part of
 //      the tokens and id, in LDS) and those of ids before its range, which is where its part of the sorted list
 //      starts; a second reading writes the list.  No work-group waits for another and no order is left to chance.
-//   2. rows: a wave adds up 64 vectors of the rows of kIds ids and writes them, zeros where no token has the id.  Ids with
+//   2. rows: a wave adds up 64 vectors of the rows of kIds ids in the order of t and writes them, zeros where no token has the id.  Ids with
 //      many tokens (more than kHot: padding, a frequent word) would keep one wave busy alone, so their sorted
 //      positions are added up in pieces of kPiece by work-groups of the same launch, in fp32;
-//   3. join: which a last launch adds in order.
+//   3. join: which a last launch adds, every fourth piece in order and the four sums.
 // Bound by bytes, and short calls by the launches: 8192 x 1024 of 32000 bf16 takes 46 us both ways, 23 at a copy's rate;
 // 16384 x 2048 of 50257 fp32, a third of the tokens one id, 205 us, 160 at that rate.
 #include <algorithm>
@@ -97,7 +97,9 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const int64_t* __res
 
 // start[v] .. start[v + 1] - 1 are the places in `order` of the tokens of id v, in the order of t.  Bound by the work-group
 // that owns the most frequent ids, whose tokens of one id take turns: 8192 tokens 12 us, 16384 20, 65536 (20000 of one
-// id) 58; more tokens in flight (16 or 32 a lane) changed nothing, the lanes of one id found by bits instead of id by id
+// id) 58; tables of more ids than 256 work-groups own read the tokens more often: both ways of 65536 tokens of 500000 x 64 bf16 190 us,
+// of 300000 of 2000000 x 64 1220, where indexing takes 103 and 385 if no id is frequent, 14000 and 91000 if half of them
+// are one; more tokens in flight (16 or 32 a lane) changed nothing, the lanes of one id found by bits instead of id by id
 // cost 73.
 __global__ __launch_bounds__(kSortWaves * 64) void embedding_sort_kernel(const int64_t* __restrict__ tokens, int T, int V,
                                                                          int ids, int* __restrict__ start,

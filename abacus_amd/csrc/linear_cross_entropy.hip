@@ -1,5 +1,5 @@
-// Cross-entropy of a linear head, x W against targets, with the gradients of both operands: the logits never whole in
-// memory.  No counterpart in the reference, whose head and loss are two steps (transformer_moe.py:75,
+// Cross-entropy of a linear head, x W against targets, with the gradients of both operands: the logits never in
+// memory, the probabilities a piece of the rows at a time.  No counterpart in the reference, whose head and loss are two steps (transformer_moe.py:75,
 // trainer.py:77-85).
 //
 //   l = x W  (fp32),   lse_t = log sum_v exp l_tv,   loss_t = lse_t - l[t, target_t]
@@ -14,7 +14,7 @@
 // One pass over a chunk of kept rows (all of them while their P takes at most kChunkBytes):
 //   1. logits: a tile of x W stays in registers; of each row and strip of columns its maximum m and the sum of
 //      exp(l - m) go out, and with gradients exp(l - m) itself, in 16 bits of which 10 are mantissa for bf16
-//      operands (it is in [0, 1], so 6 bits of exponent and no sign do; rounded four times finer than P).
+//      operands (it is in [0, 1], so 6 bits of exponent and no sign do; rounded eight times finer than P).
 //   2. rows: the strips' (m, sum) joined to lse and the loss; P in place of the exponentials, rounded once to the
 //      operands' type, which the matrix instructions take.
 //   3. dx and dw: two products on P.  Where their tiles are fewer than the CUs, slices of the reduction in fp32,

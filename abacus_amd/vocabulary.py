@@ -3,8 +3,9 @@
 ``embedding`` is embedding.py's indexing with a scale; its gradient adds the rows of each token in fp32, by tokens
 sorted by id (csrc/embedding.hip).
 
-``linear_cross_entropy`` is the cross-entropy of ``x @ w`` without its logits in memory: the products, the softmax and
-the gradients of both operands run over them piece by piece (csrc/linear_cross_entropy.hip).  The reference takes the
+``linear_cross_entropy`` is the cross-entropy of ``x @ w`` without its logits in memory: they stay in the registers they are
+formed in, and with gradients the probabilities are in memory a piece of the rows at a time, from which the products of both
+operands' gradients are taken (csrc/linear_cross_entropy.hip).  The reference takes the
 two steps one after the other (transformer_moe.py:75, kernels/liger.py:12-47).
 
 CPU tensors take the same steps in torch's operations.
@@ -130,9 +131,12 @@ def linear_cross_entropy(x: torch.Tensor, w_DV: torch.Tensor, targets: torch.Ten
     waits on the host.  Logits and sums are fp32, whatever the operands' type; ignored rows cost no products.
 
     Where a gradient is recorded, a mean's or sum's forward forms both and the backward hands them over (times the loss's
-    own, rounded once more where that is not 1).  Besides them a call holds the kept rows of x, and with gradients a piece of the
-    probabilities of at most 1 GiB in w's type, of the rows one after the other; a w of other strides than a contiguous one's,
-    or of an odd vocabulary for over 64 rows, is copied.
+    own, rounded once more where that is not 1).  The losses of rows have the logits formed again by the backward.  Besides the
+    gradients a call holds a copy of x (of all rows: how many are kept is known on the device alone) and, with gradients, the
+    probabilities in w's type of one piece of the rows after the other: up to 1 GiB, or 256 rows where those are more.  Where the
+    rows take several pieces dw's sums in fp32 (4 D V bytes) come to it, and up to 128 MiB of partial sums where the products are small:
+    2.3 GiB in all for 16384 x 4096 x 65536 in bf16.  A w of other strides than a contiguous one's, or of an odd vocabulary for over 64
+    rows, is copied.
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction is one of {', '.join(_REDUCTIONS)}, got {reduction!r}")
@@ -217,6 +221,10 @@ def embedding(tokens: torch.Tensor, w_VD: torch.Tensor, scale: float = 1.0) -> t
     Negative tokens count from the end, as in torch's indexing.  A token outside [-V, V) gives a row of NaN and no
     gradient on the GPU (on the CPU torch raises); nothing waits on the host.  The gradient of a row is the sum of its
     tokens' in fp32, times the scale, rounded once, and the same bits every run.
+
+    Text repeats tokens, and the gradient's time hardly depends on how often.  It does on the table: past some 2^18 rows every
+    2^18 more have all tokens read once more (csrc/embedding.hip), and indexing, whose time is that of the most frequent token, is
+    faster for tokens that are all different.
     """
     if tokens.dtype != torch.int64:
         raise ValueError(f"embedding takes int64 tokens, got {tokens.dtype}")

@@ -419,14 +419,15 @@ int abacus_cross_entropy_mean_bwd(const void* logits_NV, const int64_t* targets_
                                   int64_t ignore_index, int dtype, void* dlogits_NV, void* stream);
 
 /* Cross-entropy of a linear head with the gradients of both operands, the logits never
- * whole in memory (no counterpart in the reference, whose head and loss are two steps).
+ * in memory and the probabilities a piece of the rows at a time (no counterpart in the reference, whose head and loss are two steps).
  * Of l = x W, x_TD (T, D) with rows x_stride elements apart and w_DV (D, V), and int64
  * targets_T: row t's loss is log(sum_v exp(l_tv)) - l[t, targets_T[t]] in fp32, 0 where
- * its target is ignore_index, NaN where it is another value outside [0, V).
+ * its target is ignore_index, NaN where it is another value outside [0, V) (its gradients are those of
+ * a row without a target: P = s softmax).
  * reduction: ABACUS_LOSS_ROWS, loss is each row's (T values); ABACUS_LOSS_SUM and
  * ABACUS_LOSS_MEAN (over the rows not ignored), one value.  loss may be NULL where a gradient is not.
  * dx_TD (T, D), dw_DV (D, V), contiguous, `dtype`; NULL: not computed.  They are those of the
- * sum or mean, or with ABACUS_LOSS_ROWS of the sum of row_grad_T[t] (fp32) times each
+ * sum or mean, or with ABACUS_LOSS_ROWS of the sum of row_grad_T[t] (fp32; NaN and infinities reach their row's dx, and dw) times each
  * row's loss (NULL without gradients, and for the others).  Logits, sums and
  * gradients are fp32; P = s (softmax - onehot) is rounded to `dtype` for the products, the gradients once.
  * T, D and V from 1 on; x may start at any element, the other operands are 16-byte aligned.
@@ -447,8 +448,8 @@ int abacus_capture_id(int64_t* id, void* stream);
 
 /* The embedding of tokens (embedding.py:20-23): out_TD[t] = scale * w_VD[tokens_T[t]], a
  * negative token counted from the end; a token outside [-V, V) gives NaN and has no gradient.
- * Backward: dw_VD[v] = scale * the sum of d_out_TD's rows of token v in fp32, in the
- * order of t, rounded once; rows of no token are 0.  ws: abacus_embedding_bwd_ws_bytes bytes. */
+ * Backward: dw_VD[v] = scale * the sum of d_out_TD's rows of token v in fp32, in a
+ * fixed order, rounded once; rows of no token are 0.  ws: abacus_embedding_bwd_ws_bytes bytes, 16-byte aligned. */
 int abacus_embedding_fwd(const int64_t* tokens_T, const void* w_VD, int64_t T, int64_t V, int64_t D, float scale,
                          int dtype, void* out_TD, void* stream);
 int64_t abacus_embedding_bwd_ws_bytes(int64_t T, int64_t V, int64_t D);
@@ -463,7 +464,7 @@ int abacus_embedding_bwd(const int64_t* tokens_T, const void* d_out_TD, int64_t 
  * Backward, of dr and dh (NULL: zeros): dx, dy (may be dx's own memory or NULL where b is y and
  * scale 1 without a gate: they are the same), dgamma, and dpost and dgate with post_gamma and gate (each of these three
  * NULL: not formed); sums over rows in fp32, in a fixed order.  y is read with a gate or post_gamma only.
- * ws: abacus_residual_norm_bwd_ws_bytes bytes.  D: 8 to 8192 (bf16), 4 to 4096 (fp32). */
+ * ws: abacus_residual_norm_bwd_ws_bytes bytes, 16-byte aligned.  D: 8 to 8192 (bf16), 4 to 4096 (fp32). */
 int abacus_residual_norm_fwd(const void* x, const void* y, const void* gamma, const void* post_gamma, const void* gate,
                              int gate_kind, int64_t rows, int64_t D, float scale, float eps, int dtype, void* r,
                              void* h, float* rstd, float* y_rstd, void* stream);
