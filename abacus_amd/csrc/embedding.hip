@@ -7,9 +7,9 @@
 //   1. sort: a work-group owns a range of ids.  It reads all tokens, counts its own (a counter for each wave's part of
 //      the tokens and id, in LDS) and those of ids before its range, which is where its part of the sorted list
 //      starts; a second reading writes the list.  No work-group waits for another and no order is left to chance.
-//   2. rows: a wave adds up 64 vectors of the rows of kIds ids in the order of t and writes them, zeros where no token has the id.  Ids with
-//      many tokens (more than kHot: padding, a frequent word) would keep one wave busy alone, so their sorted
-//      positions are added up in pieces of kPiece by work-groups of the same launch, in fp32;
+//   2. rows: a wave adds up 64 vectors of the rows of kIds ids in the order of t and writes them, zeros where no token has
+//      the id.  Ids with many tokens (more than kHot: padding, a frequent word) would keep one wave busy alone, so their
+//      sorted positions are added up in pieces of kPiece by work-groups of the same launch, in fp32;
 //   3. join: which a last launch adds, every fourth piece in order and the four sums.
 // Bound by bytes, and short calls by the launches: 8192 x 1024 of 32000 bf16 takes 46 us both ways, 23 at a copy's rate;
 // 16384 x 2048 of 50257 fp32, a third of the tokens one id, 205 us, 160 at that rate.
@@ -97,9 +97,9 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const int64_t* __res
 
 // start[v] .. start[v + 1] - 1 are the places in `order` of the tokens of id v, in the order of t.  Bound by the work-group
 // that owns the most frequent ids, whose tokens of one id take turns: 8192 tokens 12 us, 16384 20, 65536 (20000 of one
-// id) 58; tables of more ids than 256 work-groups own read the tokens more often: both ways of 65536 tokens of 500000 x 64 bf16 190 us,
-// of 300000 of 2000000 x 64 1220, where indexing takes 103 and 385 if no id is frequent, 14000 and 91000 if half of them
-// are one; more tokens in flight (16 or 32 a lane) changed nothing, the lanes of one id found by bits instead of id by id
+// id) 58.  Tables of more ids than 256 work-groups own have the tokens read more often: both ways of 65536 tokens of
+// 500000 x 64 bf16 take 190 us, of 300000 of 2000000 x 64 1220, where indexing takes 103 and 385 if no id is frequent, 14000
+// and 91000 if half of the tokens are one.  More tokens in flight (16 or 32 a lane) changed nothing, the lanes of one id found by bits instead of id by id
 // cost 73.
 __global__ __launch_bounds__(kSortWaves * 64) void embedding_sort_kernel(const int64_t* __restrict__ tokens, int T, int V,
                                                                          int ids, int* __restrict__ start,
@@ -328,7 +328,8 @@ int backward(const int64_t* tokens, const void* dy, int64_t n, int64_t V, int64_
   const int slabs = (int)((D + 64 * VecTraits<T>::kN - 1) / (64 * VecTraits<T>::kN));
   const int64_t tasks = (V + kIds - 1) / kIds * slabs, blocks = 2 * pieces + (tasks + 3) / 4;
   // (a launch has fewer than 2^32 threads a dimension)
-  ABACUS_CHECK_ARG(blocks < (1ll << 24), "embedding_bwd: %lld tokens of a table of %lld x %lld", (long long)n, (long long)V, (long long)D);
+  ABACUS_CHECK_ARG(blocks < (1ll << 24), "embedding_bwd: %lld tokens of a table of %lld x %lld", (long long)n, (long long)V,
+                   (long long)D);
   const int ids = (int)std::min<int64_t>(kMaxIds, (V + 255) / 256);
   hipLaunchKernelGGL(embedding_sort_kernel, dim3((unsigned)((V + ids - 1) / ids)), dim3(kSortWaves * 64),
                      kSortWaves * ids * 4, s, tokens, (int)n, (int)V, ids, start, order);

@@ -1,6 +1,6 @@
 // Cross-entropy of a linear head, x W against targets, with the gradients of both operands: the logits never in
-// memory, the probabilities a piece of the rows at a time.  No counterpart in the reference, whose head and loss are two steps (transformer_moe.py:75,
-// trainer.py:77-85).
+// memory, the probabilities a piece of the rows at a time.  No counterpart in the reference, whose head and loss are two
+// steps (transformer_moe.py:75, trainer.py:77-85).
 //
 //   l = x W  (fp32),   lse_t = log sum_v exp l_tv,   loss_t = lse_t - l[t, target_t]
 //   P_tv = s_t (exp(l_tv - lse_t) - [v = target_t]),   dx = c P W^T,   dw = c x^T P

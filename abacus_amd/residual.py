@@ -112,7 +112,8 @@ class _ResidualNorm(torch.autograd.Function):
         dx = torch.empty_like(r)
         same = post_gamma is None and gate is None and ctx.scale == 1.0  # dy is dx
         dy = None if same else torch.empty_like(r)
-        dgamma, dpost, dgate = (torch.empty_like(t) if t is not None and w else None for t, w in zip((gamma, post_gamma, gate), want))
+        dgamma, dpost, dgate = (torch.empty_like(t) if w and t is not None else None
+                                for t, w in zip((gamma, post_gamma, gate), want))
         kind = _gate_kind(gate)
         nbytes = _lib.query("abacus_residual_norm_bwd_ws_bytes", rows, D, int(post_gamma is not None), kind)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)

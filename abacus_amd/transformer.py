@@ -894,7 +894,8 @@ class TransformerMoe(torch.nn.Module):
     def hidden(self, tokens_BL: torch.Tensor) -> torch.Tensor:
         """What the head multiplies: the blocks' output through the last norm, (B, L, D)."""
         x_BLD = self.embedding(tokens_BL)
-        if not (type(x_BLD) in _PLAIN and x_BLD.is_cuda and len(self.blocks) and all(_bare(b, TransformerBlockMoe) for b in self.blocks)):
+        if not (type(x_BLD) in _PLAIN and x_BLD.is_cuda and len(self.blocks)
+                and all(_bare(b, TransformerBlockMoe) for b in self.blocks)):
             for block in self.blocks:
                 x_BLD = block(x_BLD, self.rotary)
             return self.norm(x_BLD)

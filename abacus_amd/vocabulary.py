@@ -133,10 +133,10 @@ def linear_cross_entropy(x: torch.Tensor, w_DV: torch.Tensor, targets: torch.Ten
     Where a gradient is recorded, a mean's or sum's forward forms both and the backward hands them over (times the loss's
     own, rounded once more where that is not 1).  The losses of rows have the logits formed again by the backward.  Besides the
     gradients a call holds a copy of x (of all rows: how many are kept is known on the device alone) and, with gradients, the
-    probabilities in w's type of one piece of the rows after the other: up to 1 GiB, or 256 rows where those are more.  Where the
-    rows take several pieces dw's sums in fp32 (4 D V bytes) come to it, and up to 128 MiB of partial sums where the products are small:
-    2.3 GiB in all for 16384 x 4096 x 65536 in bf16.  A w of other strides than a contiguous one's, or of an odd vocabulary for over 64
-    rows, is copied.
+    probabilities in w's type of one piece of the rows after the other: up to 1 GiB, or 256 rows where those are more.  Where
+    the rows take several pieces dw's sums in fp32 (4 D V bytes) come to it, and up to 128 MiB of partial sums where the
+    products are small: 2.3 GiB in all for 16384 x 4096 x 65536 in bf16.  A w of other strides than a contiguous one's, or of an
+    odd vocabulary for over 64 rows, is copied.
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction is one of {', '.join(_REDUCTIONS)}, got {reduction!r}")

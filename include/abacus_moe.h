@@ -419,7 +419,8 @@ int abacus_cross_entropy_mean_bwd(const void* logits_NV, const int64_t* targets_
                                   int64_t ignore_index, int dtype, void* dlogits_NV, void* stream);
 
 /* Cross-entropy of a linear head with the gradients of both operands, the logits never
- * in memory and the probabilities a piece of the rows at a time (no counterpart in the reference, whose head and loss are two steps).
+ * in memory and the probabilities a piece of the rows at a time (no counterpart in the
+ * reference, whose head and loss are two steps).
  * Of l = x W, x_TD (T, D) with rows x_stride elements apart and w_DV (D, V), and int64
  * targets_T: row t's loss is log(sum_v exp(l_tv)) - l[t, targets_T[t]] in fp32, 0 where
  * its target is ignore_index, NaN where it is another value outside [0, V) (its gradients are those of
@@ -427,8 +428,8 @@ int abacus_cross_entropy_mean_bwd(const void* logits_NV, const int64_t* targets_
  * reduction: ABACUS_LOSS_ROWS, loss is each row's (T values); ABACUS_LOSS_SUM and
  * ABACUS_LOSS_MEAN (over the rows not ignored), one value.  loss may be NULL where a gradient is not.
  * dx_TD (T, D), dw_DV (D, V), contiguous, `dtype`; NULL: not computed.  They are those of the
- * sum or mean, or with ABACUS_LOSS_ROWS of the sum of row_grad_T[t] (fp32; NaN and infinities reach their row's dx, and dw) times each
- * row's loss (NULL without gradients, and for the others).  Logits, sums and
+ * sum or mean, or with ABACUS_LOSS_ROWS of the sum of row_grad_T[t] (fp32; NaN and infinities reach
+ * their row's dx, and dw) times each row's loss (NULL without gradients, and for the others).  Logits, sums and
  * gradients are fp32; P = s (softmax - onehot) is rounded to `dtype` for the products, the gradients once.
  * T, D and V from 1 on; x may start at any element, the other operands are 16-byte aligned.
  * ws: device workspace of abacus_linear_cross_entropy_ws_bytes bytes (grad: with gradients).
