@@ -99,8 +99,8 @@ __global__ __launch_bounds__(256) void embedding_fwd_kernel(const int64_t* __res
 // that owns the most frequent ids, whose tokens of one id take turns: 8192 tokens 12 us, 16384 20, 65536 (20000 of one
 // id) 58.  Tables of more ids than 256 work-groups own have the tokens read more often: both ways of 65536 tokens of
 // 500000 x 64 bf16 take 190 us, of 300000 of 2000000 x 64 1220, where indexing takes 103 and 385 if no id is frequent, 14000
-// and 91000 if half of the tokens are one.  More tokens in flight (16 or 32 a lane) changed nothing, the lanes of one id found by bits instead of id by id
-// cost 73.
+// and 91000 if half of the tokens are one.  More tokens in flight (16 or 32 a lane) changed nothing, the lanes of one id
+// found by bits instead of id by id cost 73.
 __global__ __launch_bounds__(kSortWaves * 64) void embedding_sort_kernel(const int64_t* __restrict__ tokens, int T, int V,
                                                                          int ids, int* __restrict__ start,
                                                                          int* __restrict__ order) {
